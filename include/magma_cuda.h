@@ -251,6 +251,56 @@ MAGMA_API magma_status_t magma_attention_bwd(const void* q, const void* k, const
                                    float scale, int32_t causal, magma_dtype_t dtype,
                                    void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- attention over another sequence's keys and values -----------------------
+ * nn.MultiheadAttention with a key and value of another length than the query
+ * (Module.swift:2456-2660): S = (Q K^T) * scale over the keys j < kv_lens[b],
+ * P = softmax(S), O = P V. Q and O are [batch, heads, q_len, head_dim], K and V
+ * [batch, kv_heads, kv_len, head_dim]; heads is a multiple of kv_heads and
+ * query head h reads key head h / (heads / kv_heads). Every tensor has its own
+ * (batch, head, position) strides in elements, the last dimension is
+ * contiguous; an input's stride may be 0, an output's positions may not share
+ * memory. kv_lens (int32 [batch] on the device, NULL: kv_len for all) may leave
+ * a sequence without keys: its rows of O are 0, its lse -infinity and its
+ * gradients 0. Keys and values from kv_lens[b] on have no influence, whatever
+ * they hold. A length outside [0, kv_len] is clamped and recorded in the device
+ * error word. lse [batch, heads, q_len] F32 is the row log-sum-exp of the scaled
+ * scores (NULL: not written). dtype F32 or BF16, head_dim <= 128, scale finite
+ * and not negative.
+ * workspace (16-byte aligned) may be smaller than the query's answer, or NULL:
+ * the forward pass then splits long sources into fewer parts. Calls that
+ * overlap on the GPU need workspaces of their own. */
+MAGMA_API size_t magma_cross_attention_fwd_workspace_size(int64_t batch, int64_t heads,
+                                          int64_t kv_heads, int64_t q_len, int64_t kv_len,
+                                          int64_t head_dim, magma_dtype_t dtype);
+MAGMA_API magma_status_t magma_cross_attention_fwd(const void* q, const void* k, const void* v,
+                                   void* o, float* lse, const int32_t* kv_lens,
+                                   int64_t batch, int64_t heads, int64_t kv_heads,
+                                   int64_t q_len, int64_t kv_len, int64_t head_dim,
+                                   const int64_t* q_strides, const int64_t* k_strides,
+                                   const int64_t* v_strides, const int64_t* o_strides,
+                                   float scale, magma_dtype_t dtype,
+                                   void* workspace, size_t workspace_bytes, void* stream);
+
+/* Its VJP (Autodiff.swift:309-317,379-386), with P recomputed from lse:
+ * dV = P^T dO; dS = P * (dO V^T - rowsum(dO*O)); dQ = scale * dS K;
+ * dK = scale * dS^T Q, dK and dV summed over the query heads of a key head.
+ * dQ, dK and dV are written whole (keys from kv_lens[b] on get zeros), in a
+ * fixed order of additions. The workspace of the query's size is needed. */
+MAGMA_API size_t magma_cross_attention_bwd_workspace_size(int64_t batch, int64_t heads,
+                                          int64_t kv_heads, int64_t q_len, int64_t kv_len,
+                                          int64_t head_dim, magma_dtype_t dtype);
+MAGMA_API magma_status_t magma_cross_attention_bwd(const void* q, const void* k, const void* v,
+                                   const void* o, const void* d_o, const float* lse,
+                                   const int32_t* kv_lens, void* dq, void* dk, void* dv,
+                                   int64_t batch, int64_t heads, int64_t kv_heads,
+                                   int64_t q_len, int64_t kv_len, int64_t head_dim,
+                                   const int64_t* q_strides, const int64_t* k_strides,
+                                   const int64_t* v_strides, const int64_t* o_strides,
+                                   const int64_t* do_strides, const int64_t* dq_strides,
+                                   const int64_t* dk_strides, const int64_t* dv_strides,
+                                   float scale, magma_dtype_t dtype,
+                                   void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- Adam -----------------------------------------------------------------
  * Replaces optim.Adam.step (Sources/Core/Optimizer.swift:354-412) and the value
  * Adam.update (Sources/Core/TangentOptimizer.swift:99-135), element-wise over a
@@ -314,6 +364,30 @@ MAGMA_API magma_status_t magma_adam_step_clipped(float* params, const float* gra
                                                  float grad_scale, const float* grad_norm,
                                                  float max_norm, void* stream);
 
+/* clipGradNorm over the gradients of separately held parameters
+ * (Optimizer.swift:1229-1267): norm[0] = sqrt(sum over all tensors of
+ * (grad * grad_scale)^2), and out[i] = (grads[i] * grad_scale) * c with
+ * c = max_norm / (norm + 1e-6) if that is below 1, else 1 (also 1 for a NaN
+ * norm). grads, out, sizes and the dtypes (F32 or BF16, each tensor its own) are
+ * host arrays of `count` entries, read before the call returns; a tensor of size
+ * 0 may be NULL. out[i] may be grads[i] itself (same address and dtype); apart
+ * from that an output may not share memory with any tensor of the call. The
+ * squares are added in 64 bits. norm is a device F32 scalar. workspace: 8-byte
+ * aligned, magma_grad_norm_multi_workspace_size(count) bytes of device memory.
+ * magma_grad_norm_multi writes the norm only. */
+MAGMA_API int64_t magma_grad_norm_multi_workspace_size(int32_t count);
+MAGMA_API magma_status_t magma_grad_norm_multi(const void* const* grads, const int64_t* sizes,
+                                               const magma_dtype_t* dtypes, int32_t count,
+                                               float grad_scale, float* norm, void* workspace,
+                                               int64_t workspace_bytes, void* stream);
+MAGMA_API magma_status_t magma_clip_grad_norm_multi(const void* const* grads, void* const* out,
+                                                    const int64_t* sizes,
+                                                    const magma_dtype_t* grad_dtypes,
+                                                    const magma_dtype_t* out_dtypes, int32_t count,
+                                                    float grad_scale, float max_norm, float* norm,
+                                                    void* workspace, int64_t workspace_bytes,
+                                                    void* stream);
+
 /* Learning rate of optim.WarmupCosineScheduler (Optimizer.swift:766-803) at
  * scheduler step `step` (0 for the first training step; clamped to
  * total_steps as the scheduler's step() clamps): linear warmup
@@ -361,6 +435,41 @@ MAGMA_API magma_status_t magma_embedding_bwd_deterministic(const int32_t* tokens
                                                            int32_t accumulate_dwpe,
                                                            void* workspace,
                                                            int64_t workspace_bytes, void* stream);
+
+/* nn.Embedding with a scale (Module.swift:339-410; encoder-decoder models scale
+ * by sqrt(dim)) and an optional position row:
+ *   out[b*seq+s, :] = scale * table[tokens[b*seq+s], :] + pos[s, :].
+ * table [vocab, dim] with rows table_ld elements apart, pos [>= seq, dim]
+ * (NULL: none) in table_dtype; out [batch*seq, dim] in out_dtype; F32 or BF16,
+ * F32 arithmetic. A token outside [0, vocab) contributes a zero row and is
+ * recorded in the device error word. */
+MAGMA_API magma_status_t magma_embedding_scaled_fwd(const int32_t* tokens, const void* table,
+                                   int64_t table_ld, const void* pos, void* out, int64_t batch,
+                                   int64_t seq, int64_t dim, int64_t vocab, float scale,
+                                   magma_dtype_t table_dtype, magma_dtype_t out_dtype,
+                                   void* stream);
+
+/* Its VJP by sorted tokens, in a fixed order of additions and with the same
+ * work per block however often a token repeats:
+ *   dtable[v, :] = scale * sum_{r : tokens[r] = v} dout[r, :], 0 for tokens that
+ *   do not occur and for padding_idx (-1: none); dpos[s, :] = sum_b dout[b*seq+s, :]
+ *   (all rows; dpos F32 [seq, dim], NULL: not wanted).
+ * accumulate (accumulate_dpos) != 0 adds to dtable (dpos) instead; rows of
+ * dtable that get nothing are then left alone. dout [batch*seq, dim] with rows
+ * dout_ld apart, dtable [vocab, dim] with rows dtable_ld apart, F32 or BF16;
+ * sums in F32, rounded once. Tokens outside [0, vocab) are skipped and recorded
+ * in the device error word. workspace: 16-byte aligned,
+ * magma_embedding_scaled_bwd_workspace_size bytes; calls that overlap on the GPU
+ * need workspaces of their own. */
+MAGMA_API int64_t magma_embedding_scaled_bwd_workspace_size(int64_t batch, int64_t seq,
+                                                            int64_t dim);
+MAGMA_API magma_status_t magma_embedding_scaled_bwd(const int32_t* tokens, const void* dout,
+                                   int64_t dout_ld, void* dtable, int64_t dtable_ld, float* dpos,
+                                   int64_t batch, int64_t seq, int64_t dim, int64_t vocab,
+                                   float scale, int64_t padding_idx, int32_t accumulate,
+                                   int32_t accumulate_dpos, magma_dtype_t dout_dtype,
+                                   magma_dtype_t dtable_dtype, void* workspace,
+                                   int64_t workspace_bytes, void* stream);
 
 /* Softmax cross-entropy with class-index targets, forward and backward in one
  * pass (main.swift:412-433, Loss.swift:627-699): for each row r of logits

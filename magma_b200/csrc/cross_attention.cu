@@ -1,0 +1,142 @@
+// C-ABI entry points of cross attention: argument checks and dispatch.
+#include <algorithm>
+#include <cmath>
+
+#include "cross_attention.cuh"
+
+using namespace magma;
+
+namespace {
+
+// Strides of a [d0, d1, d2, hd] tensor. An output's positions may not share
+// memory: taken from the smallest stride up, each must step over all that the
+// smaller ones span.
+magma_status_t set_strides(const char* fn, const char* what, const int64_t* from, int64_t (&to)[3],
+                           bool output, int64_t d0, int64_t d1, int64_t d2, int64_t hd) {
+  MAGMA_REQUIRE(from != nullptr, "%s: NULL strides of %s", fn, what);
+  const int64_t dims[3] = {d0, d1, d2};
+  for (int i = 0; i < 3; ++i) {
+    MAGMA_REQUIRE(from[i] >= 0 && from[i] < (1LL << 40), "%s: stride %lld of %s", fn,
+                  (long long)from[i], what);
+    to[i] = dims[i] > 1 ? from[i] : 0;
+  }
+  if (!output || d0 == 0 || d1 == 0 || d2 == 0) return MAGMA_OK;
+  int order[3] = {0, 1, 2};
+  std::sort(order, order + 3, [&](int a, int b) { return to[a] < to[b]; });
+  int64_t span = hd;
+  for (int i : order) {
+    if (dims[i] <= 1) continue;
+    MAGMA_REQUIRE(to[i] >= span, "%s: positions of %s share memory (stride %lld over %lld)", fn,
+                  what, (long long)to[i], (long long)span);
+    span += to[i] * (dims[i] - 1);
+  }
+  return MAGMA_OK;
+}
+
+magma_status_t geometry(const char* fn, const int32_t* kv_lens, int64_t batch, int64_t heads,
+                        int64_t kv_heads, int64_t q_len, int64_t kv_len, int64_t hd, float scale,
+                        magma_dtype_t dtype, CrossGeom* g) {
+  MAGMA_REQUIRE(batch >= 0 && heads >= 0 && kv_heads >= 0 && q_len >= 0 && kv_len >= 0,
+                "%s: negative size", fn);
+  MAGMA_REQUIRE(batch < 65536 && heads < 65536, "%s: batch and heads must be < 65536", fn);
+  MAGMA_REQUIRE(q_len < (1LL << 31) && kv_len < (1LL << 31), "%s: lengths must be < 2^31", fn);
+  MAGMA_REQUIRE(hd >= 1 && hd <= 128, "%s: head_dim %lld outside [1, 128]", fn, (long long)hd);
+  MAGMA_REQUIRE(kv_heads == 0 ? heads == 0 : heads % kv_heads == 0,
+                "%s: heads (%lld) must be a multiple of kv_heads (%lld)", fn, (long long)heads,
+                (long long)kv_heads);
+  MAGMA_REQUIRE(is_float_dtype(dtype), "%s: dtype must be F32 or BF16", fn);
+  MAGMA_REQUIRE(std::isfinite(scale) && scale >= 0.f, "%s: scale must be finite and not negative",
+                fn);
+  g->batch = batch;
+  g->heads = heads;
+  g->kv_heads = kv_heads;
+  g->q_len = q_len;
+  g->kv_len = kv_len;
+  g->group = kv_heads ? (int)(heads / kv_heads) : 0;
+  g->hd = (int)hd;
+  g->scale = scale;
+  g->lens = kv_lens;
+  g->err = device_error_word();
+  return MAGMA_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t magma_cross_attention_fwd_workspace_size(int64_t batch, int64_t heads, int64_t kv_heads,
+                                                int64_t q_len, int64_t kv_len, int64_t head_dim,
+                                                magma_dtype_t dtype) {
+  (void)batch, (void)heads, (void)kv_heads, (void)q_len, (void)kv_len, (void)head_dim, (void)dtype;
+  return 0;
+}
+
+magma_status_t magma_cross_attention_fwd(const void* q, const void* k, const void* v, void* o,
+                                         float* lse, const int32_t* kv_lens, int64_t batch,
+                                         int64_t heads, int64_t kv_heads, int64_t q_len,
+                                         int64_t kv_len, int64_t head_dim,
+                                         const int64_t* q_strides, const int64_t* k_strides,
+                                         const int64_t* v_strides, const int64_t* o_strides,
+                                         float scale, magma_dtype_t dtype, void* workspace,
+                                         size_t workspace_bytes, void* stream) {
+  const char* fn = "magma_cross_attention_fwd";
+  (void)workspace, (void)workspace_bytes;
+  CrossGeom g{};
+  if (magma_status_t st = geometry(fn, kv_lens, batch, heads, kv_heads, q_len, kv_len, head_dim,
+                                   scale, dtype, &g))
+    return st;
+  if (magma_status_t st = set_strides(fn, "q", q_strides, g.qs, false, batch, heads, q_len, head_dim)) return st;
+  if (magma_status_t st = set_strides(fn, "k", k_strides, g.ks, false, batch, kv_heads, kv_len, head_dim)) return st;
+  if (magma_status_t st = set_strides(fn, "v", v_strides, g.vs, false, batch, kv_heads, kv_len, head_dim)) return st;
+  if (magma_status_t st = set_strides(fn, "o", o_strides, g.os, true, batch, heads, q_len, head_dim)) return st;
+  if (batch == 0 || heads == 0 || q_len == 0) return MAGMA_OK;
+  MAGMA_REQUIRE(q && o && (kv_len == 0 || (k && v)), "%s: NULL pointer", fn);
+  return cross_fwd_simt(q, k, v, o, lse, g, dtype, (cudaStream_t)stream);
+}
+
+size_t magma_cross_attention_bwd_workspace_size(int64_t batch, int64_t heads, int64_t kv_heads,
+                                                int64_t q_len, int64_t kv_len, int64_t head_dim,
+                                                magma_dtype_t dtype) {
+  (void)kv_heads, (void)kv_len, (void)head_dim, (void)dtype;
+  if (batch <= 0 || heads <= 0 || q_len <= 0) return 0;
+  return sizeof(float) * (size_t)batch * (size_t)heads * (size_t)q_len;
+}
+
+magma_status_t magma_cross_attention_bwd(
+    const void* q, const void* k, const void* v, const void* o, const void* d_o, const float* lse,
+    const int32_t* kv_lens, void* dq, void* dk, void* dv, int64_t batch, int64_t heads,
+    int64_t kv_heads, int64_t q_len, int64_t kv_len, int64_t head_dim, const int64_t* q_strides,
+    const int64_t* k_strides, const int64_t* v_strides, const int64_t* o_strides,
+    const int64_t* do_strides, const int64_t* dq_strides, const int64_t* dk_strides,
+    const int64_t* dv_strides, float scale, magma_dtype_t dtype, void* workspace,
+    size_t workspace_bytes, void* stream) {
+  const char* fn = "magma_cross_attention_bwd";
+  CrossGeom g{};
+  if (magma_status_t st = geometry(fn, kv_lens, batch, heads, kv_heads, q_len, kv_len, head_dim,
+                                   scale, dtype, &g))
+    return st;
+  struct {
+    const char* what;
+    const int64_t* from;
+    int64_t (&to)[3];
+    bool output, keys;
+  } all[] = {{"q", q_strides, g.qs, false, false},    {"k", k_strides, g.ks, false, true},
+             {"v", v_strides, g.vs, false, true},     {"o", o_strides, g.os, false, false},
+             {"d_o", do_strides, g.dos, false, false}, {"dq", dq_strides, g.dqs, true, false},
+             {"dk", dk_strides, g.dks, true, true},   {"dv", dv_strides, g.dvs, true, true}};
+  for (auto& x : all)
+    if (magma_status_t st = set_strides(fn, x.what, x.from, x.to, x.output, batch,
+                                        x.keys ? kv_heads : heads, x.keys ? kv_len : q_len, head_dim))
+      return st;
+  const bool has_q = batch && heads && q_len, has_k = batch && kv_heads && kv_len;
+  MAGMA_REQUIRE(!has_q || (q && o && d_o && lse && dq), "%s: NULL pointer", fn);
+  MAGMA_REQUIRE(!has_k || (k && v && dk && dv), "%s: NULL pointer", fn);
+  const size_t need = magma_cross_attention_bwd_workspace_size(batch, heads, kv_heads, q_len,
+                                                               kv_len, head_dim, dtype);
+  MAGMA_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned16(workspace)),
+                "%s: a 16-byte aligned workspace of %zu bytes is needed", fn, need);
+  return cross_bwd_simt(q, k, v, o, d_o, lse, dq, dk, dv, static_cast<float*>(workspace), g, dtype,
+                        (cudaStream_t)stream);
+}
+
+}  // extern "C"

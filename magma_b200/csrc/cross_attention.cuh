@@ -1,0 +1,43 @@
+// What the cross-attention kernels share: the geometry of a call and the
+// hand-over between the entry points and the kernel files.
+#pragma once
+
+#include "common.cuh"
+
+namespace magma {
+
+// Queries [B, H, Sq, D] over keys and values [B, Hkv, Skv, D]; query head h
+// reads key head h / group. Strides (batch, head, position) are in elements,
+// the last dimension is contiguous. lens[b] keys of sequence b are there (all
+// of them where lens is NULL).
+struct CrossGeom {
+  int64_t batch, heads, kv_heads, q_len, kv_len;
+  int group, hd;
+  float scale;
+  const int32_t* lens;
+  int64_t qs[3], ks[3], vs[3], os[3];
+  // gradients: of dO, dQ, dK, dV
+  int64_t dos[3], dqs[3], dks[3], dvs[3];
+  int* err;
+};
+
+// Keys of sequence b; a length outside [0, kv_len] is clamped and reported.
+__device__ __forceinline__ int64_t cross_len(const CrossGeom& g, int64_t b) {
+  if (g.lens == nullptr) return g.kv_len;
+  const int64_t n = g.lens[b];
+  if (n < 0 || n > g.kv_len) {
+    set_device_error(g.err, kDevErrBadIndex);
+    return n < 0 ? 0 : g.kv_len;
+  }
+  return n;
+}
+
+// cross_attention_simt.cu: any types, strides and head sizes up to 128.
+magma_status_t cross_fwd_simt(const void* q, const void* k, const void* v, void* o, float* lse,
+                              const CrossGeom& g, magma_dtype_t dtype, cudaStream_t s);
+magma_status_t cross_bwd_simt(const void* q, const void* k, const void* v, const void* o,
+                              const void* d_o, const float* lse, void* dq, void* dk, void* dv,
+                              float* delta, const CrossGeom& g, magma_dtype_t dtype,
+                              cudaStream_t s);
+
+}  // namespace magma

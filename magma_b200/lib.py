@@ -109,6 +109,12 @@ SIGNATURES = {
     "magma_attention_bwd": (None, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64,
                                    _i64, C.POINTER(_i64), C.POINTER(_i64), _f, _i32, _i32, _vp,
                                    _sz, _vp]),
+    "magma_cross_attention_fwd_workspace_size": (_sz, [_i64] * 6 + [_i32]),
+    "magma_cross_attention_fwd": (None, [_vp] * 6 + [_i64] * 6 + [C.POINTER(_i64)] * 4 +
+                                  [_f, _i32, _vp, _sz, _vp]),
+    "magma_cross_attention_bwd_workspace_size": (_sz, [_i64] * 6 + [_i32]),
+    "magma_cross_attention_bwd": (None, [_vp] * 10 + [_i64] * 6 + [C.POINTER(_i64)] * 8 +
+                                  [_f, _i32, _vp, _sz, _vp]),
     "magma_adam_step": (None, [_vp, _vp, _vp, _vp, _vp, _i64, _f, _f, _f, _f, _f, _i64, _f, _vp]),
     "magma_adam_step_multi": (None, [C.POINTER(_vp), C.POINTER(_vp), C.POINTER(_vp),
                                      C.POINTER(_vp), C.POINTER(_i64), _i32, _f, _f, _f, _f, _f,
@@ -119,12 +125,21 @@ SIGNATURES = {
     "magma_grad_norm_combine": (None, [_vp, _i64, _vp, _vp]),
     "magma_adam_step_clipped": (None, [_vp, _vp, _vp, _vp, _vp, _i64, _f, _f, _f, _f, _f, _i64,
                                        _f, _vp, _f, _vp]),
+    "magma_grad_norm_multi_workspace_size": (_i64, [_i32]),
+    "magma_grad_norm_multi": (None, [_vp, _vp, _vp, _i32, _f, _vp, _vp, _i64, _vp]),
+    "magma_clip_grad_norm_multi": (None, [_vp, _vp, _vp, _vp, _vp, _i32, _f, _f, _vp, _vp, _i64,
+                                          _vp]),
     "magma_lr_warmup_cosine": (None, [_f, _f, _i64, _i64, _i64, C.POINTER(_f)]),
     "magma_embedding_fwd": (None, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp]),
     "magma_embedding_bwd": (None, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp]),
     "magma_embedding_bwd_workspace_size": (_i64, [_i64, _i64]),
     "magma_embedding_bwd_deterministic": (None, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i32,
                                                  _vp, _i64, _vp]),
+    "magma_embedding_scaled_fwd": (None, [_vp, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _f,
+                                          _i32, _i32, _vp]),
+    "magma_embedding_scaled_bwd_workspace_size": (_i64, [_i64, _i64, _i64]),
+    "magma_embedding_scaled_bwd": (None, [_vp, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64,
+                                          _f, _i64, _i32, _i32, _i32, _i32, _vp, _i64, _vp]),
     "magma_cross_entropy_fwd_bwd": (None, [_vp, _vp, _vp, _i64, _i64, _i64, _f, _i32, _vp]),
     "magma_cross_entropy_fwd_bwd_rowstats": (None, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _f,
                                                     _i32, _vp]),
@@ -176,6 +191,9 @@ KERNELS_PER_CALL = {
     # collectives run NCCL's kernels, not this library's
     "magma_allreduce": 0, "magma_reduce_scatter": 0, "magma_all_gather": 0,
     "magma_grad_sumsq": 2, "magma_grad_norm_combine": 1,
+    "magma_embedding_scaled_fwd": 1, "magma_embedding_scaled_bwd": 3,
+    "magma_cross_attention_fwd": 1, "magma_cross_attention_bwd": 3,
+    "magma_grad_norm_multi": 2, "magma_clip_grad_norm_multi": 2,
 }
 
 _lib = None

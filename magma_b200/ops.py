@@ -55,6 +55,45 @@ def workspace(nbytes: int, device: torch.device | None = None) -> torch.Tensor:
     return buf
 
 
+# Operators of encoder-decoder models run on the current stream of their
+# tensors' device, whichever device is current, and take a workspace of their
+# own from torch's allocator at each call, so that calls on several streams and
+# calls in captured graphs share none.
+def _same_device(*ts: torch.Tensor | None) -> torch.device:
+    _check_cuda(*ts)
+    devs = {t.device for t in ts if t is not None}
+    if len(devs) != 1:
+        raise ValueError(f"tensors on different devices: {sorted(map(str, devs))}")
+    return devs.pop()
+
+
+def _call_on(dev: torch.device, name: str, *args) -> None:
+    """lib.call with the device's current stream as the last argument."""
+    if dev.index == torch.cuda.current_device():
+        lib.call(name, *args, _stream())
+    else:
+        with torch.cuda.device(dev):
+            lib.call(name, *args, _stream())
+
+
+def _query_on(dev: torch.device, name: str, *args) -> int:
+    if dev.index == torch.cuda.current_device():
+        return lib.query(name, *args)
+    with torch.cuda.device(dev):
+        return lib.query(name, *args)
+
+
+def _scratch(nbytes: int, dev: torch.device) -> torch.Tensor | None:
+    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+
+
+def _rows_ld(t: torch.Tensor, what: str) -> int:
+    """Row stride of a 2-D tensor whose rows are contiguous."""
+    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError(f"{what} must be a 2-D tensor with contiguous rows")
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
 # --------------------------------------------------------------------------- LN
 def layer_norm_fwd(x: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor, eps: float = 1e-5,
                    out_dtype: torch.dtype | None = None, out: torch.Tensor | None = None):
@@ -202,6 +241,84 @@ def attention_bwd(q, k, v, o, d_o, lse, scale: float, causal: bool = True,
     return dq, dk, dv
 
 
+def _heads_view(t: torch.Tensor, what: str, shape: tuple | None = None, dtype=None):
+    """(batch, head, position) strides of a [B, H, S, D] view with unit D stride."""
+    if t.dim() != 4 or (t.shape[3] > 1 and t.stride(3) != 1):
+        raise ValueError(f"{what} must be [batch, heads, length, head_dim] with contiguous heads")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{what} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if dtype is not None and t.dtype != dtype:
+        raise TypeError(f"{what} has dtype {t.dtype}, expected {dtype}")
+    return (C.c_int64 * 3)(*t.stride()[:3])
+
+
+def _cross_sizes(q, k, v, kv_lens):
+    sq, sk = _heads_view(q, "q"), _heads_view(k, "k", None, q.dtype)
+    sv = _heads_view(v, "v", k.shape, q.dtype)
+    b, h, m, d = q.shape
+    if k.shape[0] != b or k.shape[3] != d:
+        raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} differ in batch or head_dim")
+    if kv_lens is not None and (kv_lens.dtype != torch.int32 or kv_lens.shape != (b,) or
+                                not kv_lens.is_contiguous()):
+        raise ValueError("kv_lens must be a contiguous int32 tensor of one length per sequence")
+    return (b, h, k.shape[1], m, k.shape[2], d), sq, sk, sv
+
+
+def cross_attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                        scale: float | None = None, kv_lens: torch.Tensor | None = None,
+                        out: torch.Tensor | None = None):
+    """Attention over another sequence's keys and values (nn.MultiheadAttention,
+    Module.swift:2456-2660) -> (o, lse).
+
+    q [B, H, Sq, D]; k, v [B, Hkv, Skv, D], H a multiple of Hkv; views with any
+    strides whose last dimension is contiguous. kv_lens (int32 [B]): the keys
+    that each sequence has; what k and v hold behind them has no influence, and
+    a sequence without keys gives zero rows and lse -inf. scale: D ** -0.5 by
+    default. One query per sequence (a decoding step) and few queries over long
+    sources split the keys over the GPU. out may not share memory with an input.
+    """
+    dev = _same_device(q, k, v, kv_lens, out)
+    sizes, sq, sk, sv = _cross_sizes(q, k, v, kv_lens)
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    so = _heads_view(out, "out", q.shape, q.dtype)
+    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=dev)
+    dt = _dtype(q)
+    ws = _scratch(_query_on(dev, "magma_cross_attention_fwd_workspace_size", *sizes, dt), dev)
+    _call_on(dev, "magma_cross_attention_fwd", _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse),
+             _ptr(kv_lens), *sizes, sq, sk, sv, so, sizes[5] ** -0.5 if scale is None else scale,
+             dt, _ptr(ws), 0 if ws is None else ws.numel())
+    return out, lse
+
+
+def cross_attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor,
+                        d_o: torch.Tensor, lse: torch.Tensor, scale: float | None = None,
+                        kv_lens: torch.Tensor | None = None, dq: torch.Tensor | None = None,
+                        dk: torch.Tensor | None = None, dv: torch.Tensor | None = None):
+    """VJP of cross_attention_fwd (Autodiff.swift:309-317,379-386) -> (dq, dk, dv).
+
+    o and lse are the forward pass's; dk and dv are summed over the query heads
+    that share a key head and are zero behind kv_lens. The outputs are written
+    whole; given ones may have any strides without overlap, and may not share
+    memory with an input."""
+    dev = _same_device(q, k, v, o, d_o, lse, kv_lens, dq, dk, dv)
+    sizes, sq, sk, sv = _cross_sizes(q, k, v, kv_lens)
+    if lse.dtype != torch.float32 or lse.shape != q.shape[:3] or not lse.is_contiguous():
+        raise ValueError("lse must be the forward pass's contiguous float32 [B, H, Sq]")
+    so, sg = _heads_view(o, "o", q.shape, q.dtype), _heads_view(d_o, "d_o", q.shape, q.dtype)
+    dq, dk, dv = (torch.empty_like(x) if g is None else g
+                  for x, g in ((q, dq), (k, dk), (v, dv)))
+    grads = [_heads_view(g, w, x.shape, q.dtype)
+             for g, w, x in ((dq, "dq", q), (dk, "dk", k), (dv, "dv", v))]
+    dt = _dtype(q)
+    ws = _scratch(_query_on(dev, "magma_cross_attention_bwd_workspace_size", *sizes, dt), dev)
+    _call_on(dev, "magma_cross_attention_bwd", _ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(d_o),
+             _ptr(lse), _ptr(kv_lens), _ptr(dq), _ptr(dk), _ptr(dv), *sizes, sq, sk, sv, so, sg,
+             *grads, sizes[5] ** -0.5 if scale is None else scale, dt, _ptr(ws),
+             0 if ws is None else ws.numel())
+    return dq, dk, dv
+
+
 # ------------------------------------------------------------------------- Adam
 def adam_step(params: torch.Tensor, grads: torch.Tensor, m: torch.Tensor, v: torch.Tensor, *,
               step: int, lr: float, beta1: float = 0.9, beta2: float = 0.999, eps: float = 1e-8,
@@ -252,6 +369,71 @@ def adam_step_clipped(params: torch.Tensor, grads: torch.Tensor, m: torch.Tensor
     lib.call("magma_adam_step_clipped", _ptr(params), _ptr(grads), _ptr(m), _ptr(v),
              _ptr(shadow_bf16), n, lr, beta1, beta2, eps, weight_decay, step, grad_scale,
              _ptr(grad_norm), max_norm, _stream())
+
+
+def _tensor_list(ts, what: str):
+    """Pointers, dtypes and sizes of contiguous tensors as C arrays."""
+    for t in ts:
+        if not t.is_contiguous():
+            raise ValueError(f"{what} must be contiguous tensors")
+    n = len(ts)
+    return ((C.c_void_p * n)(*[t.data_ptr() for t in ts]),
+            (C.c_int32 * n)(*[_dtype(t) for t in ts]),
+            (C.c_int64 * n)(*[t.numel() for t in ts]))
+
+
+def _norm_out(norm: torch.Tensor | None, dev: torch.device) -> torch.Tensor:
+    if norm is None:
+        return torch.empty(1, dtype=torch.float32, device=dev)
+    if norm.dtype != torch.float32 or norm.numel() != 1:
+        raise ValueError("the norm is one float32 value")
+    return norm
+
+
+def grad_norm_multi(grads, *, grad_scale: float = 1.0,
+                    out: torch.Tensor | None = None) -> torch.Tensor:
+    """Global L2 norm of grads * grad_scale over a list of float32 or bfloat16
+    tensors (optim.clipGradNorm, Optimizer.swift:1229-1247) as a one-element
+    device tensor. The squares are added in 64 bits."""
+    grads = list(grads)
+    if not grads:
+        raise ValueError("grad_norm_multi needs at least one tensor")
+    dev = _same_device(*grads, out)
+    ptrs, dtypes, sizes = _tensor_list(grads, "gradients")
+    norm = _norm_out(out, dev)
+    ws = _scratch(_query_on(dev, "magma_grad_norm_multi_workspace_size", len(grads)), dev)
+    _call_on(dev, "magma_grad_norm_multi", ptrs, sizes, dtypes, len(grads), grad_scale,
+             _ptr(norm), _ptr(ws), ws.numel())
+    return norm
+
+
+def clip_grad_norm(grads, max_norm: float, *, grad_scale: float = 1.0, out=None,
+                   norm: torch.Tensor | None = None) -> torch.Tensor:
+    """optim.clipGradNorm (Optimizer.swift:1229-1267) over a list of tensors:
+    out_i = (grads_i * grad_scale) * min(1, max_norm / (norm + 1e-6)), with norm
+    the global L2 norm of grads * grad_scale, which is returned as a one-element
+    device tensor. out: None to clip in place, else one tensor per gradient
+    (float32 or bfloat16, the gradient itself or memory of its own). Nothing is
+    copied to the host; a NaN norm leaves the gradients unclipped, as the
+    reference's mask does."""
+    grads = list(grads)
+    if not grads:
+        raise ValueError("clip_grad_norm needs at least one tensor")
+    outs = grads if out is None else list(out)
+    if len(outs) != len(grads):
+        raise ValueError(f"{len(outs)} outputs for {len(grads)} gradients")
+    dev = _same_device(*grads, *(() if out is None else outs), norm)
+    ptrs, dtypes, sizes = _tensor_list(grads, "gradients")
+    optrs, odtypes = ptrs, dtypes
+    if out is not None:
+        if any(o.shape != g.shape for o, g in zip(outs, grads)):
+            raise ValueError("an output differs in shape from its gradient")
+        optrs, odtypes, _ = _tensor_list(outs, "outputs")
+    norm = _norm_out(norm, dev)
+    ws = _scratch(_query_on(dev, "magma_grad_norm_multi_workspace_size", len(grads)), dev)
+    _call_on(dev, "magma_clip_grad_norm_multi", ptrs, optrs, sizes, dtypes, odtypes, len(grads),
+             grad_scale, max_norm, _ptr(norm), _ptr(ws), ws.numel())
+    return norm
 
 
 def lr_warmup_cosine(base_lr: float, min_lr: float, warmup_steps: int, total_steps: int,
@@ -309,6 +491,78 @@ def embedding_bwd_deterministic(tokens: torch.Tensor, dout: torch.Tensor, dwte: 
     lib.call("magma_embedding_bwd_deterministic", _ptr(tokens), _ptr(dout), _ptr(dwte),
              _ptr(dwpe), B, S, dwte.shape[1], dwte.shape[0], int(accumulate_dwpe), _ptr(ws),
              ws.numel() * ws.element_size(), _stream())
+
+
+def _tokens(tokens: torch.Tensor) -> tuple[int, int]:
+    if tokens.dim() != 2 or tokens.dtype != torch.int32 or not tokens.is_contiguous():
+        raise ValueError("tokens must be a contiguous int32 [batch, seq] tensor")
+    return tokens.shape[0], tokens.shape[1]
+
+
+def embedding_scaled_fwd(tokens: torch.Tensor, table: torch.Tensor,
+                         pos: torch.Tensor | None = None, *, scale: float = 1.0,
+                         out: torch.Tensor | None = None,
+                         out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """nn.Embedding (Module.swift:339-410) with a scale and an optional learned
+    position row: out[b*S+s] = scale * table[tokens[b, s]] + pos[s], as a
+    [B*S, D] tensor (the table's dtype by default). table [V, D] with contiguous
+    rows, pos [>= S, D] of the same dtype; float32 or bfloat16."""
+    dev = _same_device(tokens, table, pos, out)
+    b, n = _tokens(tokens)
+    ld = _rows_ld(table, "table")
+    v, d = table.shape
+    if pos is not None and (pos.dtype != table.dtype or pos.dim() != 2 or pos.shape[0] < n or
+                            pos.shape[1] != d or not pos.is_contiguous()):
+        raise ValueError(f"pos must be a contiguous {table.dtype} tensor of at least [{n}, {d}]")
+    if out is None:
+        out = torch.empty((b * n, d), dtype=out_dtype or table.dtype, device=dev)
+    elif out.shape != (b * n, d) or not out.is_contiguous():
+        raise ValueError(f"out must be a contiguous [{b * n}, {d}] tensor")
+    _call_on(dev, "magma_embedding_scaled_fwd", _ptr(tokens), _ptr(table), ld, _ptr(pos),
+             _ptr(out), b, n, d, v, scale, _dtype(table), _dtype(out))
+    return out
+
+
+def embedding_scaled_bwd(tokens: torch.Tensor, dout: torch.Tensor, vocab: int, *,
+                         scale: float = 1.0, padding_idx: int | None = None, pos: bool = False,
+                         dtable: torch.Tensor | None = None, dpos: torch.Tensor | None = None,
+                         accumulate: bool = False, accumulate_pos: bool = False,
+                         dtype: torch.dtype = torch.float32):
+    """VJP of embedding_scaled_fwd -> (dtable [V, D], dpos [S, D] or None), by
+    sorted tokens: the same bits on every run.
+
+    dout [B*S, D] with contiguous rows, float32 or bfloat16. dtable (of `dtype`,
+    or the given tensor) is written whole, zeros where a token does not occur
+    and at padding_idx, or added to with accumulate. dpos (float32; wanted with
+    pos=True or by giving it, then of at least S rows, those from S on left as
+    they are) is written, or added to with accumulate_pos."""
+    if (accumulate and dtable is None) or (accumulate_pos and dpos is None):
+        raise ValueError("accumulating needs the tensor that is added to")
+    dev = _same_device(tokens, dout, dtable, dpos)
+    b, n = _tokens(tokens)
+    ld = _rows_ld(dout, "dout")
+    d = dout.shape[1]
+    if dout.shape[0] != b * n:
+        raise ValueError(f"dout has {dout.shape[0]} rows for {b * n} tokens")
+    if dtable is None:
+        dtable = torch.empty((vocab, d), dtype=dtype, device=dev)
+    elif dtable.shape != (vocab, d):
+        raise ValueError(f"dtable must be [{vocab}, {d}]")
+    if dpos is None and pos:
+        dpos = torch.empty((n, d), dtype=torch.float32, device=dev)
+    elif dpos is not None and (dpos.dtype != torch.float32 or dpos.dim() != 2 or
+                               dpos.shape[0] < n or dpos.shape[1] != d or
+                               not dpos.is_contiguous()):
+        raise ValueError(f"dpos must be a contiguous float32 tensor of at least [{n}, {d}]")
+    pad = -1 if padding_idx is None else padding_idx
+    if padding_idx is not None and not 0 <= padding_idx < vocab:
+        raise ValueError(f"padding_idx {padding_idx} outside [0, {vocab})")
+    ws = _scratch(_query_on(dev, "magma_embedding_scaled_bwd_workspace_size", b, n, d), dev)
+    _call_on(dev, "magma_embedding_scaled_bwd", _ptr(tokens), _ptr(dout), ld, _ptr(dtable),
+             _rows_ld(dtable, "dtable"), _ptr(dpos), b, n, d, vocab, scale, pad, int(accumulate),
+             int(accumulate_pos), _dtype(dout), _dtype(dtable), _ptr(ws),
+             0 if ws is None else ws.numel())
+    return dtable, dpos
 
 
 def cross_entropy_fwd_bwd(logits: torch.Tensor, targets: torch.Tensor, classes: int | None = None,
