@@ -33,6 +33,27 @@ magma_status_t set_strides(const char* fn, const char* what, const int64_t* from
   return MAGMA_OK;
 }
 
+CrossGeom sizes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t q_len, int64_t kv_len,
+                int64_t hd) {
+  CrossGeom g{};
+  g.batch = batch;
+  g.heads = heads;
+  g.kv_heads = kv_heads;
+  g.q_len = q_len;
+  g.kv_len = kv_len;
+  g.group = kv_heads ? (int)(heads / kv_heads) : 0;
+  g.hd = (int)hd;
+  return g;
+}
+
+// Whether a workspace query is about a call that launches anything.
+bool has_work(int64_t batch, int64_t heads, int64_t kv_heads, int64_t q_len, int64_t kv_len,
+              int64_t hd) {
+  return batch > 0 && heads > 0 && kv_heads > 0 && q_len > 0 && kv_len > 0 && hd > 0 && hd <= 128 &&
+         batch < 65536 && heads < 65536 && heads % kv_heads == 0 && q_len < (1LL << 31) &&
+         kv_len < (1LL << 31);
+}
+
 magma_status_t geometry(const char* fn, const int32_t* kv_lens, int64_t batch, int64_t heads,
                         int64_t kv_heads, int64_t q_len, int64_t kv_len, int64_t hd, float scale,
                         magma_dtype_t dtype, CrossGeom* g) {
@@ -47,13 +68,7 @@ magma_status_t geometry(const char* fn, const int32_t* kv_lens, int64_t batch, i
   MAGMA_REQUIRE(is_float_dtype(dtype), "%s: dtype must be F32 or BF16", fn);
   MAGMA_REQUIRE(std::isfinite(scale) && scale >= 0.f, "%s: scale must be finite and not negative",
                 fn);
-  g->batch = batch;
-  g->heads = heads;
-  g->kv_heads = kv_heads;
-  g->q_len = q_len;
-  g->kv_len = kv_len;
-  g->group = kv_heads ? (int)(heads / kv_heads) : 0;
-  g->hd = (int)hd;
+  *g = sizes(batch, heads, kv_heads, q_len, kv_len, hd);
   g->scale = scale;
   g->lens = kv_lens;
   g->err = device_error_word();
@@ -67,8 +82,9 @@ extern "C" {
 size_t magma_cross_attention_fwd_workspace_size(int64_t batch, int64_t heads, int64_t kv_heads,
                                                 int64_t q_len, int64_t kv_len, int64_t head_dim,
                                                 magma_dtype_t dtype) {
-  (void)batch, (void)heads, (void)kv_heads, (void)q_len, (void)kv_len, (void)head_dim, (void)dtype;
-  return 0;
+  if (!has_work(batch, heads, kv_heads, q_len, kv_len, head_dim)) return 0;
+  CrossGeom g = sizes(batch, heads, kv_heads, q_len, kv_len, head_dim);
+  return dtype == MAGMA_DTYPE_BF16 && head_dim % 8 == 0 ? cross_tc_fwd_workspace(g) : 0;
 }
 
 magma_status_t magma_cross_attention_fwd(const void* q, const void* k, const void* v, void* o,
@@ -80,7 +96,6 @@ magma_status_t magma_cross_attention_fwd(const void* q, const void* k, const voi
                                          float scale, magma_dtype_t dtype, void* workspace,
                                          size_t workspace_bytes, void* stream) {
   const char* fn = "magma_cross_attention_fwd";
-  (void)workspace, (void)workspace_bytes;
   CrossGeom g{};
   if (magma_status_t st = geometry(fn, kv_lens, batch, heads, kv_heads, q_len, kv_len, head_dim,
                                    scale, dtype, &g))
@@ -91,15 +106,20 @@ magma_status_t magma_cross_attention_fwd(const void* q, const void* k, const voi
   if (magma_status_t st = set_strides(fn, "o", o_strides, g.os, true, batch, heads, q_len, head_dim)) return st;
   if (batch == 0 || heads == 0 || q_len == 0) return MAGMA_OK;
   MAGMA_REQUIRE(q && o && (kv_len == 0 || (k && v)), "%s: NULL pointer", fn);
+  if (cross_tc_fwd_supported(q, k, v, o, g, dtype))
+    return cross_fwd_tc_run(q, k, v, o, lse, g, workspace, workspace_bytes, (cudaStream_t)stream);
   return cross_fwd_simt(q, k, v, o, lse, g, dtype, (cudaStream_t)stream);
 }
 
 size_t magma_cross_attention_bwd_workspace_size(int64_t batch, int64_t heads, int64_t kv_heads,
                                                 int64_t q_len, int64_t kv_len, int64_t head_dim,
                                                 magma_dtype_t dtype) {
-  (void)kv_heads, (void)kv_len, (void)head_dim, (void)dtype;
   if (batch <= 0 || heads <= 0 || q_len <= 0) return 0;
-  return sizeof(float) * (size_t)batch * (size_t)heads * (size_t)q_len;
+  const size_t delta = sizeof(float) * (size_t)batch * (size_t)heads * (size_t)q_len;
+  if (dtype != MAGMA_DTYPE_BF16 || head_dim % 8 != 0 ||
+      !has_work(batch, heads, kv_heads, q_len, kv_len, head_dim))
+    return delta;
+  return cross_tc_bwd_workspace(sizes(batch, heads, kv_heads, q_len, kv_len, head_dim));
 }
 
 magma_status_t magma_cross_attention_bwd(
@@ -135,6 +155,8 @@ magma_status_t magma_cross_attention_bwd(
                                                                kv_len, head_dim, dtype);
   MAGMA_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned16(workspace)),
                 "%s: a 16-byte aligned workspace of %zu bytes is needed", fn, need);
+  if (cross_tc_bwd_supported(q, k, v, o, d_o, dq, dk, dv, g, dtype))
+    return cross_bwd_tc_run(q, k, v, o, d_o, lse, dq, dk, dv, workspace, g, (cudaStream_t)stream);
   return cross_bwd_simt(q, k, v, o, d_o, lse, dq, dk, dv, static_cast<float*>(workspace), g, dtype,
                         (cudaStream_t)stream);
 }

@@ -40,4 +40,20 @@ magma_status_t cross_bwd_simt(const void* q, const void* k, const void* v, const
                               float* delta, const CrossGeom& g, magma_dtype_t dtype,
                               cudaStream_t s);
 
+// cross_attention_tc.cu: BF16, head sizes that are multiples of 8, 16-byte
+// aligned positions. Workspaces in bytes; the forward pass takes less or none.
+bool cross_tc_fwd_supported(const void* q, const void* k, const void* v, const void* o,
+                            const CrossGeom& g, magma_dtype_t dtype);
+size_t cross_tc_fwd_workspace(const CrossGeom& g);
+magma_status_t cross_fwd_tc_run(const void* q, const void* k, const void* v, void* o, float* lse,
+                                const CrossGeom& g, void* workspace, size_t workspace_bytes,
+                                cudaStream_t s);
+bool cross_tc_bwd_supported(const void* q, const void* k, const void* v, const void* o,
+                            const void* d_o, const void* dq, const void* dk, const void* dv,
+                            const CrossGeom& g, magma_dtype_t dtype);
+size_t cross_tc_bwd_workspace(const CrossGeom& g);
+magma_status_t cross_bwd_tc_run(const void* q, const void* k, const void* v, const void* o,
+                                const void* d_o, const float* lse, void* dq, void* dk, void* dv,
+                                void* workspace, const CrossGeom& g, cudaStream_t s);
+
 }  // namespace magma

@@ -1,0 +1,1396 @@
+// Attention of queries over the keys and values of another sequence on the
+// tcgen05 tensor cores: BF16, F32 accumulation, head sizes that are multiples
+// of 8 up to 128 (padded to 64 or 128 columns by the tensor maps' zero fill).
+//
+//   cross_fwd_tc    O_t += P_t V_j over the key tiles j, S_t = Q_t K_j^T
+//   cross_rows      -lse log2(e) and delta = rowsum(dO O) of every query row
+//   cross_dkdv_tc   dV += P^T dO, dK += dS^T Q over the query tiles of every
+//                   head that shares the key head
+//   cross_dq_tc     dQ_t += dS_t K_j over the key tiles
+//   cross_join      the parts of a source that the forward pass has split
+//
+// Formulas as in cross_attention_simt.cu. The gradient recomputes S and dP in
+// both of its passes (14 instead of 10 products of the size of S) and needs no
+// partial tiles in memory and no atomics: every output element has one owner.
+//
+// All three products kernels have the same frame: persistent, one CTA per SM, a
+// TMA warp, a warp whose first lane issues the MMAs, and two warpgroups (thread
+// = row) that turn score tiles into probabilities; while one works the tensor
+// cores run for the other. Lengths that differ between the sequences are dealt
+// out longest first in a snake over the CTAs. Rows of V (forward) or K (dQ) from
+// the length on are set to zero in shared memory before a product reads them,
+// so whatever lies behind a length meets a probability of 0 only as 0.
+#include <cuda.h>
+
+#include <algorithm>
+
+#include "cross_attention.cuh"
+#include "sm100.cuh"
+
+namespace magma {
+namespace {
+
+using namespace sm100;
+
+constexpr int kRows = 128;            // query rows of a tile, keys of a forward tile
+constexpr int kThreads = 320;         // two warpgroups, TMA warp, MMA warp
+constexpr int kTmaWarp = 8, kMmaWarp = 9;
+constexpr int kOrder = 512;           // sequences that are dealt out by length
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kRescaleLog2 = 8.0f;
+constexpr int kBlk128 = 128 * 128;    // bytes of 64 columns of a 128-row tile
+constexpr int kBlk64 = 64 * 128;      // and of a 64-row tile
+
+struct TcArgs {
+  CrossGeom g;
+  int n_qt;                 // 128-row query tiles of a head
+  int n_pairs;              // pairs of (head, query tile) of a key head
+  int n_split;
+  int q_pad;                // query rows padded to 64 in nlse and delta
+  // 0 where a tensor's batch or head stride is 0: its map has one entry there
+  int qb, qh, kb, kh, vb, vh, db, dh;
+  void* o;
+  float* lse;
+  float* part;              // [split][b][h][q][hd] of a split source
+  float* part_lse;          // [split][b][h][q]
+  const float* nlse;        // [b][h][q_pad], -lse log2(e)
+  const float* delta;
+  void* dq;
+  void* dk;
+  void* dv;
+};
+
+// A K-major operand: rows of 128 bytes, eight rows an atom.
+__device__ __forceinline__ uint64_t desc_k(uint32_t addr) { return smem_desc_sw128(addr, 16, 1024); }
+// An MN-major operand whose 64-column blocks are `blk` bytes apart.
+__device__ __forceinline__ uint64_t desc_mn(uint32_t addr, uint32_t blk) {
+  return smem_desc_sw128(addr, blk, 1024);
+}
+// The start address is in 16-byte units in the low bits and never carries.
+__device__ __forceinline__ uint64_t desc_add(uint64_t d, uint32_t bytes) {
+  return d + (uint64_t)(bytes >> 4);
+}
+// Byte offset of columns [16 kk, 16 kk + 16) of a K-major tile.
+__device__ __forceinline__ constexpr uint32_t k_step(int kk, int blk) {
+  return (uint32_t)((kk >> 2) * blk + (kk & 3) * 32);
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&h);
+}
+
+__device__ __forceinline__ uint32_t align1024(uint8_t* raw, uint8_t** p) {
+  const uint32_t a = smem_u32(raw);
+  const uint32_t base = (a + 1023u) & ~1023u;
+  *p = raw + (base - a);
+  return base;
+}
+
+// The r-th unit of CTA c among n CTAs, even rounds in CTA order, odd ones
+// reversed; -1 past the end.
+__device__ __forceinline__ int64_t snake(int64_t r, int c, int n, int64_t units) {
+  const int64_t u = r * n + ((r & 1) ? n - 1 - c : c);
+  return u < units ? u : -1;
+}
+
+// order[rank] = sequence, longest first.
+__device__ __forceinline__ void order_by_length(const CrossGeom& g, uint16_t* order) {
+  if (g.lens == nullptr || g.batch > kOrder) return;
+  for (int i = threadIdx.x; i < (int)g.batch; i += blockDim.x) {
+    const int n = g.lens[i];
+    int rank = 0;
+    for (int j = 0; j < (int)g.batch; ++j) {
+      const int o = g.lens[j];
+      rank += o > n || (o == n && j < i);
+    }
+    order[rank] = (uint16_t)i;
+  }
+}
+__device__ __forceinline__ int64_t sequence_of(const CrossGeom& g, const uint16_t* order,
+                                               int64_t rank) {
+  return g.lens == nullptr || g.batch > kOrder ? rank : order[rank];
+}
+
+// Sets row r of a tile to zero: `blocks` blocks of 128 bytes, `blk` apart.
+__device__ __forceinline__ void zero_row(uint32_t tile, int r, int blocks, int blk) {
+  for (int i = 0; i < blocks; ++i)
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+      asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(tile + i * blk + r * 128 + c * 16),
+                   "r"(0u)
+                   : "memory");
+}
+
+// 32 F32 columns of a row times mul as BF16, those below `cols`.
+__device__ __forceinline__ void store_cols32(__nv_bfloat16* dst, const uint32_t (&v)[32], float mul,
+                                             int cols) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    if (q * 8 >= cols) break;
+    uint4 u;
+    u.x = pack_bf16(__uint_as_float(v[q * 8 + 0]) * mul, __uint_as_float(v[q * 8 + 1]) * mul);
+    u.y = pack_bf16(__uint_as_float(v[q * 8 + 2]) * mul, __uint_as_float(v[q * 8 + 3]) * mul);
+    u.z = pack_bf16(__uint_as_float(v[q * 8 + 4]) * mul, __uint_as_float(v[q * 8 + 5]) * mul);
+    u.w = pack_bf16(__uint_as_float(v[q * 8 + 6]) * mul, __uint_as_float(v[q * 8 + 7]) * mul);
+    reinterpret_cast<uint4*>(dst)[q] = u;
+  }
+}
+__device__ __forceinline__ void zero_cols(__nv_bfloat16* dst, int hd) {
+  for (int c = 0; c < hd; c += 8) *reinterpret_cast<uint4*>(dst + c) = make_uint4(0, 0, 0, 0);
+}
+
+// A pair of (head, query tile) items that read the same key head: items 2p and
+// 2p + 1 of the heads' query tiles in order.
+struct PairUnit {
+  int64_t b;
+  int kvh, split;
+  int h[2], qt[2];
+  int items;
+  int64_t len;
+  int t0, n;  // first tile of the keys, number of tiles
+};
+
+template <int KT>
+__device__ __forceinline__ PairUnit pair_unit(const TcArgs& a, const uint16_t* order, int64_t u) {
+  const CrossGeom& g = a.g;
+  PairUnit w;
+  const int64_t per_head = (int64_t)a.n_pairs * a.n_split;
+  const int64_t per_seq = per_head * g.kv_heads;
+  w.b = sequence_of(g, order, u / per_seq);
+  const int64_t rest = u % per_seq;
+  w.kvh = (int)(rest / per_head);
+  const int x = (int)(rest % per_head);
+  w.split = x / a.n_pairs;
+  const int p = x % a.n_pairs;
+  const int all = g.group * a.n_qt;
+  w.items = 2 * p + 1 < all ? 2 : 1;
+  for (int t = 0; t < 2; ++t) {
+    const int i = 2 * p + t < all ? 2 * p + t : 2 * p;
+    w.h[t] = w.kvh * g.group + i / a.n_qt;
+    w.qt[t] = i % a.n_qt;
+  }
+  w.len = cross_len(g, w.b);
+  const int tiles = (int)((w.len + KT - 1) / KT);
+  const int each = (tiles + a.n_split - 1) / a.n_split;
+  w.t0 = w.split * each < tiles ? w.split * each : tiles;
+  w.n = tiles - w.t0 < each ? tiles - w.t0 : each;
+  return w;
+}
+
+// =============================================================== forward
+// Warps 0-3 turn S_0 into P_0, warps 4-7 S_1 into P_1. TMEM columns, head size
+// 64: S_t at 128 t, O_t at 256 + 64 t, P_t (BF16 pairs, the A operand of P V) at
+// 384 + 64 t, so S_t(j + 1) is computed as soon as S_t(j) has been read. Head
+// size 128: S_t at 128 t, O_t at 256 + 128 t, and P_t takes the first half of
+// S_t's columns: S_t(j + 1) follows P_t(j) V_j, and the other tile's softmax
+// covers the wait. O_t is rescaled only when a row's maximum grows by more than
+// 2^8 (the stale maximum is exact after the final division).
+template <int HD>
+struct Fwd {
+  static constexpr bool kOver = HD == 128;
+  static constexpr int kBlocks = HD / 64;
+  static constexpr int kTile = kBlocks * kBlk128;
+  static constexpr int kQBufs = HD == 64 ? 2 : 1;
+  static constexpr int kKs = HD == 64 ? 4 : 3, kVs = HD == 64 ? 4 : 2;
+  static constexpr int kQ = 0;
+  static constexpr int kK = kQBufs * 2 * kTile;
+  static constexpr int kV = kK + kKs * kTile;
+  static constexpr int kBar = kV + kVs * kTile;
+  static constexpr int kBars = 2 * kQBufs + 2 * kKs + 2 * kVs + 8 + 1;
+  static constexpr int kOrd = kBar + kBars * 8 + 8;
+  static constexpr int kSmem = kOrd + 2 * kOrder + 1024;
+  static_assert(kSmem <= 232448, "shared memory");
+  __device__ static uint32_t tS(uint32_t t) { return t * 128; }
+  __device__ static uint32_t tO(uint32_t t) { return 256 + t * HD; }
+  __device__ static uint32_t tP(uint32_t t) { return kOver ? t * 128 : 384 + t * 64; }
+};
+
+template <int HD>
+__global__ void __launch_bounds__(kThreads, 1)
+cross_fwd_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+             const __grid_constant__ CUtensorMap tmV, const __grid_constant__ TcArgs a) {
+  using F = Fwd<HD>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* sp;
+  const uint32_t base = align1024(smem_raw, &sp);
+  auto sQ = [&](int qb, int t) { return base + F::kQ + (2 * qb + t) * F::kTile; };
+  auto sK = [&](int st) { return base + F::kK + st * F::kTile; };
+  auto sV = [&](int st) { return base + F::kV + st * F::kTile; };
+  const uint32_t bars = base + F::kBar;
+  auto q_full = [&](int i) { return bars + 8u * i; };
+  auto q_empty = [&](int i) { return bars + 8u * (F::kQBufs + i); };
+  const uint32_t kbars = bars + 16u * F::kQBufs;
+  auto k_full = [&](int i) { return kbars + 8u * i; };
+  auto k_empty = [&](int i) { return kbars + 8u * (F::kKs + i); };
+  const uint32_t vbars = kbars + 16u * F::kKs;
+  auto v_full = [&](int i) { return vbars + 8u * i; };
+  auto v_empty = [&](int i) { return vbars + 8u * (F::kVs + i); };
+  const uint32_t sbars = vbars + 16u * F::kVs;
+  auto s_full = [&](int t) { return sbars + 8u * t; };
+  auto s_free = [&](int t) { return sbars + 8u * (2 + t); };
+  auto p_full = [&](int t) { return sbars + 8u * (4 + t); };
+  auto pv_done = [&](int t) { return sbars + 8u * (6 + t); };
+  const uint32_t done_bar = sbars + 64u;
+  const uint32_t tslot = bars + 8u * F::kBars;
+  uint32_t* tslot_ptr = reinterpret_cast<uint32_t*>(sp + F::kBar + 8 * F::kBars);
+  uint16_t* order = reinterpret_cast<uint16_t*>(sp + F::kOrd);
+
+  const CrossGeom& g = a.g;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t units = (int64_t)a.n_pairs * a.n_split * g.kv_heads * g.batch;
+  const int ctas = (int)gridDim.x, cta = (int)blockIdx.x;
+
+  if (threadIdx.x == 0) {
+    prefetch_tensormap(&tmQ);
+    prefetch_tensormap(&tmK);
+    prefetch_tensormap(&tmV);
+    for (int i = 0; i < F::kBars; ++i) {
+      const uint32_t b = bars + 8u * i;
+      const bool by_warps = (b >= s_free(0) && b <= s_free(1)) || (b >= p_full(0) && b <= p_full(1));
+      mbar_init(b, by_warps ? 4 : 1);
+    }
+    fence_barrier_init();
+  }
+  if (warp == kMmaWarp) tmem_alloc(tslot, 512);
+  order_by_length(g, order);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tslot_ptr);
+
+  if (warp == kTmaWarp) {
+    if (lane == 0) {
+      bool ok = true;
+      int gk = 0;  // key tiles loaded so far
+      int ru = 0;  // units that had keys
+      for (int64_t r = 0; ok; ++r) {
+        const int64_t u = snake(r, cta, ctas, units);
+        if (u < 0) break;
+        const PairUnit w = pair_unit<kRows>(a, order, u);
+        if (w.n <= 0) continue;
+        const int qb = ru % F::kQBufs;
+        if (!mbar_wait(q_empty(qb), (uint32_t)(((ru / F::kQBufs) & 1) ^ 1), g.err)) break;
+        mbar_expect_tx(q_full(qb), w.items * F::kTile);
+        for (int t = 0; t < w.items; ++t)
+          for (int c = 0; c < F::kBlocks; ++c)
+            tma_load_4d(sQ(qb, t) + c * kBlk128, &tmQ, c * 64, w.qt[t] * kRows, w.h[t] * a.qh,
+                        (int)w.b * a.qb, q_full(qb));
+        for (int j = 0; j < w.n; ++j, ++gk) {
+          const int ks = gk % F::kKs, vs = gk % F::kVs;
+          const int row = (w.t0 + j) * kRows;
+          if (!mbar_wait(k_empty(ks), (uint32_t)(((gk / F::kKs) & 1) ^ 1), g.err)) { ok = false; break; }
+          mbar_expect_tx(k_full(ks), F::kTile);
+          for (int c = 0; c < F::kBlocks; ++c)
+            tma_load_4d(sK(ks) + c * kBlk128, &tmK, c * 64, row, w.kvh * a.kh, (int)w.b * a.kb,
+                        k_full(ks));
+          if (!mbar_wait(v_empty(vs), (uint32_t)(((gk / F::kVs) & 1) ^ 1), g.err)) { ok = false; break; }
+          mbar_expect_tx(v_full(vs), F::kTile);
+          for (int c = 0; c < F::kBlocks; ++c)
+            tma_load_4d(sV(vs) + c * kBlk128, &tmV, c * 64, row, w.kvh * a.vh, (int)w.b * a.vb,
+                        v_full(vs));
+        }
+        ++ru;
+      }
+      // every tile has been consumed before the producer leaves
+      for (int i = gk; i < gk + F::kVs && ok; ++i)
+        ok = mbar_wait(v_empty(i % F::kVs), (uint32_t)(((i / F::kVs) & 1) ^ 1), g.err);
+    }
+  } else if (warp == kMmaWarp) {
+    if (lane == 0) {
+      constexpr uint32_t idS = idesc_bf16_f32(kRows, kRows, 0, 0);
+      constexpr uint32_t idO = idesc_bf16_f32(kRows, HD, 0, 1);
+      const uint64_t dq0 = desc_k(sQ(0, 0)), dk0 = desc_k(sK(0)), dv0 = desc_mn(sV(0), kBlk128);
+      bool ok = true;
+      int gk = 0, ru = 0;
+      int ns[2] = {0, 0}, np[2] = {0, 0};
+      // S_t of the key tile at ring position kg
+      auto issue_s = [&](int t, int qb, int kg) -> bool {
+        if (!F::kOver && ns[t] >= 1 && !mbar_wait(s_free(t), (uint32_t)((ns[t] - 1) & 1), g.err))
+          return false;
+        const int st = kg % F::kKs;
+        if (!mbar_wait(k_full(st), (uint32_t)((kg / F::kKs) & 1), g.err)) return false;
+        tc_fence_after();
+        const uint64_t dq = desc_add(dq0, (uint32_t)(2 * qb + t) * F::kTile);
+        const uint64_t dk = desc_add(dk0, (uint32_t)st * F::kTile);
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; ++kk)
+          mma_bf16_ss(tmem + F::tS(t), desc_add(dq, k_step(kk, kBlk128)),
+                      desc_add(dk, k_step(kk, kBlk128)), idS, kk > 0 ? 1u : 0u);
+        mma_commit(s_full(t));
+        ++ns[t];
+        return true;
+      };
+      auto issue_pv = [&](int t, int j, int kg) -> bool {
+        const int st = kg % F::kVs;
+        if (!mbar_wait(v_full(st), (uint32_t)((kg / F::kVs) & 1), g.err)) return false;
+        if (!mbar_wait(p_full(t), (uint32_t)(np[t] & 1), g.err)) return false;
+        tc_fence_after();
+        const uint64_t dv = desc_add(dv0, (uint32_t)st * F::kTile);
+#pragma unroll
+        for (int kk = 0; kk < kRows / 16; ++kk)
+          mma_bf16_ts(tmem + F::tO(t), tmem + F::tP(t) + kk * 8, desc_add(dv, kk * 2048), idO,
+                      j > 0 || kk > 0 ? 1u : 0u);
+        mma_commit(pv_done(t));
+        ++np[t];
+        return true;
+      };
+      for (int64_t r = 0; ok; ++r) {
+        const int64_t u = snake(r, cta, ctas, units);
+        if (u < 0) break;
+        const PairUnit w = pair_unit<kRows>(a, order, u);
+        if (w.n <= 0) continue;
+        const int qb = ru % F::kQBufs;
+        if (!mbar_wait(q_full(qb), (uint32_t)((ru / F::kQBufs) & 1), g.err)) break;
+        for (int t = 0; t < w.items && ok; ++t) ok = issue_s(t, qb, gk);
+        if (!ok) break;
+        mma_commit(k_empty(gk % F::kKs));
+        for (int j = 0; j < w.n && ok; ++j) {
+          for (int t = 0; t < w.items && ok; ++t) {
+            // head size 64: S_t(j + 1) as soon as S_t(j) has been read; 128: P_t(j)
+            // lies in S_t's columns, so S_t(j + 1) goes behind P_t(j) V_j
+            if (!F::kOver && j + 1 < w.n) ok = issue_s(t, qb, gk + j + 1);
+            if (ok) ok = issue_pv(t, j, gk + j);
+            if (ok && t + 1 == w.items) mma_commit(v_empty((gk + j) % F::kVs));
+            if (F::kOver && ok && j + 1 < w.n) ok = issue_s(t, qb, gk + j + 1);
+          }
+          if (ok && j + 1 < w.n) mma_commit(k_empty((gk + j + 1) % F::kKs));
+        }
+        gk += w.n;
+        ++ru;
+        mma_commit(q_empty(qb));
+      }
+      mma_commit(done_bar);
+      mbar_wait(done_bar, 0, g.err);
+    }
+  } else {
+    const int t = warp >> 2;
+    const int row = (warp & 3) * 32 + lane;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t srow = tmem + F::tS(t) + lanes;
+    const uint32_t orow = tmem + F::tO(t) + lanes;
+    const uint32_t prow = tmem + F::tP(t) + lanes;
+    const float sl2 = g.scale * kLog2e;
+    bool ok = true;
+    int gs = 0;  // this warpgroup's steps so far
+    int gk = 0;
+    for (int64_t r = 0;; ++r) {
+      const int64_t u = snake(r, cta, ctas, units);
+      if (u < 0) break;
+      const PairUnit w = pair_unit<kRows>(a, order, u);
+      if (t >= w.items) {
+        gk += w.n > 0 ? w.n : 0;
+        continue;
+      }
+      const int64_t qi = (int64_t)w.qt[t] * kRows + row;
+      float m_run = -INFINITY, l_run = 0.f;
+      for (int j = 0; j < w.n; ++j, ++gs, ++gk) {
+        const int64_t left = w.len - (int64_t)(w.t0 + j) * kRows;
+        const bool tail = left < kRows;
+        const int lim = tail ? (int)left - 1 : kRows - 1;  // last key of the tile
+        if (ok && !mbar_wait(s_full(t), (uint32_t)(gs & 1), g.err)) ok = false;
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) continue;
+        tc_fence_after();
+        // the row's maximum, two halves of 64 columns, eight chains
+        float mx8[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) mx8[i] = -INFINITY;
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+          uint32_t v[2][32];
+          tmem_ld32(srow + hh * 64, v[0]);
+          tmem_ld32(srow + hh * 64 + 32, v[1]);
+          tmem_wait_ld();
+          if (!tail) {
+#pragma unroll
+            for (int e = 0; e < 64; ++e)
+              mx8[e & 7] = fmaxf(mx8[e & 7], __uint_as_float(v[e >> 5][e & 31]));
+          } else {
+#pragma unroll
+            for (int e = 0; e < 64; ++e)
+              if (hh * 64 + e <= lim)
+                mx8[e & 7] = fmaxf(mx8[e & 7], __uint_as_float(v[e >> 5][e & 31]));
+          }
+        }
+        const float mx = fmaxf(fmaxf(fmaxf(mx8[0], mx8[1]), fmaxf(mx8[2], mx8[3])),
+                               fmaxf(fmaxf(mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7])));
+        const float m_new = fmaxf(m_run, mx * sl2);
+        // the previous P V has read P_t and added into O_t
+        if (gs >= 1 && !mbar_wait(pv_done(t), (uint32_t)((gs - 1) & 1), g.err)) ok = false;
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) continue;
+        tc_fence_after();
+        if (j == 0) {
+          m_run = m_new == -INFINITY ? 0.f : m_new;
+        } else if (__any_sync(0xffffffffu, m_new > m_run + kRescaleLog2)) {
+          const float alpha = ex2_approx(m_run - m_new);
+          m_run = m_new;
+          l_run *= alpha;
+#pragma unroll
+          for (int c = 0; c < HD / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld32(orow + c * 32, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            tmem_st32(orow + c * 32, o);
+          }
+          tmem_wait_st();
+        }
+        // P = exp2(S scale log2(e) - m), two columns per instruction
+        unsigned long long rs2[2] = {0ull, 0ull};
+        const unsigned long long sl22 = f2_pack(sl2, sl2), nm2 = f2_pack(-m_run, -m_run);
+        auto exp32 = [&](const uint32_t (&v)[32], int c) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            float x0, x1;
+            f2_unpack(f2_fma(f2_pack(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])),
+                             sl22, nm2), x0, x1);
+            float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
+            if (tail) {
+              if (c + 2 * e > lim) p0 = 0.f;
+              if (c + 2 * e + 1 > lim) p1 = 0.f;
+            }
+            rs2[e & 1] = f2_add(rs2[e & 1], f2_pack(p0, p1));
+            pk[e] = pack_bf16(p0, p1);
+          }
+          tmem_st16(prow + c / 2, pk);
+        };
+        uint32_t va[2][32], vb[32], vc[32];
+        tmem_ld32(srow, va[0]);
+        tmem_ld32(srow + 32, va[1]);
+        tmem_wait_ld();
+        exp32(va[0], 0);
+        tmem_ld32(srow + 64, vb);
+        exp32(va[1], 32);
+        tmem_wait_ld();
+        tmem_ld32(srow + 96, vc);
+        exp32(vb, 64);
+        tmem_wait_ld();
+        if (!F::kOver) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(s_free(t));
+        }
+        exp32(vc, 96);
+        float a0, a1, b0, b1;
+        f2_unpack(rs2[0], a0, a1);
+        f2_unpack(rs2[1], b0, b1);
+        l_run += (a0 + a1) + (b0 + b1);
+        if (tail && t == 0) {  // P_0 V goes first: both tiles find the rows zeroed
+          const int vs = gk % F::kVs;
+          if (!mbar_wait(v_full(vs), (uint32_t)((gk / F::kVs) & 1), g.err)) ok = false;
+          ok = __all_sync(0xffffffffu, ok);
+          if (ok && row > lim) zero_row(sV(vs), row, F::kBlocks, kBlk128);
+          fence_proxy_async_smem();
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (ok && lane == 0) mbar_arrive(p_full(t));
+      }
+      if (ok && w.n > 0 && !mbar_wait(pv_done(t), (uint32_t)((gs - 1) & 1), g.err)) ok = false;
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) continue;
+      tc_fence_after();
+      const float inv = l_run == 0.f ? 0.f : 1.0f / l_run;  // no keys: a zero row
+      const float lse = l_run == 0.f ? -INFINITY : m_run * kLn2 + logf(l_run);
+      const int64_t at = (w.b * g.heads + w.h[t]) * g.q_len + qi;
+      const bool in = qi < g.q_len;
+      __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(a.o) + w.b * g.os[0] + w.h[t] * g.os[1] +
+                           qi * g.os[2];
+      const int64_t pat = w.split * g.batch * g.heads * g.q_len + at;
+#pragma unroll
+      for (int c = 0; c < HD / 32; ++c) {
+        uint32_t v[32];
+        if (w.n > 0) {
+          tmem_ld32(orow + c * 32, v);
+          tmem_wait_ld();
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) v[e] = 0u;
+        }
+        if (!in || c * 32 >= g.hd) continue;
+        if (a.n_split == 1) {
+          store_cols32(dst + c * 32, v, inv, g.hd - c * 32);
+        } else {
+          float4* pd = reinterpret_cast<float4*>(a.part + pat * g.hd + c * 32);
+#pragma unroll
+          for (int q = 0; q < 8; ++q)
+            if (c * 32 + q * 4 < g.hd)
+              pd[q] = make_float4(__uint_as_float(v[4 * q]) * inv, __uint_as_float(v[4 * q + 1]) * inv,
+                                  __uint_as_float(v[4 * q + 2]) * inv,
+                                  __uint_as_float(v[4 * q + 3]) * inv);
+        }
+      }
+      if (in) {
+        if (a.n_split > 1) a.part_lse[pat] = lse;
+        else if (a.lse != nullptr) a.lse[at] = lse;
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// =========================================================== rows of the gradient
+// nlse = -lse log2(e), delta = rowsum(dO O), rows padded to a multiple of 64 with
+// (-inf, 0): the exponential of a row that is not there, or that had no
+// probabilities, is 0. Eight threads a row.
+__global__ void __launch_bounds__(256)
+cross_rows(const __nv_bfloat16* __restrict__ o, const __nv_bfloat16* __restrict__ d_o,
+           const float* __restrict__ lse, float* __restrict__ nlse, float* __restrict__ delta,
+           const CrossGeom g, int q_pad) {
+  const int64_t i = (int64_t)blockIdx.x * 32 + (threadIdx.x >> 3);
+  const int part = threadIdx.x & 7;
+  const int64_t rows = g.batch * g.heads * q_pad;
+  if (i >= rows) return;  // rows is a multiple of 32: whole warps leave
+  const int64_t bh = i / q_pad, q = i % q_pad, b = bh / g.heads, h = bh % g.heads;
+  float acc = 0.f;
+  if (q < g.q_len) {
+    const __nv_bfloat16* po = o + b * g.os[0] + h * g.os[1] + q * g.os[2];
+    const __nv_bfloat16* pd = d_o + b * g.dos[0] + h * g.dos[1] + q * g.dos[2];
+    for (int c = part * 8; c < g.hd; c += 64) {
+      float x[8], y[8];
+      load8(po + c, x);
+      load8(pd + c, y);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc = fmaf(x[e], y[e], acc);
+    }
+  }
+#pragma unroll
+  for (int w = 4; w > 0; w >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, w);
+  if (part != 0) return;
+  float l = -INFINITY;
+  if (q < g.q_len) {
+    const float v = lse[bh * g.q_len + q];
+    l = v == -INFINITY ? -INFINITY : -v * kLog2e;
+  }
+  nlse[i] = l;
+  delta[i] = q < g.q_len ? acc : 0.f;
+}
+
+// P and dS of 32 columns of a row as BF16 pairs, two columns per instruction.
+// nl and dl: the rows' terms of each column pair.
+template <typename NL, typename DL>
+__device__ __forceinline__ void grad32(const uint32_t (&vs)[32], const uint32_t (&vd)[32],
+                                       unsigned long long sl22, NL nl, DL dl, uint32_t (&pp)[16],
+                                       uint32_t (&pd)[16], int lim) {
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    float x0, x1, d0, d1;
+    f2_unpack(f2_fma(f2_pack(__uint_as_float(vs[2 * e]), __uint_as_float(vs[2 * e + 1])), sl22,
+                     nl(e)), x0, x1);
+    const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
+    f2_unpack(f2_mul(f2_pack(p0, p1),
+                     f2_sub(f2_pack(__uint_as_float(vd[2 * e]), __uint_as_float(vd[2 * e + 1])),
+                            dl(e))), d0, d1);
+    if (2 * e > lim) d0 = 0.f;
+    if (2 * e + 1 > lim) d1 = 0.f;
+    pp[e] = pack_bf16(p0, p1);
+    pd[e] = pack_bf16(d0, d1);
+  }
+}
+
+// =================================================================== dQ
+// As the forward kernel, over 64-key tiles: S_t, dP_t = dO_t V_j^T; dS_t as BF16
+// pairs in S_t's columns is the A operand of dQ_t += dS_t K_j. TMEM columns of
+// tile t from 256 t: S, dP, dQ.
+template <int HD>
+struct Dq {
+  static constexpr int kKeys = 64;
+  static constexpr int kBlocks = HD / 64;
+  static constexpr int kTile = kBlocks * kBlk128;   // Q, dO
+  static constexpr int kKv = kBlocks * kBlk64;      // K, V
+  static constexpr int kStages = HD == 64 ? 6 : 3;
+  static constexpr int kQ = 0;                      // [t][Q, dO]
+  static constexpr int kRing = 4 * kTile;           // [stage][K, V]
+  static constexpr int kBar = kRing + kStages * 2 * kKv;
+  static constexpr int kBars = 2 + 2 * kStages + 6 + 1;
+  static constexpr int kOrd = kBar + kBars * 8 + 8;
+  static constexpr int kSmem = kOrd + 2 * kOrder + 1024;
+  static_assert(kSmem <= 232448, "shared memory");
+};
+
+template <int HD>
+__global__ void __launch_bounds__(kThreads, 1)
+cross_dq_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmG,
+            const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+            const __grid_constant__ TcArgs a) {
+  using F = Dq<HD>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* sp;
+  const uint32_t base = align1024(smem_raw, &sp);
+  auto sQ = [&](int t) { return base + F::kQ + 2 * t * F::kTile; };
+  auto sG = [&](int t) { return base + F::kQ + (2 * t + 1) * F::kTile; };
+  auto sK = [&](int st) { return base + F::kRing + 2 * st * F::kKv; };
+  auto sV = [&](int st) { return base + F::kRing + (2 * st + 1) * F::kKv; };
+  const uint32_t bars = base + F::kBar;
+  const uint32_t q_full = bars, q_empty = bars + 8;
+  auto kv_full = [&](int i) { return bars + 8u * (2 + i); };
+  auto kv_empty = [&](int i) { return bars + 8u * (2 + F::kStages + i); };
+  const uint32_t sbars = bars + 8u * (2 + 2 * F::kStages);
+  auto s_full = [&](int t) { return sbars + 8u * t; };
+  auto ds_full = [&](int t) { return sbars + 8u * (2 + t); };
+  auto dq_done = [&](int t) { return sbars + 8u * (4 + t); };
+  const uint32_t done_bar = sbars + 48u;
+  const uint32_t tslot = bars + 8u * F::kBars;
+  uint32_t* tslot_ptr = reinterpret_cast<uint32_t*>(sp + F::kBar + 8 * F::kBars);
+  uint16_t* order = reinterpret_cast<uint16_t*>(sp + F::kOrd);
+
+  const CrossGeom& g = a.g;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t units = (int64_t)a.n_pairs * g.kv_heads * g.batch;
+  const int ctas = (int)gridDim.x, cta = (int)blockIdx.x;
+
+  if (threadIdx.x == 0) {
+    prefetch_tensormap(&tmQ);
+    prefetch_tensormap(&tmG);
+    prefetch_tensormap(&tmK);
+    prefetch_tensormap(&tmV);
+    for (int i = 0; i < F::kBars; ++i) {
+      const uint32_t b = bars + 8u * i;
+      mbar_init(b, b == ds_full(0) || b == ds_full(1) ? 4 : 1);
+    }
+    fence_barrier_init();
+  }
+  if (warp == kMmaWarp) tmem_alloc(tslot, 512);
+  order_by_length(g, order);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tslot_ptr);
+  auto tS = [&](int t) { return tmem + 256u * t; };
+  auto tDp = [&](int t) { return tmem + 256u * t + 64u; };
+  auto tDq = [&](int t) { return tmem + 256u * t + 128u; };
+
+  if (warp == kTmaWarp) {
+    if (lane == 0) {
+      bool ok = true;
+      int gk = 0, ru = 0;
+      for (int64_t r = 0; ok; ++r) {
+        const int64_t u = snake(r, cta, ctas, units);
+        if (u < 0) break;
+        const PairUnit w = pair_unit<F::kKeys>(a, order, u);
+        if (w.n <= 0) continue;
+        if (!mbar_wait(q_empty, (uint32_t)((ru & 1) ^ 1), g.err)) break;
+        mbar_expect_tx(q_full, w.items * 2 * F::kTile);
+        for (int t = 0; t < w.items; ++t)
+          for (int c = 0; c < F::kBlocks; ++c) {
+            tma_load_4d(sQ(t) + c * kBlk128, &tmQ, c * 64, w.qt[t] * kRows, w.h[t] * a.qh,
+                        (int)w.b * a.qb, q_full);
+            tma_load_4d(sG(t) + c * kBlk128, &tmG, c * 64, w.qt[t] * kRows, w.h[t] * a.dh,
+                        (int)w.b * a.db, q_full);
+          }
+        for (int j = 0; j < w.n; ++j, ++gk) {
+          const int st = gk % F::kStages, row = j * F::kKeys;
+          if (!mbar_wait(kv_empty(st), (uint32_t)(((gk / F::kStages) & 1) ^ 1), g.err)) {
+            ok = false;
+            break;
+          }
+          mbar_expect_tx(kv_full(st), 2 * F::kKv);
+          for (int c = 0; c < F::kBlocks; ++c) {
+            tma_load_4d(sK(st) + c * kBlk64, &tmK, c * 64, row, w.kvh * a.kh, (int)w.b * a.kb,
+                        kv_full(st));
+            tma_load_4d(sV(st) + c * kBlk64, &tmV, c * 64, row, w.kvh * a.vh, (int)w.b * a.vb,
+                        kv_full(st));
+          }
+        }
+        ++ru;
+      }
+      for (int i = gk; i < gk + F::kStages && ok; ++i)
+        ok = mbar_wait(kv_empty(i % F::kStages), (uint32_t)(((i / F::kStages) & 1) ^ 1), g.err);
+    }
+  } else if (warp == kMmaWarp) {
+    if (lane == 0) {
+      constexpr uint32_t idS = idesc_bf16_f32(kRows, F::kKeys, 0, 0);
+      constexpr uint32_t idQ = idesc_bf16_f32(kRows, HD, 0, 1);
+      bool ok = true;
+      int gk = 0, ru = 0;
+      int nd[2] = {0, 0};
+      const uint64_t dq0 = desc_k(sQ(0)), dg0 = desc_k(sG(0)), dk0 = desc_k(sK(0)),
+                     dv0 = desc_k(sV(0)), dkm0 = desc_mn(sK(0), kBlk64);
+      auto issue_s = [&](int t, int kg) -> bool {
+        const int st = kg % F::kStages;
+        if (!mbar_wait(kv_full(st), (uint32_t)((kg / F::kStages) & 1), g.err)) return false;
+        tc_fence_after();
+        const uint32_t at = (uint32_t)t * 2 * F::kTile, ak = (uint32_t)st * 2 * F::kKv;
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; ++kk)
+          mma_bf16_ss(tS(t), desc_add(dq0, at + k_step(kk, kBlk128)),
+                      desc_add(dk0, ak + k_step(kk, kBlk64)), idS, kk > 0 ? 1u : 0u);
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; ++kk)
+          mma_bf16_ss(tDp(t), desc_add(dg0, at + k_step(kk, kBlk128)),
+                      desc_add(dv0, ak + k_step(kk, kBlk64)), idS, kk > 0 ? 1u : 0u);
+        mma_commit(s_full(t));
+        return true;
+      };
+      for (int64_t r = 0; ok; ++r) {
+        const int64_t u = snake(r, cta, ctas, units);
+        if (u < 0) break;
+        const PairUnit w = pair_unit<F::kKeys>(a, order, u);
+        if (w.n <= 0) continue;
+        if (!mbar_wait(q_full, (uint32_t)(ru & 1), g.err)) break;
+        for (int t = 0; t < w.items && ok; ++t) ok = issue_s(t, gk);
+        for (int j = 0; j < w.n && ok; ++j) {
+          const int st = (gk + j) % F::kStages;
+          for (int t = 0; t < w.items && ok; ++t) {
+            ok = mbar_wait(ds_full(t), (uint32_t)(nd[t] & 1), g.err);
+            if (!ok) break;
+            ++nd[t];
+            tc_fence_after();
+            const uint64_t dk = desc_add(dkm0, (uint32_t)st * 2 * F::kKv);
+#pragma unroll
+            for (int kk = 0; kk < F::kKeys / 16; ++kk)
+              mma_bf16_ts(tDq(t), tS(t) + kk * 8, desc_add(dk, kk * 2048), idQ,
+                          j > 0 || kk > 0 ? 1u : 0u);
+            if (t + 1 == w.items) mma_commit(kv_empty(st));
+            if (j + 1 < w.n) ok = issue_s(t, gk + j + 1);
+            else mma_commit(dq_done(t));
+          }
+        }
+        gk += w.n;
+        ++ru;
+        mma_commit(q_empty);
+      }
+      mma_commit(done_bar);
+      mbar_wait(done_bar, 0, g.err);
+    }
+  } else {
+    const int t = warp >> 2;
+    const int row = (warp & 3) * 32 + lane;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const float sl2 = g.scale * kLog2e;
+    const unsigned long long sl22 = f2_pack(sl2, sl2);
+    bool ok = true;
+    int gs = 0, gk = 0, gu = 0;
+    for (int64_t r = 0;; ++r) {
+      const int64_t u = snake(r, cta, ctas, units);
+      if (u < 0) break;
+      const PairUnit w = pair_unit<F::kKeys>(a, order, u);
+      if (t >= w.items) {
+        gk += w.n > 0 ? w.n : 0;
+        continue;
+      }
+      const int64_t qi = (int64_t)w.qt[t] * kRows + row;
+      const bool in = qi < g.q_len;
+      const int64_t at = (w.b * g.heads + w.h[t]) * a.q_pad + qi;
+      const float nl = in ? a.nlse[at] : -INFINITY, dl = in ? a.delta[at] : 0.f;
+      const unsigned long long nl2 = f2_pack(nl, nl), dl2 = f2_pack(dl, dl);
+      for (int j = 0; j < w.n; ++j, ++gs, ++gk) {
+        const int64_t left = w.len - (int64_t)j * F::kKeys;
+        const bool tail = left < F::kKeys;
+        const int lim = tail ? (int)left - 1 : F::kKeys - 1;
+        if (ok && !mbar_wait(s_full(t), (uint32_t)(gs & 1), g.err)) ok = false;
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) continue;
+        tc_fence_after();
+        uint32_t vs[2][32], vd[2][32];
+        tmem_ld32(tS(t) + lanes, vs[0]);
+        tmem_ld32(tDp(t) + lanes, vd[0]);
+        tmem_wait_ld();
+        tmem_ld32(tS(t) + lanes + 32, vs[1]);
+        tmem_ld32(tDp(t) + lanes + 32, vd[1]);
+        uint32_t pp[16], pd[16];
+        auto n = [&](int) { return nl2; };
+        auto d = [&](int) { return dl2; };
+        if (tail) grad32(vs[0], vd[0], sl22, n, d, pp, pd, lim);
+        else grad32(vs[0], vd[0], sl22, n, d, pp, pd, 64);
+        tmem_wait_ld();  // all of S_t is in registers: dS_t may take its columns
+        tmem_st16(tS(t) + lanes, pd);
+        if (tail) grad32(vs[1], vd[1], sl22, n, d, pp, pd, lim - 32);
+        else grad32(vs[1], vd[1], sl22, n, d, pp, pd, 64);
+        tmem_st16(tS(t) + lanes + 16, pd);
+        if (tail && t == 0 && row < F::kKeys) {  // warps 0 and 1
+          const int st = gk % F::kStages;
+          if (!mbar_wait(kv_full(st), (uint32_t)((gk / F::kStages) & 1), g.err)) ok = false;
+          ok = __all_sync(0xffffffffu, ok);
+          if (ok && row > lim) zero_row(sK(st), row, F::kBlocks, kBlk64);
+          fence_proxy_async_smem();
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (ok && lane == 0) mbar_arrive(ds_full(t));
+      }
+      __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(a.dq) + w.b * g.dqs[0] + w.h[t] * g.dqs[1] +
+                           qi * g.dqs[2];
+      if (w.n <= 0) {
+        if (in) zero_cols(dst, g.hd);
+        continue;
+      }
+      if (ok && !mbar_wait(dq_done(t), (uint32_t)(gu & 1), g.err)) ok = false;
+      ++gu;
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) continue;
+      tc_fence_after();
+#pragma unroll
+      for (int c = 0; c < HD / 32; ++c) {
+        uint32_t v[32];
+        tmem_ld32(tDq(t) + lanes + c * 32, v);
+        tmem_wait_ld();
+        if (in && c * 32 < g.hd) store_cols32(dst + c * 32, v, g.scale, g.hd - c * 32);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// ================================================================ dK and dV
+// A unit is a 128-key tile of a key head; its steps are the 64-query tiles of
+// all query heads that share it. Steps alternate between two score buffers and
+// the two warpgroups: S^T = K Q^T, dP^T = V dO^T (thread = key row); P^T and
+// dS^T as BF16 pairs in the same columns are the A operands of dV += P^T dO and
+// dK += dS^T Q. TMEM columns of buffer t from 128 t: S^T, dP^T; then dV, dK.
+// Nothing is masked: a row of a key behind the length only reaches its own
+// output row, which is stored as zeros, and the terms of a query row behind
+// q_len make its probabilities 0.
+template <int HD>
+struct Dkv {
+  static constexpr int kQ = 64;                     // query rows of a step
+  static constexpr int kBlocks = HD / 64;
+  static constexpr int kTile = kBlocks * kBlk128;   // K, V
+  static constexpr int kQd = kBlocks * kBlk64;      // Q, dO
+  static constexpr int kKvBufs = HD == 64 ? 2 : 1;
+  static constexpr int kStages = HD == 64 ? 6 : 4;
+  static constexpr int kStage = 2 * kQd;
+  static constexpr int kKv = 0;                     // [buffer][K, V]
+  static constexpr int kRing = kKvBufs * 2 * kTile;
+  static constexpr int kStats = kRing + kStages * kStage;   // [stage][nlse, delta]
+  static constexpr int kBar = kStats + kStages * 2 * kQ * 4;
+  static constexpr int kBars = 2 * kKvBufs + 2 * kStages + 4 + 3;
+  static constexpr int kSmem = kBar + kBars * 8 + 16 + 8 * kOrder + 16 + 1024;
+  static_assert(kSmem <= 232448, "shared memory");
+};
+
+template <int HD>
+__global__ void __launch_bounds__(kThreads, 1)
+cross_dkdv_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmG,
+              const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+              const __grid_constant__ TcArgs a) {
+  using F = Dkv<HD>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* sp;
+  const uint32_t base = align1024(smem_raw, &sp);
+  auto sK = [&](int kb) { return base + F::kKv + 2 * kb * F::kTile; };
+  auto sV = [&](int kb) { return base + F::kKv + (2 * kb + 1) * F::kTile; };
+  auto sQ = [&](int st) { return base + F::kRing + st * F::kStage; };
+  auto sG = [&](int st) { return base + F::kRing + st * F::kStage + F::kQd; };
+  const uint32_t bars = base + F::kBar;
+  auto kv_full = [&](int i) { return bars + 8u * i; };
+  auto kv_empty = [&](int i) { return bars + 8u * (F::kKvBufs + i); };
+  const uint32_t qbars = bars + 16u * F::kKvBufs;
+  auto q_full = [&](int i) { return qbars + 8u * i; };
+  auto q_empty = [&](int i) { return qbars + 8u * (F::kStages + i); };
+  const uint32_t sbars = qbars + 16u * F::kStages;
+  auto s_full = [&](int t) { return sbars + 8u * t; };
+  auto p_full = [&](int t) { return sbars + 8u * (2 + t); };
+  const uint32_t acc_full = sbars + 32u, acc_empty = sbars + 40u, done_bar = sbars + 48u;
+  const uint32_t tslot = bars + 8u * F::kBars;
+  uint32_t* tslot_ptr = reinterpret_cast<uint32_t*>(sp + F::kBar + 8 * F::kBars);
+  // first[i]: key tiles of the sequences before i
+  int64_t* first = reinterpret_cast<int64_t*>(
+      sp + ((F::kBar + 8 * F::kBars + 8 + 15) / 16) * 16);
+
+  const CrossGeom& g = a.g;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int ctas = (int)gridDim.x, cta = (int)blockIdx.x;
+  const int64_t all_tiles = (g.kv_len + kRows - 1) / kRows;
+  // With a table of the sequences' tiles the units are exactly the tiles that
+  // have keys; without one every tile is a unit.
+  const bool table = g.lens != nullptr && g.batch < kOrder;
+  const int q_steps = a.q_pad / F::kQ;
+  const int n_it = g.group * q_steps;
+
+  if (threadIdx.x == 0) {
+    prefetch_tensormap(&tmQ);
+    prefetch_tensormap(&tmG);
+    prefetch_tensormap(&tmK);
+    prefetch_tensormap(&tmV);
+    for (int i = 0; i < F::kBars; ++i) {
+      const uint32_t b = bars + 8u * i;
+      mbar_init(b, b == p_full(0) || b == p_full(1) ? 4 : b == acc_empty ? 8 : 1);
+    }
+    fence_barrier_init();
+  }
+  if (warp == kMmaWarp) tmem_alloc(tslot, 512);
+  if (table && warp == 0) {
+    int64_t sum = 0;
+    for (int64_t i0 = 0; i0 < g.batch; i0 += 32) {
+      const int64_t i = i0 + lane;
+      int64_t n = i < g.batch ? (cross_len(g, i) + kRows - 1) / kRows : 0;
+      int64_t inc = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t x = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += x;
+      }
+      if (i < g.batch) first[i] = sum + inc - n;
+      sum += __shfl_sync(0xffffffffu, inc, 31);
+    }
+    if (lane == 0) first[g.batch] = sum;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tslot_ptr);
+  auto tS = [&](int t) { return tmem + 128u * t; };
+  auto tDp = [&](int t) { return tmem + 128u * t + 64u; };
+  const uint32_t tDv = tmem + 256u, tDk = tmem + 256u + HD;
+  const int64_t units = (table ? first[g.batch] : all_tiles * g.batch) * g.kv_heads;
+
+  struct Unit {
+    int64_t b, len;
+    int kvh, kt, n;
+  };
+  // sequences outermost, then key heads, then tiles: tiles that run at the same
+  // time read the same queries
+  auto unit = [&](int64_t u) {
+    Unit w;
+    if (table) {
+      int64_t lo = 0, hi = g.batch;  // first[lo] * kv_heads <= u < first[hi] * kv_heads
+      while (hi - lo > 1) {
+        const int64_t mid = (lo + hi) >> 1;
+        if (first[mid] * g.kv_heads <= u) lo = mid;
+        else hi = mid;
+      }
+      w.b = lo;
+      const int64_t tiles = first[lo + 1] - first[lo];
+      const int64_t rest = u - first[lo] * g.kv_heads;
+      w.kvh = (int)(rest / tiles);
+      w.kt = (int)(rest % tiles);
+    } else {
+      w.b = u / (all_tiles * g.kv_heads);
+      const int64_t rest = u % (all_tiles * g.kv_heads);
+      w.kvh = (int)(rest / all_tiles);
+      w.kt = (int)(rest % all_tiles);
+    }
+    w.len = cross_len(g, w.b);
+    w.n = (int64_t)w.kt * kRows < w.len ? n_it : 0;
+    return w;
+  };
+
+  if (warp == kTmaWarp) {
+    if (lane == 0) {
+      bool ok = true;
+      int gq = 0, ru = 0;
+      for (int64_t r = 0; ok; ++r) {
+        const int64_t u = snake(r, cta, ctas, units);
+        if (u < 0) break;
+        const Unit w = unit(u);
+        if (w.n == 0) continue;
+        const int kb = ru % F::kKvBufs;
+        if (!mbar_wait(kv_empty(kb), (uint32_t)(((ru / F::kKvBufs) & 1) ^ 1), g.err)) break;
+        mbar_expect_tx(kv_full(kb), 2 * F::kTile);
+        for (int c = 0; c < F::kBlocks; ++c) {
+          tma_load_4d(sK(kb) + c * kBlk128, &tmK, c * 64, w.kt * kRows, w.kvh * a.kh,
+                      (int)w.b * a.kb, kv_full(kb));
+          tma_load_4d(sV(kb) + c * kBlk128, &tmV, c * 64, w.kt * kRows, w.kvh * a.vh,
+                      (int)w.b * a.vb, kv_full(kb));
+        }
+        for (int i = 0; i < w.n; ++i, ++gq) {
+          const int st = gq % F::kStages;
+          if (!mbar_wait(q_empty(st), (uint32_t)(((gq / F::kStages) & 1) ^ 1), g.err)) {
+            ok = false;
+            break;
+          }
+          const int h = w.kvh * g.group + i / q_steps, q0 = i % q_steps * F::kQ;
+          const int64_t at = (w.b * g.heads + h) * a.q_pad + q0;
+          mbar_expect_tx(q_full(st), F::kStage + 2 * F::kQ * 4);
+          for (int c = 0; c < F::kBlocks; ++c) {
+            tma_load_4d(sQ(st) + c * kBlk64, &tmQ, c * 64, q0, h * a.qh, (int)w.b * a.qb, q_full(st));
+            tma_load_4d(sG(st) + c * kBlk64, &tmG, c * 64, q0, h * a.dh, (int)w.b * a.db, q_full(st));
+          }
+          const uint32_t stats = base + F::kStats + st * 2 * F::kQ * 4;
+          bulk_load(stats, a.nlse + at, F::kQ * 4, q_full(st));
+          bulk_load(stats + F::kQ * 4, a.delta + at, F::kQ * 4, q_full(st));
+        }
+        ++ru;
+      }
+      for (int i = gq; i < gq + F::kStages && ok; ++i)
+        ok = mbar_wait(q_empty(i % F::kStages), (uint32_t)(((i / F::kStages) & 1) ^ 1), g.err);
+    }
+  } else if (warp == kMmaWarp) {
+    if (lane == 0) {
+      constexpr uint32_t idS = idesc_bf16_f32(kRows, F::kQ, 0, 0);
+      constexpr uint32_t idG = idesc_bf16_f32(kRows, HD, 0, 1);
+      const uint64_t dk0 = desc_k(sK(0)), dv0 = desc_k(sV(0)), dq0 = desc_k(sQ(0)),
+                     dg0 = desc_k(sG(0)), dqm0 = desc_mn(sQ(0), kBlk64),
+                     dgm0 = desc_mn(sG(0), kBlk64);
+      bool ok = true;
+      int gs = 0, ru = 0;
+      auto issue_s = [&](int i, int kb) -> bool {  // step i of all units
+        const int st = i % F::kStages, t = i & 1;
+        if (!mbar_wait(q_full(st), (uint32_t)((i / F::kStages) & 1), g.err)) return false;
+        tc_fence_after();
+        const uint32_t aq = (uint32_t)st * F::kStage, ak = (uint32_t)kb * 2 * F::kTile;
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; ++kk)
+          mma_bf16_ss(tS(t), desc_add(dk0, ak + k_step(kk, kBlk128)),
+                      desc_add(dq0, aq + k_step(kk, kBlk64)), idS, kk > 0 ? 1u : 0u);
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; ++kk)
+          mma_bf16_ss(tDp(t), desc_add(dv0, ak + k_step(kk, kBlk128)),
+                      desc_add(dg0, aq + k_step(kk, kBlk64)), idS, kk > 0 ? 1u : 0u);
+        mma_commit(s_full(t));
+        return true;
+      };
+      for (int64_t r = 0; ok; ++r) {
+        const int64_t u = snake(r, cta, ctas, units);
+        if (u < 0) break;
+        const Unit w = unit(u);
+        if (w.n == 0) continue;
+        const int kb = ru % F::kKvBufs;
+        if (!mbar_wait(kv_full(kb), (uint32_t)((ru / F::kKvBufs) & 1), g.err)) break;
+        for (int i = 0; i < 2 && i < w.n && ok; ++i) ok = issue_s(gs + i, kb);
+        for (int i = 0; i < w.n && ok; ++i) {
+          const int s = gs + i, t = s & 1, st = s % F::kStages;
+          ok = mbar_wait(p_full(t), (uint32_t)((s >> 1) & 1), g.err);
+          // the previous unit's dV and dK have been read
+          if (ok && i == 0 && ru >= 1) ok = mbar_wait(acc_empty, (uint32_t)((ru - 1) & 1), g.err);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t aq = (uint32_t)st * F::kStage;
+#pragma unroll
+          for (int kk = 0; kk < F::kQ / 16; ++kk)
+            mma_bf16_ts(tDv, tS(t) + kk * 8, desc_add(dgm0, aq + kk * 2048), idG,
+                        i > 0 || kk > 0 ? 1u : 0u);
+#pragma unroll
+          for (int kk = 0; kk < F::kQ / 16; ++kk)
+            mma_bf16_ts(tDk, tDp(t) + kk * 8, desc_add(dqm0, aq + kk * 2048), idG,
+                        i > 0 || kk > 0 ? 1u : 0u);
+          mma_commit(q_empty(st));
+          if (i + 2 < w.n) ok = issue_s(s + 2, kb);
+        }
+        gs += w.n;
+        ++ru;
+        mma_commit(kv_empty(kb));
+        mma_commit(acc_full);
+      }
+      mma_commit(done_bar);
+      mbar_wait(done_bar, 0, g.err);
+    }
+  } else {
+    const int t = warp >> 2;
+    const int row = (warp & 3) * 32 + lane;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const float sl2 = g.scale * kLog2e;
+    const unsigned long long sl22 = f2_pack(sl2, sl2);
+    bool ok = true;
+    int gs = 0, ru = 0;
+    for (int64_t r = 0;; ++r) {
+      const int64_t u = snake(r, cta, ctas, units);
+      if (u < 0) break;
+      const Unit w = unit(u);
+      for (int i = 0; i < w.n; ++i) {
+        const int s = gs + i;
+        if ((s & 1) != t) continue;
+        const int st = s % F::kStages;
+        if (ok && !mbar_wait(s_full(t), (uint32_t)((s >> 1) & 1), g.err)) ok = false;
+        // the step's row terms came with its tiles
+        if (ok && !mbar_wait(q_full(st), (uint32_t)((s / F::kStages) & 1), g.err)) ok = false;
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) continue;
+        tc_fence_after();
+        const ulonglong2* nl =
+            reinterpret_cast<const ulonglong2*>(sp + F::kStats + st * 2 * F::kQ * 4);
+        const ulonglong2* dl = nl + F::kQ / 4;
+        uint32_t vs[2][32], vd[2][32];
+        tmem_ld32(tS(t) + lanes, vs[0]);
+        tmem_ld32(tDp(t) + lanes, vd[0]);
+        tmem_wait_ld();
+        tmem_ld32(tS(t) + lanes + 32, vs[1]);
+        tmem_ld32(tDp(t) + lanes + 32, vd[1]);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t pp[16], pd[16];
+          ulonglong2 n4, d4;
+          auto n = [&](int e) {
+            if ((e & 1) == 0) n4 = nl[c * 8 + (e >> 1)];
+            return (e & 1) ? n4.y : n4.x;
+          };
+          auto d = [&](int e) {
+            if ((e & 1) == 0) d4 = dl[c * 8 + (e >> 1)];
+            return (e & 1) ? d4.y : d4.x;
+          };
+          grad32(vs[c], vd[c], sl22, n, d, pp, pd, 64);
+          if (c == 0) tmem_wait_ld();  // both tiles are in registers
+          tmem_st16(tS(t) + lanes + 16 * c, pp);
+          tmem_st16(tDp(t) + lanes + 16 * c, pd);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full(t));
+      }
+      gs += w.n;
+      // warpgroup 0 stores dV, warpgroup 1 dK
+      const int64_t kj = (int64_t)w.kt * kRows + row;
+      const bool in = kj < g.kv_len;
+      __nv_bfloat16* dst =
+          t == 0 ? static_cast<__nv_bfloat16*>(a.dv) + w.b * g.dvs[0] + w.kvh * g.dvs[1] + kj * g.dvs[2]
+                 : static_cast<__nv_bfloat16*>(a.dk) + w.b * g.dks[0] + w.kvh * g.dks[1] + kj * g.dks[2];
+      if (w.n == 0) {
+        if (in) zero_cols(dst, g.hd);
+        continue;
+      }
+      if (ok && !mbar_wait(acc_full, (uint32_t)(ru & 1), g.err)) ok = false;
+      ++ru;
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) continue;
+      tc_fence_after();
+      const float mul = t == 0 ? 1.f : g.scale;
+#pragma unroll
+      for (int c = 0; c < HD / 32; ++c) {
+        uint32_t v[32];
+        tmem_ld32((t == 0 ? tDv : tDk) + lanes + c * 32, v);
+        tmem_wait_ld();
+        if (c + 1 == HD / 32) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(acc_empty);
+        }
+        if (!in || c * 32 >= g.hd) continue;
+        if (kj < w.len) store_cols32(dst + c * 32, v, mul, g.hd - c * 32);
+      }
+      if (in && kj >= w.len) zero_cols(dst, g.hd);
+    }
+    if (table) {  // the tiles without keys, which are no units
+      for (int64_t i = cta; i < all_tiles * g.kv_heads * g.batch; i += ctas) {
+        const int64_t kt = i % all_tiles, kvh = i / all_tiles % g.kv_heads,
+                      b = i / all_tiles / g.kv_heads;
+        if (kt < first[b + 1] - first[b]) continue;
+        const int64_t kj = kt * kRows + row;
+        if (kj >= g.kv_len) continue;
+        zero_cols(t == 0 ? static_cast<__nv_bfloat16*>(a.dv) + b * g.dvs[0] + kvh * g.dvs[1] + kj * g.dvs[2]
+                         : static_cast<__nv_bfloat16*>(a.dk) + b * g.dks[0] + kvh * g.dks[1] + kj * g.dks[2],
+                  g.hd);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// =================================================================== join
+// O and lse of a row from its parts: with M the largest lse of the parts,
+// O = sum_s exp(lse_s - M) O_s / sum_s exp(lse_s - M). A part without keys has
+// lse -inf and is not read. One warp a row.
+__global__ void __launch_bounds__(256)
+cross_join(const float* __restrict__ part, const float* __restrict__ part_lse,
+           __nv_bfloat16* __restrict__ o, float* __restrict__ lse, const CrossGeom g, int n_split) {
+  const int lane = threadIdx.x & 31;
+  const int64_t rows = g.batch * g.heads * g.q_len;
+  const int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (i >= rows) return;
+  float m = -INFINITY;
+  for (int s = lane; s < n_split; s += 32) m = fmaxf(m, part_lse[s * rows + i]);
+  m = warp_max(m);
+  float total = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  const int c = lane * 4;
+  if (m != -INFINITY) {
+    for (int s = 0; s < n_split; ++s) {
+      const float w = expf(part_lse[s * rows + i] - m);
+      if (w == 0.f) continue;
+      total += w;
+      if (c < g.hd) {
+        const float4 v = *reinterpret_cast<const float4*>(part + (s * rows + i) * g.hd + c);
+        acc.x = fmaf(w, v.x, acc.x);
+        acc.y = fmaf(w, v.y, acc.y);
+        acc.z = fmaf(w, v.z, acc.z);
+        acc.w = fmaf(w, v.w, acc.w);
+      }
+    }
+  }
+  const float inv = total == 0.f ? 0.f : 1.f / total;
+  const int64_t q = i % g.q_len, bh = i / g.q_len, h = bh % g.heads, b = bh / g.heads;
+  if (c < g.hd) {
+    const float v[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
+    store4(o + b * g.os[0] + h * g.os[1] + q * g.os[2] + c, v);
+  }
+  if (lane == 0 && lse != nullptr) lse[i] = total == 0.f ? -INFINITY : m + logf(total);
+}
+
+// ------------------------------------------------------------------ host side
+// Map of a [batch, heads, positions, hd] view: boxes of 64 columns and `rows`
+// positions. A batch or head stride of 0 becomes an extent of 1, and *bm or *hm
+// 0: the kernels multiply the coordinate by it.
+magma_status_t view_map(CUtensorMap* map, const void* p, int64_t hd, int64_t n, int64_t heads,
+                        int64_t batch, const int64_t (&st)[3], int rows, int* bm, int* hm) {
+  *bm = st[0] != 0;
+  *hm = st[1] != 0;
+  const uint64_t dims[4] = {(uint64_t)hd, (uint64_t)n, (uint64_t)(*hm ? heads : 1),
+                            (uint64_t)(*bm ? batch : 1)};
+  auto bytes = [](int64_t s) { return (uint64_t)(s ? 2 * s : 256); };
+  const uint64_t strides[3] = {bytes(st[2]), bytes(st[1]), bytes(st[0])};
+  const uint32_t box[4] = {64, (uint32_t)rows, 1, 1};
+  return encode_tensor_map_nd(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p, 4, dims, strides, box,
+                              CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+// Strides in 16-byte steps; positions may not share an address.
+bool tc_strides(const void* p, const int64_t (&st)[3], int64_t n) {
+  return aligned16(p) && st[0] % 8 == 0 && st[1] % 8 == 0 && st[2] % 8 == 0 &&
+         (st[2] != 0 || n <= 1) && st[0] < (1LL << 38) && st[1] < (1LL << 38) &&
+         st[2] < (1LL << 38);
+}
+
+template <typename K>
+magma_status_t smem_for(K kernel, int bytes) {
+  return cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes),
+                     "cross attention shared memory");
+}
+
+TcArgs args_of(const CrossGeom& g) {
+  TcArgs a{};
+  a.g = g;
+  a.n_qt = (int)ceil_div(g.q_len, kRows);
+  a.n_pairs = (int)ceil_div((int64_t)g.group * a.n_qt, 2);
+  a.n_split = 1;
+  a.q_pad = (int)(ceil_div(g.q_len, 64) * 64);
+  return a;
+}
+
+template <int HD>
+magma_status_t fwd_tc(const void* q, const void* k, const void* v, TcArgs a, cudaStream_t s) {
+  const CrossGeom& g = a.g;
+  CUtensorMap mq, mk, mv;
+  if (magma_status_t st = view_map(&mq, q, g.hd, g.q_len, g.heads, g.batch, g.qs, kRows, &a.qb, &a.qh)) return st;
+  if (magma_status_t st = view_map(&mk, k, g.hd, g.kv_len, g.kv_heads, g.batch, g.ks, kRows, &a.kb, &a.kh)) return st;
+  if (magma_status_t st = view_map(&mv, v, g.hd, g.kv_len, g.kv_heads, g.batch, g.vs, kRows, &a.vb, &a.vh)) return st;
+  if (magma_status_t st = smem_for(cross_fwd_tc<HD>, Fwd<HD>::kSmem)) return st;
+  const int64_t units = (int64_t)a.n_pairs * a.n_split * g.kv_heads * g.batch;
+  const unsigned ctas = (unsigned)std::min<int64_t>(units, num_sms());
+  cross_fwd_tc<HD><<<ctas, kThreads, Fwd<HD>::kSmem, s>>>(mq, mk, mv, a);
+  return check_launch("cross_fwd_tc");
+}
+
+template <int HD>
+magma_status_t bwd_tc(const void* q, const void* k, const void* v, const void* d_o, TcArgs a,
+                      cudaStream_t s) {
+  const CrossGeom& g = a.g;
+  CUtensorMap mq, mg, mk, mv;
+  {
+    using F = Dkv<HD>;
+    if (magma_status_t st = view_map(&mq, q, g.hd, g.q_len, g.heads, g.batch, g.qs, F::kQ, &a.qb, &a.qh)) return st;
+    if (magma_status_t st = view_map(&mg, d_o, g.hd, g.q_len, g.heads, g.batch, g.dos, F::kQ, &a.db, &a.dh)) return st;
+    if (magma_status_t st = view_map(&mk, k, g.hd, g.kv_len, g.kv_heads, g.batch, g.ks, kRows, &a.kb, &a.kh)) return st;
+    if (magma_status_t st = view_map(&mv, v, g.hd, g.kv_len, g.kv_heads, g.batch, g.vs, kRows, &a.vb, &a.vh)) return st;
+    if (magma_status_t st = smem_for(cross_dkdv_tc<HD>, F::kSmem)) return st;
+    const int64_t units = ceil_div(g.kv_len, kRows) * g.kv_heads * g.batch;
+    const unsigned ctas = (unsigned)std::min<int64_t>(units, num_sms());
+    cross_dkdv_tc<HD><<<ctas, kThreads, F::kSmem, s>>>(mq, mg, mk, mv, a);
+    if (magma_status_t st = check_launch("cross_dkdv_tc")) return st;
+  }
+  using F = Dq<HD>;
+  if (magma_status_t st = view_map(&mq, q, g.hd, g.q_len, g.heads, g.batch, g.qs, kRows, &a.qb, &a.qh)) return st;
+  if (magma_status_t st = view_map(&mg, d_o, g.hd, g.q_len, g.heads, g.batch, g.dos, kRows, &a.db, &a.dh)) return st;
+  if (magma_status_t st = view_map(&mk, k, g.hd, g.kv_len, g.kv_heads, g.batch, g.ks, F::kKeys, &a.kb, &a.kh)) return st;
+  if (magma_status_t st = view_map(&mv, v, g.hd, g.kv_len, g.kv_heads, g.batch, g.vs, F::kKeys, &a.vb, &a.vh)) return st;
+  if (magma_status_t st = smem_for(cross_dq_tc<HD>, F::kSmem)) return st;
+  const int64_t units = (int64_t)a.n_pairs * g.kv_heads * g.batch;
+  const unsigned ctas = (unsigned)std::min<int64_t>(units, num_sms());
+  cross_dq_tc<HD><<<ctas, kThreads, F::kSmem, s>>>(mq, mg, mk, mv, a);
+  return check_launch("cross_dq_tc");
+}
+
+}  // namespace
+
+bool cross_tc_fwd_supported(const void* q, const void* k, const void* v, const void* o,
+                            const CrossGeom& g, magma_dtype_t dtype) {
+  return dtype == MAGMA_DTYPE_BF16 && g.hd % 8 == 0 && g.kv_len > 0 && g.q_len > 0 &&
+         tc_strides(q, g.qs, g.q_len) && tc_strides(k, g.ks, g.kv_len) &&
+         tc_strides(v, g.vs, g.kv_len) && tc_strides(o, g.os, g.q_len) &&
+         (int64_t)g.group * ceil_div(g.q_len, kRows) < (1LL << 30);
+}
+
+bool cross_tc_bwd_supported(const void* q, const void* k, const void* v, const void* o,
+                            const void* d_o, const void* dq, const void* dk, const void* dv,
+                            const CrossGeom& g, magma_dtype_t dtype) {
+  return cross_tc_fwd_supported(q, k, v, o, g, dtype) && tc_strides(d_o, g.dos, g.q_len) &&
+         tc_strides(dq, g.dqs, g.q_len) && tc_strides(dk, g.dks, g.kv_len) &&
+         tc_strides(dv, g.dvs, g.kv_len) &&
+         (int64_t)g.group * ceil_div(g.q_len, 64) < (1LL << 31);
+}
+
+// Parts of a source: as many as fill the SMs, at least four key tiles each (a
+// part costs its share of the join: one F32 row per query and part).
+static int64_t wanted_splits(const CrossGeom& g) {
+  const TcArgs a = args_of(g);
+  const int64_t units = (int64_t)a.n_pairs * g.kv_heads * g.batch;
+  const int64_t tiles = ceil_div(g.kv_len, kRows);
+  return std::max<int64_t>(1, std::min<int64_t>(num_sms() / std::max<int64_t>(units, 1), tiles / 4));
+}
+
+size_t cross_tc_fwd_workspace(const CrossGeom& g) {
+  const int64_t n = wanted_splits(g);
+  return n <= 1 ? 0 : (size_t)n * g.batch * g.heads * g.q_len * (g.hd + 1) * sizeof(float);
+}
+
+magma_status_t cross_fwd_tc_run(const void* q, const void* k, const void* v, void* o, float* lse,
+                                const CrossGeom& g, void* workspace, size_t workspace_bytes,
+                                cudaStream_t s) {
+  TcArgs a = args_of(g);
+  a.o = o;
+  a.lse = lse;
+  const int64_t rows = g.batch * g.heads * g.q_len;
+  const size_t each = (size_t)rows * (g.hd + 1) * sizeof(float);
+  if (workspace != nullptr && aligned16(workspace))
+    a.n_split = (int)std::max<int64_t>(1, std::min<int64_t>(wanted_splits(g), workspace_bytes / each));
+  if (a.n_split > 1) {
+    a.part = static_cast<float*>(workspace);
+    a.part_lse = a.part + (size_t)a.n_split * rows * g.hd;
+  }
+  if (magma_status_t st = g.hd <= 64 ? fwd_tc<64>(q, k, v, a, s) : fwd_tc<128>(q, k, v, a, s))
+    return st;
+  if (a.n_split == 1) return MAGMA_OK;
+  cross_join<<<(unsigned)ceil_div(rows, 8), 256, 0, s>>>(
+      a.part, a.part_lse, static_cast<__nv_bfloat16*>(o), lse, g, a.n_split);
+  return check_launch("cross_join");
+}
+
+size_t cross_tc_bwd_workspace(const CrossGeom& g) {
+  return 2 * sizeof(float) * (size_t)g.batch * g.heads * (ceil_div(g.q_len, 64) * 64);
+}
+
+magma_status_t cross_bwd_tc_run(const void* q, const void* k, const void* v, const void* o,
+                                const void* d_o, const float* lse, void* dq, void* dk, void* dv,
+                                void* workspace, const CrossGeom& g, cudaStream_t s) {
+  TcArgs a = args_of(g);
+  const int64_t rows = g.batch * g.heads * a.q_pad;
+  float* nlse = static_cast<float*>(workspace);
+  float* delta = nlse + rows;
+  a.nlse = nlse;
+  a.delta = delta;
+  a.dq = dq;
+  a.dk = dk;
+  a.dv = dv;
+  cross_rows<<<(unsigned)ceil_div(rows, 32), 256, 0, s>>>(
+      static_cast<const __nv_bfloat16*>(o), static_cast<const __nv_bfloat16*>(d_o), lse, nlse, delta,
+      g, a.q_pad);
+  if (magma_status_t st = check_launch("cross_rows")) return st;
+  return g.hd <= 64 ? bwd_tc<64>(q, k, v, d_o, a, s) : bwd_tc<128>(q, k, v, d_o, a, s);
+}
+
+}  // namespace magma
