@@ -84,6 +84,7 @@ size_t magma_cross_attention_fwd_workspace_size(int64_t batch, int64_t heads, in
                                                 magma_dtype_t dtype) {
   if (!has_work(batch, heads, kv_heads, q_len, kv_len, head_dim)) return 0;
   CrossGeom g = sizes(batch, heads, kv_heads, q_len, kv_len, head_dim);
+  if (cross_step_rows(g, dtype)) return cross_step_workspace(g, dtype);
   return dtype == MAGMA_DTYPE_BF16 && head_dim % 8 == 0 ? cross_tc_fwd_workspace(g) : 0;
 }
 
@@ -106,6 +107,9 @@ magma_status_t magma_cross_attention_fwd(const void* q, const void* k, const voi
   if (magma_status_t st = set_strides(fn, "o", o_strides, g.os, true, batch, heads, q_len, head_dim)) return st;
   if (batch == 0 || heads == 0 || q_len == 0) return MAGMA_OK;
   MAGMA_REQUIRE(q && o && (kv_len == 0 || (k && v)), "%s: NULL pointer", fn);
+  if (cross_step_supported(q, k, v, o, g, dtype))
+    return cross_step_run(q, k, v, o, lse, g, dtype, workspace, workspace_bytes,
+                          (cudaStream_t)stream);
   if (cross_tc_fwd_supported(q, k, v, o, g, dtype))
     return cross_fwd_tc_run(q, k, v, o, lse, g, workspace, workspace_bytes, (cudaStream_t)stream);
   return cross_fwd_simt(q, k, v, o, lse, g, dtype, (cudaStream_t)stream);

@@ -40,6 +40,21 @@ magma_status_t cross_bwd_simt(const void* q, const void* k, const void* v, const
                               float* delta, const CrossGeom& g, magma_dtype_t dtype,
                               cudaStream_t s);
 
+// cross_attention_step.cu: few query rows per key head (_rows: as far as sizes
+// say), 16-byte aligned positions.
+bool cross_step_rows(const CrossGeom& g, magma_dtype_t dtype);
+bool cross_step_supported(const void* q, const void* k, const void* v, const void* o,
+                          const CrossGeom& g, magma_dtype_t dtype);
+size_t cross_step_workspace(const CrossGeom& g, magma_dtype_t dtype);
+magma_status_t cross_step_run(const void* q, const void* k, const void* v, void* o, float* lse,
+                              const CrossGeom& g, magma_dtype_t dtype, void* workspace,
+                              size_t workspace_bytes, cudaStream_t s);
+
+// cross_attention_join.cu: parts [n_part][batch][heads][q_len][hd] and their lse.
+magma_status_t cross_join_parts(const float* part, const float* part_lse, void* o, float* lse,
+                                const CrossGeom& g, int n_part, magma_dtype_t dtype,
+                                cudaStream_t s);
+
 // cross_attention_tc.cu: BF16, head sizes that are multiples of 8, 16-byte
 // aligned positions. Workspaces in bytes; the forward pass takes less or none.
 bool cross_tc_fwd_supported(const void* q, const void* k, const void* v, const void* o,

@@ -1,0 +1,573 @@
+// Attention of a few queries over long sources: one query per sequence (a
+// decoding step) or a handful, times the heads that share a key head.
+//
+// The work is one read of K and V (4 flops per byte and query row), so the
+// source is cut into chunks, a CTA takes one chunk of one key head with all
+// query rows that read it (row = shared head * q_len + query), and the parts
+// are joined by their log-sum-exp (cross_join_parts). Tiles of K and V stream
+// through a cp.async ring; keys from the length on are filled with zeros there,
+// so what lies behind a length is never read.
+//
+//   cross_step_bf16  warp-level MMA (m16n8k16): WM x (4 / WM) warps over rows
+//                    and keys, each with its own running maximum and sum. The
+//                    16-row tile holds one query of up to 16 heads; the tcgen05
+//                    tile of 128 rows would be empty, and the products are not
+//                    what bounds this.
+//   cross_step_f32   FMA pipe: scores by key, sums by column.
+#include <cmath>
+
+#include <algorithm>
+
+#include "cross_attention.cuh"
+#include "sm100.cuh"
+
+namespace magma {
+namespace {
+
+using namespace sm100;
+
+constexpr int kThreads = 128;
+constexpr int kKeys = 64;  // keys of a BF16 tile
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+struct StepArgs {
+  CrossGeom g;
+  int rows;             // shared heads * q_len
+  int n_chunk;          // chunks of the longest source
+  int64_t chunk;        // keys of a chunk, a multiple of the tile
+  void* o;
+  float* lse;
+  float* part;          // [chunk][b][h][q][hd], if n_chunk > 1
+  float* part_lse;      // [chunk][b][h][q], natural logarithm
+};
+
+// One CTA's chunk: sequence, key head, keys [k0, k1).
+struct Chunk {
+  int64_t b, kvh, k0, k1;
+  int index;
+};
+__device__ __forceinline__ Chunk chunk_of(const StepArgs& a) {
+  Chunk c;
+  const int64_t i = blockIdx.x;
+  c.index = (int)(i % a.n_chunk);
+  c.kvh = i / a.n_chunk % a.g.kv_heads;
+  c.b = i / a.n_chunk / a.g.kv_heads;
+  const int64_t len = cross_len(a.g, c.b);
+  c.k0 = c.index * a.chunk < len ? c.index * a.chunk : len;
+  c.k1 = len - c.k0 < a.chunk ? len : c.k0 + a.chunk;
+  return c;
+}
+
+// Index of packed row r in a [b][h][q] array, and its head and query.
+__device__ __forceinline__ int64_t row_at(const CrossGeom& g, const Chunk& c, int r, int64_t* h,
+                                          int64_t* q) {
+  *h = c.kvh * g.group + r / (int)g.q_len;
+  *q = r % (int)g.q_len;
+  return (c.b * g.heads + *h) * g.q_len + *q;
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+               "r"(on ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&h);
+}
+
+// Stores a row's result: the output itself, or a chunk's normalised part.
+template <typename T>
+__device__ __forceinline__ void store_part(const StepArgs& a, const Chunk& c, int r, int col,
+                                           const float (&v)[4], float lse) {
+  int64_t h, q;
+  const int64_t at = row_at(a.g, c, r, &h, &q);
+  const int64_t rows = a.g.batch * a.g.heads * a.g.q_len;
+  if (a.n_chunk > 1) {
+    store4(a.part + (c.index * rows + at) * a.g.hd + col, v);
+    if (col == 0) a.part_lse[c.index * rows + at] = lse;
+  } else {
+    store4(static_cast<T*>(a.o) + c.b * a.g.os[0] + h * a.g.os[1] + q * a.g.os[2] + col, v);
+    if (col == 0 && a.lse != nullptr) a.lse[at] = lse;
+  }
+}
+
+// ---------------------------------------------------------------- BF16
+template <int HD>
+struct Bf {
+  static constexpr int kStages = HD == 64 ? 3 : 2;
+  static constexpr int kChunks = HD / 8;            // 16-byte pieces of a row
+  static constexpr int kTile = kKeys * HD * 2;
+  static constexpr int kSmem = kStages * 2 * kTile;
+  static constexpr int kJoin = 4 * 16 * (HD + 4) * 4;  // the warps' sums at the end
+  static_assert(kJoin + 4 * 16 * 8 <= kSmem, "shared memory");
+};
+
+template <int HD, int WM>
+__global__ void __launch_bounds__(kThreads)
+cross_step_bf16(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __restrict__ k,
+                const __nv_bfloat16* __restrict__ v, const __grid_constant__ StepArgs a) {
+  using F = Bf<HD>;
+  constexpr int WN = 4 / WM;         // warps over the keys of a tile
+  constexpr int KW = kKeys / WN;     // keys of a warp
+  constexpr int NT = KW / 8;         // its 8-key tiles
+  constexpr int DT = HD / 8;         // 8-column tiles of the output
+  extern __shared__ __align__(128) uint8_t sm[];
+  const uint32_t base = smem_u32(sm);
+  const CrossGeom& g = a.g;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int wm = warp / WN, wn = warp % WN;
+  const Chunk c = chunk_of(a);
+  const int tiles = (int)((c.k1 - c.k0 + kKeys - 1) / kKeys);
+
+  // tile loads: 16 bytes a thread, a row's pieces side by side
+  const int piece = tid % F::kChunks, row0 = tid / F::kChunks;
+  constexpr int kRowStep = kThreads / F::kChunks;
+  const bool piece_on = piece * 8 < g.hd;
+  const __nv_bfloat16* kh = k + c.b * g.ks[0] + c.kvh * g.ks[1] + (piece_on ? piece * 8 : 0);
+  const __nv_bfloat16* vh = v + c.b * g.vs[0] + c.kvh * g.vs[1] + (piece_on ? piece * 8 : 0);
+  auto load = [&](int j) {
+    const uint32_t dst = base + (j % F::kStages) * 2 * F::kTile;
+    const int64_t kj = c.k0 + (int64_t)j * kKeys;
+#pragma unroll
+    for (int i = 0; i < kKeys / kRowStep; ++i) {
+      const int r = row0 + i * kRowStep;
+      const bool on = piece_on && kj + r < c.k1;
+      const int64_t at = on ? kj + r : c.k0;
+      const uint32_t o = r * HD * 2 + ((piece ^ (r & 7)) << 4);
+      cp_async16(dst + o, kh + at * g.ks[2], on);
+      cp_async16(dst + F::kTile + o, vh + at * g.vs[2], on);
+    }
+  };
+#pragma unroll
+  for (int j = 0; j < F::kStages - 1; ++j) {
+    if (j < tiles) load(j);
+    cp_commit();
+  }
+
+  // Q fragments: rows lane / 4 and + 8 of the warp's 16
+  uint32_t qf[HD / 16][4];
+  {
+    const __nv_bfloat16* qp[2];
+    bool on[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = wm * 16 + (lane >> 2) + 8 * i;
+      on[i] = r < a.rows;
+      int64_t h, qi;
+      row_at(g, c, on[i] ? r : 0, &h, &qi);
+      qp[i] = q + c.b * g.qs[0] + h * g.qs[1] + qi * g.qs[2];
+    }
+#pragma unroll
+    for (int kk = 0; kk < HD / 16; ++kk)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int col = kk * 16 + (lane & 3) * 2 + (e >> 1) * 8;
+        qf[kk][e] = on[e & 1] && col < g.hd
+                        ? *reinterpret_cast<const uint32_t*>(qp[e & 1] + col) : 0u;
+      }
+  }
+  const float sl2 = g.scale * kLog2e;
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  float acc[DT][4];
+#pragma unroll
+  for (int i = 0; i < DT; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[i][e] = 0.f;
+
+  for (int j = 0; j < tiles; ++j) {
+    cp_wait<F::kStages - 2>();
+    __syncthreads();
+    if (j + F::kStages - 1 < tiles) load(j + F::kStages - 1);
+    cp_commit();
+    const uint32_t sk = base + (j % F::kStages) * 2 * F::kTile, sv = sk + F::kTile;
+    const int left = (int)(c.k1 - c.k0 - (int64_t)j * kKeys) - wn * KW;  // keys of this warp
+    if (left <= 0) continue;
+    float s[NT][4];
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[i][e] = 0.f;
+#pragma unroll
+    for (int kk = 0; kk < HD / 16; ++kk)
+#pragma unroll
+      for (int p = 0; p < NT / 2; ++p) {
+        // keys 16 p .. + 15, columns 16 kk .. + 15: lanes 0-7, 8-15 the first eight
+        // keys' two halves, 16-31 the other eight keys'
+        const int r = wn * KW + p * 16 + (lane & 7) + ((lane >> 4) << 3);
+        const int ch = kk * 2 + ((lane >> 3) & 1);
+        uint32_t b[4];
+        ldmatrix4(sk + r * HD * 2 + ((ch ^ (r & 7)) << 4), b);
+        mma16816(s[2 * p], qf[kk], b[0], b[1]);
+        mma16816(s[2 * p + 1], qf[kk], b[2], b[3]);
+      }
+    float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int key = i * 8 + (lane & 3) * 2 + (e & 1);
+        s[i][e] = key < left ? s[i][e] * sl2 : -INFINITY;
+        mx[e >> 1] = fmaxf(mx[e >> 1], s[i][e]);
+      }
+    float alpha[2], ref[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
+      mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
+      const float mn = fmaxf(m[i], mx[i]);
+      ref[i] = mn == -INFINITY ? 0.f : mn;
+      alpha[i] = ex2_approx(m[i] - ref[i]);
+      m[i] = mn;
+      l[i] *= alpha[i];
+    }
+    uint32_t pf[NT / 2][4];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      float p[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        p[e] = ex2_approx(s[i][e] - ref[e >> 1]);
+        l[e >> 1] += p[e];
+      }
+      // P goes into the second product as BF16, as the operands are
+      pf[i >> 1][(i & 1) * 2] = pack_bf16(p[0], p[1]);
+      pf[i >> 1][(i & 1) * 2 + 1] = pack_bf16(p[2], p[3]);
+    }
+#pragma unroll
+    for (int i = 0; i < DT; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[i][e] *= alpha[e >> 1];
+#pragma unroll
+    for (int p = 0; p < NT / 2; ++p)
+#pragma unroll
+      for (int d = 0; d < HD / 16; ++d) {
+        const int r = wn * KW + p * 16 + (lane & 15);
+        const int ch = d * 2 + (lane >> 4);
+        uint32_t b[4];
+        ldmatrix4_t(sv + r * HD * 2 + ((ch ^ (r & 7)) << 4), b);
+        mma16816(acc[2 * d], pf[p], b[0], b[1]);
+        mma16816(acc[2 * d + 1], pf[p], b[2], b[3]);
+      }
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+  }
+  // the warps' sums meet in shared memory: [warp][16][HD + 4], then (m, l)
+  cp_wait<0>();
+  __syncthreads();
+  float* so = reinterpret_cast<float*>(sm);
+  float2* sml = reinterpret_cast<float2*>(sm + F::kJoin);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = (lane >> 2) + 8 * i;
+    float* dst = so + (warp * 16 + r) * (HD + 4) + (lane & 3) * 2;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+      *reinterpret_cast<float2*>(dst + d * 8) = make_float2(acc[d][2 * i], acc[d][2 * i + 1]);
+    if ((lane & 3) == 0) sml[warp * 16 + r] = make_float2(m[i], l[i]);
+  }
+  __syncthreads();
+  constexpr int kVec = HD / 4;
+  for (int i = tid; i < WM * 16 * kVec; i += kThreads) {
+    const int r = i / kVec, col = i % kVec * 4;
+    if (r >= a.rows || col >= g.hd) continue;
+    const int w0 = (r / 16) * WN, rr = r % 16;
+    float mm = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < WN; ++w) mm = fmaxf(mm, sml[(w0 + w) * 16 + rr].x);
+    float total = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < WN; ++w) {
+      const float2 ml = sml[(w0 + w) * 16 + rr];
+      const float f = mm == -INFINITY ? 0.f : ex2_approx(ml.x - mm);
+      total += f * ml.y;
+      float x[4];
+      load4(so + ((w0 + w) * 16 + rr) * (HD + 4) + col, x);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = fmaf(f, x[e], o[e]);
+    }
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] *= inv;
+    store_part<__nv_bfloat16>(a, c, r, col, o, total == 0.f ? -INFINITY : mm * kLn2 + logf(total));
+  }
+}
+
+// ----------------------------------------------------------------- F32
+constexpr int kF32Keys = 32;
+
+template <int HD>
+struct Ff {
+  static constexpr int kStages = 2;
+  static constexpr int kPitch = HD + 4;  // floats: rows a quarter-warp reads lie in other banks
+  static constexpr int kTile = kF32Keys * kPitch * 4;
+  static constexpr int kRing = kStages * 2 * kTile;
+};
+
+// RT rows (shared heads x queries). Scores: warp = row modulo 4, lane = key.
+// Sums: thread = column (and, head size 64, half of the keys).
+template <int HD, int RT>
+__global__ void __launch_bounds__(kThreads)
+cross_step_f32(const float* __restrict__ q, const float* __restrict__ k,
+               const float* __restrict__ v, const __grid_constant__ StepArgs a) {
+  using F = Ff<HD>;
+  constexpr int kHalves = kThreads / HD;  // threads that share a column
+  constexpr int kVec = HD / 4;
+  extern __shared__ __align__(128) uint8_t sm[];
+  const uint32_t base = smem_u32(sm);
+  float* qs = reinterpret_cast<float*>(sm + F::kRing);  // [RT][HD], times scale log2(e)
+  float* ps = qs + RT * HD;                             // [key][RT]
+  float* as = ps + kF32Keys * RT;                       // [RT] this tile's rescaling
+  const CrossGeom& g = a.g;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const Chunk c = chunk_of(a);
+  const int tiles = (int)((c.k1 - c.k0 + kF32Keys - 1) / kF32Keys);
+  const float* kh = k + c.b * g.ks[0] + c.kvh * g.ks[1];
+  const float* vh = v + c.b * g.vs[0] + c.kvh * g.vs[1];
+  auto load = [&](int j) {
+    const uint32_t dst = base + (j % F::kStages) * 2 * F::kTile;
+    const int64_t kj = c.k0 + (int64_t)j * kF32Keys;
+#pragma unroll
+    for (int i = 0; i < kF32Keys * kVec / kThreads; ++i) {
+      const int x = tid + i * kThreads, r = x / kVec, col = x % kVec * 4;
+      const bool on = col < g.hd && kj + r < c.k1;
+      const int64_t at = on ? kj + r : c.k0;
+      const uint32_t o = (r * F::kPitch + col) * 4;
+      cp_async16(dst + o, kh + at * g.ks[2] + (on ? col : 0), on);
+      cp_async16(dst + F::kTile + o, vh + at * g.vs[2] + (on ? col : 0), on);
+    }
+  };
+  if (tiles > 0) load(0);
+  cp_commit();
+  for (int i = tid; i < RT * HD; i += kThreads) {
+    const int r = i / HD, col = i % HD;
+    float x = 0.f;
+    if (r < a.rows && col < g.hd) {
+      int64_t h, qi;
+      row_at(g, c, r, &h, &qi);
+      x = q[c.b * g.qs[0] + h * g.qs[1] + qi * g.qs[2] + col];
+    }
+    qs[i] = x;
+  }
+  constexpr int RW = (RT + 3) / 4;  // rows of a warp
+  float m[RW], l[RW], acc[RT];
+#pragma unroll
+  for (int i = 0; i < RW; ++i) m[i] = -INFINITY, l[i] = 0.f;
+#pragma unroll
+  for (int r = 0; r < RT; ++r) acc[r] = 0.f;
+  const int col = tid % HD, half = tid / HD;
+  for (int j = 0; j < tiles; ++j) {
+    if (j + 1 < tiles) load(j + 1);
+    cp_commit();
+    cp_wait<1>();
+    __syncthreads();
+    const float* sk = reinterpret_cast<const float*>(sm + (j % F::kStages) * 2 * F::kTile);
+    const float* sv = sk + F::kTile / 4;
+    const int left = (int)(c.k1 - c.k0 - (int64_t)j * kF32Keys);
+    float s[RW];
+#pragma unroll
+    for (int i = 0; i < RW; ++i) s[i] = 0.f;
+#pragma unroll 8
+    for (int d = 0; d < HD; d += 4) {
+      const float4 x = *reinterpret_cast<const float4*>(sk + lane * F::kPitch + d);
+#pragma unroll
+      for (int i = 0; i < RW; ++i) {
+        const int r = warp + 4 * i;
+        if (r >= RT) continue;
+        const float4 y = *reinterpret_cast<const float4*>(qs + r * HD + d);
+        s[i] = fmaf(x.x, y.x, s[i]);
+        s[i] = fmaf(x.y, y.y, s[i]);
+        s[i] = fmaf(x.z, y.z, s[i]);
+        s[i] = fmaf(x.w, y.w, s[i]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < RW; ++i) {
+      const int r = warp + 4 * i;
+      if (r >= RT) continue;
+      const float x = lane < left ? s[i] * g.scale : -INFINITY;
+      const float mn = fmaxf(m[i], warp_max(x));
+      const float ref = mn == -INFINITY ? 0.f : mn;
+      const float p = expf(x - ref), alpha = expf(m[i] - ref);
+      m[i] = mn;
+      l[i] = l[i] * alpha + warp_sum(p);
+      ps[lane * RT + r] = p;
+      if (lane == 0) as[r] = alpha;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < RT; ++r) acc[r] *= as[r];
+    constexpr int KH = kF32Keys / kHalves;
+#pragma unroll 8
+    for (int i = 0; i < KH; ++i) {
+      const int key = half * KH + i;
+      const float x = sv[key * F::kPitch + col];
+#pragma unroll
+      for (int r = 0; r < RT; r += 4) {
+        const float4 p = *reinterpret_cast<const float4*>(ps + key * RT + r);
+        acc[r] = fmaf(p.x, x, acc[r]);
+        acc[r + 1] = fmaf(p.y, x, acc[r + 1]);
+        acc[r + 2] = fmaf(p.z, x, acc[r + 2]);
+        acc[r + 3] = fmaf(p.w, x, acc[r + 3]);
+      }
+    }
+    __syncthreads();
+  }
+  cp_wait<0>();
+  __syncthreads();
+  float* so = reinterpret_cast<float*>(sm);  // [half][RT][HD]
+#pragma unroll
+  for (int r = 0; r < RT; ++r) so[(half * RT + r) * HD + col] = acc[r];
+  float2* sml = reinterpret_cast<float2*>(ps);
+#pragma unroll
+  for (int i = 0; i < RW; ++i)
+    if (lane == 0 && warp + 4 * i < RT) sml[warp + 4 * i] = make_float2(m[i], l[i]);
+  __syncthreads();
+  for (int i = tid; i < RT * kVec; i += kThreads) {
+    const int r = i / kVec, d = i % kVec * 4;
+    if (r >= a.rows || d >= g.hd) continue;
+    const float2 ml = sml[r];
+    const float inv = ml.y == 0.f ? 0.f : 1.f / ml.y;
+    float o[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int hh = 0; hh < kHalves; ++hh) {
+      float x[4];
+      load4(so + (hh * RT + r) * HD + d, x);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] += x[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] *= inv;
+    store_part<float>(a, c, r, d, o, ml.y == 0.f ? -INFINITY : ml.x + logf(ml.y));
+  }
+}
+
+// ---------------------------------------------------------------- host side
+bool step_aligned(const void* p, const int64_t (&st)[3], int64_t per16) {
+  return aligned16(p) && st[0] % per16 == 0 && st[1] % per16 == 0 && st[2] % per16 == 0;
+}
+
+int64_t tile_keys(magma_dtype_t dtype) { return dtype == MAGMA_DTYPE_F32 ? kF32Keys : kKeys; }
+
+// Keys of a chunk: about eight CTAs' worth of chunks per SM, so that lengths that
+// differ even out, but no more chunks than that, since each costs a part.
+int64_t chunk_keys(const CrossGeom& g, magma_dtype_t dtype) {
+  const int64_t tile = tile_keys(dtype);
+  const int64_t heads = g.batch * g.kv_heads;
+  const int64_t want = std::max<int64_t>(1, 8LL * num_sms() / heads);
+  return std::max<int64_t>(1, ceil_div(g.kv_len, want * tile)) * tile;
+}
+
+template <int HD, int WM>
+magma_status_t launch_bf16(const void* q, const void* k, const void* v, const StepArgs& a,
+                           unsigned ctas, cudaStream_t s) {
+  const int smem = Bf<HD>::kSmem;
+  if (magma_status_t st = cuda_status(
+          cudaFuncSetAttribute(cross_step_bf16<HD, WM>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               smem), "cross_step shared memory"))
+    return st;
+  cross_step_bf16<HD, WM><<<ctas, kThreads, smem, s>>>(
+      static_cast<const __nv_bfloat16*>(q), static_cast<const __nv_bfloat16*>(k),
+      static_cast<const __nv_bfloat16*>(v), a);
+  return check_launch("cross_step_bf16");
+}
+
+template <int HD, int RT>
+magma_status_t launch_f32(const void* q, const void* k, const void* v, const StepArgs& a,
+                          unsigned ctas, cudaStream_t s) {
+  const int smem = Ff<HD>::kRing + (RT * HD + kF32Keys * RT + RT) * 4;
+  if (magma_status_t st = cuda_status(
+          cudaFuncSetAttribute(cross_step_f32<HD, RT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               smem), "cross_step shared memory"))
+    return st;
+  cross_step_f32<HD, RT><<<ctas, kThreads, smem, s>>>(
+      static_cast<const float*>(q), static_cast<const float*>(k), static_cast<const float*>(v), a);
+  return check_launch("cross_step_f32");
+}
+
+}  // namespace
+
+bool cross_step_supported(const void* q, const void* k, const void* v, const void* o,
+                          const CrossGeom& g, magma_dtype_t dtype) {
+  const int64_t per16 = dtype == MAGMA_DTYPE_F32 ? 4 : 8;
+  return cross_step_rows(g, dtype) && step_aligned(q, g.qs, per16) && step_aligned(k, g.ks, per16) &&
+         step_aligned(v, g.vs, per16) && step_aligned(o, g.os, per16);
+}
+
+bool cross_step_rows(const CrossGeom& g, magma_dtype_t dtype) {
+  const int64_t rows = (int64_t)g.group * g.q_len;
+  const bool f32 = dtype == MAGMA_DTYPE_F32;
+  return rows >= 1 && rows <= (f32 ? 16 : 64) && g.kv_len > 0 && g.hd % (f32 ? 4 : 8) == 0 &&
+         g.batch * g.kv_heads * (8LL * num_sms() + 1) < (1LL << 31);
+}
+
+size_t cross_step_workspace(const CrossGeom& g, magma_dtype_t dtype) {
+  const int64_t n = ceil_div(g.kv_len, chunk_keys(g, dtype));
+  return n <= 1 ? 0 : (size_t)n * g.batch * g.heads * g.q_len * (g.hd + 1) * sizeof(float);
+}
+
+magma_status_t cross_step_run(const void* q, const void* k, const void* v, void* o, float* lse,
+                              const CrossGeom& g, magma_dtype_t dtype, void* workspace,
+                              size_t workspace_bytes, cudaStream_t s) {
+  StepArgs a{};
+  a.g = g;
+  a.rows = (int)(g.group * g.q_len);
+  a.o = o;
+  a.lse = lse;
+  const int64_t tile = tile_keys(dtype);
+  const int64_t rows = g.batch * g.heads * g.q_len;
+  const size_t each = (size_t)rows * (g.hd + 1) * sizeof(float);
+  a.chunk = chunk_keys(g, dtype);
+  const int64_t room = workspace && aligned16(workspace) ? (int64_t)(workspace_bytes / each) : 0;
+  if (ceil_div(g.kv_len, a.chunk) > std::max<int64_t>(1, room))
+    a.chunk = ceil_div(g.kv_len, std::max<int64_t>(1, room) * tile) * tile;
+  a.n_chunk = (int)ceil_div(g.kv_len, a.chunk);
+  if (a.n_chunk > 1) {
+    a.part = static_cast<float*>(workspace);
+    a.part_lse = a.part + (size_t)a.n_chunk * rows * g.hd;
+  }
+  const unsigned ctas = (unsigned)(a.n_chunk * g.kv_heads * g.batch);
+  magma_status_t st;
+  if (dtype == MAGMA_DTYPE_F32) {
+    const bool few = a.rows <= 4;
+    st = g.hd <= 64 ? (few ? launch_f32<64, 4>(q, k, v, a, ctas, s) : launch_f32<64, 16>(q, k, v, a, ctas, s))
+                    : (few ? launch_f32<128, 4>(q, k, v, a, ctas, s) : launch_f32<128, 16>(q, k, v, a, ctas, s));
+  } else {
+    auto* run = g.hd <= 64 ? (a.rows <= 16 ? launch_bf16<64, 1> : a.rows <= 32 ? launch_bf16<64, 2> : launch_bf16<64, 4>)
+                           : (a.rows <= 16 ? launch_bf16<128, 1> : a.rows <= 32 ? launch_bf16<128, 2> : launch_bf16<128, 4>);
+    st = run(q, k, v, a, ctas, s);
+  }
+  if (st || a.n_chunk == 1) return st;
+  return cross_join_parts(a.part, a.part_lse, o, lse, g, a.n_chunk, dtype, s);
+}
+
+}  // namespace magma

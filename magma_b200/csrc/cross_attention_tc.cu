@@ -7,7 +7,6 @@
 //   cross_dkdv_tc   dV += P^T dO, dK += dS^T Q over the query tiles of every
 //                   head that shares the key head
 //   cross_dq_tc     dQ_t += dS_t K_j over the key tiles
-//   cross_join      the parts of a source that the forward pass has split
 //
 // Formulas as in cross_attention_simt.cu. The gradient recomputes S and dP in
 // both of its passes (14 instead of 10 products of the size of S) and needs no
@@ -1192,46 +1191,6 @@ cross_dkdv_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
   }
 }
 
-// =================================================================== join
-// O and lse of a row from its parts: with M the largest lse of the parts,
-// O = sum_s exp(lse_s - M) O_s / sum_s exp(lse_s - M). A part without keys has
-// lse -inf and is not read. One warp a row.
-__global__ void __launch_bounds__(256)
-cross_join(const float* __restrict__ part, const float* __restrict__ part_lse,
-           __nv_bfloat16* __restrict__ o, float* __restrict__ lse, const CrossGeom g, int n_split) {
-  const int lane = threadIdx.x & 31;
-  const int64_t rows = g.batch * g.heads * g.q_len;
-  const int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (i >= rows) return;
-  float m = -INFINITY;
-  for (int s = lane; s < n_split; s += 32) m = fmaxf(m, part_lse[s * rows + i]);
-  m = warp_max(m);
-  float total = 0.f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  const int c = lane * 4;
-  if (m != -INFINITY) {
-    for (int s = 0; s < n_split; ++s) {
-      const float w = expf(part_lse[s * rows + i] - m);
-      if (w == 0.f) continue;
-      total += w;
-      if (c < g.hd) {
-        const float4 v = *reinterpret_cast<const float4*>(part + (s * rows + i) * g.hd + c);
-        acc.x = fmaf(w, v.x, acc.x);
-        acc.y = fmaf(w, v.y, acc.y);
-        acc.z = fmaf(w, v.z, acc.z);
-        acc.w = fmaf(w, v.w, acc.w);
-      }
-    }
-  }
-  const float inv = total == 0.f ? 0.f : 1.f / total;
-  const int64_t q = i % g.q_len, bh = i / g.q_len, h = bh % g.heads, b = bh / g.heads;
-  if (c < g.hd) {
-    const float v[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
-    store4(o + b * g.os[0] + h * g.os[1] + q * g.os[2] + c, v);
-  }
-  if (lane == 0 && lse != nullptr) lse[i] = total == 0.f ? -INFINITY : m + logf(total);
-}
-
 // ------------------------------------------------------------------ host side
 // Map of a [batch, heads, positions, hd] view: boxes of 64 columns and `rows`
 // positions. A batch or head stride of 0 becomes an extent of 1, and *bm or *hm
@@ -1365,9 +1324,7 @@ magma_status_t cross_fwd_tc_run(const void* q, const void* k, const void* v, voi
   if (magma_status_t st = g.hd <= 64 ? fwd_tc<64>(q, k, v, a, s) : fwd_tc<128>(q, k, v, a, s))
     return st;
   if (a.n_split == 1) return MAGMA_OK;
-  cross_join<<<(unsigned)ceil_div(rows, 8), 256, 0, s>>>(
-      a.part, a.part_lse, static_cast<__nv_bfloat16*>(o), lse, g, a.n_split);
-  return check_launch("cross_join");
+  return cross_join_parts(a.part, a.part_lse, o, lse, g, a.n_split, MAGMA_DTYPE_BF16, s);
 }
 
 size_t cross_tc_bwd_workspace(const CrossGeom& g) {
