@@ -32,6 +32,22 @@ __device__ __forceinline__ int64_t cross_len(const CrossGeom& g, int64_t b) {
   return n;
 }
 
+// Lets a kernel use `bytes` of dynamic shared memory, asked once per kernel and
+// device (`Kernel` is a type of its own for each kernel).
+template <auto Kernel>
+magma_status_t cross_smem(int bytes) {
+  static bool done[64] = {};
+  int dev = 0;
+  if (magma_status_t st = cuda_status(cudaGetDevice(&dev), "cudaGetDevice")) return st;
+  if (dev < 64 && done[dev]) return MAGMA_OK;
+  if (magma_status_t st = cuda_status(
+          cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes),
+          "cross attention shared memory"))
+    return st;
+  if (dev < 64) done[dev] = true;
+  return MAGMA_OK;
+}
+
 // cross_attention_simt.cu: any types, strides and head sizes up to 128.
 magma_status_t cross_fwd_simt(const void* q, const void* k, const void* v, void* o, float* lse,
                               const CrossGeom& g, magma_dtype_t dtype, cudaStream_t s);

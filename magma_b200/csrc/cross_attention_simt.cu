@@ -345,12 +345,6 @@ cross_dq(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__
   }
 }
 
-template <typename K>
-magma_status_t prepare(K kernel, size_t smem, const char* what) {
-  return cuda_status(
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), what);
-}
-
 magma_status_t blocks_of(int64_t tiles, int64_t heads, int64_t batch, unsigned* n) {
   const double all = (double)tiles * (double)heads * (double)batch;
   if (all > 2147483647.0)
@@ -364,7 +358,7 @@ magma_status_t fwd(const void* q, const void* k, const void* v, void* o, float* 
                    const CrossGeom& g, cudaStream_t s) {
   const size_t smem = (3 * kT * (HD + 1) + kT * (kT + 1)) * sizeof(float);
   unsigned n;
-  if (magma_status_t st = prepare(cross_fwd<HD, T>, smem, "cross_fwd smem")) return st;
+  if (magma_status_t st = cross_smem<cross_fwd<HD, T>>((int)smem)) return st;
   if (magma_status_t st = blocks_of(ceil_div(g.q_len, kT), g.heads, g.batch, &n)) return st;
   cross_fwd<HD, T><<<n, kThreads, smem, s>>>((const T*)q, (const T*)k, (const T*)v, (T*)o, lse, g);
   return check_launch("cross_fwd");
@@ -377,8 +371,8 @@ magma_status_t bwd(const void* q, const void* k, const void* v, const void* o, c
   const size_t kv_smem =
       (4 * kT * (HD + 1) + 2 * kT * (kT + 1) + 2 * kT) * sizeof(float);
   const size_t q_smem = (4 * kT * (HD + 1) + kT * (kT + 1)) * sizeof(float);
-  if (magma_status_t st = prepare(cross_dkdv<HD, T>, kv_smem, "cross_dkdv smem")) return st;
-  if (magma_status_t st = prepare(cross_dq<HD, T>, q_smem, "cross_dq smem")) return st;
+  if (magma_status_t st = cross_smem<cross_dkdv<HD, T>>((int)kv_smem)) return st;
+  if (magma_status_t st = cross_smem<cross_dq<HD, T>>((int)q_smem)) return st;
   unsigned nq = 0, nk = 0;
   if (magma_status_t st = blocks_of(ceil_div(g.q_len, kT), g.heads, g.batch, &nq)) return st;
   if (magma_status_t st = blocks_of(ceil_div(g.kv_len, kT), g.kv_heads, g.batch, &nk)) return st;

@@ -491,10 +491,7 @@ template <int HD, int WM>
 magma_status_t launch_bf16(const void* q, const void* k, const void* v, const StepArgs& a,
                            unsigned ctas, cudaStream_t s) {
   const int smem = Bf<HD>::kSmem;
-  if (magma_status_t st = cuda_status(
-          cudaFuncSetAttribute(cross_step_bf16<HD, WM>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               smem), "cross_step shared memory"))
-    return st;
+  if (magma_status_t st = cross_smem<cross_step_bf16<HD, WM>>(smem)) return st;
   cross_step_bf16<HD, WM><<<ctas, kThreads, smem, s>>>(
       static_cast<const __nv_bfloat16*>(q), static_cast<const __nv_bfloat16*>(k),
       static_cast<const __nv_bfloat16*>(v), a);
@@ -505,10 +502,7 @@ template <int HD, int RT>
 magma_status_t launch_f32(const void* q, const void* k, const void* v, const StepArgs& a,
                           unsigned ctas, cudaStream_t s) {
   const int smem = Ff<HD>::kRing + (RT * HD + kF32Keys * RT + RT) * 4;
-  if (magma_status_t st = cuda_status(
-          cudaFuncSetAttribute(cross_step_f32<HD, RT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               smem), "cross_step shared memory"))
-    return st;
+  if (magma_status_t st = cross_smem<cross_step_f32<HD, RT>>(smem)) return st;
   cross_step_f32<HD, RT><<<ctas, kThreads, smem, s>>>(
       static_cast<const float*>(q), static_cast<const float*>(k), static_cast<const float*>(v), a);
   return check_launch("cross_step_f32");

@@ -1215,12 +1215,6 @@ bool tc_strides(const void* p, const int64_t (&st)[3], int64_t n) {
          st[2] < (1LL << 38);
 }
 
-template <typename K>
-magma_status_t smem_for(K kernel, int bytes) {
-  return cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes),
-                     "cross attention shared memory");
-}
-
 TcArgs args_of(const CrossGeom& g) {
   TcArgs a{};
   a.g = g;
@@ -1238,7 +1232,7 @@ magma_status_t fwd_tc(const void* q, const void* k, const void* v, TcArgs a, cud
   if (magma_status_t st = view_map(&mq, q, g.hd, g.q_len, g.heads, g.batch, g.qs, kRows, &a.qb, &a.qh)) return st;
   if (magma_status_t st = view_map(&mk, k, g.hd, g.kv_len, g.kv_heads, g.batch, g.ks, kRows, &a.kb, &a.kh)) return st;
   if (magma_status_t st = view_map(&mv, v, g.hd, g.kv_len, g.kv_heads, g.batch, g.vs, kRows, &a.vb, &a.vh)) return st;
-  if (magma_status_t st = smem_for(cross_fwd_tc<HD>, Fwd<HD>::kSmem)) return st;
+  if (magma_status_t st = cross_smem<cross_fwd_tc<HD>>(Fwd<HD>::kSmem)) return st;
   const int64_t units = (int64_t)a.n_pairs * a.n_split * g.kv_heads * g.batch;
   const unsigned ctas = (unsigned)std::min<int64_t>(units, num_sms());
   cross_fwd_tc<HD><<<ctas, kThreads, Fwd<HD>::kSmem, s>>>(mq, mk, mv, a);
@@ -1256,7 +1250,7 @@ magma_status_t bwd_tc(const void* q, const void* k, const void* v, const void* d
     if (magma_status_t st = view_map(&mg, d_o, g.hd, g.q_len, g.heads, g.batch, g.dos, F::kQ, &a.db, &a.dh)) return st;
     if (magma_status_t st = view_map(&mk, k, g.hd, g.kv_len, g.kv_heads, g.batch, g.ks, kRows, &a.kb, &a.kh)) return st;
     if (magma_status_t st = view_map(&mv, v, g.hd, g.kv_len, g.kv_heads, g.batch, g.vs, kRows, &a.vb, &a.vh)) return st;
-    if (magma_status_t st = smem_for(cross_dkdv_tc<HD>, F::kSmem)) return st;
+    if (magma_status_t st = cross_smem<cross_dkdv_tc<HD>>(F::kSmem)) return st;
     const int64_t units = ceil_div(g.kv_len, kRows) * g.kv_heads * g.batch;
     const unsigned ctas = (unsigned)std::min<int64_t>(units, num_sms());
     cross_dkdv_tc<HD><<<ctas, kThreads, F::kSmem, s>>>(mq, mg, mk, mv, a);
@@ -1267,7 +1261,7 @@ magma_status_t bwd_tc(const void* q, const void* k, const void* v, const void* d
   if (magma_status_t st = view_map(&mg, d_o, g.hd, g.q_len, g.heads, g.batch, g.dos, kRows, &a.db, &a.dh)) return st;
   if (magma_status_t st = view_map(&mk, k, g.hd, g.kv_len, g.kv_heads, g.batch, g.ks, F::kKeys, &a.kb, &a.kh)) return st;
   if (magma_status_t st = view_map(&mv, v, g.hd, g.kv_len, g.kv_heads, g.batch, g.vs, F::kKeys, &a.vb, &a.vh)) return st;
-  if (magma_status_t st = smem_for(cross_dq_tc<HD>, F::kSmem)) return st;
+  if (magma_status_t st = cross_smem<cross_dq_tc<HD>>(F::kSmem)) return st;
   const int64_t units = (int64_t)a.n_pairs * g.kv_heads * g.batch;
   const unsigned ctas = (unsigned)std::min<int64_t>(units, num_sms());
   cross_dq_tc<HD><<<ctas, kThreads, F::kSmem, s>>>(mq, mg, mk, mv, a);

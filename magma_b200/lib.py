@@ -110,10 +110,10 @@ SIGNATURES = {
                                    _i64, C.POINTER(_i64), C.POINTER(_i64), _f, _i32, _i32, _vp,
                                    _sz, _vp]),
     "magma_cross_attention_fwd_workspace_size": (_sz, [_i64] * 6 + [_i32]),
-    "magma_cross_attention_fwd": (None, [_vp] * 6 + [_i64] * 6 + [C.POINTER(_i64)] * 4 +
+    "magma_cross_attention_fwd": (None, [_vp] * 6 + [_i64] * 6 + [_vp] * 4 +
                                   [_f, _i32, _vp, _sz, _vp]),
     "magma_cross_attention_bwd_workspace_size": (_sz, [_i64] * 6 + [_i32]),
-    "magma_cross_attention_bwd": (None, [_vp] * 10 + [_i64] * 6 + [C.POINTER(_i64)] * 8 +
+    "magma_cross_attention_bwd": (None, [_vp] * 10 + [_i64] * 6 + [_vp] * 8 +
                                   [_f, _i32, _vp, _sz, _vp]),
     "magma_adam_step": (None, [_vp, _vp, _vp, _vp, _vp, _i64, _f, _f, _f, _f, _f, _i64, _f, _vp]),
     "magma_adam_step_multi": (None, [C.POINTER(_vp), C.POINTER(_vp), C.POINTER(_vp),

@@ -10,6 +10,7 @@ semantics (cited per function).
 from __future__ import annotations
 
 import ctypes as C
+import functools
 
 import torch
 
@@ -58,33 +59,38 @@ def workspace(nbytes: int, device: torch.device | None = None) -> torch.Tensor:
 # Operators of encoder-decoder models run on the current stream of their
 # tensors' device, whichever device is current, and take a workspace of their
 # own from torch's allocator at each call, so that calls on several streams and
-# calls in captured graphs share none.
-def _same_device(*ts: torch.Tensor | None) -> torch.device:
-    _check_cuda(*ts)
-    devs = {t.device for t in ts if t is not None}
-    if len(devs) != 1:
-        raise ValueError(f"tensors on different devices: {sorted(map(str, devs))}")
-    return devs.pop()
+# calls in captured graphs share none. Their smallest calls take a few
+# microseconds on the GPU, so the checks on the way there are kept short.
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_I64x12, _I64x24 = C.c_int64 * 12, C.c_int64 * 24
 
 
-def _call_on(dev: torch.device, name: str, *args) -> None:
-    """lib.call with the device's current stream as the last argument."""
-    if dev.index == torch.cuda.current_device():
-        lib.call(name, *args, _stream())
+def _same_device(first: torch.Tensor, *ts: torch.Tensor | None) -> int:
+    """The CUDA device index that all tensors share."""
+    i = first.get_device()
+    if i < 0:
+        raise ValueError("magma_b200 ops take CUDA tensors")
+    for t in ts:
+        if t is not None and t.get_device() != i:
+            _check_cuda(t)
+            raise ValueError(f"tensors on different devices: cuda:{i} and {t.device}")
+    return i
+
+
+def _call_on(i: int, name: str, *args) -> None:
+    """lib.call on device i with its current stream as the last argument."""
+    if i == torch.cuda.current_device():
+        lib.call(name, *args, _raw_stream(i))
     else:
-        with torch.cuda.device(dev):
-            lib.call(name, *args, _stream())
+        with torch.cuda.device(i):
+            lib.call(name, *args, _raw_stream(i))
 
 
-def _query_on(dev: torch.device, name: str, *args) -> int:
-    if dev.index == torch.cuda.current_device():
-        return lib.query(name, *args)
-    with torch.cuda.device(dev):
-        return lib.query(name, *args)
-
-
-def _scratch(nbytes: int, dev: torch.device) -> torch.Tensor | None:
-    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+@functools.lru_cache(maxsize=256)
+def _bytes_on(i: int, name: str, *sizes) -> int:
+    """A workspace query: it depends on the sizes and the device's SM count."""
+    with torch.cuda.device(i):
+        return lib.query(name, *sizes)
 
 
 def _rows_ld(t: torch.Tensor, what: str) -> int:
@@ -241,27 +247,30 @@ def attention_bwd(q, k, v, o, d_o, lse, scale: float, causal: bool = True,
     return dq, dk, dv
 
 
-def _heads_view(t: torch.Tensor, what: str, shape: tuple | None = None, dtype=None):
-    """(batch, head, position) strides of a [B, H, S, D] view with unit D stride."""
-    if t.dim() != 4 or (t.shape[3] > 1 and t.stride(3) != 1):
-        raise ValueError(f"{what} must be [batch, heads, length, head_dim] with contiguous heads")
-    if shape is not None and tuple(t.shape) != tuple(shape):
+def _heads_view(t: torch.Tensor, what: str, shape, dtype) -> tuple:
+    """Strides of a [B, H, S, D] view with unit D stride."""
+    if t.shape != shape:
         raise ValueError(f"{what} has shape {tuple(t.shape)}, expected {tuple(shape)}")
-    if dtype is not None and t.dtype != dtype:
+    if t.dtype is not dtype:
         raise TypeError(f"{what} has dtype {t.dtype}, expected {dtype}")
-    return (C.c_int64 * 3)(*t.stride()[:3])
+    st = t.stride()
+    if st[3] != 1 and shape[3] > 1:
+        raise ValueError(f"the last dimension of {what} must be contiguous")
+    return st[:3]
 
 
 def _cross_sizes(q, k, v, kv_lens):
-    sq, sk = _heads_view(q, "q"), _heads_view(k, "k", None, q.dtype)
-    sv = _heads_view(v, "v", k.shape, q.dtype)
-    b, h, m, d = q.shape
-    if k.shape[0] != b or k.shape[3] != d:
-        raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} differ in batch or head_dim")
-    if kv_lens is not None and (kv_lens.dtype != torch.int32 or kv_lens.shape != (b,) or
+    qs, ks, dt = q.shape, k.shape, q.dtype
+    if len(qs) != 4 or len(ks) != 4:
+        raise ValueError("q, k and v must be [batch, heads, length, head_dim]")
+    if ks[0] != qs[0] or ks[3] != qs[3]:
+        raise ValueError(f"q {tuple(qs)} and k {tuple(ks)} differ in batch or head_dim")
+    if kv_lens is not None and (kv_lens.dtype is not torch.int32 or kv_lens.shape != qs[:1] or
                                 not kv_lens.is_contiguous()):
         raise ValueError("kv_lens must be a contiguous int32 tensor of one length per sequence")
-    return (b, h, k.shape[1], m, k.shape[2], d), sq, sk, sv
+    strides = (*_heads_view(q, "q", qs, dt), *_heads_view(k, "k", ks, dt),
+               *_heads_view(v, "v", ks, dt))
+    return (qs[0], qs[1], ks[1], qs[2], ks[2], qs[3]), strides
 
 
 def cross_attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
@@ -275,19 +284,22 @@ def cross_attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     that each sequence has; what k and v hold behind them has no influence, and
     a sequence without keys gives zero rows and lse -inf. scale: D ** -0.5 by
     default. One query per sequence (a decoding step) and few queries over long
-    sources split the keys over the GPU. out may not share memory with an input.
+    sources split the keys over the GPU. out (by default like q, with q's strides
+    where they are dense) may not share memory with an input.
     """
-    dev = _same_device(q, k, v, kv_lens, out)
-    sizes, sq, sk, sv = _cross_sizes(q, k, v, kv_lens)
+    i = _same_device(q, k, v, kv_lens, out)
+    sizes, st = _cross_sizes(q, k, v, kv_lens)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    so = _heads_view(out, "out", q.shape, q.dtype)
-    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=dev)
+        out = torch.empty_like(q)
+    at = C.addressof(stb := _I64x12(*st, *_heads_view(out, "out", q.shape, q.dtype)))
+    lse = q.new_empty(q.shape[:3], dtype=torch.float32)
     dt = _dtype(q)
-    ws = _scratch(_query_on(dev, "magma_cross_attention_fwd_workspace_size", *sizes, dt), dev)
-    _call_on(dev, "magma_cross_attention_fwd", _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse),
-             _ptr(kv_lens), *sizes, sq, sk, sv, so, sizes[5] ** -0.5 if scale is None else scale,
-             dt, _ptr(ws), 0 if ws is None else ws.numel())
+    n = _bytes_on(i, "magma_cross_attention_fwd_workspace_size", *sizes, dt)
+    ws = q.new_empty(n, dtype=torch.uint8) if n else None
+    _call_on(i, "magma_cross_attention_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(),
+             out.data_ptr(), lse.data_ptr(), _ptr(kv_lens), *sizes, at, at + 24, at + 48, at + 72,
+             sizes[5] ** -0.5 if scale is None else scale, dt, _ptr(ws), n)
+    del stb
     return out, lse
 
 
@@ -301,21 +313,28 @@ def cross_attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: to
     that share a key head and are zero behind kv_lens. The outputs are written
     whole; given ones may have any strides without overlap, and may not share
     memory with an input."""
-    dev = _same_device(q, k, v, o, d_o, lse, kv_lens, dq, dk, dv)
-    sizes, sq, sk, sv = _cross_sizes(q, k, v, kv_lens)
+    i = _same_device(q, k, v, o, d_o, lse, kv_lens, dq, dk, dv)
+    sizes, st = _cross_sizes(q, k, v, kv_lens)
     if lse.dtype != torch.float32 or lse.shape != q.shape[:3] or not lse.is_contiguous():
         raise ValueError("lse must be the forward pass's contiguous float32 [B, H, Sq]")
-    so, sg = _heads_view(o, "o", q.shape, q.dtype), _heads_view(d_o, "d_o", q.shape, q.dtype)
-    dq, dk, dv = (torch.empty_like(x) if g is None else g
-                  for x, g in ((q, dq), (k, dk), (v, dv)))
-    grads = [_heads_view(g, w, x.shape, q.dtype)
-             for g, w, x in ((dq, "dq", q), (dk, "dk", k), (dv, "dv", v))]
+    if dq is None:
+        dq = torch.empty_like(q)
+    if dk is None:
+        dk = torch.empty_like(k)
+    if dv is None:
+        dv = torch.empty_like(v)
+    qs, ks, t = q.shape, k.shape, q.dtype
+    stb = _I64x24(*st, *_heads_view(o, "o", qs, t), *_heads_view(d_o, "d_o", qs, t),
+                  *_heads_view(dq, "dq", qs, t), *_heads_view(dk, "dk", ks, t),
+                  *_heads_view(dv, "dv", ks, t))
+    at = C.addressof(stb)
     dt = _dtype(q)
-    ws = _scratch(_query_on(dev, "magma_cross_attention_bwd_workspace_size", *sizes, dt), dev)
-    _call_on(dev, "magma_cross_attention_bwd", _ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(d_o),
-             _ptr(lse), _ptr(kv_lens), _ptr(dq), _ptr(dk), _ptr(dv), *sizes, sq, sk, sv, so, sg,
-             *grads, sizes[5] ** -0.5 if scale is None else scale, dt, _ptr(ws),
-             0 if ws is None else ws.numel())
+    n = _bytes_on(i, "magma_cross_attention_bwd_workspace_size", *sizes, dt)
+    ws = q.new_empty(n, dtype=torch.uint8) if n else None
+    _call_on(i, "magma_cross_attention_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(),
+             o.data_ptr(), d_o.data_ptr(), lse.data_ptr(), _ptr(kv_lens), dq.data_ptr(),
+             dk.data_ptr(), dv.data_ptr(), *sizes, *range(at, at + 192, 24),
+             sizes[5] ** -0.5 if scale is None else scale, dt, _ptr(ws), n)
     return dq, dk, dv
 
 
@@ -371,22 +390,30 @@ def adam_step_clipped(params: torch.Tensor, grads: torch.Tensor, m: torch.Tensor
              _ptr(grad_norm), max_norm, _stream())
 
 
-def _tensor_list(ts, what: str):
-    """Pointers, dtypes and sizes of contiguous tensors as C arrays."""
+def _tensor_list(ts, what: str, i: int | None = None):
+    """Device index, pointers, dtypes and sizes of contiguous tensors as C arrays."""
+    n = len(ts)
+    if n == 0:
+        raise ValueError(f"at least one of the {what} is needed")
+    if i is None:
+        i = ts[0].get_device()
     for t in ts:
+        if t.get_device() != i or i < 0:
+            _same_device(ts[0], t)
+            raise ValueError(f"{what} on another device than cuda:{i}")
         if not t.is_contiguous():
             raise ValueError(f"{what} must be contiguous tensors")
-    n = len(ts)
-    return ((C.c_void_p * n)(*[t.data_ptr() for t in ts]),
+    return (i, (C.c_void_p * n)(*[t.data_ptr() for t in ts]),
             (C.c_int32 * n)(*[_dtype(t) for t in ts]),
             (C.c_int64 * n)(*[t.numel() for t in ts]))
 
 
-def _norm_out(norm: torch.Tensor | None, dev: torch.device) -> torch.Tensor:
+def _norm_out(norm: torch.Tensor | None, first: torch.Tensor) -> torch.Tensor:
     if norm is None:
-        return torch.empty(1, dtype=torch.float32, device=dev)
+        return first.new_empty(1, dtype=torch.float32)
     if norm.dtype != torch.float32 or norm.numel() != 1:
         raise ValueError("the norm is one float32 value")
+    _same_device(first, norm)
     return norm
 
 
@@ -396,14 +423,12 @@ def grad_norm_multi(grads, *, grad_scale: float = 1.0,
     tensors (optim.clipGradNorm, Optimizer.swift:1229-1247) as a one-element
     device tensor. The squares are added in 64 bits."""
     grads = list(grads)
-    if not grads:
-        raise ValueError("grad_norm_multi needs at least one tensor")
-    dev = _same_device(*grads, out)
-    ptrs, dtypes, sizes = _tensor_list(grads, "gradients")
-    norm = _norm_out(out, dev)
-    ws = _scratch(_query_on(dev, "magma_grad_norm_multi_workspace_size", len(grads)), dev)
-    _call_on(dev, "magma_grad_norm_multi", ptrs, sizes, dtypes, len(grads), grad_scale,
-             _ptr(norm), _ptr(ws), ws.numel())
+    i, ptrs, dtypes, sizes = _tensor_list(grads, "gradients")
+    norm = _norm_out(out, grads[0])
+    n = _bytes_on(i, "magma_grad_norm_multi_workspace_size", len(grads))
+    ws = norm.new_empty(n, dtype=torch.uint8)
+    _call_on(i, "magma_grad_norm_multi", ptrs, sizes, dtypes, len(grads), grad_scale,
+             norm.data_ptr(), ws.data_ptr(), n)
     return norm
 
 
@@ -417,22 +442,21 @@ def clip_grad_norm(grads, max_norm: float, *, grad_scale: float = 1.0, out=None,
     copied to the host; a NaN norm leaves the gradients unclipped, as the
     reference's mask does."""
     grads = list(grads)
-    if not grads:
-        raise ValueError("clip_grad_norm needs at least one tensor")
     outs = grads if out is None else list(out)
     if len(outs) != len(grads):
         raise ValueError(f"{len(outs)} outputs for {len(grads)} gradients")
-    dev = _same_device(*grads, *(() if out is None else outs), norm)
-    ptrs, dtypes, sizes = _tensor_list(grads, "gradients")
+    i, ptrs, dtypes, sizes = _tensor_list(grads, "gradients")
     optrs, odtypes = ptrs, dtypes
     if out is not None:
-        if any(o.shape != g.shape for o, g in zip(outs, grads)):
-            raise ValueError("an output differs in shape from its gradient")
-        optrs, odtypes, _ = _tensor_list(outs, "outputs")
-    norm = _norm_out(norm, dev)
-    ws = _scratch(_query_on(dev, "magma_grad_norm_multi_workspace_size", len(grads)), dev)
-    _call_on(dev, "magma_clip_grad_norm_multi", ptrs, optrs, sizes, dtypes, odtypes, len(grads),
-             grad_scale, max_norm, _ptr(norm), _ptr(ws), ws.numel())
+        for o, g in zip(outs, grads):
+            if o.shape != g.shape:
+                raise ValueError("an output differs in shape from its gradient")
+        _, optrs, odtypes, _ = _tensor_list(outs, "outputs", i)
+    norm = _norm_out(norm, grads[0])
+    n = _bytes_on(i, "magma_grad_norm_multi_workspace_size", len(grads))
+    ws = norm.new_empty(n, dtype=torch.uint8)
+    _call_on(i, "magma_clip_grad_norm_multi", ptrs, optrs, sizes, dtypes, odtypes, len(grads),
+             grad_scale, max_norm, norm.data_ptr(), ws.data_ptr(), n)
     return norm
 
 
@@ -507,7 +531,7 @@ def embedding_scaled_fwd(tokens: torch.Tensor, table: torch.Tensor,
     position row: out[b*S+s] = scale * table[tokens[b, s]] + pos[s], as a
     [B*S, D] tensor (the table's dtype by default). table [V, D] with contiguous
     rows, pos [>= S, D] of the same dtype; float32 or bfloat16."""
-    dev = _same_device(tokens, table, pos, out)
+    i = _same_device(tokens, table, pos, out)
     b, n = _tokens(tokens)
     ld = _rows_ld(table, "table")
     v, d = table.shape
@@ -515,11 +539,11 @@ def embedding_scaled_fwd(tokens: torch.Tensor, table: torch.Tensor,
                             pos.shape[1] != d or not pos.is_contiguous()):
         raise ValueError(f"pos must be a contiguous {table.dtype} tensor of at least [{n}, {d}]")
     if out is None:
-        out = torch.empty((b * n, d), dtype=out_dtype or table.dtype, device=dev)
+        out = table.new_empty((b * n, d), dtype=out_dtype)
     elif out.shape != (b * n, d) or not out.is_contiguous():
         raise ValueError(f"out must be a contiguous [{b * n}, {d}] tensor")
-    _call_on(dev, "magma_embedding_scaled_fwd", _ptr(tokens), _ptr(table), ld, _ptr(pos),
-             _ptr(out), b, n, d, v, scale, _dtype(table), _dtype(out))
+    _call_on(i, "magma_embedding_scaled_fwd", tokens.data_ptr(), table.data_ptr(), ld, _ptr(pos),
+             out.data_ptr(), b, n, d, v, scale, _dtype(table), _dtype(out))
     return out
 
 
@@ -538,18 +562,18 @@ def embedding_scaled_bwd(tokens: torch.Tensor, dout: torch.Tensor, vocab: int, *
     they are) is written, or added to with accumulate_pos."""
     if (accumulate and dtable is None) or (accumulate_pos and dpos is None):
         raise ValueError("accumulating needs the tensor that is added to")
-    dev = _same_device(tokens, dout, dtable, dpos)
+    i = _same_device(tokens, dout, dtable, dpos)
     b, n = _tokens(tokens)
     ld = _rows_ld(dout, "dout")
     d = dout.shape[1]
     if dout.shape[0] != b * n:
         raise ValueError(f"dout has {dout.shape[0]} rows for {b * n} tokens")
     if dtable is None:
-        dtable = torch.empty((vocab, d), dtype=dtype, device=dev)
+        dtable = dout.new_empty((vocab, d), dtype=dtype)
     elif dtable.shape != (vocab, d):
         raise ValueError(f"dtable must be [{vocab}, {d}]")
     if dpos is None and pos:
-        dpos = torch.empty((n, d), dtype=torch.float32, device=dev)
+        dpos = dout.new_empty((n, d), dtype=torch.float32)
     elif dpos is not None and (dpos.dtype != torch.float32 or dpos.dim() != 2 or
                                dpos.shape[0] < n or dpos.shape[1] != d or
                                not dpos.is_contiguous()):
@@ -557,11 +581,11 @@ def embedding_scaled_bwd(tokens: torch.Tensor, dout: torch.Tensor, vocab: int, *
     pad = -1 if padding_idx is None else padding_idx
     if padding_idx is not None and not 0 <= padding_idx < vocab:
         raise ValueError(f"padding_idx {padding_idx} outside [0, {vocab})")
-    ws = _scratch(_query_on(dev, "magma_embedding_scaled_bwd_workspace_size", b, n, d), dev)
-    _call_on(dev, "magma_embedding_scaled_bwd", _ptr(tokens), _ptr(dout), ld, _ptr(dtable),
-             _rows_ld(dtable, "dtable"), _ptr(dpos), b, n, d, vocab, scale, pad, int(accumulate),
-             int(accumulate_pos), _dtype(dout), _dtype(dtable), _ptr(ws),
-             0 if ws is None else ws.numel())
+    nws = _bytes_on(i, "magma_embedding_scaled_bwd_workspace_size", b, n, d)
+    ws = dout.new_empty(nws, dtype=torch.uint8) if nws else None
+    _call_on(i, "magma_embedding_scaled_bwd", tokens.data_ptr(), dout.data_ptr(), ld,
+             dtable.data_ptr(), _rows_ld(dtable, "dtable"), _ptr(dpos), b, n, d, vocab, scale, pad,
+             int(accumulate), int(accumulate_pos), _dtype(dout), _dtype(dtable), _ptr(ws), nws)
     return dtable, dpos
 
 
