@@ -279,6 +279,30 @@ template <> __device__ __forceinline__ float gelu_grad_t<__nv_bfloat16>(float x)
 
 }  // namespace magma
 
+namespace magma {
+// A kernel that may start while the launch before it on the stream is ending:
+// its blocks are brought up meanwhile and wait_for_launch_before() holds them
+// until that launch is done and its writes are visible.
+__device__ __forceinline__ void wait_for_launch_before() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+template <typename... P, typename... A>
+magma_status_t launch_after(void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem,
+                            cudaStream_t stream, const char* what, A&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cuda_status(cudaLaunchKernelEx(&cfg, kernel, static_cast<A&&>(args)...), what);
+}
+}  // namespace magma
+
 // Argument-check helper used at the top of every entry point.
 #define MAGMA_REQUIRE(cond, ...)                                   \
   do {                                                             \

@@ -16,6 +16,7 @@ template <typename T>
 __global__ void __launch_bounds__(256)
 cross_join(const float* __restrict__ part, const float* __restrict__ part_lse, T* __restrict__ o,
            float* __restrict__ lse, const CrossGeom g, int n_part) {
+  wait_for_launch_before();
   const int lane = threadIdx.x & 31;
   const int64_t rows = g.batch * g.heads * g.q_len;
   const int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
@@ -55,11 +56,10 @@ magma_status_t cross_join_parts(const float* part, const float* part_lse, void* 
                                 cudaStream_t s) {
   const unsigned blocks = (unsigned)ceil_div(g.batch * g.heads * g.q_len, 8);
   if (dtype == MAGMA_DTYPE_F32)
-    cross_join<float><<<blocks, 256, 0, s>>>(part, part_lse, static_cast<float*>(o), lse, g, n_part);
-  else
-    cross_join<__nv_bfloat16><<<blocks, 256, 0, s>>>(part, part_lse, static_cast<__nv_bfloat16*>(o),
-                                                     lse, g, n_part);
-  return check_launch("cross_join");
+    return launch_after(cross_join<float>, dim3(blocks), 256, 0, s, "cross_join", part, part_lse,
+                        static_cast<float*>(o), lse, g, n_part);
+  return launch_after(cross_join<__nv_bfloat16>, dim3(blocks), 256, 0, s, "cross_join", part, part_lse,
+                      static_cast<__nv_bfloat16*>(o), lse, g, n_part);
 }
 
 }  // namespace magma

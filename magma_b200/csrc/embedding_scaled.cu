@@ -13,13 +13,15 @@
 //  1. emb_sort     one cluster of up to 8 CTAs sorts the rows by (token, row)
 //                  with a stable radix sort, 8 bits a pass; rows whose token
 //                  is padding or outside the table get the key `vocab` and
-//                  end up last.
+//                  end up last. The other clusters meanwhile set the table's
+//                  gradient to zero and write dpos: neither needs the order,
+//                  and the sort alone would leave 140 SMs idle. (The rows of
+//                  tokens that occur are written twice.)
 //  2. emb_sum      a CTA adds the dout rows of P consecutive places of the
 //                  sorted order, so that every CTA has the same work however
 //                  often a token repeats. A run of equal tokens inside the P
 //                  places is stored at once; the part of a run that crosses a
-//                  border goes to the workspace. Further CTAs write the zero
-//                  rows of tokens that do not occur, and dpos.
+//                  border goes to the workspace.
 //  3. emb_join     adds the parts of each crossing run in order.
 // The order of the additions depends on the tokens alone (no atomics on
 // floating values), so the result is the same on every run.
@@ -28,6 +30,7 @@
 #include <algorithm>
 
 #include "common.cuh"
+#include "sm100.cuh"
 
 namespace magma {
 namespace {
@@ -82,27 +85,78 @@ emb_lookup(const int32_t* __restrict__ tokens, const TI* __restrict__ table, int
   }
 }
 
-// ---- sort ----------------------------------------------------------------------
+// ---- 16-byte accesses -----------------------------------------------------------
+// V elements of T as they lie in memory, kept packed until they are added.
+template <typename T, int V>
+struct Raw {
+  static constexpr int kWords = (V * (int)sizeof(T) + 3) / 4;
+  uint32_t w[kWords];
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (kWords == 4) {
+      const uint4 u = *reinterpret_cast<const uint4*>(p);
+      w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
+    } else if constexpr (sizeof(T) == 4) {
+      w[0] = *reinterpret_cast<const uint32_t*>(p);
+    } else {
+      w[0] = *reinterpret_cast<const uint16_t*>(p);
+    }
+  }
+  __device__ __forceinline__ void add_to(float (&acc)[V]) const {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) acc[e] += __uint_as_float(w[e]);
+    } else if constexpr (V == 1) {
+      acc[0] += __uint_as_float(w[0] << 16);
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; e += 2) {
+        acc[e] += __uint_as_float(w[e / 2] << 16);
+        acc[e + 1] += __uint_as_float(w[e / 2] & 0xFFFF0000u);
+      }
+    }
+  }
+};
+template <typename T, int V>
+__device__ __forceinline__ void load_v(const T* p, float (&v)[V]) {
+  if constexpr (V == 8) load8(p, v);
+  else if constexpr (V == 4) load4(p, v);
+  else v[0] = to_f32(p[0]);
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_v(T* p, const float (&v)[V]) {
+  if constexpr (V == 8) store8(p, v);
+  else if constexpr (V == 4) store4(p, v);
+  else p[0] = from_f32<T>(v[0]);
+}
+
+struct GradArgs {
+  const int32_t* tokens;
+  uint32_t* key[2];  // ping-pong buffers of the sort
+  uint32_t* row[2];
+  const void* dout;
+  int64_t dout_ld;
+  void* dtable;
+  int64_t dtable_ld;
+  float* head;  // [tile][dim]: the tile's part of a run that began before it
+  float* tail;  // [tile][dim]: the tile's part of a run that began in it and goes on
+  float* dpos;
+  int64_t rows, vocab, batch, seq, padding, tiles;
+  int dim, places, passes, accumulate, accumulate_dpos;
+  float scale;
+  int* err;
+};
+
+// ---- sort, zero rows, dpos ---------------------------------------------------------
 constexpr int kSortThreads = 1024;
 constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kMaxCluster = 8;
 constexpr int kDigits = 256;
+constexpr int kCountBytes = kSortWarps * kDigits * 4;
 // A CTA of the cluster takes at least this many rows: below it the exchange of
 // the counts costs more than the rows.
 constexpr int kSortRows = 2048;
 
-struct SortArgs {
-  const int32_t* tokens;
-  uint32_t* key[2];  // ping-pong buffers
-  uint32_t* row[2];
-  int64_t rows;
-  int64_t vocab;
-  int64_t padding;
-  int passes;
-  int* err;
-};
-
-__device__ __forceinline__ uint32_t sort_key(const SortArgs& a, int64_t i, bool report) {
+__device__ __forceinline__ uint32_t sort_key(const GradArgs& a, int64_t i, bool report) {
   const int32_t t = a.tokens[i];
   if (t < 0 || t >= a.vocab) {
     if (report) set_device_error(a.err, kDevErrBadIndex);
@@ -114,11 +168,9 @@ __device__ __forceinline__ uint32_t sort_key(const SortArgs& a, int64_t i, bool 
 // Every warp owns a contiguous piece of the rows. A pass counts the digits of
 // each piece, turns the counts into the first place of (digit, CTA, warp) in
 // that order, and moves the rows; within 32 rows the place follows the lane,
-// so equal digits keep their order.
-__global__ void __launch_bounds__(kSortThreads, 1) emb_sort(const SortArgs a) {
-  extern __shared__ uint32_t counts[];                  // [warp][digit]
-  __shared__ uint32_t cta_count[kDigits], scan[kDigits];
-  cg::cluster_group cluster = cg::this_cluster();
+// so equal digits keep their order. All CTAs of the first cluster are here.
+__device__ void sort_rows(const GradArgs& a, cg::cluster_group cluster, uint32_t* counts,
+                          uint32_t* cta_count, uint32_t* scan) {
   const int nc = (int)cluster.num_blocks(), c = (int)cluster.block_rank();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t pieces = (int64_t)nc * kSortWarps;
@@ -130,12 +182,13 @@ __global__ void __launch_bounds__(kSortThreads, 1) emb_sort(const SortArgs a) {
   uint32_t* mine = counts + warp * kDigits;
   for (int p = 0; p < a.passes; ++p) {
     const int shift = 8 * p;
-    const uint32_t* kin = a.key[(p + 1) & 1];
-    const uint32_t* rin = a.row[(p + 1) & 1];
-    uint32_t* kout = a.key[p & 1];
-    uint32_t* rout = a.row[p & 1];
+    const uint32_t* kin = p & 1 ? a.key[0] : a.key[1];
+    const uint32_t* rin = p & 1 ? a.row[0] : a.row[1];
+    uint32_t* kout = p & 1 ? a.key[1] : a.key[0];
+    uint32_t* rout = p & 1 ? a.row[1] : a.row[0];
     for (int d = lane; d < kDigits; d += 32) mine[d] = 0;
     __syncwarp();
+#pragma unroll 4
     for (int64_t i = i0 + lane; i < i1; i += 32) {
       const uint32_t k = p == 0 ? sort_key(a, i, true) : kin[i];
       atomicAdd(&mine[(k >> shift) & (kDigits - 1)], 1u);
@@ -144,7 +197,7 @@ __global__ void __launch_bounds__(kSortThreads, 1) emb_sort(const SortArgs a) {
     // counts[w][d] -> rows of digit d in earlier warps of this CTA
     if (threadIdx.x < kDigits) {
       uint32_t run = 0;
-#pragma unroll 8
+#pragma unroll
       for (int w = 0; w < kSortWarps; ++w) {
         const uint32_t n = counts[w * kDigits + threadIdx.x];
         counts[w * kDigits + threadIdx.x] = run;
@@ -155,8 +208,9 @@ __global__ void __launch_bounds__(kSortThreads, 1) emb_sort(const SortArgs a) {
     cluster.sync();
     uint32_t before = 0, all = 0;  // rows of this digit in earlier CTAs, in all
     if (threadIdx.x < kDigits) {
-      for (int o = 0; o < nc; ++o) {
-        const uint32_t n = cluster.map_shared_rank(cta_count, o)[threadIdx.x];
+#pragma unroll
+      for (int o = 0; o < kMaxCluster; ++o) {
+        const uint32_t n = o < nc ? cluster.map_shared_rank(cta_count, o)[threadIdx.x] : 0u;
         if (o < c) before += n;
         all += n;
       }
@@ -186,7 +240,7 @@ __global__ void __launch_bounds__(kSortThreads, 1) emb_sort(const SortArgs a) {
     __syncthreads();
     if (threadIdx.x < kDigits) {
       const uint32_t base = scan[threadIdx.x] + before;
-#pragma unroll 8
+#pragma unroll
       for (int w = 0; w < kSortWarps; ++w) counts[w * kDigits + threadIdx.x] += base;
     }
     __syncthreads();
@@ -207,10 +261,102 @@ __global__ void __launch_bounds__(kSortThreads, 1) emb_sort(const SortArgs a) {
       }
       __syncwarp();
     }
-    // the next pass reads what other CTAs of the cluster wrote, and the counts
-    // of this one are read by them until here
-    __threadfence();
+    // The next pass reads what the other CTAs wrote, and this CTA's counts are
+    // read by them until here.
+    if (p + 1 < a.passes) __threadfence();
     cluster.sync();
+  }
+}
+
+// dpos: a thread has V columns of one position and every G-th stretch of the
+// batch; the G sums of a column meet in shared memory and are added in order.
+template <typename TD, int V>
+__device__ void sum_positions(const GradArgs& a, int64_t cta, int64_t ctas, float* sums) {
+  const int64_t nv = a.dim / V, items = a.seq * nv;
+  // as many stretches as fill the CTAs, of at least eight rows
+  int G = 1;
+  while (G < 8 && items * G * 2 <= ctas * kSortThreads && a.batch >= G * 16) G *= 2;
+  const int per = kSortThreads / G, g = threadIdx.x / per, x = threadIdx.x % per;
+  const int64_t b0 = a.batch * g / G, b1 = a.batch * (g + 1) / G;
+  const int64_t step = a.seq * a.dout_ld;
+  for (int64_t i0 = cta * per; i0 < items; i0 += ctas * per) {
+    const int64_t i = i0 + x, s = i / nv;
+    const int col = (int)(i % nv) * V;
+    float acc[V] = {};
+    if (i < items) {
+      const TD* src = static_cast<const TD*>(a.dout) + s * a.dout_ld + col;
+      for (int64_t b = b0; b < b1; b += 8) {
+        Raw<TD, V> v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+          if (b + u < b1) v[u].load(src + (b + u) * step);
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+          if (b + u < b1) v[u].add_to(acc);
+      }
+    }
+    if (G > 1) {
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < V; ++e) sums[e * kSortThreads + threadIdx.x] = acc[e];
+      __syncthreads();
+      if (g != 0) continue;
+      for (int o = 1; o < G; ++o)
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc[e] += sums[e * kSortThreads + o * per + x];
+    }
+    if (i >= items) continue;
+    float* dst = a.dpos + s * a.dim + col;
+    if (a.accumulate_dpos) {
+      float old[V];
+      load_v<float, V>(dst, old);
+#pragma unroll
+      for (int e = 0; e < V; ++e) acc[e] += old[e];
+    }
+    store_v<float, V>(dst, acc);
+  }
+}
+
+template <typename TD, typename TT, int V>
+__global__ void __launch_bounds__(kSortThreads, 1) emb_sort(const __grid_constant__ GradArgs a) {
+  extern __shared__ __align__(128) uint32_t counts[];  // [warp][digit]
+  __shared__ uint32_t cta_count[kDigits], scan[kDigits];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int nc = (int)cluster.num_blocks();
+  if ((int)blockIdx.x < nc) {
+    if (a.rows > 0) sort_rows(a, cluster, counts, cta_count, scan);
+    if ((int)gridDim.x > nc) return;  // the other clusters do the rest
+  }
+  const int64_t first = (int)gridDim.x > nc ? nc : 0;
+  const int64_t cta = (int64_t)blockIdx.x - first, ctas = (int64_t)gridDim.x - first;
+  __syncthreads();
+  if (a.dpos != nullptr) sum_positions<TD, V>(a, cta, ctas, reinterpret_cast<float*>(counts));
+  if (a.accumulate) return;
+  TT* table = static_cast<TT*>(a.dtable);
+  if constexpr (V > 1) {
+    // Rows of whole 16-byte pieces: bulk copies of a zeroed stretch of shared
+    // memory, 32 lanes issuing a row each.
+    __syncthreads();
+    uint4* z = reinterpret_cast<uint4*>(counts);
+    for (int i = threadIdx.x; i < kCountBytes / 16; i += kSortThreads) z[i] = make_uint4(0, 0, 0, 0);
+    sm100::fence_proxy_async_smem();
+    __syncthreads();
+    if (threadIdx.x >= 32) return;
+    const uint32_t src = sm100::smem_u32(counts);
+    const int64_t bytes = (int64_t)a.dim * sizeof(TT);
+    for (int64_t v = cta * 32 + threadIdx.x; v < a.vocab; v += ctas * 32) {
+      uint8_t* dst = reinterpret_cast<uint8_t*>(table + v * a.dtable_ld);
+      for (int64_t at = 0; at < bytes; at += kCountBytes)
+        sm100::bulk_store(dst + at, src,
+                          (uint32_t)(bytes - at < kCountBytes ? bytes - at : kCountBytes));
+    }
+    sm100::bulk_commit_group();
+    sm100::bulk_wait_group_all();
+  } else {
+    const int lane = threadIdx.x & 31;
+    const int64_t w0 = (cta * kSortThreads + threadIdx.x) >> 5, warps = ctas * kSortWarps;
+    for (int64_t v = w0; v < a.vocab; v += warps)
+      for (int c = lane; c < a.dim; c += 32) table[v * a.dtable_ld + c] = from_f32<TT>(0.f);
   }
 }
 
@@ -218,37 +364,8 @@ __global__ void __launch_bounds__(kSortThreads, 1) emb_sort(const SortArgs a) {
 constexpr int kSumThreads = 128;
 constexpr int kMaxPlaces = 128;
 
-struct SumArgs {
-  const uint32_t* key;
-  const uint32_t* row;
-  const void* dout;
-  int64_t dout_ld;
-  void* dtable;
-  int64_t dtable_ld;
-  float* head;  // [tile][dim]: the tile's part of a run that began before it
-  float* tail;  // [tile][dim]: the tile's part of a run that began in it and goes on
-  float* dpos;
-  int64_t rows, vocab, batch, seq;
-  int64_t tiles, zero_blocks, pos_blocks;
-  int dim, places, accumulate, accumulate_dpos;
-  float scale;
-};
-
 template <typename T, int V>
-__device__ __forceinline__ void load_v(const T* p, float (&v)[V]) {
-  if constexpr (V == 8) load8(p, v);
-  else if constexpr (V == 4) load4(p, v);
-  else v[0] = to_f32(p[0]);
-}
-template <typename T, int V>
-__device__ __forceinline__ void store_v(T* p, const float (&v)[V]) {
-  if constexpr (V == 8) store8(p, v);
-  else if constexpr (V == 4) store4(p, v);
-  else p[0] = from_f32<T>(v[0]);
-}
-
-template <typename T, int V>
-__device__ __forceinline__ void store_grad(const SumArgs& a, uint32_t token, int col,
+__device__ __forceinline__ void store_grad(const GradArgs& a, uint32_t token, int col,
                                            const float (&acc)[V]) {
   T* dst = static_cast<T*>(a.dtable) + (int64_t)token * a.dtable_ld + col;
   float v[V];
@@ -261,77 +378,27 @@ __device__ __forceinline__ void store_grad(const SumArgs& a, uint32_t token, int
   store_v<T, V>(dst, v);
 }
 
-// First place whose key is at least x.
-__device__ __forceinline__ int64_t lower_bound(const uint32_t* key, int64_t n, uint32_t x) {
-  int64_t lo = 0, hi = n;
-  while (lo < hi) {
-    const int64_t mid = (lo + hi) >> 1;
-    if (key[mid] < x) lo = mid + 1;
-    else hi = mid;
-  }
-  return lo;
+__device__ __forceinline__ const uint32_t* sorted_key(const GradArgs& a) {
+  return a.passes & 1 ? a.key[0] : a.key[1];
 }
-
-constexpr int kZeroRows = 8;  // vocabulary rows of a warp that writes zero rows
-
-template <typename T, int V>
-__device__ __forceinline__ void zero_rows(const SumArgs& a, int64_t block) {
-  const int lane = threadIdx.x & 31;
-  const int64_t v0 = (block * (kSumThreads / 32) + (threadIdx.x >> 5)) * kZeroRows;
-  bool absent = false;
-  if (lane < kZeroRows && v0 + lane < a.vocab) {
-    const uint32_t v = (uint32_t)(v0 + lane);
-    const int64_t p = lower_bound(a.key, a.rows, v);
-    absent = p == a.rows || a.key[p] != v;
-  }
-  const uint32_t mask = __ballot_sync(0xffffffffu, absent);
-  const float zero[V] = {};
-  for (int j = 0; j < kZeroRows; ++j) {
-    if (!(mask >> j & 1u)) continue;
-    T* dst = static_cast<T*>(a.dtable) + (v0 + j) * a.dtable_ld;
-    for (int c = lane * V; c < a.dim; c += 32 * V) store_v<T, V>(dst + c, zero);
-  }
-}
-
-template <typename TD, int V>
-__device__ __forceinline__ void sum_positions(const SumArgs& a, int64_t block) {
-  const int64_t nv = a.dim / V;
-  const int64_t i = block * kSumThreads + threadIdx.x;
-  if (i >= a.seq * nv) return;
-  const int64_t s = i / nv;
-  const int col = (int)(i % nv) * V;
-  float acc[V] = {};
-  const TD* src = static_cast<const TD*>(a.dout) + s * a.dout_ld + col;
-  float* dst = a.dpos + s * a.dim + col;
-#pragma unroll 4
-  for (int64_t b = 0; b < a.batch; ++b) {
-    float v[V];
-    load_v<TD, V>(src + b * a.seq * a.dout_ld, v);
-#pragma unroll
-    for (int e = 0; e < V; ++e) acc[e] += v[e];
-  }
-#pragma unroll
-  for (int e = 0; e < V; ++e) dst[e] = a.accumulate_dpos ? dst[e] + acc[e] : acc[e];
+__device__ __forceinline__ const uint32_t* sorted_row(const GradArgs& a) {
+  return a.passes & 1 ? a.row[0] : a.row[1];
 }
 
 // TD: dout, TT: dtable. The dout rows of eight places are in flight at a time.
 template <typename TD, typename TT, int V>
-__global__ void __launch_bounds__(kSumThreads) emb_sum(const SumArgs a) {
-  if ((int64_t)blockIdx.x >= a.tiles) {
-    const int64_t b = (int64_t)blockIdx.x - a.tiles;
-    if (blockIdx.y != 0) return;
-    if (b < a.zero_blocks) zero_rows<TT, V>(a, b);
-    else sum_positions<TD, V>(a, b - a.zero_blocks);
-    return;
-  }
+__global__ void __launch_bounds__(kSumThreads) emb_sum(const __grid_constant__ GradArgs a) {
   __shared__ uint32_t key[kMaxPlaces + 2], row[kMaxPlaces];
+  wait_for_launch_before();
   const int64_t tile = blockIdx.x, p0 = tile * a.places;
   const int n = (int)(a.rows - p0 < a.places ? a.rows - p0 : a.places);
+  const uint32_t* skey = sorted_key(a);
+  const uint32_t* srow = sorted_row(a);
   // key[0]: the place before the tile, key[n + 1]: the place behind it
   for (int i = threadIdx.x; i < n + 2; i += kSumThreads) {
     const int64_t p = p0 + i - 1;
-    key[i] = p >= 0 && p < a.rows ? a.key[p] : 0xFFFFFFFFu;
-    if (i >= 1 && i <= n) row[i - 1] = a.row[p];
+    key[i] = p >= 0 && p < a.rows ? skey[p] : 0xFFFFFFFFu;
+    if (i >= 1 && i <= n) row[i - 1] = srow[p];
   }
   __syncthreads();
   const int col = (blockIdx.y * kSumThreads + threadIdx.x) * V;
@@ -341,19 +408,18 @@ __global__ void __launch_bounds__(kSumThreads) emb_sum(const SumArgs a) {
   bool began = key[0] != key[1];  // the current run begins in this tile
   constexpr int kAhead = 8;
   for (int i0 = 0; i0 < n; i0 += kAhead) {
-    float v[kAhead][V];
+    Raw<TD, V> v[kAhead];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u)
       if (i0 + u < n && key[i0 + u + 1] < (uint32_t)a.vocab)
-        load_v<TD, V>(src + (int64_t)row[i0 + u] * a.dout_ld, v[u]);
+        v[u].load(src + (int64_t)row[i0 + u] * a.dout_ld);
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       const int i = i0 + u;
       if (i >= n) break;
       const uint32_t t = key[i + 1];
       if (t >= (uint32_t)a.vocab) return;  // padding and bad tokens are last
-#pragma unroll
-      for (int e = 0; e < V; ++e) acc[e] += v[u][e];
+      v[u].add_to(acc);
       const bool ends = key[i + 2] != t;
       if (!ends && i + 1 < n) continue;
       if (began && ends) {
@@ -369,28 +435,60 @@ __global__ void __launch_bounds__(kSumThreads) emb_sum(const SumArgs a) {
   }
 }
 
-// One CTA per tile: if a run begins in the tile and goes on behind it, adds its
-// parts in order.
+// Number of tiles right behind `tile` that begin with token t: the keys are
+// sorted, so they are the first ones, and 32 lanes narrow the range at a time.
+__device__ __forceinline__ int64_t tiles_of_run(const GradArgs& a, const uint32_t* key, int64_t tile,
+                                                uint32_t t) {
+  const int lane = threadIdx.x & 31;
+  int64_t lo = 0, hi = a.tiles - 1 - tile;  // the first lo do, none behind the first hi does
+  while (lo < hi) {
+    const int64_t step = (hi - lo + 31) / 32, at = lo + (lane + 1) * step;
+    const bool on = at <= hi && key[(tile + at) * a.places] == t;
+    const int n = __popc(__ballot_sync(0xffffffffu, on));
+    const int64_t next = lo + (int64_t)(n + 1) * step - 1;  // the one behind the last hit fails
+    lo += (int64_t)n * step;
+    hi = next < hi ? next : hi;
+  }
+  return lo;
+}
+
+// One CTA per tile and 32 V columns: if a run begins in the tile and goes on
+// behind it, its parts are added in four stretches of tiles, a warp each, and
+// the stretches in order.
 template <typename TT, int V>
-__global__ void __launch_bounds__(kSumThreads) emb_join(const SumArgs a) {
+__global__ void __launch_bounds__(kSumThreads) emb_join(const __grid_constant__ GradArgs a) {
+  __shared__ float part[kSumThreads / 32][32 * V];
+  wait_for_launch_before();
   const int64_t tile = blockIdx.x, p0 = tile * a.places, last = p0 + a.places - 1;
   if (last + 1 >= a.rows) return;
-  const uint32_t t = a.key[last];
-  if (t >= (uint32_t)a.vocab || a.key[last + 1] != t) return;
-  if (p0 > 0 && a.key[p0] == t && a.key[p0 - 1] == t) return;  // began earlier
-  const int64_t end = lower_bound(a.key, a.rows, t + 1);       // behind the run
-  const int64_t last_tile = (end - 1) / a.places;
-  const int col = (blockIdx.y * kSumThreads + threadIdx.x) * V;
-  if (col >= a.dim) return;
-  float acc[V];
-  load_v<float, V>(a.tail + tile * a.dim + col, acc);
+  const uint32_t* key = sorted_key(a);
+  const uint32_t t = key[last];
+  if (t >= (uint32_t)a.vocab || key[last + 1] != t) return;
+  if (p0 > 0 && key[p0] == t && key[p0 - 1] == t) return;  // began earlier
+  const int64_t n = tiles_of_run(a, key, tile, t);  // tiles with a head part
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int col = (blockIdx.y * 32 + lane) * V;
+  const int64_t j0 = tile + 1 + n * warp / 4, j1 = tile + 1 + n * (warp + 1) / 4;
+  float acc[V] = {};
+  if (col < a.dim) {
+    if (warp == 0) load_v<float, V>(a.tail + tile * a.dim + col, acc);
+    const float* src = a.head + col;
 #pragma unroll 8
-  for (int64_t j = tile + 1; j <= last_tile; ++j) {
-    float v[V];
-    load_v<float, V>(a.head + j * a.dim + col, v);
+    for (int64_t j = j0; j < j1; ++j) {
+      float v[V];
+      load_v<float, V>(src + j * a.dim, v);
 #pragma unroll
-    for (int e = 0; e < V; ++e) acc[e] += v[e];
+      for (int e = 0; e < V; ++e) acc[e] += v[e];
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e) part[warp][lane * V + e] = acc[e];
   }
+  __syncthreads();
+  if (warp != 0 || col >= a.dim) return;
+#pragma unroll
+  for (int w = 1; w < kSumThreads / 32; ++w)
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc[e] += part[w][lane * V + e];
   store_grad<TT, V>(a, t, col, acc);
 }
 
@@ -418,15 +516,46 @@ bool vec_ok(const void* p, int64_t ld, magma_dtype_t t, int v) {
 }
 
 template <typename TD, typename TT, int V>
-magma_status_t launch_sum(const SumArgs& a, cudaStream_t cs) {
+magma_status_t launch_grad(const GradArgs& a, cudaStream_t cs) {
+  // the cluster that sorts, and as many others as there is other work for
+  int64_t n = 1;
+  while (n < kMaxCluster && n * kSortRows < a.rows) n *= 2;
+  const int64_t other = (a.accumulate ? 0 : a.vocab * (int64_t)a.dim) +
+                        (a.dpos ? a.seq * a.dim * (a.batch + 1) : 0);
+  if (a.rows == 0 && other == 0) return MAGMA_OK;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)n);
+  cfg.blockDim = dim3(kSortThreads);
+  cfg.dynamicSmemBytes = kCountBytes;
+  cfg.stream = cs;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)n;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (other > 0) {
+    // No more clusters than run at once: a cluster needs its CTAs on one GPC,
+    // and the last ones of a second wave would take as long as all of the first.
+    int most = 0;
+    if (magma_status_t st = cuda_status(
+            cudaOccupancyMaxActiveClusters(&most, emb_sort<TD, TT, V>, &cfg), "emb_sort clusters"))
+      return st;
+    const int64_t more =
+        std::min<int64_t>(ceil_div(other, (int64_t)n * kSortThreads * V * 4), most - 1);
+    cfg.gridDim = dim3((unsigned)(n * (1 + std::max<int64_t>(more, 0))));
+  }
+  if (magma_status_t st = cuda_status(cudaLaunchKernelEx(&cfg, emb_sort<TD, TT, V>, a), "emb_sort"))
+    return st;
+  if (a.tiles == 0) return MAGMA_OK;
   const unsigned cols = (unsigned)ceil_div(a.dim, kSumThreads * V);
-  const int64_t blocks = a.tiles + a.zero_blocks + a.pos_blocks;
-  if (blocks > 0x7FFFFFFFLL) return fail(MAGMA_INVALID_ARGUMENT, "magma_embedding_scaled_bwd: too large");
-  emb_sum<TD, TT, V><<<dim3((unsigned)blocks, cols), kSumThreads, 0, cs>>>(a);
-  if (magma_status_t st = check_launch("emb_sum")) return st;
+  if (magma_status_t st = launch_after(emb_sum<TD, TT, V>, dim3((unsigned)a.tiles, cols),
+                                       kSumThreads, 0, cs, "emb_sum", a))
+    return st;
   if (a.tiles < 2) return MAGMA_OK;  // no border for a run to cross
-  emb_join<TT, V><<<dim3((unsigned)(a.tiles - 1), cols), kSumThreads, 0, cs>>>(a);
-  return check_launch("emb_join");
+  return launch_after(emb_join<TT, V>,
+                      dim3((unsigned)(a.tiles - 1), (unsigned)ceil_div(a.dim, 32 * V)), kSumThreads, 0,
+                      cs, "emb_join", a);
 }
 
 template <typename TI, typename TO>
@@ -445,6 +574,7 @@ magma_status_t check_sizes(const char* fn, int64_t batch, int64_t seq, int64_t d
   MAGMA_REQUIRE(batch >= 0 && seq >= 0 && dim >= 0 && vocab >= 0, "%s: negative size", fn);
   MAGMA_REQUIRE(vocab < 0x7FFFFFFFLL && dim <= (1LL << 22), "%s: vocab or dim too large", fn);
   MAGMA_REQUIRE(batch == 0 || seq <= 0x7FFFFFFFLL / batch, "%s: more than 2^31 - 1 rows", fn);
+  MAGMA_REQUIRE(batch > 0 || seq < 0x7FFFFFFFLL, "%s: more than 2^31 - 1 rows", fn);
   return MAGMA_OK;
 }
 
@@ -509,73 +639,48 @@ magma_status_t magma_embedding_scaled_bwd(const int32_t* tokens, const void* dou
                 "%s: a 16-byte aligned workspace of %lld bytes is needed", fn, (long long)l.total);
   cudaStream_t cs = (cudaStream_t)stream;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  SortArgs s{};
-  s.tokens = tokens;
+  GradArgs a{};
+  a.tokens = tokens;
   for (int i = 0; i < 2; ++i) {
-    s.key[i] = reinterpret_cast<uint32_t*>(ws + i * l.rows_bytes);
-    s.row[i] = reinterpret_cast<uint32_t*>(ws + (2 + i) * l.rows_bytes);
+    a.key[i] = reinterpret_cast<uint32_t*>(ws + i * l.rows_bytes);
+    a.row[i] = reinterpret_cast<uint32_t*>(ws + (2 + i) * l.rows_bytes);
   }
-  s.rows = rows;
-  s.vocab = vocab;
-  s.padding = padding_idx;
-  s.passes = vocab < (1 << 8) ? 1 : vocab < (1 << 16) ? 2 : vocab < (1 << 24) ? 3 : 4;
-  s.err = device_error_word();
-  if (rows > 0) {
-    int64_t n = 1;
-    while (n < kMaxCluster && n * kSortRows < rows) n *= 2;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)n);
-    cfg.blockDim = dim3(kSortThreads);
-    cfg.dynamicSmemBytes = kSortWarps * kDigits * 4;
-    cfg.stream = cs;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)n;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    if (magma_status_t st = cuda_status(cudaLaunchKernelEx(&cfg, emb_sort, s), "emb_sort"))
-      return st;
-  }
-  SumArgs a{};
-  a.key = s.key[(s.passes - 1) & 1];
-  a.row = s.row[(s.passes - 1) & 1];
+  a.head = reinterpret_cast<float*>(ws + 4 * l.rows_bytes);
+  a.tail = reinterpret_cast<float*>(ws + 4 * l.rows_bytes + l.part_bytes);
   a.dout = dout;
   a.dout_ld = dout_ld;
   a.dtable = dtable;
   a.dtable_ld = dtable_ld;
-  a.head = reinterpret_cast<float*>(ws + 4 * l.rows_bytes);
-  a.tail = reinterpret_cast<float*>(ws + 4 * l.rows_bytes + l.part_bytes);
   a.dpos = dpos;
   a.rows = rows;
   a.vocab = vocab;
   a.batch = batch;
   a.seq = seq;
+  a.padding = padding_idx;
+  a.tiles = l.tiles;
   a.dim = (int)dim;
   a.places = l.places;
-  a.tiles = l.tiles;
+  // the largest key is `vocab`
+  a.passes = vocab < (1 << 8) ? 1 : vocab < (1 << 16) ? 2 : vocab < (1 << 24) ? 3 : 4;
   a.accumulate = accumulate;
   a.accumulate_dpos = accumulate_dpos;
   a.scale = scale;
+  a.err = device_error_word();
   // Sixteen-byte accesses of dout where everything is aligned for them.
   const int vmax = dout_dtype == MAGMA_DTYPE_BF16 ? 8 : 4;
-  const bool vec = vec_ok(dout, dout_ld, dout_dtype, vmax) && dim % vmax == 0 &&
-                   vec_ok(dtable, dtable_ld, dtable_dtype, vmax) &&
+  const bool vec = vec_ok(dout, dout_ld, dout_dtype, vmax) && dim % 8 == 0 &&
+                   aligned16(dtable) && vec_ok(dtable, dtable_ld, dtable_dtype, 8) &&
                    (dpos == nullptr || vec_ok(dpos, dim, MAGMA_DTYPE_F32, vmax));
-  const int v = vec ? vmax : 1;
-  a.zero_blocks = accumulate ? 0 : ceil_div(vocab, kZeroRows * (kSumThreads / 32));
-  a.pos_blocks = dpos == nullptr ? 0 : ceil_div(seq * (dim / v), kSumThreads);
-  if (a.tiles + a.zero_blocks + a.pos_blocks == 0) return MAGMA_OK;
   const bool bd = dout_dtype == MAGMA_DTYPE_BF16, bt = dtable_dtype == MAGMA_DTYPE_BF16;
   if (vec)
-    return bd ? (bt ? launch_sum<__nv_bfloat16, __nv_bfloat16, 8>(a, cs)
-                    : launch_sum<__nv_bfloat16, float, 8>(a, cs))
-              : (bt ? launch_sum<float, __nv_bfloat16, 4>(a, cs)
-                    : launch_sum<float, float, 4>(a, cs));
-  return bd ? (bt ? launch_sum<__nv_bfloat16, __nv_bfloat16, 1>(a, cs)
-                  : launch_sum<__nv_bfloat16, float, 1>(a, cs))
-            : (bt ? launch_sum<float, __nv_bfloat16, 1>(a, cs)
-                  : launch_sum<float, float, 1>(a, cs));
+    return bd ? (bt ? launch_grad<__nv_bfloat16, __nv_bfloat16, 8>(a, cs)
+                    : launch_grad<__nv_bfloat16, float, 8>(a, cs))
+              : (bt ? launch_grad<float, __nv_bfloat16, 4>(a, cs)
+                    : launch_grad<float, float, 4>(a, cs));
+  return bd ? (bt ? launch_grad<__nv_bfloat16, __nv_bfloat16, 1>(a, cs)
+                  : launch_grad<__nv_bfloat16, float, 1>(a, cs))
+            : (bt ? launch_grad<float, __nv_bfloat16, 1>(a, cs)
+                  : launch_grad<float, float, 1>(a, cs));
 }
 
 }  // extern "C"

@@ -11,9 +11,10 @@
 //   grad_multi_scale  every block adds all partial sums in the same order,
 //                     forms c, and scales its share; block 0 writes the norm.
 // The list travels in the kernel's parameters, so a captured graph holds its
-// own copy and nothing is uploaded. A block's share is a contiguous run of
-// kTile-element tiles of the concatenated list (a tile never spans two
-// tensors), so one binary search finds its first tensor.
+// own copy and nothing is uploaded. The concatenated list is cut into
+// kTile-element tiles (a tile never spans two tensors), which the blocks take
+// in turn, so that the GPU reads one front through memory; one binary search
+// finds a block's first tensor, and from there it walks along the list.
 //
 // The squares are added in 64 bits: a square of an F32 value neither overflows
 // nor vanishes there, and the order of the additions does not show in the F32
@@ -30,8 +31,9 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kTile = 4096;       // elements of a tile
-constexpr int kSmallList = 48;    // tensors per launch, parameters of about 1 KB
-constexpr int kBigList = 1024;    // and of about 26 KB (the limit is 32764 bytes)
+constexpr int kSmallList = 48;    // tensors per launch, parameters of about 1 KB,
+constexpr int kMidList = 256;     // 7 KB
+constexpr int kBigList = 1024;    // and 29 KB (the limit is 32764 bytes)
 constexpr int kBlocksPerSm = 8;
 
 template <int N>
@@ -46,13 +48,7 @@ struct GradList {
 
 constexpr int kKindBf16In = 1, kKindBf16Out = 2, kKindVec = 4;
 
-// The block's share of the tiles, and the tensor that holds tile t.
-template <int N>
-__device__ __forceinline__ void share(const GradList<N>& l, uint32_t& t0, uint32_t& t1) {
-  const uint64_t tiles = l.first[l.count];
-  t0 = (uint32_t)(tiles * blockIdx.x / gridDim.x);
-  t1 = (uint32_t)(tiles * (blockIdx.x + 1) / gridDim.x);
-}
+// The tensor that holds tile t.
 template <int N>
 __device__ __forceinline__ int tensor_of(const GradList<N>& l, uint32_t t) {
   int lo = 0, hi = l.count;  // first[lo] <= t < first[hi]
@@ -105,12 +101,11 @@ __global__ void __launch_bounds__(kThreads)
 grad_multi_sumsq(const __grid_constant__ GradList<N> l, float scale,
                  double* __restrict__ partial) {
   __shared__ double red[kThreads / 32];
-  uint32_t t0, t1;
-  share(l, t0, t1);
+  const uint32_t tiles = l.first[l.count];
   double acc = 0.0;
-  if (t0 < t1) {
-    int k = tensor_of(l, t0);
-    for (uint32_t t = t0; t < t1; ++t) {
+  if (blockIdx.x < tiles) {
+    int k = tensor_of(l, blockIdx.x);
+    for (uint32_t t = blockIdx.x; t < tiles; t += gridDim.x) {
       while (t >= l.first[k + 1]) ++k;
       const int64_t e0 = (int64_t)(t - l.first[k]) * kTile;
       const int64_t left = l.n[k] - e0;
@@ -135,8 +130,20 @@ __device__ __forceinline__ float norm_of(const double* partial, int nb, double* 
 __global__ void __launch_bounds__(kThreads)
 grad_multi_finish(const double* __restrict__ partial, int nb, float* __restrict__ norm) {
   __shared__ double red[kThreads / 32];
+  wait_for_launch_before();
   const float v = norm_of(partial, nb, red);
   if (threadIdx.x == 0) norm[0] = v;
+}
+
+// Outputs are not read again here: they need not push gradients out of the L2.
+__device__ __forceinline__ void stream4(float* p, const float (&v)[4]) {
+  __stcs(reinterpret_cast<float4*>(p), make_float4(v[0], v[1], v[2], v[3]));
+}
+__device__ __forceinline__ void stream4(__nv_bfloat16* p, const float (&v)[4]) {
+  uint2 u;
+  *reinterpret_cast<__nv_bfloat162*>(&u.x) = __floats2bfloat162_rn(v[0], v[1]);
+  *reinterpret_cast<__nv_bfloat162*>(&u.y) = __floats2bfloat162_rn(v[2], v[3]);
+  __stcs(reinterpret_cast<uint2*>(p), u);
 }
 
 template <typename TI, typename TO>
@@ -151,7 +158,7 @@ __device__ __forceinline__ void tile_scale(const TI* g, TO* out, int n, bool vec
     for (int i = 0; i < kPer; ++i) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[i][e] = __fmul_rn(__fmul_rn(v[i][e], scale), c);
-      store4(out + 4 * (threadIdx.x + i * kThreads), v[i]);
+      stream4(out + 4 * (threadIdx.x + i * kThreads), v[i]);
     }
   } else {
     for (int i = threadIdx.x; i < n; i += kThreads)
@@ -159,22 +166,23 @@ __device__ __forceinline__ void tile_scale(const TI* g, TO* out, int n, bool vec
   }
 }
 
-// A block walks its share backwards: what grad_multi_sumsq read last is what
-// the L2 still holds.
+// The list is walked backwards: what grad_multi_sumsq read last is what the L2
+// still holds.
 template <int N>
 __global__ void __launch_bounds__(kThreads)
 grad_multi_scale(const __grid_constant__ GradList<N> l, float scale, float max_norm,
                  const double* __restrict__ partial, int nb, float* __restrict__ norm) {
   __shared__ double red[kThreads / 32];
+  wait_for_launch_before();
   const float v = norm_of(partial, nb, red);
   if (norm != nullptr && blockIdx.x == 0 && threadIdx.x == 0) norm[0] = v;
   const float raw = __fdiv_rn(max_norm, __fadd_rn(v, 1e-6f));
   const float c = raw < 1.f ? raw : 1.f;
-  uint32_t t0, t1;
-  share(l, t0, t1);
-  if (t0 >= t1) return;
-  int k = tensor_of(l, t1 - 1);
-  for (uint32_t t = t1; t-- > t0;) {
+  const uint32_t tiles = l.first[l.count];
+  if (blockIdx.x >= tiles) return;
+  int k = tensor_of(l, tiles - 1 - blockIdx.x);
+  for (int64_t at = (int64_t)tiles - 1 - blockIdx.x; at >= 0; at -= gridDim.x) {
+    const uint32_t t = (uint32_t)at;
     while (t < l.first[k]) --k;
     if (l.g[k] == l.out[k] && scale == 1.f && c == 1.f) continue;  // in place, unchanged
     const int64_t e0 = (int64_t)(t - l.first[k]) * kTile;
@@ -305,16 +313,17 @@ magma_status_t run_lists(const char* fn, const Tensors& t, float grad_scale, flo
     nb += b;
   }
   if (t.out == nullptr || nb == 0) {
-    grad_multi_finish<<<1, kThreads, 0, cs>>>(partial, nb, norm);
-    return check_launch("grad_multi_finish");
+    return launch_after(grad_multi_finish, dim3(1), kThreads, 0, cs, "grad_multi_finish", partial, nb,
+                        norm);
   }
   bool first = true;
   for (int32_t k = 0; k < t.count;) {
     k = fill(t, k, &l);
     if (l.count == 0) continue;
-    grad_multi_scale<N><<<blocks_for(l.first[l.count]), kThreads, 0, cs>>>(
-        l, grad_scale, max_norm, partial, nb, first ? norm : nullptr);
-    if (magma_status_t st = check_launch("grad_multi_scale")) return st;
+    if (magma_status_t st = launch_after(grad_multi_scale<N>, dim3(blocks_for(l.first[l.count])),
+                                         kThreads, 0, cs, "grad_multi_scale", l, grad_scale, max_norm,
+                                         partial, nb, first ? norm : nullptr))
+      return st;
     first = false;
   }
   return MAGMA_OK;
@@ -339,6 +348,8 @@ magma_status_t run(const char* fn, const Tensors& t, float grad_scale, float max
   return t.count <= kSmallList
              ? run_lists<kSmallList>(fn, t, grad_scale, max_norm, norm, partial,
                                      workspace_bytes / 8, cs)
+         : t.count <= kMidList
+             ? run_lists<kMidList>(fn, t, grad_scale, max_norm, norm, partial, workspace_bytes / 8, cs)
              : run_lists<kBigList>(fn, t, grad_scale, max_norm, norm, partial,
                                    workspace_bytes / 8, cs);
 }

@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
+from array import array
 
 import torch
 
@@ -391,21 +392,27 @@ def adam_step_clipped(params: torch.Tensor, grads: torch.Tensor, m: torch.Tensor
 
 
 def _tensor_list(ts, what: str, i: int | None = None):
-    """Device index, pointers, dtypes and sizes of contiguous tensors as C arrays."""
+    """Device index, pointers, dtypes and sizes of contiguous tensors."""
     n = len(ts)
     if n == 0:
         raise ValueError(f"at least one of the {what} is needed")
     if i is None:
         i = ts[0].get_device()
-    for t in ts:
-        if t.get_device() != i or i < 0:
-            _same_device(ts[0], t)
-            raise ValueError(f"{what} on another device than cuda:{i}")
-        if not t.is_contiguous():
-            raise ValueError(f"{what} must be contiguous tensors")
-    return (i, (C.c_void_p * n)(*[t.data_ptr() for t in ts]),
-            (C.c_int32 * n)(*[_dtype(t) for t in ts]),
-            (C.c_int64 * n)(*[t.numel() for t in ts]))
+    if i < 0 or [t.get_device() for t in ts] != [i] * n:
+        _same_device(ts[0], *ts)
+        raise ValueError(f"{what} on another device than cuda:{i}")
+    if not all([t.is_contiguous() for t in ts]):
+        raise ValueError(f"{what} must be contiguous tensors")
+    try:
+        dtypes = [_DT[t.dtype] for t in ts]
+    except KeyError as e:
+        raise TypeError(f"unsupported dtype {e.args[0]}; expected float32 or bfloat16") from None
+    return (i, array("Q", [t.data_ptr() for t in ts]), array("i", dtypes),
+            array("q", [t.numel() for t in ts]))
+
+
+def _addr(a: array) -> int:
+    return a.buffer_info()[0]
 
 
 def _norm_out(norm: torch.Tensor | None, first: torch.Tensor) -> torch.Tensor:
@@ -427,8 +434,8 @@ def grad_norm_multi(grads, *, grad_scale: float = 1.0,
     norm = _norm_out(out, grads[0])
     n = _bytes_on(i, "magma_grad_norm_multi_workspace_size", len(grads))
     ws = norm.new_empty(n, dtype=torch.uint8)
-    _call_on(i, "magma_grad_norm_multi", ptrs, sizes, dtypes, len(grads), grad_scale,
-             norm.data_ptr(), ws.data_ptr(), n)
+    _call_on(i, "magma_grad_norm_multi", _addr(ptrs), _addr(sizes), _addr(dtypes), len(grads),
+             grad_scale, norm.data_ptr(), ws.data_ptr(), n)
     return norm
 
 
@@ -448,15 +455,15 @@ def clip_grad_norm(grads, max_norm: float, *, grad_scale: float = 1.0, out=None,
     i, ptrs, dtypes, sizes = _tensor_list(grads, "gradients")
     optrs, odtypes = ptrs, dtypes
     if out is not None:
-        for o, g in zip(outs, grads):
-            if o.shape != g.shape:
-                raise ValueError("an output differs in shape from its gradient")
+        if [o.shape for o in outs] != [g.shape for g in grads]:
+            raise ValueError("an output differs in shape from its gradient")
         _, optrs, odtypes, _ = _tensor_list(outs, "outputs", i)
     norm = _norm_out(norm, grads[0])
     n = _bytes_on(i, "magma_grad_norm_multi_workspace_size", len(grads))
     ws = norm.new_empty(n, dtype=torch.uint8)
-    _call_on(i, "magma_clip_grad_norm_multi", ptrs, optrs, sizes, dtypes, odtypes, len(grads),
-             grad_scale, max_norm, norm.data_ptr(), ws.data_ptr(), n)
+    _call_on(i, "magma_clip_grad_norm_multi", _addr(ptrs), _addr(optrs), _addr(sizes),
+             _addr(dtypes), _addr(odtypes), len(grads), grad_scale, max_norm, norm.data_ptr(),
+             ws.data_ptr(), n)
     return norm
 
 
