@@ -41,6 +41,11 @@ constexpr float kRescaleLog2 = 8.0f;
 constexpr int kBlk128 = 128 * 128;    // bytes of 64 columns of a 128-row tile
 constexpr int kBlk64 = 64 * 128;      // and of a 64-row tile
 
+// The exponent's scale in base 2. A scale of 0 becomes the smallest normal
+// number: products of finite scores with it leave every exponential at 1, and a
+// masked score of -inf still gives 0.
+__device__ __forceinline__ float scale_log2(float scale) { return fmaxf(scale * kLog2e, 1.17549435e-38f); }
+
 struct TcArgs {
   CrossGeom g;
   int n_qt;                 // 128-row query tiles of a head
@@ -197,7 +202,7 @@ struct Fwd {
   static constexpr int kK = kQBufs * 2 * kTile;
   static constexpr int kV = kK + kKs * kTile;
   static constexpr int kBar = kV + kVs * kTile;
-  static constexpr int kBars = 2 * kQBufs + 2 * kKs + 2 * kVs + 8 + 1;
+  static constexpr int kBars = 2 * kQBufs + 2 * kKs + 2 * kVs + 10 + 1;
   static constexpr int kOrd = kBar + kBars * 8 + 8;
   static constexpr int kSmem = kOrd + 2 * kOrder + 1024;
   static_assert(kSmem <= 232448, "shared memory");
@@ -230,8 +235,9 @@ cross_fwd_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
   auto s_full = [&](int t) { return sbars + 8u * t; };
   auto s_free = [&](int t) { return sbars + 8u * (2 + t); };
   auto p_full = [&](int t) { return sbars + 8u * (4 + t); };
-  auto pv_done = [&](int t) { return sbars + 8u * (6 + t); };
-  const uint32_t done_bar = sbars + 64u;
+  auto p_half = [&](int t) { return sbars + 8u * (6 + t); };
+  auto pv_done = [&](int t) { return sbars + 8u * (8 + t); };
+  const uint32_t done_bar = sbars + 80u;
   const uint32_t tslot = bars + 8u * F::kBars;
   uint32_t* tslot_ptr = reinterpret_cast<uint32_t*>(sp + F::kBar + 8 * F::kBars);
   uint16_t* order = reinterpret_cast<uint16_t*>(sp + F::kOrd);
@@ -247,7 +253,7 @@ cross_fwd_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
     prefetch_tensormap(&tmV);
     for (int i = 0; i < F::kBars; ++i) {
       const uint32_t b = bars + 8u * i;
-      const bool by_warps = (b >= s_free(0) && b <= s_free(1)) || (b >= p_full(0) && b <= p_full(1));
+      const bool by_warps = b >= s_free(0) && b <= p_half(1);
       mbar_init(b, by_warps ? 4 : 1);
     }
     fence_barrier_init();
@@ -324,13 +330,19 @@ cross_fwd_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
       auto issue_pv = [&](int t, int j, int kg) -> bool {
         const int st = kg % F::kVs;
         if (!mbar_wait(v_full(st), (uint32_t)((kg / F::kVs) & 1), g.err)) return false;
-        if (!mbar_wait(p_full(t), (uint32_t)(np[t] & 1), g.err)) return false;
-        tc_fence_after();
         const uint64_t dv = desc_add(dv0, (uint32_t)st * F::kTile);
+        // the first 64 keys while the softmax is at the others
 #pragma unroll
-        for (int kk = 0; kk < kRows / 16; ++kk)
-          mma_bf16_ts(tmem + F::tO(t), tmem + F::tP(t) + kk * 8, desc_add(dv, kk * 2048), idO,
-                      j > 0 || kk > 0 ? 1u : 0u);
+        for (int half = 0; half < 2; ++half) {
+          if (!mbar_wait(half ? p_full(t) : p_half(t), (uint32_t)(np[t] & 1), g.err)) return false;
+          tc_fence_after();
+#pragma unroll
+          for (int k4 = 0; k4 < 4; ++k4) {
+            const int kk = half * 4 + k4;
+            mma_bf16_ts(tmem + F::tO(t), tmem + F::tP(t) + kk * 8, desc_add(dv, kk * 2048), idO,
+                        j > 0 || kk > 0 ? 1u : 0u);
+          }
+        }
         mma_commit(pv_done(t));
         ++np[t];
         return true;
@@ -370,7 +382,7 @@ cross_fwd_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
     const uint32_t srow = tmem + F::tS(t) + lanes;
     const uint32_t orow = tmem + F::tO(t) + lanes;
     const uint32_t prow = tmem + F::tP(t) + lanes;
-    const float sl2 = g.scale * kLog2e;
+    const float sl2 = scale_log2(g.scale);
     bool ok = true;
     int gs = 0;  // this warpgroup's steps so far
     int gk = 0;
@@ -392,27 +404,33 @@ cross_fwd_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) continue;
         tc_fence_after();
-        // the row's maximum, two halves of 64 columns, eight chains
+        // The first 96 columns of the row stay in registers from the maximum to
+        // the exponentials; the last 32 are read again (128 would not fit beside
+        // the rest of the 168 a thread has).
+        uint32_t v[3][32], w4[32];
+        // -inf: no part in maximum or sum
+        auto mask = [&](uint32_t(&x)[32], int c) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (c * 32 + e > lim) x[e] = 0xFF800000u;
+        };
+        tmem_ld32(srow + 96, w4);
+#pragma unroll
+        for (int c = 0; c < 3; ++c) tmem_ld32(srow + c * 32, v[c]);
+        tmem_wait_ld();
+        if (tail) {
+          mask(w4, 3);
+#pragma unroll
+          for (int c = 0; c < 3; ++c) mask(v[c], c);
+        }
         float mx8[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) mx8[i] = -INFINITY;
+        for (int i = 0; i < 8; ++i) mx8[i] = __uint_as_float(w4[i]);
 #pragma unroll
-        for (int hh = 0; hh < 2; ++hh) {
-          uint32_t v[2][32];
-          tmem_ld32(srow + hh * 64, v[0]);
-          tmem_ld32(srow + hh * 64 + 32, v[1]);
-          tmem_wait_ld();
-          if (!tail) {
+        for (int e = 8; e < 32; ++e) mx8[e & 7] = fmaxf(mx8[e & 7], __uint_as_float(w4[e]));
 #pragma unroll
-            for (int e = 0; e < 64; ++e)
-              mx8[e & 7] = fmaxf(mx8[e & 7], __uint_as_float(v[e >> 5][e & 31]));
-          } else {
-#pragma unroll
-            for (int e = 0; e < 64; ++e)
-              if (hh * 64 + e <= lim)
-                mx8[e & 7] = fmaxf(mx8[e & 7], __uint_as_float(v[e >> 5][e & 31]));
-          }
-        }
+        for (int e = 0; e < 96; ++e)
+          mx8[e & 7] = fmaxf(mx8[e & 7], __uint_as_float(v[e >> 5][e & 31]));
         const float mx = fmaxf(fmaxf(fmaxf(mx8[0], mx8[1]), fmaxf(mx8[2], mx8[3])),
                                fmaxf(fmaxf(mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7])));
         const float m_new = fmaxf(m_run, mx * sl2);
@@ -428,57 +446,19 @@ cross_fwd_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
           m_run = m_new;
           l_run *= alpha;
 #pragma unroll
-          for (int c = 0; c < HD / 32; ++c) {
-            uint32_t o[32];
-            tmem_ld32(orow + c * 32, o);
+          for (int c = 0; c < HD / 16; ++c) {
+            uint32_t o[16];
+            tmem_ld16(orow + c * 16, o);
             tmem_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-            tmem_st32(orow + c * 32, o);
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            tmem_st16(orow + c * 16, o);
           }
           tmem_wait_st();
         }
         // P = exp2(S scale log2(e) - m), two columns per instruction
         unsigned long long rs2[2] = {0ull, 0ull};
         const unsigned long long sl22 = f2_pack(sl2, sl2), nm2 = f2_pack(-m_run, -m_run);
-        auto exp32 = [&](const uint32_t (&v)[32], int c) {
-          uint32_t pk[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            float x0, x1;
-            f2_unpack(f2_fma(f2_pack(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])),
-                             sl22, nm2), x0, x1);
-            float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
-            if (tail) {
-              if (c + 2 * e > lim) p0 = 0.f;
-              if (c + 2 * e + 1 > lim) p1 = 0.f;
-            }
-            rs2[e & 1] = f2_add(rs2[e & 1], f2_pack(p0, p1));
-            pk[e] = pack_bf16(p0, p1);
-          }
-          tmem_st16(prow + c / 2, pk);
-        };
-        uint32_t va[2][32], vb[32], vc[32];
-        tmem_ld32(srow, va[0]);
-        tmem_ld32(srow + 32, va[1]);
-        tmem_wait_ld();
-        exp32(va[0], 0);
-        tmem_ld32(srow + 64, vb);
-        exp32(va[1], 32);
-        tmem_wait_ld();
-        tmem_ld32(srow + 96, vc);
-        exp32(vb, 64);
-        tmem_wait_ld();
-        if (!F::kOver) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(s_free(t));
-        }
-        exp32(vc, 96);
-        float a0, a1, b0, b1;
-        f2_unpack(rs2[0], a0, a1);
-        f2_unpack(rs2[1], b0, b1);
-        l_run += (a0 + a1) + (b0 + b1);
         if (tail && t == 0) {  // P_0 V goes first: both tiles find the rows zeroed
           const int vs = gk % F::kVs;
           if (!mbar_wait(v_full(vs), (uint32_t)((gk / F::kVs) & 1), g.err)) ok = false;
@@ -486,10 +466,43 @@ cross_fwd_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
           if (ok && row > lim) zero_row(sV(vs), row, F::kBlocks, kBlk128);
           fence_proxy_async_smem();
         }
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (ok && lane == 0) mbar_arrive(p_full(t));
+        auto exp32 = [&](const uint32_t(&x)[32], int c) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            float x0, x1;
+            f2_unpack(f2_fma(f2_pack(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), sl22,
+                             nm2), x0, x1);
+            const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
+            rs2[e & 1] = f2_add(rs2[e & 1], f2_pack(p0, p1));
+            pk[e] = pack_bf16(p0, p1);
+          }
+          tmem_st16(prow + c * 16, pk);
+        };
+        auto arrive = [&](uint32_t bar) {
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (ok && lane == 0) mbar_arrive(bar);
+        };
+        exp32(v[0], 0);
+        exp32(v[1], 1);
+        arrive(p_half(t));
+        tmem_ld32(srow + 96, w4);
+        exp32(v[2], 2);
+        tmem_wait_ld();
+        if (!F::kOver) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(s_free(t));
+        }
+        if (tail) mask(w4, 3);
+        exp32(w4, 3);
+        arrive(p_full(t));
+        float a0, a1, b0, b1;
+        f2_unpack(rs2[0], a0, a1);
+        f2_unpack(rs2[1], b0, b1);
+        l_run += (a0 + a1) + (b0 + b1);
       }
       if (ok && w.n > 0 && !mbar_wait(pv_done(t), (uint32_t)((gs - 1) & 1), g.err)) ok = false;
       ok = __all_sync(0xffffffffu, ok);
@@ -768,7 +781,7 @@ cross_dq_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
     const int t = warp >> 2;
     const int row = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const float sl2 = g.scale * kLog2e;
+    const float sl2 = scale_log2(g.scale);
     const unsigned long long sl22 = f2_pack(sl2, sl2);
     bool ok = true;
     int gs = 0, gk = 0, gu = 0;
@@ -1088,7 +1101,7 @@ cross_dkdv_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
     const int t = warp >> 2;
     const int row = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const float sl2 = g.scale * kLog2e;
+    const float sl2 = scale_log2(g.scale);
     const unsigned long long sl22 = f2_pack(sl2, sl2);
     bool ok = true;
     int gs = 0, ru = 0;
