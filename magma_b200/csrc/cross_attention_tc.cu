@@ -22,6 +22,7 @@
 #include <cuda.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "cross_attention.cuh"
 #include "sm100.cuh"
@@ -149,12 +150,19 @@ __device__ __forceinline__ void zero_cols(__nv_bfloat16* dst, int hd) {
 // 2p + 1 of the heads' query tiles in order.
 struct PairUnit {
   int64_t b;
-  int kvh, split;
-  int h[2], qt[2];
+  int kvh, split, first;  // first item: (head in the group) * n_qt + query tile
   int items;
   int64_t len;
   int t0, n;  // first tile of the keys, number of tiles
 };
+
+// Head and query tile of a unit's tile t.
+__device__ __forceinline__ int head_of(const TcArgs& a, const PairUnit& w, int t) {
+  return w.kvh * a.g.group + (w.first + t) / a.n_qt;
+}
+__device__ __forceinline__ int tile_of(const TcArgs& a, const PairUnit& w, int t) {
+  return (w.first + t) % a.n_qt;
+}
 
 template <int KT>
 __device__ __forceinline__ PairUnit pair_unit(const TcArgs& a, const uint16_t* order, int64_t u) {
@@ -169,12 +177,8 @@ __device__ __forceinline__ PairUnit pair_unit(const TcArgs& a, const uint16_t* o
   w.split = x / a.n_pairs;
   const int p = x % a.n_pairs;
   const int all = g.group * a.n_qt;
+  w.first = 2 * p;
   w.items = 2 * p + 1 < all ? 2 : 1;
-  for (int t = 0; t < 2; ++t) {
-    const int i = 2 * p + t < all ? 2 * p + t : 2 * p;
-    w.h[t] = w.kvh * g.group + i / a.n_qt;
-    w.qt[t] = i % a.n_qt;
-  }
   w.len = cross_len(g, w.b);
   const int tiles = (int)((w.len + KT - 1) / KT);
   const int each = (tiles + a.n_split - 1) / a.n_split;
@@ -280,8 +284,8 @@ cross_fwd_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
         mbar_expect_tx(q_full(qb), w.items * F::kTile);
         for (int t = 0; t < w.items; ++t)
           for (int c = 0; c < F::kBlocks; ++c)
-            tma_load_4d(sQ(qb, t) + c * kBlk128, &tmQ, c * 64, w.qt[t] * kRows, w.h[t] * a.qh,
-                        (int)w.b * a.qb, q_full(qb));
+            tma_load_4d(sQ(qb, t) + c * kBlk128, &tmQ, c * 64, tile_of(a, w, t) * kRows,
+                        head_of(a, w, t) * a.qh, (int)w.b * a.qb, q_full(qb));
         for (int j = 0; j < w.n; ++j, ++gk) {
           const int ks = gk % F::kKs, vs = gk % F::kVs;
           const int row = (w.t0 + j) * kRows;
@@ -308,67 +312,94 @@ cross_fwd_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
       constexpr uint32_t idO = idesc_bf16_f32(kRows, HD, 0, 1);
       const uint64_t dq0 = desc_k(sQ(0, 0)), dk0 = desc_k(sK(0)), dv0 = desc_mn(sV(0), kBlk128);
       bool ok = true;
-      int gk = 0, ru = 0;
-      int ns[2] = {0, 0}, np[2] = {0, 0};
-      // S_t of the key tile at ring position kg
-      auto issue_s = [&](int t, int qb, int kg) -> bool {
-        if (!F::kOver && ns[t] >= 1 && !mbar_wait(s_free(t), (uint32_t)((ns[t] - 1) & 1), g.err))
-          return false;
-        const int st = kg % F::kKs;
-        if (!mbar_wait(k_full(st), (uint32_t)((kg / F::kKs) & 1), g.err)) return false;
+      int ru = 0;
+      // ring positions of the next key tile of S and of P V, and the parities of
+      // their stages: counted up, so that nothing is divided per step
+      int ks = 0, vs = 0;
+      uint32_t kp = 0, vp = 0;
+      uint32_t ns0 = 0, ns1 = 0, np0 = 0, np1 = 0;  // S_t, P_t V issued
+      auto k_wait = [&]() {
+        if (!mbar_wait(k_full(ks), kp, g.err)) return false;
+        tc_fence_after();
+        return true;
+      };
+      auto k_next = [&]() {  // both tiles' S have been issued
+        mma_commit(k_empty(ks));
+        if (++ks == F::kKs) ks = 0, kp ^= 1u;
+      };
+      auto issue_s = [&](auto tc, int qb) -> bool {
+        constexpr int t = decltype(tc)::value;
+        uint32_t& ns = t ? ns1 : ns0;
+        if (!F::kOver && ns >= 1 && !mbar_wait(s_free(t), (ns - 1) & 1u, g.err)) return false;
         tc_fence_after();
         const uint64_t dq = desc_add(dq0, (uint32_t)(2 * qb + t) * F::kTile);
-        const uint64_t dk = desc_add(dk0, (uint32_t)st * F::kTile);
+        const uint64_t dk = desc_add(dk0, (uint32_t)ks * F::kTile);
+        const uint32_t d = tmem + F::tS(t);
 #pragma unroll
         for (int kk = 0; kk < HD / 16; ++kk)
-          mma_bf16_ss(tmem + F::tS(t), desc_add(dq, k_step(kk, kBlk128)),
-                      desc_add(dk, k_step(kk, kBlk128)), idS, kk > 0 ? 1u : 0u);
+          mma_bf16_ss(d, desc_add(dq, k_step(kk, kBlk128)), desc_add(dk, k_step(kk, kBlk128)), idS,
+                      kk > 0 ? 1u : 0u);
         mma_commit(s_full(t));
-        ++ns[t];
+        ++ns;
         return true;
       };
-      auto issue_pv = [&](int t, int j, int kg) -> bool {
-        const int st = kg % F::kVs;
-        if (!mbar_wait(v_full(st), (uint32_t)((kg / F::kVs) & 1), g.err)) return false;
-        const uint64_t dv = desc_add(dv0, (uint32_t)st * F::kTile);
+      auto issue_pv = [&](auto tc, uint32_t more) -> bool {
+        constexpr int t = decltype(tc)::value;
+        uint32_t& np = t ? np1 : np0;
+        const uint64_t dv = desc_add(dv0, (uint32_t)vs * F::kTile);
+        const uint32_t d = tmem + F::tO(t), p = tmem + F::tP(t);
         // the first 64 keys while the softmax is at the others
+        if (!mbar_wait(p_half(t), np & 1u, g.err)) return false;
+        tc_fence_after();
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          if (!mbar_wait(half ? p_full(t) : p_half(t), (uint32_t)(np[t] & 1), g.err)) return false;
-          tc_fence_after();
+        for (int kk = 0; kk < 4; ++kk)
+          mma_bf16_ts(d, p + kk * 8, desc_add(dv, kk * 2048), idO, kk > 0 ? 1u : more);
+        if (!mbar_wait(p_full(t), np & 1u, g.err)) return false;
+        tc_fence_after();
 #pragma unroll
-          for (int k4 = 0; k4 < 4; ++k4) {
-            const int kk = half * 4 + k4;
-            mma_bf16_ts(tmem + F::tO(t), tmem + F::tP(t) + kk * 8, desc_add(dv, kk * 2048), idO,
-                        j > 0 || kk > 0 ? 1u : 0u);
-          }
-        }
+        for (int kk = 4; kk < 8; ++kk)
+          mma_bf16_ts(d, p + kk * 8, desc_add(dv, kk * 2048), idO, 1u);
         mma_commit(pv_done(t));
-        ++np[t];
+        ++np;
         return true;
       };
+      using t0 = std::integral_constant<int, 0>;
+      using t1 = std::integral_constant<int, 1>;
       for (int64_t r = 0; ok; ++r) {
         const int64_t u = snake(r, cta, ctas, units);
         if (u < 0) break;
         const PairUnit w = pair_unit<kRows>(a, order, u);
         if (w.n <= 0) continue;
         const int qb = ru % F::kQBufs;
-        if (!mbar_wait(q_full(qb), (uint32_t)((ru / F::kQBufs) & 1), g.err)) break;
-        for (int t = 0; t < w.items && ok; ++t) ok = issue_s(t, qb, gk);
+        const bool two = w.items > 1;
+        ok = mbar_wait(q_full(qb), (uint32_t)((ru / F::kQBufs) & 1), g.err) && k_wait() &&
+             issue_s(t0{}, qb) && (!two || issue_s(t1{}, qb));
         if (!ok) break;
-        mma_commit(k_empty(gk % F::kKs));
-        for (int j = 0; j < w.n && ok; ++j) {
-          for (int t = 0; t < w.items && ok; ++t) {
-            // head size 64: S_t(j + 1) as soon as S_t(j) has been read; 128: P_t(j)
-            // lies in S_t's columns, so S_t(j + 1) goes behind P_t(j) V_j
-            if (!F::kOver && j + 1 < w.n) ok = issue_s(t, qb, gk + j + 1);
-            if (ok) ok = issue_pv(t, j, gk + j);
-            if (ok && t + 1 == w.items) mma_commit(v_empty((gk + j) % F::kVs));
-            if (F::kOver && ok && j + 1 < w.n) ok = issue_s(t, qb, gk + j + 1);
+        k_next();
+        for (int j = 0; j < w.n; ++j) {
+          const bool last = j + 1 == w.n;
+          const uint32_t more = j > 0 ? 1u : 0u;
+          ok = mbar_wait(v_full(vs), vp, g.err) && (last || k_wait());
+          if (!ok) break;
+          // head size 64: S_t(j + 1) as soon as S_t(j) has been read; 128: P_t(j)
+          // lies in S_t's columns, so S_t(j + 1) goes behind P_t(j) V_j
+          if constexpr (F::kOver) {
+            ok = issue_pv(t0{}, more) && (last || issue_s(t0{}, qb)) &&
+                 (!two || issue_pv(t1{}, more));
+            if (!ok) break;
+            mma_commit(v_empty(vs));
+            if (two && !last) ok = issue_s(t1{}, qb);
+          } else {
+            ok = (last || issue_s(t0{}, qb)) && issue_pv(t0{}, more) &&
+                 (!two || ((last || issue_s(t1{}, qb)) && issue_pv(t1{}, more)));
+            if (!ok) break;
+            mma_commit(v_empty(vs));
           }
-          if (ok && j + 1 < w.n) mma_commit(k_empty((gk + j + 1) % F::kKs));
+          if (!ok) break;
+          if (!last) k_next();
+          if (++vs == F::kVs) vs = 0, vp ^= 1u;
         }
-        gk += w.n;
+        if (!ok) break;
         ++ru;
         mma_commit(q_empty(qb));
       }
@@ -394,7 +425,8 @@ cross_fwd_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
         gk += w.n > 0 ? w.n : 0;
         continue;
       }
-      const int64_t qi = (int64_t)w.qt[t] * kRows + row;
+      const int h = head_of(a, w, t);
+      const int64_t qi = (int64_t)tile_of(a, w, t) * kRows + row;
       float m_run = -INFINITY, l_run = 0.f;
       for (int j = 0; j < w.n; ++j, ++gs, ++gk) {
         const int64_t left = w.len - (int64_t)(w.t0 + j) * kRows;
@@ -510,9 +542,9 @@ cross_fwd_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
       tc_fence_after();
       const float inv = l_run == 0.f ? 0.f : 1.0f / l_run;  // no keys: a zero row
       const float lse = l_run == 0.f ? -INFINITY : m_run * kLn2 + logf(l_run);
-      const int64_t at = (w.b * g.heads + w.h[t]) * g.q_len + qi;
+      const int64_t at = (w.b * g.heads + h) * g.q_len + qi;
       const bool in = qi < g.q_len;
-      __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(a.o) + w.b * g.os[0] + w.h[t] * g.os[1] +
+      __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(a.o) + w.b * g.os[0] + h * g.os[1] +
                            qi * g.os[2];
       const int64_t pat = w.split * g.batch * g.heads * g.q_len + at;
 #pragma unroll
@@ -590,24 +622,29 @@ cross_rows(const __nv_bfloat16* __restrict__ o, const __nv_bfloat16* __restrict_
   delta[i] = q < g.q_len ? acc : 0.f;
 }
 
-// P and dS of 32 columns of a row as BF16 pairs, two columns per instruction.
-// nl and dl: the rows' terms of each column pair.
-template <typename NL, typename DL>
-__device__ __forceinline__ void grad32(const uint32_t (&vs)[32], const uint32_t (&vd)[32],
-                                       unsigned long long sl22, NL nl, DL dl, uint32_t (&pp)[16],
-                                       uint32_t (&pd)[16], int lim) {
+// P of 32 columns of a row in place of S, two columns per instruction; nl: the
+// -lse log2(e) of a column pair.
+template <typename NL>
+__device__ __forceinline__ void probs32(uint32_t (&v)[32], unsigned long long sl22, NL nl) {
 #pragma unroll
   for (int e = 0; e < 16; ++e) {
-    float x0, x1, d0, d1;
-    f2_unpack(f2_fma(f2_pack(__uint_as_float(vs[2 * e]), __uint_as_float(vs[2 * e + 1])), sl22,
-                     nl(e)), x0, x1);
-    const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
-    f2_unpack(f2_mul(f2_pack(p0, p1),
+    float x0, x1;
+    f2_unpack(f2_fma(f2_pack(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), sl22, nl(e)),
+              x0, x1);
+    v[2 * e] = __float_as_uint(ex2_approx(x0));
+    v[2 * e + 1] = __float_as_uint(ex2_approx(x1));
+  }
+}
+// dS = P (dP - delta) of 32 columns as BF16 pairs; dl: the delta of a column pair.
+template <typename DL>
+__device__ __forceinline__ void grads32(const uint32_t (&p)[32], const uint32_t (&vd)[32], DL dl,
+                                        uint32_t (&pd)[16]) {
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    float d0, d1;
+    f2_unpack(f2_mul(f2_pack(__uint_as_float(p[2 * e]), __uint_as_float(p[2 * e + 1])),
                      f2_sub(f2_pack(__uint_as_float(vd[2 * e]), __uint_as_float(vd[2 * e + 1])),
                             dl(e))), d0, d1);
-    if (2 * e > lim) d0 = 0.f;
-    if (2 * e + 1 > lim) d1 = 0.f;
-    pp[e] = pack_bf16(p0, p1);
     pd[e] = pack_bf16(d0, d1);
   }
 }
@@ -626,7 +663,7 @@ struct Dq {
   static constexpr int kQ = 0;                      // [t][Q, dO]
   static constexpr int kRing = 4 * kTile;           // [stage][K, V]
   static constexpr int kBar = kRing + kStages * 2 * kKv;
-  static constexpr int kBars = 2 + 2 * kStages + 6 + 1;
+  static constexpr int kBars = 2 + 2 * kStages + 8 + 1;
   static constexpr int kOrd = kBar + kBars * 8 + 8;
   static constexpr int kSmem = kOrd + 2 * kOrder + 1024;
   static_assert(kSmem <= 232448, "shared memory");
@@ -653,7 +690,8 @@ cross_dq_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
   auto s_full = [&](int t) { return sbars + 8u * t; };
   auto ds_full = [&](int t) { return sbars + 8u * (2 + t); };
   auto dq_done = [&](int t) { return sbars + 8u * (4 + t); };
-  const uint32_t done_bar = sbars + 48u;
+  auto dp_full = [&](int t) { return sbars + 8u * (6 + t); };
+  const uint32_t done_bar = sbars + 64u;
   const uint32_t tslot = bars + 8u * F::kBars;
   uint32_t* tslot_ptr = reinterpret_cast<uint32_t*>(sp + F::kBar + 8 * F::kBars);
   uint16_t* order = reinterpret_cast<uint16_t*>(sp + F::kOrd);
@@ -697,10 +735,9 @@ cross_dq_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
         mbar_expect_tx(q_full, w.items * 2 * F::kTile);
         for (int t = 0; t < w.items; ++t)
           for (int c = 0; c < F::kBlocks; ++c) {
-            tma_load_4d(sQ(t) + c * kBlk128, &tmQ, c * 64, w.qt[t] * kRows, w.h[t] * a.qh,
-                        (int)w.b * a.qb, q_full);
-            tma_load_4d(sG(t) + c * kBlk128, &tmG, c * 64, w.qt[t] * kRows, w.h[t] * a.dh,
-                        (int)w.b * a.db, q_full);
+            const int row = tile_of(a, w, t) * kRows, h = head_of(a, w, t);
+            tma_load_4d(sQ(t) + c * kBlk128, &tmQ, c * 64, row, h * a.qh, (int)w.b * a.qb, q_full);
+            tma_load_4d(sG(t) + c * kBlk128, &tmG, c * 64, row, h * a.dh, (int)w.b * a.db, q_full);
           }
         for (int j = 0; j < w.n; ++j, ++gk) {
           const int st = gk % F::kStages, row = j * F::kKeys;
@@ -726,51 +763,81 @@ cross_dq_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
       constexpr uint32_t idS = idesc_bf16_f32(kRows, F::kKeys, 0, 0);
       constexpr uint32_t idQ = idesc_bf16_f32(kRows, HD, 0, 1);
       bool ok = true;
-      int gk = 0, ru = 0;
-      int nd[2] = {0, 0};
+      int ru = 0;
       const uint64_t dq0 = desc_k(sQ(0)), dg0 = desc_k(sG(0)), dk0 = desc_k(sK(0)),
                      dv0 = desc_k(sV(0)), dkm0 = desc_mn(sK(0), kBlk64);
-      auto issue_s = [&](int t, int kg) -> bool {
-        const int st = kg % F::kStages;
-        if (!mbar_wait(kv_full(st), (uint32_t)((kg / F::kStages) & 1), g.err)) return false;
+      int sst = 0, gst = 0;      // ring stages of the next S / dP and of the next dQ
+      uint32_t sph = 0;
+      uint32_t nd0 = 0, nd1 = 0;  // dS_t used
+      auto kv_wait = [&]() {
+        if (!mbar_wait(kv_full(sst), sph, g.err)) return false;
         tc_fence_after();
-        const uint32_t at = (uint32_t)t * 2 * F::kTile, ak = (uint32_t)st * 2 * F::kKv;
+        return true;
+      };
+      auto kv_next = [&]() {
+        if (++sst == F::kStages) sst = 0, sph ^= 1u;
+      };
+      auto issue_s = [&](auto tc) {
+        constexpr int t = decltype(tc)::value;
+        const uint64_t dk = desc_add(dk0, (uint32_t)sst * 2 * F::kKv);
+        const uint64_t dv = desc_add(dv0, (uint32_t)sst * 2 * F::kKv);
+        constexpr uint32_t at = (uint32_t)t * 2 * F::kTile;
 #pragma unroll
         for (int kk = 0; kk < HD / 16; ++kk)
-          mma_bf16_ss(tS(t), desc_add(dq0, at + k_step(kk, kBlk128)),
-                      desc_add(dk0, ak + k_step(kk, kBlk64)), idS, kk > 0 ? 1u : 0u);
+          mma_bf16_ss(tS(t), desc_add(dq0, at + k_step(kk, kBlk128)), desc_add(dk, k_step(kk, kBlk64)),
+                      idS, kk > 0 ? 1u : 0u);
+        mma_commit(s_full(t));
 #pragma unroll
         for (int kk = 0; kk < HD / 16; ++kk)
           mma_bf16_ss(tDp(t), desc_add(dg0, at + k_step(kk, kBlk128)),
-                      desc_add(dv0, ak + k_step(kk, kBlk64)), idS, kk > 0 ? 1u : 0u);
-        mma_commit(s_full(t));
+                      desc_add(dv, k_step(kk, kBlk64)), idS, kk > 0 ? 1u : 0u);
+        mma_commit(dp_full(t));
+      };
+      auto issue_dq = [&](auto tc, uint32_t more) -> bool {
+        constexpr int t = decltype(tc)::value;
+        uint32_t& nd = t ? nd1 : nd0;
+        if (!mbar_wait(ds_full(t), nd & 1u, g.err)) return false;
+        ++nd;
+        tc_fence_after();
+        const uint64_t dk = desc_add(dkm0, (uint32_t)gst * 2 * F::kKv);
+#pragma unroll
+        for (int kk = 0; kk < F::kKeys / 16; ++kk)
+          mma_bf16_ts(tDq(t), tS(t) + kk * 8, desc_add(dk, kk * 2048), idQ, kk > 0 ? 1u : more);
         return true;
       };
+      using t0 = std::integral_constant<int, 0>;
+      using t1 = std::integral_constant<int, 1>;
       for (int64_t r = 0; ok; ++r) {
         const int64_t u = snake(r, cta, ctas, units);
         if (u < 0) break;
         const PairUnit w = pair_unit<F::kKeys>(a, order, u);
         if (w.n <= 0) continue;
-        if (!mbar_wait(q_full, (uint32_t)(ru & 1), g.err)) break;
-        for (int t = 0; t < w.items && ok; ++t) ok = issue_s(t, gk);
-        for (int j = 0; j < w.n && ok; ++j) {
-          const int st = (gk + j) % F::kStages;
-          for (int t = 0; t < w.items && ok; ++t) {
-            ok = mbar_wait(ds_full(t), (uint32_t)(nd[t] & 1), g.err);
+        const bool two = w.items > 1;
+        ok = mbar_wait(q_full, (uint32_t)(ru & 1), g.err) && kv_wait();
+        if (!ok) break;
+        issue_s(t0{});
+        if (two) issue_s(t1{});
+        kv_next();
+        for (int j = 0; j < w.n; ++j) {
+          const bool last = j + 1 == w.n;
+          const uint32_t more = j > 0 ? 1u : 0u;
+          ok = (last || kv_wait()) && issue_dq(t0{}, more);
+          if (!ok) break;
+          if (last) mma_commit(dq_done(0));
+          else issue_s(t0{});
+          if (two) {
+            ok = issue_dq(t1{}, more);
             if (!ok) break;
-            ++nd[t];
-            tc_fence_after();
-            const uint64_t dk = desc_add(dkm0, (uint32_t)st * 2 * F::kKv);
-#pragma unroll
-            for (int kk = 0; kk < F::kKeys / 16; ++kk)
-              mma_bf16_ts(tDq(t), tS(t) + kk * 8, desc_add(dk, kk * 2048), idQ,
-                          j > 0 || kk > 0 ? 1u : 0u);
-            if (t + 1 == w.items) mma_commit(kv_empty(st));
-            if (j + 1 < w.n) ok = issue_s(t, gk + j + 1);
-            else mma_commit(dq_done(t));
           }
+          mma_commit(kv_empty(gst));
+          if (two) {
+            if (last) mma_commit(dq_done(1));
+            else issue_s(t1{});
+          }
+          if (!last) kv_next();
+          if (++gst == F::kStages) gst = 0;
         }
-        gk += w.n;
+        if (!ok) break;
         ++ru;
         mma_commit(q_empty);
       }
@@ -793,9 +860,10 @@ cross_dq_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
         gk += w.n > 0 ? w.n : 0;
         continue;
       }
-      const int64_t qi = (int64_t)w.qt[t] * kRows + row;
+      const int h = head_of(a, w, t);
+      const int64_t qi = (int64_t)tile_of(a, w, t) * kRows + row;
       const bool in = qi < g.q_len;
-      const int64_t at = (w.b * g.heads + w.h[t]) * a.q_pad + qi;
+      const int64_t at = (w.b * g.heads + h) * a.q_pad + qi;
       const float nl = in ? a.nlse[at] : -INFINITY, dl = in ? a.delta[at] : 0.f;
       const unsigned long long nl2 = f2_pack(nl, nl), dl2 = f2_pack(dl, dl);
       for (int j = 0; j < w.n; ++j, ++gs, ++gk) {
@@ -806,22 +874,32 @@ cross_dq_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) continue;
         tc_fence_after();
-        uint32_t vs[2][32], vd[2][32];
+        uint32_t vs[2][32];
         tmem_ld32(tS(t) + lanes, vs[0]);
-        tmem_ld32(tDp(t) + lanes, vd[0]);
-        tmem_wait_ld();
         tmem_ld32(tS(t) + lanes + 32, vs[1]);
-        tmem_ld32(tDp(t) + lanes + 32, vd[1]);
-        uint32_t pp[16], pd[16];
-        auto n = [&](int) { return nl2; };
-        auto d = [&](int) { return dl2; };
-        if (tail) grad32(vs[0], vd[0], sl22, n, d, pp, pd, lim);
-        else grad32(vs[0], vd[0], sl22, n, d, pp, pd, 64);
-        tmem_wait_ld();  // all of S_t is in registers: dS_t may take its columns
-        tmem_st16(tS(t) + lanes, pd);
-        if (tail) grad32(vs[1], vd[1], sl22, n, d, pp, pd, lim - 32);
-        else grad32(vs[1], vd[1], sl22, n, d, pp, pd, 64);
-        tmem_st16(tS(t) + lanes + 16, pd);
+        tmem_wait_ld();
+        // P while dP is being computed
+#pragma unroll
+        for (int c = 0; c < 2; ++c) probs32(vs[c], sl22, [&](int) { return nl2; });
+        if (!mbar_wait(dp_full(t), (uint32_t)(gs & 1), g.err)) ok = false;
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) continue;
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t vd[32], pd[16];
+          tmem_ld32(tDp(t) + lanes + 32 * c, vd);
+          tmem_wait_ld();
+          grads32(vs[c], vd, [&](int) { return dl2; }, pd);
+          if (tail) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              if (32 * c + 2 * e > lim) pd[e] &= 0xFFFF0000u;
+              if (32 * c + 2 * e + 1 > lim) pd[e] &= 0x0000FFFFu;
+            }
+          }
+          tmem_st16(tS(t) + lanes + 16 * c, pd);  // S_t is in registers
+        }
         if (tail && t == 0 && row < F::kKeys) {  // warps 0 and 1
           const int st = gk % F::kStages;
           if (!mbar_wait(kv_full(st), (uint32_t)((gk / F::kStages) & 1), g.err)) ok = false;
@@ -834,7 +912,7 @@ cross_dq_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
         __syncwarp();
         if (ok && lane == 0) mbar_arrive(ds_full(t));
       }
-      __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(a.dq) + w.b * g.dqs[0] + w.h[t] * g.dqs[1] +
+      __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(a.dq) + w.b * g.dqs[0] + h * g.dqs[1] +
                            qi * g.dqs[2];
       if (w.n <= 0) {
         if (in) zero_cols(dst, g.hd);
@@ -885,7 +963,7 @@ struct Dkv {
   static constexpr int kRing = kKvBufs * 2 * kTile;
   static constexpr int kStats = kRing + kStages * kStage;   // [stage][nlse, delta]
   static constexpr int kBar = kStats + kStages * 2 * kQ * 4;
-  static constexpr int kBars = 2 * kKvBufs + 2 * kStages + 4 + 3;
+  static constexpr int kBars = 2 * kKvBufs + 2 * kStages + 8 + 3;
   static constexpr int kSmem = kBar + kBars * 8 + 16 + 8 * kOrder + 16 + 1024;
   static_assert(kSmem <= 232448, "shared memory");
 };
@@ -912,7 +990,9 @@ cross_dkdv_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
   const uint32_t sbars = qbars + 16u * F::kStages;
   auto s_full = [&](int t) { return sbars + 8u * t; };
   auto p_full = [&](int t) { return sbars + 8u * (2 + t); };
-  const uint32_t acc_full = sbars + 32u, acc_empty = sbars + 40u, done_bar = sbars + 48u;
+  auto dp_full = [&](int t) { return sbars + 8u * (4 + t); };
+  auto ds_full = [&](int t) { return sbars + 8u * (6 + t); };
+  const uint32_t acc_full = sbars + 64u, acc_empty = sbars + 72u, done_bar = sbars + 80u;
   const uint32_t tslot = bars + 8u * F::kBars;
   uint32_t* tslot_ptr = reinterpret_cast<uint32_t*>(sp + F::kBar + 8 * F::kBars);
   // first[i]: key tiles of the sequences before i
@@ -936,7 +1016,8 @@ cross_dkdv_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
     prefetch_tensormap(&tmV);
     for (int i = 0; i < F::kBars; ++i) {
       const uint32_t b = bars + 8u * i;
-      mbar_init(b, b == p_full(0) || b == p_full(1) ? 4 : b == acc_empty ? 8 : 1);
+      const bool by_warps = b == p_full(0) || b == p_full(1) || b == ds_full(0) || b == ds_full(1);
+      mbar_init(b, by_warps ? 4 : b == acc_empty ? 8 : 1);
     }
     fence_barrier_init();
   }
@@ -1045,22 +1126,39 @@ cross_dkdv_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
                      dg0 = desc_k(sG(0)), dqm0 = desc_mn(sQ(0), kBlk64),
                      dgm0 = desc_mn(sG(0), kBlk64);
       bool ok = true;
-      int gs = 0, ru = 0;
-      auto issue_s = [&](int i, int kb) -> bool {  // step i of all units
-        const int st = i % F::kStages, t = i & 1;
-        if (!mbar_wait(q_full(st), (uint32_t)((i / F::kStages) & 1), g.err)) return false;
+      int ru = 0;
+      // the next step whose S^T / dP^T, and whose dV / dK, are issued: its ring
+      // stage, its score buffer (alternating), and the parity of that buffer
+      int sst = 0, gst = 0, dst = 0;
+      uint32_t sph = 0, tb = 0, gp = 0, db = 0;
+      auto q_wait = [&]() {
+        if (!mbar_wait(q_full(sst), sph, g.err)) return false;
         tc_fence_after();
-        const uint32_t aq = (uint32_t)st * F::kStage, ak = (uint32_t)kb * 2 * F::kTile;
-#pragma unroll
-        for (int kk = 0; kk < HD / 16; ++kk)
-          mma_bf16_ss(tS(t), desc_add(dk0, ak + k_step(kk, kBlk128)),
-                      desc_add(dq0, aq + k_step(kk, kBlk64)), idS, kk > 0 ? 1u : 0u);
-#pragma unroll
-        for (int kk = 0; kk < HD / 16; ++kk)
-          mma_bf16_ss(tDp(t), desc_add(dv0, ak + k_step(kk, kBlk128)),
-                      desc_add(dg0, aq + k_step(kk, kBlk64)), idS, kk > 0 ? 1u : 0u);
-        mma_commit(s_full(t));
         return true;
+      };
+      auto issue_s = [&](uint32_t t, int kb) {
+        const uint32_t ak = (uint32_t)kb * 2 * F::kTile;
+        const uint64_t dk = desc_add(dk0, ak), dq = desc_add(dq0, (uint32_t)sst * F::kStage);
+        const uint32_t d = tmem + 128u * t;
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; ++kk)
+          mma_bf16_ss(d, desc_add(dk, k_step(kk, kBlk128)), desc_add(dq, k_step(kk, kBlk64)), idS,
+                      kk > 0 ? 1u : 0u);
+        mma_commit(s_full(t));
+      };
+      auto issue_dp = [&](uint32_t t, int kb) {
+        const uint32_t ak = (uint32_t)kb * 2 * F::kTile;
+        const uint64_t dv = desc_add(dv0, ak), dg = desc_add(dg0, (uint32_t)dst * F::kStage);
+        const uint32_t d = tmem + 128u * t + 64u;
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; ++kk)
+          mma_bf16_ss(d, desc_add(dv, k_step(kk, kBlk128)), desc_add(dg, k_step(kk, kBlk64)), idS,
+                      kk > 0 ? 1u : 0u);
+        mma_commit(dp_full(t));
+        if (++dst == F::kStages) dst = 0;
+      };
+      auto s_next = [&]() {
+        if (++sst == F::kStages) sst = 0, sph ^= 1u;
       };
       for (int64_t r = 0; ok; ++r) {
         const int64_t u = snake(r, cta, ctas, units);
@@ -1068,28 +1166,54 @@ cross_dkdv_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
         const Unit w = unit(u);
         if (w.n == 0) continue;
         const int kb = ru % F::kKvBufs;
-        if (!mbar_wait(kv_full(kb), (uint32_t)((ru / F::kKvBufs) & 1), g.err)) break;
-        for (int i = 0; i < 2 && i < w.n && ok; ++i) ok = issue_s(gs + i, kb);
-        for (int i = 0; i < w.n && ok; ++i) {
-          const int s = gs + i, t = s & 1, st = s % F::kStages;
-          ok = mbar_wait(p_full(t), (uint32_t)((s >> 1) & 1), g.err);
-          // the previous unit's dV and dK have been read
-          if (ok && i == 0 && ru >= 1) ok = mbar_wait(acc_empty, (uint32_t)((ru - 1) & 1), g.err);
+        ok = mbar_wait(kv_full(kb), (uint32_t)((ru / F::kKvBufs) & 1), g.err);
+        for (int i = 0; i < 2 && i < w.n && ok; ++i) {
+          ok = q_wait();
+          if (!ok) break;
+          issue_s(tb, kb);
+          issue_dp(tb, kb);
+          s_next();
+          tb ^= 1u;
+        }
+        if (!ok) break;
+        for (int i = 0; i < w.n; ++i) {
+          const uint32_t t = db;
+          const uint32_t more = i > 0 ? 1u : 0u;
+          const bool next = i + 2 < w.n;
+          const uint32_t aq = (uint32_t)gst * F::kStage, sc = tmem + 128u * t;
+          ok = mbar_wait(p_full(t), gp, g.err) &&
+               // the previous unit's dV and dK have been read
+               (i > 0 || ru == 0 || mbar_wait(acc_empty, (uint32_t)((ru - 1) & 1), g.err)) &&
+               (!next || q_wait());
           if (!ok) break;
           tc_fence_after();
-          const uint32_t aq = (uint32_t)st * F::kStage;
+          {
+            const uint64_t dgm = desc_add(dgm0, aq);
 #pragma unroll
-          for (int kk = 0; kk < F::kQ / 16; ++kk)
-            mma_bf16_ts(tDv, tS(t) + kk * 8, desc_add(dgm0, aq + kk * 2048), idG,
-                        i > 0 || kk > 0 ? 1u : 0u);
+            for (int kk = 0; kk < F::kQ / 16; ++kk)
+              mma_bf16_ts(tDv, sc + kk * 8, desc_add(dgm, kk * 2048), idG, kk > 0 ? 1u : more);
+          }
+          if (next) issue_s(t, kb);  // behind dV, which reads P^T in the same columns
+          ok = mbar_wait(ds_full(t), gp, g.err);
+          if (!ok) break;
+          tc_fence_after();
+          {
+            const uint64_t dqm = desc_add(dqm0, aq);
 #pragma unroll
-          for (int kk = 0; kk < F::kQ / 16; ++kk)
-            mma_bf16_ts(tDk, tDp(t) + kk * 8, desc_add(dqm0, aq + kk * 2048), idG,
-                        i > 0 || kk > 0 ? 1u : 0u);
-          mma_commit(q_empty(st));
-          if (i + 2 < w.n) ok = issue_s(s + 2, kb);
+            for (int kk = 0; kk < F::kQ / 16; ++kk)
+              mma_bf16_ts(tDk, sc + 64u + kk * 8, desc_add(dqm, kk * 2048), idG, kk > 0 ? 1u : more);
+          }
+          mma_commit(q_empty(gst));
+          if (next) {
+            issue_dp(t, kb);
+            s_next();
+            tb ^= 1u;
+          }
+          if (++gst == F::kStages) gst = 0;
+          gp ^= db;  // the parity of both buffers turns after the second one
+          db ^= 1u;
         }
-        gs += w.n;
+        if (!ok) break;
         ++ru;
         mma_commit(kv_empty(kb));
         mma_commit(acc_full);
@@ -1122,33 +1246,48 @@ cross_dkdv_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
         const ulonglong2* nl =
             reinterpret_cast<const ulonglong2*>(sp + F::kStats + st * 2 * F::kQ * 4);
         const ulonglong2* dl = nl + F::kQ / 4;
-        uint32_t vs[2][32], vd[2][32];
+        uint32_t vs[2][32];
         tmem_ld32(tS(t) + lanes, vs[0]);
-        tmem_ld32(tDp(t) + lanes, vd[0]);
-        tmem_wait_ld();
         tmem_ld32(tS(t) + lanes + 32, vs[1]);
-        tmem_ld32(tDp(t) + lanes + 32, vd[1]);
+        tmem_wait_ld();
+        auto terms = [&](const ulonglong2* p, int c) {
+          return [p, c, x = ulonglong2{}](int e) mutable {
+            if ((e & 1) == 0) x = p[c * 8 + (e >> 1)];
+            return (e & 1) ? x.y : x.x;
+          };
+        };
+        // P^T while dP^T is being computed
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          uint32_t pp[16], pd[16];
-          ulonglong2 n4, d4;
-          auto n = [&](int e) {
-            if ((e & 1) == 0) n4 = nl[c * 8 + (e >> 1)];
-            return (e & 1) ? n4.y : n4.x;
-          };
-          auto d = [&](int e) {
-            if ((e & 1) == 0) d4 = dl[c * 8 + (e >> 1)];
-            return (e & 1) ? d4.y : d4.x;
-          };
-          grad32(vs[c], vd[c], sl22, n, d, pp, pd, 64);
-          if (c == 0) tmem_wait_ld();  // both tiles are in registers
-          tmem_st16(tS(t) + lanes + 16 * c, pp);
-          tmem_st16(tDp(t) + lanes + 16 * c, pd);
+          probs32(vs[c], sl22, terms(nl, c));
+          uint32_t pp[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            pp[e] = pack_bf16(__uint_as_float(vs[c][2 * e]), __uint_as_float(vs[c][2 * e + 1]));
+          tmem_st16(tS(t) + lanes + 16 * c, pp);  // S^T is in registers
         }
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(p_full(t));
+        if (!mbar_wait(dp_full(t), (uint32_t)((s >> 1) & 1), g.err)) ok = false;
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) continue;
+        tc_fence_after();
+        uint32_t vd[2][32];
+        tmem_ld32(tDp(t) + lanes, vd[0]);
+        tmem_ld32(tDp(t) + lanes + 32, vd[1]);
+        tmem_wait_ld();
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t pd[16];
+          grads32(vs[c], vd[c], terms(dl, c), pd);
+          tmem_st16(tDp(t) + lanes + 16 * c, pd);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(ds_full(t));
       }
       gs += w.n;
       // warpgroup 0 stores dV, warpgroup 1 dK
