@@ -66,6 +66,17 @@ struct TcArgs {
   void* dv;
 };
 
+// True in one lane of a converged warp. The compiler knows that a single lane
+// runs what depends on it, and keeps the operands of the MMAs and copies issued
+// there in uniform registers (with `lane == 0` it serialises over the lanes).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(p));
+  return p != 0;
+}
+
 // A K-major operand: rows of 128 bytes, eight rows an atom.
 __device__ __forceinline__ uint64_t desc_k(uint32_t addr) { return smem_desc_sw128(addr, 16, 1024); }
 // An MN-major operand whose 64-column blocks are `blk` bytes apart.
@@ -270,7 +281,7 @@ cross_fwd_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tslot_ptr);
 
   if (warp == kTmaWarp) {
-    if (lane == 0) {
+    if (elect_one()) {
       bool ok = true;
       int gk = 0;  // key tiles loaded so far
       int ru = 0;  // units that had keys
@@ -307,7 +318,7 @@ cross_fwd_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
         ok = mbar_wait(v_empty(i % F::kVs), (uint32_t)(((i / F::kVs) & 1) ^ 1), g.err);
     }
   } else if (warp == kMmaWarp) {
-    if (lane == 0) {
+    if (elect_one()) {
       constexpr uint32_t idS = idesc_bf16_f32(kRows, kRows, 0, 0);
       constexpr uint32_t idO = idesc_bf16_f32(kRows, HD, 0, 1);
       const uint64_t dq0 = desc_k(sQ(0, 0)), dk0 = desc_k(sK(0)), dv0 = desc_mn(sV(0), kBlk128);
@@ -723,7 +734,7 @@ cross_dq_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
   auto tDq = [&](int t) { return tmem + 256u * t + 128u; };
 
   if (warp == kTmaWarp) {
-    if (lane == 0) {
+    if (elect_one()) {
       bool ok = true;
       int gk = 0, ru = 0;
       for (int64_t r = 0; ok; ++r) {
@@ -759,7 +770,7 @@ cross_dq_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
         ok = mbar_wait(kv_empty(i % F::kStages), (uint32_t)(((i / F::kStages) & 1) ^ 1), g.err);
     }
   } else if (warp == kMmaWarp) {
-    if (lane == 0) {
+    if (elect_one()) {
       constexpr uint32_t idS = idesc_bf16_f32(kRows, F::kKeys, 0, 0);
       constexpr uint32_t idQ = idesc_bf16_f32(kRows, HD, 0, 1);
       bool ok = true;
@@ -1079,7 +1090,7 @@ cross_dkdv_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
   };
 
   if (warp == kTmaWarp) {
-    if (lane == 0) {
+    if (elect_one()) {
       bool ok = true;
       int gq = 0, ru = 0;
       for (int64_t r = 0; ok; ++r) {
@@ -1119,7 +1130,7 @@ cross_dkdv_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
         ok = mbar_wait(q_empty(i % F::kStages), (uint32_t)(((i / F::kStages) & 1) ^ 1), g.err);
     }
   } else if (warp == kMmaWarp) {
-    if (lane == 0) {
+    if (elect_one()) {
       constexpr uint32_t idS = idesc_bf16_f32(kRows, F::kQ, 0, 0);
       constexpr uint32_t idG = idesc_bf16_f32(kRows, HD, 0, 1);
       const uint64_t dk0 = desc_k(sK(0)), dv0 = desc_k(sV(0)), dq0 = desc_k(sQ(0)),
