@@ -85,7 +85,8 @@ size_t magma_cross_attention_fwd_workspace_size(int64_t batch, int64_t heads, in
   if (!has_work(batch, heads, kv_heads, q_len, kv_len, head_dim)) return 0;
   CrossGeom g = sizes(batch, heads, kv_heads, q_len, kv_len, head_dim);
   if (cross_step_rows(g, dtype)) return cross_step_workspace(g, dtype);
-  return dtype == MAGMA_DTYPE_BF16 && head_dim % 8 == 0 ? cross_tc_fwd_workspace(g) : 0;
+  return dtype == MAGMA_DTYPE_BF16 && head_dim % 8 == 0 ? cross_tc_fwd_workspace(g)
+                                                        : cross_simt_fwd_workspace(g);
 }
 
 magma_status_t magma_cross_attention_fwd(const void* q, const void* k, const void* v, void* o,
@@ -112,7 +113,8 @@ magma_status_t magma_cross_attention_fwd(const void* q, const void* k, const voi
                           (cudaStream_t)stream);
   if (cross_tc_fwd_supported(q, k, v, o, g, dtype))
     return cross_fwd_tc_run(q, k, v, o, lse, g, workspace, workspace_bytes, (cudaStream_t)stream);
-  return cross_fwd_simt(q, k, v, o, lse, g, dtype, (cudaStream_t)stream);
+  return cross_fwd_simt(q, k, v, o, lse, g, dtype, workspace, workspace_bytes,
+                        (cudaStream_t)stream);
 }
 
 size_t magma_cross_attention_bwd_workspace_size(int64_t batch, int64_t heads, int64_t kv_heads,

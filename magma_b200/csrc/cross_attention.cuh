@@ -48,9 +48,12 @@ magma_status_t cross_smem(int bytes) {
   return MAGMA_OK;
 }
 
-// cross_attention_simt.cu: any types, strides and head sizes up to 128.
+// cross_attention_simt.cu: any types, strides and head sizes up to 128. The
+// forward pass takes less workspace or none.
+size_t cross_simt_fwd_workspace(const CrossGeom& g);
 magma_status_t cross_fwd_simt(const void* q, const void* k, const void* v, void* o, float* lse,
-                              const CrossGeom& g, magma_dtype_t dtype, cudaStream_t s);
+                              const CrossGeom& g, magma_dtype_t dtype, void* workspace,
+                              size_t workspace_bytes, cudaStream_t s);
 magma_status_t cross_bwd_simt(const void* q, const void* k, const void* v, const void* o,
                               const void* d_o, const float* lse, void* dq, void* dk, void* dv,
                               float* delta, const CrossGeom& g, magma_dtype_t dtype,

@@ -14,153 +14,302 @@
 // every output element is added up by one thread in a fixed order. Keys from
 // len_b on are never read: their tiles are filled with zeros.
 //
-// 64 x 64 tiles, 256 threads; thread (ty, tx) = (tid / 16, tid % 16) owns rows
-// ty + 16i and columns tx + 16j.
+// The query rows of the heads that share a key head form one list (row =
+// shared head * q_len + query), cut into 64-row tiles, so that short queries
+// fill a tile together. Everything is bound by the FMA pipe and what feeds it:
+// a thread holds a block of products and adds two terms per instruction
+// (fma.f32x2): pairs along d for the scores, whose tiles lie in rows of d, and
+// pairs along the row index for the second products, whose left operand is
+// written to shared memory with that index contiguous. Rows are padded by 16
+// bytes, which spreads 16-byte reads of neighbouring rows over the banks.
+#include <algorithm>
 #include <cmath>
 
 #include "cross_attention.cuh"
+#include "sm100.cuh"
 
 namespace magma {
 namespace {
 
-constexpr int kT = 64;
-constexpr int kThreads = 256;
+using u64 = unsigned long long;
 
-// Rows [r0, r0 + 64) x [0, hd) of a head as F32 into dst[64][HD + 1], zeros
-// from row `rows` and column hd on.
-template <int HD, typename T>
-__device__ __forceinline__ void load_tile(float* dst, const T* src, int64_t stride, int64_t r0,
-                                          int64_t rows, int hd) {
-  for (int i = threadIdx.x; i < kT * HD; i += kThreads) {
-    const int r = i / HD, d = i % HD;
-    dst[r * (HD + 1) + d] =
-        r0 + r < rows && d < hd ? to_f32(src[(r0 + r) * stride + d]) : 0.f;
-  }
+constexpr int kRows = 64;       // query rows, and keys of a gradient tile
+constexpr int kP = kRows + 4;   // pitch of a tile of probabilities
+
+// A tile of rows: pitch in floats.
+template <int HD> constexpr int kPitch = HD + 4;
+
+__device__ __forceinline__ void cp_async16(float* dst, const float* src, bool on) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(sm100::smem_u32(dst)), "l"(src),
+               "r"(on ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// acc[i][j] += sum_d a[ty + 16i][d] * b[tx + 16j][d]
-template <int HD>
-__device__ __forceinline__ void dot_tile(float (&acc)[4][4], const float* a, const float* b,
-                                         int ty, int tx) {
+// ROWS rows into dst[ROWS][HD + 4] as F32; `at(r)` is row r's offset from src,
+// negative for a row that is not there. Those rows, and columns from hd on,
+// become zeros. VEC: F32 rows in 16-byte pieces, asynchronously.
+template <int HD, int ROWS, bool VEC, typename T, typename At>
+__device__ __forceinline__ void load_rows(float* dst, const T* src, int hd, At at) {
+  if constexpr (VEC) {
+    constexpr int kPieces = HD / 4;
 #pragma unroll 4
-  for (int d = 0; d < HD; ++d) {
-    float x[4], y[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = a[(ty + 16 * i) * (HD + 1) + d];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) y[j] = b[(tx + 16 * j) * (HD + 1) + d];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(x[i], y[j], acc[i][j]);
+    for (int i = threadIdx.x; i < ROWS * kPieces; i += blockDim.x) {
+      const int r = i / kPieces, c = i % kPieces * 4;
+      const int64_t o = at(r);
+      const bool on = o >= 0 && c < hd;
+      cp_async16(dst + r * kPitch<HD> + c, src + (on ? o + c : 0), on);
+    }
+  } else {
+    for (int i = threadIdx.x; i < ROWS * HD; i += blockDim.x) {
+      const int r = i / HD, c = i % HD;
+      const int64_t o = at(r);
+      dst[r * kPitch<HD> + c] = o >= 0 && c < hd ? to_f32(src[o + c]) : 0.f;
+    }
   }
 }
 
+// s[i][j] = sum_d a[row_a(i)][d] b[row_b(j)][d], even and odd d apart.
+template <int HD, int NI, int NJ, typename RA, typename RB>
+__device__ __forceinline__ void dots(float (&s)[NI][NJ], const float* a, const float* b, RA row_a,
+                                     RB row_b) {
+  u64 acc[NI][NJ];
+#pragma unroll
+  for (int i = 0; i < NI; ++i)
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) acc[i][j] = 0ull;
+#pragma unroll 4
+  for (int d = 0; d < HD; d += 4) {
+    ulonglong2 x[NI], y[NJ];
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+      x[i] = *reinterpret_cast<const ulonglong2*>(a + row_a(i) * kPitch<HD> + d);
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+      y[j] = *reinterpret_cast<const ulonglong2*>(b + row_b(j) * kPitch<HD> + d);
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        acc[i][j] = f2_fma(x[i].x, y[j].x, acc[i][j]);
+        acc[i][j] = f2_fma(x[i].y, y[j].y, acc[i][j]);
+      }
+  }
+#pragma unroll
+  for (int i = 0; i < NI; ++i)
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      float lo, hi;
+      f2_unpack(acc[i][j], lo, hi);
+      s[i][j] = lo + hi;
+    }
+}
+
+// Column c of a thread's ND columns: groups of four, 64 apart.
+__device__ __forceinline__ int col_of(int tx, int c) { return tx * 4 + (c & 3) + 64 * (c >> 2); }
+
+// acc[p][c] += (left pair p) * right[c]: the columns' values doubled into pairs.
+template <int NP, int ND>
+__device__ __forceinline__ void add_products(u64 (&acc)[NP][ND], const u64 (&left)[NP],
+                                             const float* right, int tx) {
+#pragma unroll
+  for (int q = 0; q < ND / 4; ++q) {
+    const float4 v = *reinterpret_cast<const float4*>(right + tx * 4 + 64 * q);
+    const u64 w[4] = {f2_pack(v.x, v.x), f2_pack(v.y, v.y), f2_pack(v.z, v.z), f2_pack(v.w, v.w)};
+#pragma unroll
+    for (int p = 0; p < NP; ++p)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) acc[p][4 * q + c] = f2_fma(left[p], w[c], acc[p][4 * q + c]);
+  }
+}
+
+// A CTA's place: tile, key head, sequence, part of the source.
 struct Block {
-  int64_t tile, h, b;
+  int64_t tile, kvh, b;
+  int part;
 };
-__device__ __forceinline__ Block block_of(int64_t tiles, int64_t heads) {
+__device__ __forceinline__ Block block_of(int64_t tiles, int64_t heads, int parts) {
   Block x;
-  const int64_t i = blockIdx.x;
+  int64_t i = blockIdx.x;
+  x.part = (int)(i % parts);
+  i /= parts;
   x.tile = i % tiles;
-  x.h = i / tiles % heads;
+  x.kvh = i / tiles % heads;
   x.b = i / tiles / heads;
   return x;
 }
 
-template <int HD, typename T>
-__global__ void __launch_bounds__(kThreads)
+// Offset of listed query row r of a [B, H, Sq, D] tensor, -1 behind the last.
+__device__ __forceinline__ int64_t row_offset(const CrossGeom& g, const Block& x,
+                                              const int64_t (&st)[3], int64_t r) {
+  if (r >= g.group * g.q_len) return -1;
+  return x.b * st[0] + (x.kvh * g.group + r / g.q_len) * st[1] + r % g.q_len * st[2];
+}
+// Its index in [B, H, Sq].
+__device__ __forceinline__ int64_t row_index(const CrossGeom& g, const Block& x, int64_t r) {
+  return (x.b * g.heads + x.kvh * g.group + r / g.q_len) * g.q_len + r % g.q_len;
+}
+
+struct FwdArgs {
+  CrossGeom g;
+  int parts;
+  float* part;      // [part][b][h][q][hd] of a split source
+  float* part_lse;  // [part][b][h][q]
+};
+
+// ------------------------------------------------------------------ forward
+// 128 threads; thread (ty, tx) has rows ty 4 + {0..3} and + 32, keys tx + 16 j,
+// columns tx 4 + {0..3} and + 64. K and V of a tile have a buffer each: V comes
+// in under the scores, the next K under the sums.
+template <int HD>
+struct FwdTile {
+  static constexpr int kKeys = HD == 64 ? 64 : 32;
+  static constexpr int kSmem =
+      ((kRows + 2 * kKeys) * kPitch<HD> + kKeys * kP) * 4 + kRows * 8;
+};
+
+template <int HD, typename T, bool VEC>
+__global__ void __launch_bounds__(128)
 cross_fwd(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
-          T* __restrict__ o, float* __restrict__ lse, const CrossGeom g) {
-  extern __shared__ float sm[];
+          T* __restrict__ o, float* __restrict__ lse, const __grid_constant__ FwdArgs a) {
+  constexpr int BN = FwdTile<HD>::kKeys, NK = BN / 16, ND = HD / 16;
+  extern __shared__ __align__(16) float sm[];
   float* Qs = sm;
-  float* Ks = Qs + kT * (HD + 1);
-  float* Vs = Ks + kT * (HD + 1);
-  float* Ps = Vs + kT * (HD + 1);  // [64][65]
+  float* Ks = Qs + kRows * kPitch<HD>;
+  float* Vs = Ks + BN * kPitch<HD>;
+  float* Ps = Vs + BN * kPitch<HD>;                        // [key][row]
+  int64_t* offs = reinterpret_cast<int64_t*>(Ps + BN * kP);  // of the query rows
+  const CrossGeom& g = a.g;
   const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
-  const Block x = block_of((g.q_len + kT - 1) / kT, g.heads);
-  const int64_t q0 = x.tile * kT, kvh = x.h / g.group, len = cross_len(g, x.b);
-  const T* kh = k + x.b * g.ks[0] + kvh * g.ks[1];
-  const T* vh = v + x.b * g.vs[0] + kvh * g.vs[1];
-  load_tile<HD>(Qs, q + x.b * g.qs[0] + x.h * g.qs[1], g.qs[2], q0, g.q_len, g.hd);
-  constexpr int DJ = HD / 16;
-  float acc[4][DJ] = {}, m[4], l[4] = {};
+  const int64_t rows = (int64_t)g.group * g.q_len;
+  const Block x = block_of((rows + kRows - 1) / kRows, g.kv_heads, a.parts);
+  const int64_t r0 = x.tile * kRows, len = cross_len(g, x.b);
+  const int64_t tiles = (len + BN - 1) / BN, each = (tiles + a.parts - 1) / a.parts;
+  const int64_t t0 = x.part * each < tiles ? x.part * each : tiles;
+  const int64_t t1 = tiles - t0 < each ? tiles : t0 + each;
+  const T* kh = k + x.b * g.ks[0] + x.kvh * g.ks[1];
+  const T* vh = v + x.b * g.vs[0] + x.kvh * g.vs[1];
+  auto row = [&](int i) { return ty * 4 + (i & 3) + 32 * (i >> 2); };
+  auto load_k = [&](int64_t t) {
+    load_rows<HD, BN, VEC>(Ks, kh, g.hd, [&](int r) {
+      return t * BN + r < len ? (t * BN + r) * g.ks[2] : (int64_t)-1;
+    });
+  };
+  auto load_v = [&](int64_t t) {
+    load_rows<HD, BN, VEC>(Vs, vh, g.hd, [&](int r) {
+      return t * BN + r < len ? (t * BN + r) * g.vs[2] : (int64_t)-1;
+    });
+  };
+  if (tid < kRows) offs[tid] = row_offset(g, x, g.qs, r0 + tid);
+  __syncthreads();
+  load_rows<HD, kRows, VEC>(Qs, q, g.hd, [&](int r) { return offs[r]; });
+  if (t0 < t1) load_k(t0);
+  cp_commit();
+  u64 acc[4][ND];
+  float m[8], l[8];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) m[i] = -INFINITY;
-  for (int64_t k0 = 0; k0 < len; k0 += kT) {
-    __syncthreads();
-    load_tile<HD>(Ks, kh, g.ks[2], k0, len, g.hd);
-    load_tile<HD>(Vs, vh, g.vs[2], k0, len, g.hd);
-    __syncthreads();
-    float s[4][4] = {};
-    dot_tile<HD>(s, Qs, Ks, ty, tx);
+  for (int p = 0; p < 4; ++p)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int c = 0; c < ND; ++c) acc[p][c] = 0ull;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m[i] = -INFINITY, l[i] = 0.f;
+  for (int64_t t = t0; t < t1; ++t) {
+    cp_wait<0>();
+    __syncthreads();  // K is there; the last tile's V and P have been used
+    load_v(t);
+    cp_commit();
+    float s[8][NK];
+    dots<HD>(s, Qs, Ks, row, [&](int j) { return tx + 16 * j; });
+    float alpha[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
       float mx = -INFINITY;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        s[i][j] = k0 + tx + 16 * j < len ? s[i][j] * g.scale : -INFINITY;
+      for (int j = 0; j < NK; ++j) {
+        s[i][j] = t * BN + tx + 16 * j < len ? s[i][j] * g.scale : -INFINITY;
         mx = fmaxf(mx, s[i][j]);
       }
 #pragma unroll
       for (int w = 8; w > 0; w >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
       const float mn = fmaxf(m[i], mx);
       const float ref = mn == -INFINITY ? 0.f : mn;  // a row of -inf scores
-      const float alpha = expf(m[i] - ref);
+      alpha[i] = expf(m[i] - ref);
+      m[i] = mn;
       float rs = 0.f;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < NK; ++j) {
         s[i][j] = expf(s[i][j] - ref);
         rs += s[i][j];
       }
-#pragma unroll
-      for (int w = 8; w > 0; w >>= 1) rs += __shfl_xor_sync(0xffffffffu, rs, w);
-      l[i] = l[i] * alpha + rs;
-      m[i] = mn;
-#pragma unroll
-      for (int j = 0; j < DJ; ++j) acc[i][j] *= alpha;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) Ps[(ty + 16 * i) * (kT + 1) + tx + 16 * j] = s[i][j];
+      l[i] = l[i] * alpha[i] + rs;  // the thread's keys; the 16 threads meet at the end
     }
-    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < NK; ++j)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        *reinterpret_cast<float4*>(Ps + (tx + 16 * j) * kP + ty * 4 + 32 * h) =
+            make_float4(s[4 * h][j], s[4 * h + 1][j], s[4 * h + 2][j], s[4 * h + 3][j]);
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      const u64 f = f2_pack(alpha[2 * p], alpha[2 * p + 1]);
+#pragma unroll
+      for (int c = 0; c < ND; ++c) acc[p][c] = f2_mul(acc[p][c], f);
+    }
+    cp_wait<0>();
+    __syncthreads();  // V and P are there; K has been used
+    if (t + 1 < t1) load_k(t + 1);
+    cp_commit();
 #pragma unroll 4
-    for (int c = 0; c < kT; ++c) {
-      float pv[4], vv[DJ];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) pv[i] = Ps[(ty + 16 * i) * (kT + 1) + c];
-#pragma unroll
-      for (int j = 0; j < DJ; ++j) vv[j] = Vs[c * (HD + 1) + tx + 16 * j];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < DJ; ++j) acc[i][j] = fmaf(pv[i], vv[j], acc[i][j]);
+    for (int key = 0; key < BN; ++key) {
+      const ulonglong2 lo = *reinterpret_cast<const ulonglong2*>(Ps + key * kP + ty * 4);
+      const ulonglong2 hi = *reinterpret_cast<const ulonglong2*>(Ps + key * kP + ty * 4 + 32);
+      const u64 left[4] = {lo.x, lo.y, hi.x, hi.y};
+      add_products(acc, left, Vs + key * kPitch<HD>, tx);
     }
   }
-  T* oh = o + x.b * g.os[0] + x.h * g.os[1];
+  cp_wait<0>();
+  const int64_t all = g.batch * g.heads * g.q_len;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t qi = q0 + ty + 16 * i;
-    if (qi >= g.q_len) continue;
+  for (int i = 0; i < 8; ++i) {
+#pragma unroll
+    for (int w = 8; w > 0; w >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], w);
+    const int64_t r = r0 + row(i);
+    if (r >= rows) continue;
     const float inv = l[i] == 0.f ? 0.f : 1.0f / l[i];  // no keys: a zero row
-#pragma unroll
-    for (int j = 0; j < DJ; ++j) {
-      const int d = tx + 16 * j;
-      if (d < g.hd) oh[qi * g.os[2] + d] = from_f32<T>(acc[i][j] * inv);
+    const float out_lse = l[i] == 0.f ? -INFINITY : m[i] + logf(l[i]);
+    const int64_t at = row_index(g, x, r);
+    if (a.parts > 1) {
+      if (tx == 0) a.part_lse[x.part * all + at] = out_lse;
+    } else if (tx == 0 && lse != nullptr) {
+      lse[at] = out_lse;
     }
-    if (tx == 0 && lse != nullptr)
-      lse[(x.b * g.heads + x.h) * g.q_len + qi] = l[i] == 0.f ? -INFINITY : m[i] + logf(l[i]);
+    const int64_t oo = row_offset(g, x, g.os, r);
+#pragma unroll
+    for (int c = 0; c < ND; ++c) {
+      float lo, hi;
+      f2_unpack(acc[i >> 1][c], lo, hi);
+      const float y = (i & 1 ? hi : lo) * inv;
+      const int d = col_of(tx, c);
+      if (d >= g.hd) continue;
+      if (a.parts > 1) a.part[(x.part * all + at) * g.hd + d] = y;
+      else o[oo + d] = from_f32<T>(y);
+    }
   }
 }
 
 // delta[b, h, i] = sum_d dO[i, d] * O[i, d]; one warp per row.
 template <typename T>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(256)
 cross_delta(const T* __restrict__ o, const T* __restrict__ d_o, float* __restrict__ delta,
             const CrossGeom g) {
   const int lane = threadIdx.x & 31;
   const int64_t rows = g.batch * g.heads * g.q_len;
-  for (int64_t r = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); r < rows;
-       r += (int64_t)gridDim.x * (kThreads / 32)) {
+  for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < rows;
+       r += (int64_t)gridDim.x * 8) {
     const int64_t s = r % g.q_len, bh = r / g.q_len, h = bh % g.heads, b = bh / g.heads;
     const T* po = o + b * g.os[0] + h * g.os[1] + s * g.os[2];
     const T* pd = d_o + b * g.dos[0] + h * g.dos[1] + s * g.dos[2];
@@ -174,8 +323,17 @@ cross_delta(const T* __restrict__ o, const T* __restrict__ d_o, float* __restric
 // A row without probabilities (lse = -inf) gets none in the gradient either.
 __device__ __forceinline__ float row_lse(float lse) { return lse == -INFINITY ? INFINITY : lse; }
 
-// P and dS of a 64 x 64 tile from its dot products; keys from len on and
-// queries from q_len on take no part.
+// The terms of the query rows of a tile: lse and delta, (inf, 0) behind the last.
+__device__ __forceinline__ void row_terms(const CrossGeom& g, const Block& x, int64_t r,
+                                          const float* lse, const float* delta, float& l, float& e) {
+  const bool on = r < (int64_t)g.group * g.q_len;
+  const int64_t at = on ? row_index(g, x, r) : 0;
+  l = on ? row_lse(lse[at]) : INFINITY;
+  e = on ? delta[at] : 0.f;
+}
+
+// P and dS from the dot products; a key from len on takes no part, a query row
+// that is not there has lse = inf.
 __device__ __forceinline__ void probs(float& s, float& dp, bool on, float scale, float lse,
                                       float delta) {
   const float p = on ? expf(s * scale - lse) : 0.f;
@@ -183,239 +341,302 @@ __device__ __forceinline__ void probs(float& s, float& dp, bool on, float scale,
   dp = on ? p * (dp - delta) : 0.f;
 }
 
-// One CTA per (key tile, key head, sequence): dK and dV of 64 keys.
-template <int HD, typename T>
-__global__ void __launch_bounds__(kThreads)
+// --------------------------------------------------------------- dK and dV
+// One CTA of 256 threads per (key tile, key head, sequence). Scores: thread (ty,
+// tx) has rows ty 4 + {0..3}, keys tx + 16 j. Sums: keys ty 4 + {0..3}, columns
+// as above.
+template <int HD> constexpr int kDkvSmem = (4 * kRows * kPitch<HD> + 2 * kRows * kP + 2 * kRows) * 4 + 2 * kRows * 8;
+
+template <int HD, typename T, bool VEC>
+__global__ void __launch_bounds__(256, HD == 64 ? 2 : 1)
 cross_dkdv(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
            const T* __restrict__ d_o, const float* __restrict__ lse,
            const float* __restrict__ delta, T* __restrict__ dk, T* __restrict__ dv,
-           const CrossGeom g) {
-  extern __shared__ float sm[];
+           const __grid_constant__ CrossGeom g) {
+  constexpr int ND = HD / 16;
+  extern __shared__ __align__(16) float sm[];
   float* Ks = sm;
-  float* Vs = Ks + kT * (HD + 1);
-  float* Qs = Vs + kT * (HD + 1);
-  float* Gs = Qs + kT * (HD + 1);   // dO
-  float* Ps = Gs + kT * (HD + 1);   // [q][k], 64 x 65
-  float* Ds = Ps + kT * (kT + 1);   // dS
-  float* Ls = Ds + kT * (kT + 1);   // lse of the query tile
-  float* Es = Ls + kT;              // delta of the query tile
+  float* Vs = Ks + kRows * kPitch<HD>;
+  float* Qs = Vs + kRows * kPitch<HD>;
+  float* Gs = Qs + kRows * kPitch<HD>;  // dO
+  float* Ps = Gs + kRows * kPitch<HD>;  // [row][key]
+  float* Ds = Ps + kRows * kP;          // dS, [row][key]
+  float* Ls = Ds + kRows * kP;          // lse of the query rows
+  float* Es = Ls + kRows;               // delta
+  int64_t* qo = reinterpret_cast<int64_t*>(Es + kRows);
+  int64_t* go = qo + kRows;
   const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
-  const Block x = block_of((g.kv_len + kT - 1) / kT, g.kv_heads);
-  const int64_t k0 = x.tile * kT, len = cross_len(g, x.b);
-  constexpr int DJ = HD / 16;
-  float adk[4][DJ] = {}, adv[4][DJ] = {};
+  const Block x = block_of((g.kv_len + kRows - 1) / kRows, g.kv_heads, 1);
+  const int64_t k0 = x.tile * kRows, len = cross_len(g, x.b);
+  const int64_t rows = (int64_t)g.group * g.q_len;
+  u64 adk[2][ND], adv[2][ND];
+#pragma unroll
+  for (int p = 0; p < 2; ++p)
+#pragma unroll
+    for (int c = 0; c < ND; ++c) adk[p][c] = adv[p][c] = 0ull;
   if (k0 < len) {
-    load_tile<HD>(Ks, k + x.b * g.ks[0] + x.h * g.ks[1], g.ks[2], k0, len, g.hd);
-    load_tile<HD>(Vs, v + x.b * g.vs[0] + x.h * g.vs[1], g.vs[2], k0, len, g.hd);
-    for (int gi = 0; gi < g.group; ++gi) {
-      const int64_t h = x.h * g.group + gi, bh = x.b * g.heads + h;
-      const T* qh = q + x.b * g.qs[0] + h * g.qs[1];
-      const T* doh = d_o + x.b * g.dos[0] + h * g.dos[1];
-      for (int64_t q0 = 0; q0 < g.q_len; q0 += kT) {
-        __syncthreads();
-        load_tile<HD>(Qs, qh, g.qs[2], q0, g.q_len, g.hd);
-        load_tile<HD>(Gs, doh, g.dos[2], q0, g.q_len, g.hd);
-        if (tid < kT) {
-          const bool on = q0 + tid < g.q_len;
-          Ls[tid] = on ? row_lse(lse[bh * g.q_len + q0 + tid]) : 0.f;
-          Es[tid] = on ? delta[bh * g.q_len + q0 + tid] : 0.f;
-        }
-        __syncthreads();
-        float s[4][4] = {}, dp[4][4] = {};
-        dot_tile<HD>(s, Qs, Ks, ty, tx);
-        dot_tile<HD>(dp, Gs, Vs, ty, tx);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int r = ty + 16 * i, c = tx + 16 * j;
-            probs(s[i][j], dp[i][j], k0 + c < len && q0 + r < g.q_len, g.scale, Ls[r], Es[r]);
-            Ps[r * (kT + 1) + c] = s[i][j];
-            Ds[r * (kT + 1) + c] = dp[i][j];
-          }
-        __syncthreads();
-        // dV[key][d] += sum_q P[q][key] dO[q][d]: keys ty + 16i, columns tx + 16j
-#pragma unroll 2
-        for (int r = 0; r < kT; ++r) {
-          float p[4], ds[4], qv[DJ], gv[DJ];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            p[i] = Ps[r * (kT + 1) + ty + 16 * i];
-            ds[i] = Ds[r * (kT + 1) + ty + 16 * i];
-          }
-#pragma unroll
-          for (int j = 0; j < DJ; ++j) {
-            qv[j] = Qs[r * (HD + 1) + tx + 16 * j];
-            gv[j] = Gs[r * (HD + 1) + tx + 16 * j];
-          }
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int j = 0; j < DJ; ++j) {
-              adv[i][j] = fmaf(p[i], gv[j], adv[i][j]);
-              adk[i][j] = fmaf(ds[i], qv[j], adk[i][j]);
-            }
-        }
+    auto key = [&](int64_t st) {
+      return [&g, k0, len, st](int r) { return k0 + r < len ? (k0 + r) * st : (int64_t)-1; };
+    };
+    load_rows<HD, kRows, VEC>(Ks, k + x.b * g.ks[0] + x.kvh * g.ks[1], g.hd, key(g.ks[2]));
+    load_rows<HD, kRows, VEC>(Vs, v + x.b * g.vs[0] + x.kvh * g.vs[1], g.hd, key(g.vs[2]));
+    for (int64_t r0 = 0; r0 < rows; r0 += kRows) {
+      __syncthreads();
+      if (tid < kRows) {
+        qo[tid] = row_offset(g, x, g.qs, r0 + tid);
+        go[tid] = row_offset(g, x, g.dos, r0 + tid);
+        row_terms(g, x, r0 + tid, lse, delta, Ls[tid], Es[tid]);
       }
-    }
-  }
-  T* dkh = dk + x.b * g.dks[0] + x.h * g.dks[1];
-  T* dvh = dv + x.b * g.dvs[0] + x.h * g.dvs[1];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t kj = k0 + ty + 16 * i;
-    if (kj >= g.kv_len) continue;
-#pragma unroll
-    for (int j = 0; j < DJ; ++j) {
-      const int d = tx + 16 * j;
-      if (d >= g.hd) continue;
-      dkh[kj * g.dks[2] + d] = from_f32<T>(adk[i][j] * g.scale);
-      dvh[kj * g.dvs[2] + d] = from_f32<T>(adv[i][j]);
-    }
-  }
-}
-
-// One CTA per (query tile, head, sequence): dQ of 64 queries.
-template <int HD, typename T>
-__global__ void __launch_bounds__(kThreads)
-cross_dq(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
-         const T* __restrict__ d_o, const float* __restrict__ lse,
-         const float* __restrict__ delta, T* __restrict__ dq, const CrossGeom g) {
-  extern __shared__ float sm[];
-  float* Qs = sm;
-  float* Gs = Qs + kT * (HD + 1);
-  float* Ks = Gs + kT * (HD + 1);
-  float* Vs = Ks + kT * (HD + 1);
-  float* Ds = Vs + kT * (HD + 1);  // [q][k], 64 x 65
-  const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
-  const Block x = block_of((g.q_len + kT - 1) / kT, g.heads);
-  const int64_t q0 = x.tile * kT, kvh = x.h / g.group, len = cross_len(g, x.b);
-  const int64_t bh = x.b * g.heads + x.h;
-  load_tile<HD>(Qs, q + x.b * g.qs[0] + x.h * g.qs[1], g.qs[2], q0, g.q_len, g.hd);
-  load_tile<HD>(Gs, d_o + x.b * g.dos[0] + x.h * g.dos[1], g.dos[2], q0, g.q_len, g.hd);
-  float ls[4], es[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t qi = q0 + ty + 16 * i;
-    ls[i] = qi < g.q_len ? row_lse(lse[bh * g.q_len + qi]) : 0.f;
-    es[i] = qi < g.q_len ? delta[bh * g.q_len + qi] : 0.f;
-  }
-  constexpr int DJ = HD / 16;
-  float acc[4][DJ] = {};
-  for (int64_t k0 = 0; k0 < len; k0 += kT) {
-    __syncthreads();
-    load_tile<HD>(Ks, k + x.b * g.ks[0] + kvh * g.ks[1], g.ks[2], k0, len, g.hd);
-    load_tile<HD>(Vs, v + x.b * g.vs[0] + kvh * g.vs[1], g.vs[2], k0, len, g.hd);
-    __syncthreads();
-    float s[4][4] = {}, dp[4][4] = {};
-    dot_tile<HD>(s, Qs, Ks, ty, tx);
-    dot_tile<HD>(dp, Gs, Vs, ty, tx);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int r = ty + 16 * i, c = tx + 16 * j;
-        probs(s[i][j], dp[i][j], k0 + c < len && q0 + r < g.q_len, g.scale, ls[i], es[i]);
-        Ds[r * (kT + 1) + c] = dp[i][j];
-      }
-    __syncthreads();
-#pragma unroll 4
-    for (int c = 0; c < kT; ++c) {
-      float ds[4], kv[DJ];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) ds[i] = Ds[(ty + 16 * i) * (kT + 1) + c];
-#pragma unroll
-      for (int j = 0; j < DJ; ++j) kv[j] = Ks[c * (HD + 1) + tx + 16 * j];
+      __syncthreads();
+      load_rows<HD, kRows, VEC>(Qs, q, g.hd, [&](int r) { return qo[r]; });
+      load_rows<HD, kRows, VEC>(Gs, d_o, g.hd, [&](int r) { return go[r]; });
+      cp_commit();
+      cp_wait<0>();
+      __syncthreads();
+      float s[4][4], dp[4][4];
+      auto row = [&](int i) { return ty * 4 + i; };
+      auto col = [&](int j) { return tx + 16 * j; };
+      dots<HD>(s, Qs, Ks, row, col);
+      dots<HD>(dp, Gs, Vs, row, col);
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < DJ; ++j) acc[i][j] = fmaf(ds[i], kv[j], acc[i][j]);
+        for (int j = 0; j < 4; ++j) {
+          const int r = row(i), c = col(j);
+          probs(s[i][j], dp[i][j], k0 + c < len, g.scale, Ls[r], Es[r]);
+          Ps[r * kP + c] = s[i][j];
+          Ds[r * kP + c] = dp[i][j];
+        }
+      __syncthreads();
+#pragma unroll 4
+      for (int r = 0; r < kRows; ++r) {
+        const ulonglong2 p = *reinterpret_cast<const ulonglong2*>(Ps + r * kP + ty * 4);
+        const ulonglong2 d = *reinterpret_cast<const ulonglong2*>(Ds + r * kP + ty * 4);
+        const u64 lp[2] = {p.x, p.y}, ld[2] = {d.x, d.y};
+        add_products(adv, lp, Gs + r * kPitch<HD>, tx);
+        add_products(adk, ld, Qs + r * kPitch<HD>, tx);
+      }
     }
   }
-  T* dqh = dq + x.b * g.dqs[0] + x.h * g.dqs[1];
+  cp_wait<0>();
+  T* dkh = dk + x.b * g.dks[0] + x.kvh * g.dks[1];
+  T* dvh = dv + x.b * g.dvs[0] + x.kvh * g.dvs[1];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int64_t qi = q0 + ty + 16 * i;
-    if (qi >= g.q_len) continue;
+    const int64_t kj = k0 + ty * 4 + i;
+    if (kj >= g.kv_len) continue;
 #pragma unroll
-    for (int j = 0; j < DJ; ++j) {
-      const int d = tx + 16 * j;
-      if (d < g.hd) dqh[qi * g.dqs[2] + d] = from_f32<T>(acc[i][j] * g.scale);
+    for (int c = 0; c < ND; ++c) {
+      const int d = col_of(tx, c);
+      if (d >= g.hd) continue;
+      float a0, a1, b0, b1;
+      f2_unpack(adk[i >> 1][c], a0, a1);
+      f2_unpack(adv[i >> 1][c], b0, b1);
+      dkh[kj * g.dks[2] + d] = from_f32<T>((i & 1 ? a1 : a0) * g.scale);
+      dvh[kj * g.dvs[2] + d] = from_f32<T>(i & 1 ? b1 : b0);
     }
   }
 }
 
-magma_status_t blocks_of(int64_t tiles, int64_t heads, int64_t batch, unsigned* n) {
-  const double all = (double)tiles * (double)heads * (double)batch;
+// ---------------------------------------------------------------------- dQ
+// One CTA of 256 threads per (row tile, key head, sequence); sums: rows ty 4 +
+// {0..3}, columns as above.
+template <int HD> constexpr int kDqSmem = (4 * kRows * kPitch<HD> + kRows * kP) * 4 + 2 * kRows * 8;
+
+template <int HD, typename T, bool VEC>
+__global__ void __launch_bounds__(256, HD == 64 ? 2 : 1)
+cross_dq(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
+         const T* __restrict__ d_o, const float* __restrict__ lse,
+         const float* __restrict__ delta, T* __restrict__ dq, const __grid_constant__ CrossGeom g) {
+  constexpr int ND = HD / 16;
+  extern __shared__ __align__(16) float sm[];
+  float* Qs = sm;
+  float* Gs = Qs + kRows * kPitch<HD>;
+  float* Ks = Gs + kRows * kPitch<HD>;
+  float* Vs = Ks + kRows * kPitch<HD>;
+  float* Ds = Vs + kRows * kPitch<HD>;  // dS, [key][row]
+  int64_t* qo = reinterpret_cast<int64_t*>(Ds + kRows * kP);
+  int64_t* go = qo + kRows;
+  const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
+  const int64_t rows = (int64_t)g.group * g.q_len;
+  const Block x = block_of((rows + kRows - 1) / kRows, g.kv_heads, 1);
+  const int64_t r0 = x.tile * kRows, len = cross_len(g, x.b);
+  const T* kh = k + x.b * g.ks[0] + x.kvh * g.ks[1];
+  const T* vh = v + x.b * g.vs[0] + x.kvh * g.vs[1];
+  if (tid < kRows) {
+    qo[tid] = row_offset(g, x, g.qs, r0 + tid);
+    go[tid] = row_offset(g, x, g.dos, r0 + tid);
+  }
+  __syncthreads();
+  load_rows<HD, kRows, VEC>(Qs, q, g.hd, [&](int r) { return qo[r]; });
+  load_rows<HD, kRows, VEC>(Gs, d_o, g.hd, [&](int r) { return go[r]; });
+  auto row = [&](int i) { return ty * 4 + i; };
+  auto col = [&](int j) { return tx + 16 * j; };
+  float ls[4], es[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) row_terms(g, x, r0 + row(i), lse, delta, ls[i], es[i]);
+  u64 acc[2][ND];
+#pragma unroll
+  for (int p = 0; p < 2; ++p)
+#pragma unroll
+    for (int c = 0; c < ND; ++c) acc[p][c] = 0ull;
+  for (int64_t k0 = 0; k0 < len; k0 += kRows) {
+    __syncthreads();
+    auto key = [&](int64_t st) {
+      return [&g, k0, len, st](int r) { return k0 + r < len ? (k0 + r) * st : (int64_t)-1; };
+    };
+    load_rows<HD, kRows, VEC>(Ks, kh, g.hd, key(g.ks[2]));
+    load_rows<HD, kRows, VEC>(Vs, vh, g.hd, key(g.vs[2]));
+    cp_commit();
+    cp_wait<0>();
+    __syncthreads();
+    float s[4][4], dp[4][4];
+    dots<HD>(s, Qs, Ks, row, col);
+    dots<HD>(dp, Gs, Vs, row, col);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        probs(s[i][j], dp[i][j], k0 + col(j) < len, g.scale, ls[i], es[i]);
+      *reinterpret_cast<float4*>(Ds + col(j) * kP + ty * 4) =
+          make_float4(dp[0][j], dp[1][j], dp[2][j], dp[3][j]);
+    }
+    __syncthreads();
+#pragma unroll 4
+    for (int c = 0; c < kRows; ++c) {
+      const ulonglong2 d = *reinterpret_cast<const ulonglong2*>(Ds + c * kP + ty * 4);
+      const u64 left[2] = {d.x, d.y};
+      add_products(acc, left, Ks + c * kPitch<HD>, tx);
+    }
+  }
+  cp_wait<0>();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t o = row_offset(g, x, g.dqs, r0 + row(i));
+    if (o < 0) continue;
+#pragma unroll
+    for (int c = 0; c < ND; ++c) {
+      const int d = col_of(tx, c);
+      if (d >= g.hd) continue;
+      float lo, hi;
+      f2_unpack(acc[i >> 1][c], lo, hi);
+      dq[o + d] = from_f32<T>((i & 1 ? hi : lo) * g.scale);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- host side
+magma_status_t blocks_of(int64_t tiles, int64_t heads, int64_t batch, int64_t parts, unsigned* n) {
+  const double all = (double)tiles * (double)heads * (double)batch * (double)parts;
   if (all > 2147483647.0)
     return fail(MAGMA_INVALID_ARGUMENT, "cross attention: more than 2^31 - 1 tiles");
-  *n = (unsigned)(tiles * heads * batch);
+  *n = (unsigned)(tiles * heads * batch * parts);
   return MAGMA_OK;
 }
 
-template <int HD, typename T>
+int64_t row_tiles(const CrossGeom& g) { return ceil_div((int64_t)g.group * g.q_len, kRows); }
+
+// Rows in 16-byte pieces.
+bool pieces(const void* p, const int64_t (&st)[3]) {
+  return aligned16(p) && st[0] % 4 == 0 && st[1] % 4 == 0 && st[2] % 4 == 0;
+}
+
+template <int HD, typename T, bool VEC>
 magma_status_t fwd(const void* q, const void* k, const void* v, void* o, float* lse,
-                   const CrossGeom& g, cudaStream_t s) {
-  const size_t smem = (3 * kT * (HD + 1) + kT * (kT + 1)) * sizeof(float);
+                   const FwdArgs& a, cudaStream_t s) {
+  const CrossGeom& g = a.g;
+  constexpr int smem = FwdTile<HD>::kSmem;
   unsigned n;
-  if (magma_status_t st = cross_smem<cross_fwd<HD, T>>((int)smem)) return st;
-  if (magma_status_t st = blocks_of(ceil_div(g.q_len, kT), g.heads, g.batch, &n)) return st;
-  cross_fwd<HD, T><<<n, kThreads, smem, s>>>((const T*)q, (const T*)k, (const T*)v, (T*)o, lse, g);
+  if (magma_status_t st = cross_smem<cross_fwd<HD, T, VEC>>(smem)) return st;
+  if (magma_status_t st = blocks_of(row_tiles(g), g.kv_heads, g.batch, a.parts, &n)) return st;
+  cross_fwd<HD, T, VEC><<<n, 128, smem, s>>>((const T*)q, (const T*)k, (const T*)v, (T*)o, lse, a);
   return check_launch("cross_fwd");
 }
 
-template <int HD, typename T>
+template <int HD, typename T, bool VEC>
 magma_status_t bwd(const void* q, const void* k, const void* v, const void* o, const void* d_o,
                    const float* lse, void* dq, void* dk, void* dv, float* delta,
                    const CrossGeom& g, cudaStream_t s) {
-  const size_t kv_smem =
-      (4 * kT * (HD + 1) + 2 * kT * (kT + 1) + 2 * kT) * sizeof(float);
-  const size_t q_smem = (4 * kT * (HD + 1) + kT * (kT + 1)) * sizeof(float);
-  if (magma_status_t st = cross_smem<cross_dkdv<HD, T>>((int)kv_smem)) return st;
-  if (magma_status_t st = cross_smem<cross_dq<HD, T>>((int)q_smem)) return st;
+  if (magma_status_t st = cross_smem<cross_dkdv<HD, T, VEC>>(kDkvSmem<HD>)) return st;
+  if (magma_status_t st = cross_smem<cross_dq<HD, T, VEC>>(kDqSmem<HD>)) return st;
   unsigned nq = 0, nk = 0;
-  if (magma_status_t st = blocks_of(ceil_div(g.q_len, kT), g.heads, g.batch, &nq)) return st;
-  if (magma_status_t st = blocks_of(ceil_div(g.kv_len, kT), g.kv_heads, g.batch, &nk)) return st;
+  if (magma_status_t st = blocks_of(row_tiles(g), g.kv_heads, g.batch, 1, &nq)) return st;
+  if (magma_status_t st = blocks_of(ceil_div(g.kv_len, kRows), g.kv_heads, g.batch, 1, &nk)) return st;
   if (nq > 0) {
-    const int64_t rows = g.batch * g.heads * g.q_len;
     const int64_t cap = 16LL * num_sms();
-    const int64_t nd = ceil_div(rows, kThreads / 32);
-    cross_delta<T><<<(unsigned)(nd > cap ? cap : nd), kThreads, 0, s>>>((const T*)o, (const T*)d_o,
-                                                                     delta, g);
+    const int64_t nd = ceil_div(g.batch * g.heads * g.q_len, 8);
+    cross_delta<T><<<(unsigned)std::min(cap, nd), 256, 0, s>>>((const T*)o, (const T*)d_o, delta, g);
     if (magma_status_t st = check_launch("cross_delta")) return st;
   }
   if (nk > 0) {
-    cross_dkdv<HD, T><<<nk, kThreads, kv_smem, s>>>((const T*)q, (const T*)k, (const T*)v,
-                                                    (const T*)d_o, lse, delta, (T*)dk, (T*)dv, g);
+    cross_dkdv<HD, T, VEC><<<nk, 256, kDkvSmem<HD>, s>>>((const T*)q, (const T*)k, (const T*)v,
+                                                         (const T*)d_o, lse, delta, (T*)dk, (T*)dv, g);
     if (magma_status_t st = check_launch("cross_dkdv")) return st;
   }
   if (nq > 0) {
-    cross_dq<HD, T><<<nq, kThreads, q_smem, s>>>((const T*)q, (const T*)k, (const T*)v,
-                                                 (const T*)d_o, lse, delta, (T*)dq, g);
+    cross_dq<HD, T, VEC><<<nq, 256, kDqSmem<HD>, s>>>((const T*)q, (const T*)k, (const T*)v,
+                                                      (const T*)d_o, lse, delta, (T*)dq, g);
     return check_launch("cross_dq");
   }
   return MAGMA_OK;
 }
 
+// Parts of a source: as many as give every SM two CTAs, of at least four tiles.
+int64_t wanted_parts(const CrossGeom& g) {
+  const int64_t ctas = std::max<int64_t>(row_tiles(g) * g.kv_heads * g.batch, 1);
+  const int64_t tiles = ceil_div(g.kv_len, g.hd <= 64 ? 64 : 32);
+  return std::max<int64_t>(1, std::min<int64_t>(2LL * num_sms() / ctas, tiles / 4));
+}
+
 }  // namespace
 
+size_t cross_simt_fwd_workspace(const CrossGeom& g) {
+  const int64_t n = g.hd % 4 == 0 ? wanted_parts(g) : 1;
+  return n <= 1 ? 0 : (size_t)n * g.batch * g.heads * g.q_len * (g.hd + 1) * sizeof(float);
+}
+
 magma_status_t cross_fwd_simt(const void* q, const void* k, const void* v, void* o, float* lse,
-                              const CrossGeom& g, magma_dtype_t dtype, cudaStream_t s) {
+                              const CrossGeom& g, magma_dtype_t dtype, void* workspace,
+                              size_t workspace_bytes, cudaStream_t s) {
+  FwdArgs a{};
+  a.g = g;
+  a.parts = 1;
+  const int64_t rows = g.batch * g.heads * g.q_len;
+  const size_t each = (size_t)rows * (g.hd + 1) * sizeof(float);
+  const bool join_ok = g.hd % 4 == 0 && g.os[0] % 4 == 0 && g.os[1] % 4 == 0 && g.os[2] % 4 == 0 &&
+                       aligned16(o);
+  if (workspace != nullptr && aligned16(workspace) && join_ok)
+    a.parts = (int)std::max<int64_t>(1, std::min<int64_t>(wanted_parts(g), workspace_bytes / each));
+  if (a.parts > 1) {
+    a.part = static_cast<float*>(workspace);
+    a.part_lse = a.part + (size_t)a.parts * rows * g.hd;
+  }
+  const bool vec = dtype == MAGMA_DTYPE_F32 && g.hd % 4 == 0 && pieces(q, g.qs) &&
+                   pieces(k, g.ks) && pieces(v, g.vs);
+  magma_status_t st;
   if (dtype == MAGMA_DTYPE_F32)
-    return g.hd <= 64 ? fwd<64, float>(q, k, v, o, lse, g, s) : fwd<128, float>(q, k, v, o, lse, g, s);
-  return g.hd <= 64 ? fwd<64, __nv_bfloat16>(q, k, v, o, lse, g, s)
-                    : fwd<128, __nv_bfloat16>(q, k, v, o, lse, g, s);
+    st = g.hd <= 64 ? (vec ? fwd<64, float, true>(q, k, v, o, lse, a, s) : fwd<64, float, false>(q, k, v, o, lse, a, s))
+                    : (vec ? fwd<128, float, true>(q, k, v, o, lse, a, s) : fwd<128, float, false>(q, k, v, o, lse, a, s));
+  else
+    st = g.hd <= 64 ? fwd<64, __nv_bfloat16, false>(q, k, v, o, lse, a, s)
+                    : fwd<128, __nv_bfloat16, false>(q, k, v, o, lse, a, s);
+  if (st || a.parts == 1) return st;
+  return cross_join_parts(a.part, a.part_lse, o, lse, g, a.parts, dtype, s);
 }
 
 magma_status_t cross_bwd_simt(const void* q, const void* k, const void* v, const void* o,
                               const void* d_o, const float* lse, void* dq, void* dk, void* dv,
                               float* delta, const CrossGeom& g, magma_dtype_t dtype,
                               cudaStream_t s) {
+  const bool vec = dtype == MAGMA_DTYPE_F32 && g.hd % 4 == 0 && pieces(q, g.qs) &&
+                   pieces(k, g.ks) && pieces(v, g.vs) && pieces(d_o, g.dos);
   if (dtype == MAGMA_DTYPE_F32)
-    return g.hd <= 64 ? bwd<64, float>(q, k, v, o, d_o, lse, dq, dk, dv, delta, g, s)
-                      : bwd<128, float>(q, k, v, o, d_o, lse, dq, dk, dv, delta, g, s);
-  return g.hd <= 64 ? bwd<64, __nv_bfloat16>(q, k, v, o, d_o, lse, dq, dk, dv, delta, g, s)
-                    : bwd<128, __nv_bfloat16>(q, k, v, o, d_o, lse, dq, dk, dv, delta, g, s);
+    return g.hd <= 64 ? (vec ? bwd<64, float, true>(q, k, v, o, d_o, lse, dq, dk, dv, delta, g, s)
+                             : bwd<64, float, false>(q, k, v, o, d_o, lse, dq, dk, dv, delta, g, s))
+                      : (vec ? bwd<128, float, true>(q, k, v, o, d_o, lse, dq, dk, dv, delta, g, s)
+                             : bwd<128, float, false>(q, k, v, o, d_o, lse, dq, dk, dv, delta, g, s));
+  return g.hd <= 64 ? bwd<64, __nv_bfloat16, false>(q, k, v, o, d_o, lse, dq, dk, dv, delta, g, s)
+                    : bwd<128, __nv_bfloat16, false>(q, k, v, o, d_o, lse, dq, dk, dv, delta, g, s);
 }
 
 }  // namespace magma
