@@ -3,8 +3,8 @@
 // Each part holds a row's normalised O_s and lse_s. With M the largest lse_s,
 //   O = sum_s exp(lse_s - M) O_s / sum_s exp(lse_s - M),
 //   lse = M + log sum_s exp(lse_s - M).
-// A part without keys has lse -inf and is not read. One warp a row, four columns
-// a lane; the parts of a few rows come out of L2.
+// A part without keys has lse -inf and is not read. W warps a row (four for many
+// parts, whose reads would follow one another otherwise), four columns a lane.
 #include <cmath>
 
 #include "cross_attention.cuh"
@@ -12,33 +12,54 @@
 namespace magma {
 namespace {
 
-template <typename T>
-__global__ void __launch_bounds__(256)
+constexpr int kThreads = 256;
+constexpr int kManyParts = 8;
+
+template <typename T, int W>
+__global__ void __launch_bounds__(kThreads)
 cross_join(const float* __restrict__ part, const float* __restrict__ part_lse, T* __restrict__ o,
            float* __restrict__ lse, const CrossGeom g, int n_part) {
+  constexpr int kRows = kThreads / 32 / W;
+  __shared__ float4 sums[W > 1 ? kThreads : 1];
+  __shared__ float totals[W > 1 ? kThreads / 32 : 1];
   wait_for_launch_before();
-  const int lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, w = warp % W;
   const int64_t rows = g.batch * g.heads * g.q_len;
-  const int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (i >= rows) return;
+  const int64_t i = (int64_t)blockIdx.x * kRows + warp / W;
+  const bool row_on = i < rows;
   float m = -INFINITY;
-  for (int s = lane; s < n_part; s += 32) m = fmaxf(m, part_lse[s * rows + i]);
+  if (row_on)
+    for (int s = lane; s < n_part; s += 32) m = fmaxf(m, part_lse[s * rows + i]);
   m = warp_max(m);
   float total = 0.f;
   float acc[4] = {0.f, 0.f, 0.f, 0.f};
   const int c = lane * 4;
   if (m != -INFINITY) {
-#pragma unroll 4
-    for (int s = 0; s < n_part; ++s) {
-      const float w = expf(part_lse[s * rows + i] - m);
-      total += w;
+    const int s0 = n_part * w / W, s1 = n_part * (w + 1) / W;
+#pragma unroll 8
+    for (int s = s0; s < s1; ++s) {
+      const float f = expf(part_lse[s * rows + i] - m);
+      total += f;
       if (c >= g.hd) continue;
       float v[4];
       load4(part + (s * rows + i) * g.hd + c, v);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[e] = fmaf(w, v[e], acc[e]);
+      for (int e = 0; e < 4; ++e) acc[e] = fmaf(f, v[e], acc[e]);
     }
   }
+  if constexpr (W > 1) {
+    sums[threadIdx.x] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+    if (lane == 0) totals[warp] = total;
+    __syncthreads();
+    if (w != 0) return;
+#pragma unroll
+    for (int x = 1; x < W; ++x) {
+      const float4 v = sums[threadIdx.x + 32 * x];
+      acc[0] += v.x, acc[1] += v.y, acc[2] += v.z, acc[3] += v.w;
+      total += totals[warp + x];
+    }
+  }
+  if (!row_on) return;
   const float inv = total == 0.f ? 0.f : 1.f / total;
   const int64_t q = i % g.q_len, bh = i / g.q_len, h = bh % g.heads, b = bh / g.heads;
   if (c < g.hd) {
@@ -49,17 +70,23 @@ cross_join(const float* __restrict__ part, const float* __restrict__ part_lse, T
   if (lane == 0 && lse != nullptr) lse[i] = total == 0.f ? -INFINITY : m + logf(total);
 }
 
+template <typename T>
+magma_status_t join(const float* part, const float* part_lse, void* o, float* lse,
+                    const CrossGeom& g, int n_part, cudaStream_t s) {
+  const int64_t rows = g.batch * g.heads * g.q_len;
+  const bool many = n_part > kManyParts;
+  const unsigned blocks = (unsigned)ceil_div(rows, many ? 2 : 8);
+  return launch_after(many ? cross_join<T, 4> : cross_join<T, 1>, dim3(blocks), kThreads, 0, s,
+                      "cross_join", part, part_lse, static_cast<T*>(o), lse, g, n_part);
+}
+
 }  // namespace
 
 magma_status_t cross_join_parts(const float* part, const float* part_lse, void* o, float* lse,
                                 const CrossGeom& g, int n_part, magma_dtype_t dtype,
                                 cudaStream_t s) {
-  const unsigned blocks = (unsigned)ceil_div(g.batch * g.heads * g.q_len, 8);
-  if (dtype == MAGMA_DTYPE_F32)
-    return launch_after(cross_join<float>, dim3(blocks), 256, 0, s, "cross_join", part, part_lse,
-                        static_cast<float*>(o), lse, g, n_part);
-  return launch_after(cross_join<__nv_bfloat16>, dim3(blocks), 256, 0, s, "cross_join", part, part_lse,
-                      static_cast<__nv_bfloat16*>(o), lse, g, n_part);
+  return dtype == MAGMA_DTYPE_F32 ? join<float>(part, part_lse, o, lse, g, n_part, s)
+                                  : join<__nv_bfloat16>(part, part_lse, o, lse, g, n_part, s);
 }
 
 }  // namespace magma

@@ -581,11 +581,12 @@ magma_status_t bwd(const void* q, const void* k, const void* v, const void* o, c
   return MAGMA_OK;
 }
 
-// Parts of a source: as many as give every SM two CTAs, of at least four tiles.
+// Parts of a source: as many as give every SM six CTAs, two rounds of those that
+// run at once, so that lengths that differ even out; of at least two tiles.
 int64_t wanted_parts(const CrossGeom& g) {
   const int64_t ctas = std::max<int64_t>(row_tiles(g) * g.kv_heads * g.batch, 1);
   const int64_t tiles = ceil_div(g.kv_len, g.hd <= 64 ? 64 : 32);
-  return std::max<int64_t>(1, std::min<int64_t>(2LL * num_sms() / ctas, tiles / 4));
+  return std::max<int64_t>(1, std::min<int64_t>(6LL * num_sms() / ctas, tiles / 2));
 }
 
 }  // namespace

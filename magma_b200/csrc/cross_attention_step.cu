@@ -4,16 +4,16 @@
 // The work is one read of K and V (4 flops per byte and query row), so the
 // source is cut into chunks, a CTA takes one chunk of one key head with all
 // query rows that read it (row = shared head * q_len + query), and the parts
-// are joined by their log-sum-exp (cross_join_parts). Tiles of K and V stream
-// through a cp.async ring; keys from the length on are filled with zeros there,
-// so what lies behind a length is never read.
+// are joined by their log-sum-exp (cross_join_parts). Keys from the length on
+// are filled with zeros: what lies behind a length is never read.
 //
 //   cross_step_bf16  warp-level MMA (m16n8k16): WM x (4 / WM) warps over rows
 //                    and keys, each with its own running maximum and sum. The
 //                    16-row tile holds one query of up to 16 heads; the tcgen05
 //                    tile of 128 rows would be empty, and the products are not
-//                    what bounds this.
-//   cross_step_f32   FMA pipe: scores by key, sums by column.
+//                    what bounds this. K and V tiles come through a cp.async ring.
+//   cross_step_f32   FMA pipe: scores by key, sums by column, four warps over
+//                    the keys.
 #include <cmath>
 
 #include <algorithm>
@@ -34,6 +34,7 @@ constexpr float kLn2 = 0.6931471805599453f;
 struct StepArgs {
   CrossGeom g;
   int rows;             // shared heads * q_len
+  int groups, each;     // CTAs that share a chunk's rows, rows of one of them
   int n_chunk;          // chunks of the longest source
   int64_t chunk;        // keys of a chunk, a multiple of the tile
   void* o;
@@ -42,14 +43,16 @@ struct StepArgs {
   float* part_lse;      // [chunk][b][h][q], natural logarithm
 };
 
-// One CTA's chunk: sequence, key head, keys [k0, k1).
+// One CTA's chunk: sequence, key head, keys [k0, k1), first of its query rows.
 struct Chunk {
   int64_t b, kvh, k0, k1;
-  int index;
+  int index, r0;
 };
 __device__ __forceinline__ Chunk chunk_of(const StepArgs& a) {
   Chunk c;
-  const int64_t i = blockIdx.x;
+  int64_t i = blockIdx.x;
+  c.r0 = (int)(i % a.groups) * a.each;
+  i /= a.groups;
   c.index = (int)(i % a.n_chunk);
   c.kvh = i / a.n_chunk % a.g.kv_heads;
   c.b = i / a.n_chunk / a.g.kv_heads;
@@ -324,150 +327,155 @@ cross_step_bf16(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __rest
 }
 
 // ----------------------------------------------------------------- F32
-constexpr int kF32Keys = 32;
+// A warp takes groups of eight keys straight from memory into registers (no
+// value of K or V is used by two warps) and has its own maximum and sum, so the
+// warps run free of one another. Scores: lane = (key, every fourth 16-byte piece
+// of d); the next group's K is on its way under the sums, its V under the next
+// scores. Sums: lane = four columns, of every key (head size 128) or of every
+// second one (64).
+constexpr int kF32Keys = 32;  // keys of the four warps' groups
 
-template <int HD>
-struct Ff {
-  static constexpr int kStages = 2;
-  static constexpr int kPitch = HD + 4;  // floats: rows a quarter-warp reads lie in other banks
-  static constexpr int kTile = kF32Keys * kPitch * 4;
-  static constexpr int kRing = kStages * 2 * kTile;
-};
-
-// RT rows (shared heads x queries). Scores: warp = row modulo 4, lane = key.
-// Sums: thread = column (and, head size 64, half of the keys).
 template <int HD, int RT>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, RT == 8 ? 3 : HD == 128 ? 4 : 5)
 cross_step_f32(const float* __restrict__ q, const float* __restrict__ k,
                const float* __restrict__ v, const __grid_constant__ StepArgs a) {
-  using F = Ff<HD>;
-  constexpr int kHalves = kThreads / HD;  // threads that share a column
+  constexpr int kPieces = HD / 16;         // of a lane's share of a K row
+  constexpr int kHalves = 128 / HD;        // keys that a V load covers
+  constexpr int kLoads = 8 / kHalves;      // V loads of a group
   constexpr int kVec = HD / 4;
-  extern __shared__ __align__(128) uint8_t sm[];
-  const uint32_t base = smem_u32(sm);
-  float* qs = reinterpret_cast<float*>(sm + F::kRing);  // [RT][HD], times scale log2(e)
-  float* ps = qs + RT * HD;                             // [key][RT]
-  float* as = ps + kF32Keys * RT;                       // [RT] this tile's rescaling
+  __shared__ float sh[4 * RT * HD];        // q, at the end the warps' sums
+  __shared__ float2 sml[4 * RT];
   const CrossGeom& g = a.g;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int kk = lane >> 2, part = lane & 3;
+  const int vk = lane / kVec, vcol = lane % kVec * 4;  // key of a pair, first column
   const Chunk c = chunk_of(a);
-  const int tiles = (int)((c.k1 - c.k0 + kF32Keys - 1) / kF32Keys);
-  const float* kh = k + c.b * g.ks[0] + c.kvh * g.ks[1];
-  const float* vh = v + c.b * g.vs[0] + c.kvh * g.vs[1];
-  auto load = [&](int j) {
-    const uint32_t dst = base + (j % F::kStages) * 2 * F::kTile;
-    const int64_t kj = c.k0 + (int64_t)j * kF32Keys;
+  const int keys = (int)(c.k1 - c.k0), groups = (keys + 7) / 8;
+  const float* kh = k + c.b * g.ks[0] + c.kvh * g.ks[1] + c.k0 * g.ks[2];
+  const float* vh = v + c.b * g.vs[0] + c.kvh * g.vs[1] + c.k0 * g.vs[2];
+  const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+  float4 kx[kPieces], vx[kLoads];
+  auto load_k = [&](int grp) {
+    const int key = grp * 8 + kk;
+    const float* src = kh + key * g.ks[2];
 #pragma unroll
-    for (int i = 0; i < kF32Keys * kVec / kThreads; ++i) {
-      const int x = tid + i * kThreads, r = x / kVec, col = x % kVec * 4;
-      const bool on = col < g.hd && kj + r < c.k1;
-      const int64_t at = on ? kj + r : c.k0;
-      const uint32_t o = (r * F::kPitch + col) * 4;
-      cp_async16(dst + o, kh + at * g.ks[2] + (on ? col : 0), on);
-      cp_async16(dst + F::kTile + o, vh + at * g.vs[2] + (on ? col : 0), on);
+    for (int i = 0; i < kPieces; ++i) {
+      const int d = (part + 4 * i) * 4;
+      kx[i] = key < keys && d < g.hd ? __ldg(reinterpret_cast<const float4*>(src + d)) : zero;
     }
   };
-  if (tiles > 0) load(0);
-  cp_commit();
+  auto load_v = [&](int grp) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int key = grp * 8 + i * kHalves + vk;
+      vx[i] = key < keys && vcol < g.hd
+                  ? __ldg(reinterpret_cast<const float4*>(vh + key * g.vs[2] + vcol)) : zero;
+    }
+  };
+  if (warp < groups) {
+    load_k(warp);
+    load_v(warp);
+  }
   for (int i = tid; i < RT * HD; i += kThreads) {
     const int r = i / HD, col = i % HD;
     float x = 0.f;
-    if (r < a.rows && col < g.hd) {
+    if (c.r0 + r < a.rows && col < g.hd) {
       int64_t h, qi;
-      row_at(g, c, r, &h, &qi);
+      row_at(g, c, c.r0 + r, &h, &qi);
       x = q[c.b * g.qs[0] + h * g.qs[1] + qi * g.qs[2] + col];
     }
-    qs[i] = x;
+    sh[i] = x;
   }
-  constexpr int RW = (RT + 3) / 4;  // rows of a warp
-  float m[RW], l[RW], acc[RT];
-#pragma unroll
-  for (int i = 0; i < RW; ++i) m[i] = -INFINITY, l[i] = 0.f;
-#pragma unroll
-  for (int r = 0; r < RT; ++r) acc[r] = 0.f;
-  const int col = tid % HD, half = tid / HD;
-  for (int j = 0; j < tiles; ++j) {
-    if (j + 1 < tiles) load(j + 1);
-    cp_commit();
-    cp_wait<1>();
-    __syncthreads();
-    const float* sk = reinterpret_cast<const float*>(sm + (j % F::kStages) * 2 * F::kTile);
-    const float* sv = sk + F::kTile / 4;
-    const int left = (int)(c.k1 - c.k0 - (int64_t)j * kF32Keys);
-    float s[RW];
-#pragma unroll
-    for (int i = 0; i < RW; ++i) s[i] = 0.f;
-#pragma unroll 8
-    for (int d = 0; d < HD; d += 4) {
-      const float4 x = *reinterpret_cast<const float4*>(sk + lane * F::kPitch + d);
-#pragma unroll
-      for (int i = 0; i < RW; ++i) {
-        const int r = warp + 4 * i;
-        if (r >= RT) continue;
-        const float4 y = *reinterpret_cast<const float4*>(qs + r * HD + d);
-        s[i] = fmaf(x.x, y.x, s[i]);
-        s[i] = fmaf(x.y, y.y, s[i]);
-        s[i] = fmaf(x.z, y.z, s[i]);
-        s[i] = fmaf(x.w, y.w, s[i]);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < RW; ++i) {
-      const int r = warp + 4 * i;
-      if (r >= RT) continue;
-      const float x = lane < left ? s[i] * g.scale : -INFINITY;
-      const float mn = fmaxf(m[i], warp_max(x));
-      const float ref = mn == -INFINITY ? 0.f : mn;
-      const float p = expf(x - ref), alpha = expf(m[i] - ref);
-      m[i] = mn;
-      l[i] = l[i] * alpha + warp_sum(p);
-      ps[lane * RT + r] = p;
-      if (lane == 0) as[r] = alpha;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int r = 0; r < RT; ++r) acc[r] *= as[r];
-    constexpr int KH = kF32Keys / kHalves;
-#pragma unroll 8
-    for (int i = 0; i < KH; ++i) {
-      const int key = half * KH + i;
-      const float x = sv[key * F::kPitch + col];
-#pragma unroll
-      for (int r = 0; r < RT; r += 4) {
-        const float4 p = *reinterpret_cast<const float4*>(ps + key * RT + r);
-        acc[r] = fmaf(p.x, x, acc[r]);
-        acc[r + 1] = fmaf(p.y, x, acc[r + 1]);
-        acc[r + 2] = fmaf(p.z, x, acc[r + 2]);
-        acc[r + 3] = fmaf(p.w, x, acc[r + 3]);
-      }
-    }
-    __syncthreads();
-  }
-  cp_wait<0>();
   __syncthreads();
-  float* so = reinterpret_cast<float*>(sm);  // [half][RT][HD]
+  float m[RT], l[RT], acc[RT][4];
 #pragma unroll
-  for (int r = 0; r < RT; ++r) so[(half * RT + r) * HD + col] = acc[r];
-  float2* sml = reinterpret_cast<float2*>(ps);
+  for (int r = 0; r < RT; ++r) {
+    m[r] = -INFINITY;
+    l[r] = 0.f;
 #pragma unroll
-  for (int i = 0; i < RW; ++i)
-    if (lane == 0 && warp + 4 * i < RT) sml[warp + 4 * i] = make_float2(m[i], l[i]);
+    for (int e = 0; e < 4; ++e) acc[r][e] = 0.f;
+  }
+  for (int grp = warp; grp < groups; grp += 4) {
+    const int left = keys - grp * 8;
+    float s[RT];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) s[r] = 0.f;
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i)
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        const float4 y = *reinterpret_cast<const float4*>(sh + r * HD + (part + 4 * i) * 4);
+        s[r] = fmaf(kx[i].x, y.x, s[r]);
+        s[r] = fmaf(kx[i].y, y.y, s[r]);
+        s[r] = fmaf(kx[i].z, y.z, s[r]);
+        s[r] = fmaf(kx[i].w, y.w, s[r]);
+      }
+    if (grp + 4 < groups) load_k(grp + 4);
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      s[r] += __shfl_xor_sync(0xffffffffu, s[r], 1);
+      s[r] += __shfl_xor_sync(0xffffffffu, s[r], 2);
+    }
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      const float x = kk < left ? s[r] * g.scale : -INFINITY;
+      float mx = x;
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      const float mn = fmaxf(m[r], mx);
+      const float ref = mn == -INFINITY ? 0.f : mn;
+      const float alpha = expf(m[r] - ref);
+      m[r] = mn;
+      s[r] = expf(x - ref);
+      l[r] = l[r] * alpha + s[r];  // the lane's key; a key's four lanes hold the same
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[r][e] *= alpha;
+    }
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i)
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        const float p = __shfl_sync(0xffffffffu, s[r], (i * kHalves + vk) * 4);
+        acc[r][0] = fmaf(p, vx[i].x, acc[r][0]);
+        acc[r][1] = fmaf(p, vx[i].y, acc[r][1]);
+        acc[r][2] = fmaf(p, vx[i].z, acc[r][2]);
+        acc[r][3] = fmaf(p, vx[i].w, acc[r][3]);
+      }
+    if (grp + 4 < groups) load_v(grp + 4);
+  }
+  __syncthreads();  // q has been used
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], o);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (kHalves == 2) acc[r][e] += __shfl_xor_sync(0xffffffffu, acc[r][e], 16);
+    if (vk == 0) store4(sh + (warp * RT + r) * HD + vcol, acc[r]);
+    if (lane == 0) sml[warp * RT + r] = make_float2(m[r], l[r]);
+  }
   __syncthreads();
   for (int i = tid; i < RT * kVec; i += kThreads) {
     const int r = i / kVec, d = i % kVec * 4;
-    if (r >= a.rows || d >= g.hd) continue;
-    const float2 ml = sml[r];
-    const float inv = ml.y == 0.f ? 0.f : 1.f / ml.y;
-    float o[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int hh = 0; hh < kHalves; ++hh) {
-      float x[4];
-      load4(so + (hh * RT + r) * HD + d, x);
+    if (c.r0 + r >= a.rows || d >= g.hd) continue;
+    float mm = -INFINITY;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] += x[e];
+    for (int w = 0; w < 4; ++w) mm = fmaxf(mm, sml[w * RT + r].x);
+    float total = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float2 ml = sml[w * RT + r];
+      const float f = mm == -INFINITY ? 0.f : expf(ml.x - mm);
+      total += f * ml.y;
+      float x[4];
+      load4(sh + (w * RT + r) * HD + d, x);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = fmaf(f, x[e], o[e]);
     }
+    const float inv = total == 0.f ? 0.f : 1.f / total;
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] *= inv;
-    store_part<float>(a, c, r, d, o, ml.y == 0.f ? -INFINITY : ml.x + logf(ml.y));
+    store_part<float>(a, c, c.r0 + r, d, o, total == 0.f ? -INFINITY : mm + logf(total));
   }
 }
 
@@ -478,13 +486,25 @@ bool step_aligned(const void* p, const int64_t (&st)[3], int64_t per16) {
 
 int64_t tile_keys(magma_dtype_t dtype) { return dtype == MAGMA_DTYPE_F32 ? kF32Keys : kKeys; }
 
-// Keys of a chunk: about eight CTAs' worth of chunks per SM, so that lengths that
-// differ even out, but no more chunks than that, since each costs a part.
+// Rows of a CTA: F32 rows beyond eight go to further CTAs, which read the chunk
+// again out of L2 (16 rows in one CTA took half again as long: a thread's sums
+// leave no room for enough CTAs to cover the loads).
+int rows_each(const CrossGeom& g, magma_dtype_t dtype) {
+  const int64_t rows = (int64_t)g.group * g.q_len;
+  return dtype == MAGMA_DTYPE_F32 ? (rows <= 4 ? 4 : 8) : (int)rows;
+}
+
+// Keys of a chunk: sixteen CTAs per SM, so that lengths that differ even out, but
+// chunks below 256 keys only where there are not six CTAs per SM: each chunk costs
+// a part and its share of the join.
 int64_t chunk_keys(const CrossGeom& g, magma_dtype_t dtype) {
   const int64_t tile = tile_keys(dtype);
-  const int64_t heads = g.batch * g.kv_heads;
-  const int64_t want = std::max<int64_t>(1, 8LL * num_sms() / heads);
-  return std::max<int64_t>(1, ceil_div(g.kv_len, want * tile)) * tile;
+  const int64_t heads =
+      g.batch * g.kv_heads * ceil_div((int64_t)g.group * g.q_len, rows_each(g, dtype));
+  const int64_t many = ceil_div(g.kv_len * heads, 16LL * num_sms());
+  const int64_t few = ceil_div(g.kv_len * heads, 6LL * num_sms());
+  const int64_t keys = std::max(many, std::min<int64_t>(256, few));
+  return ceil_div(keys, tile) * tile;
 }
 
 template <int HD, int WM>
@@ -501,9 +521,7 @@ magma_status_t launch_bf16(const void* q, const void* k, const void* v, const St
 template <int HD, int RT>
 magma_status_t launch_f32(const void* q, const void* k, const void* v, const StepArgs& a,
                           unsigned ctas, cudaStream_t s) {
-  const int smem = Ff<HD>::kRing + (RT * HD + kF32Keys * RT + RT) * 4;
-  if (magma_status_t st = cross_smem<cross_step_f32<HD, RT>>(smem)) return st;
-  cross_step_f32<HD, RT><<<ctas, kThreads, smem, s>>>(
+  cross_step_f32<HD, RT><<<ctas, kThreads, 0, s>>>(
       static_cast<const float*>(q), static_cast<const float*>(k), static_cast<const float*>(v), a);
   return check_launch("cross_step_f32");
 }
@@ -521,7 +539,7 @@ bool cross_step_rows(const CrossGeom& g, magma_dtype_t dtype) {
   const int64_t rows = (int64_t)g.group * g.q_len;
   const bool f32 = dtype == MAGMA_DTYPE_F32;
   return rows >= 1 && rows <= (f32 ? 16 : 64) && g.kv_len > 0 && g.hd % (f32 ? 4 : 8) == 0 &&
-         g.batch * g.kv_heads * (8LL * num_sms() + 1) < (1LL << 31);
+         g.batch * g.kv_heads * 64 * ceil_div(g.kv_len, 32) < (1LL << 31);
 }
 
 size_t cross_step_workspace(const CrossGeom& g, magma_dtype_t dtype) {
@@ -535,6 +553,8 @@ magma_status_t cross_step_run(const void* q, const void* k, const void* v, void*
   StepArgs a{};
   a.g = g;
   a.rows = (int)(g.group * g.q_len);
+  a.each = rows_each(g, dtype);
+  a.groups = (int)ceil_div(a.rows, a.each);
   a.o = o;
   a.lse = lse;
   const int64_t tile = tile_keys(dtype);
@@ -549,12 +569,12 @@ magma_status_t cross_step_run(const void* q, const void* k, const void* v, void*
     a.part = static_cast<float*>(workspace);
     a.part_lse = a.part + (size_t)a.n_chunk * rows * g.hd;
   }
-  const unsigned ctas = (unsigned)(a.n_chunk * g.kv_heads * g.batch);
+  const unsigned ctas = (unsigned)(a.groups * a.n_chunk * g.kv_heads * g.batch);
   magma_status_t st;
   if (dtype == MAGMA_DTYPE_F32) {
     const bool few = a.rows <= 4;
-    st = g.hd <= 64 ? (few ? launch_f32<64, 4>(q, k, v, a, ctas, s) : launch_f32<64, 16>(q, k, v, a, ctas, s))
-                    : (few ? launch_f32<128, 4>(q, k, v, a, ctas, s) : launch_f32<128, 16>(q, k, v, a, ctas, s));
+    st = g.hd <= 64 ? (few ? launch_f32<64, 4>(q, k, v, a, ctas, s) : launch_f32<64, 8>(q, k, v, a, ctas, s))
+                    : (few ? launch_f32<128, 4>(q, k, v, a, ctas, s) : launch_f32<128, 8>(q, k, v, a, ctas, s));
   } else {
     auto* run = g.hd <= 64 ? (a.rows <= 16 ? launch_bf16<64, 1> : a.rows <= 32 ? launch_bf16<64, 2> : launch_bf16<64, 4>)
                            : (a.rows <= 16 ? launch_bf16<128, 1> : a.rows <= 32 ? launch_bf16<128, 2> : launch_bf16<128, 4>);
