@@ -61,6 +61,7 @@ struct TcArgs {
   float* part_lse;          // [split][b][h][q]
   const float* nlse;        // [b][h][q_pad], -lse log2(e)
   const float* delta;
+  float* piece;             // partial sums of units that several CTAs share, or NULL
   void* dq;
   void* dk;
   void* dv;
@@ -157,6 +158,48 @@ __device__ __forceinline__ void zero_cols(__nv_bfloat16* dst, int hd) {
   for (int c = 0; c < hd; c += 8) *reinterpret_cast<uint4*>(dst + c) = make_uint4(0, 0, 0, 0);
 }
 
+// ------------------------------------------------------- steps dealt out evenly
+// Where whole units would leave many CTAs idle at the end, the gradient's steps
+// (a unit's key or query tiles) are dealt out instead: CTA c of G takes steps
+// [T c / G, T (c + 1) / G) of T. A unit that a border cuts is added up in pieces:
+// every CTA stores the F32 sums of the first and the last unit of its range if it
+// has them in part (slots 0 and 1), and a second kernel adds a unit's pieces in
+// the order of the CTAs.
+__device__ __forceinline__ int64_t border(int64_t total, int64_t c, int64_t ctas) {
+  return total * c / ctas;
+}
+// 128 rows of HD F32 sums, two of them for each slot.
+template <int HD>
+__device__ __forceinline__ float* piece_rows(const TcArgs& a, int64_t cta, int slot, int t) {
+  return a.piece + ((cta * 2 + slot) * 2 + t) * (int64_t)kRows * HD;
+}
+template <int HD>
+__device__ __forceinline__ void store_piece32(float* row, const uint32_t (&v)[32]) {
+#pragma unroll
+  for (int q = 0; q < 8; ++q)
+    reinterpret_cast<uint4*>(row)[q] = make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+}
+// The unit of steps [begin, begin + n) that border c cuts: the sum over its
+// pieces of row `row`, columns [col, col + 4). Slot 0 of a CTA whose range begins
+// in the unit, slot 1 of the one whose range ends in it.
+template <int HD>
+__device__ __forceinline__ float4 sum_pieces(const TcArgs& a, int64_t total, int64_t ctas, int64_t c,
+                                             int64_t begin, int64_t n, int t, int row, int col) {
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int64_t i = c - 1; i < ctas && border(total, i, ctas) < begin + n; ++i) {
+    if (border(total, i, ctas) == border(total, i + 1, ctas)) continue;  // nothing of its own
+    const int slot = border(total, i, ctas) >= begin ? 0 : 1;
+    const float4 v = *reinterpret_cast<const float4*>(
+        piece_rows<HD>(a, i, slot, t) + (int64_t)row * HD + col);
+    s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+  }
+  return s;
+}
+__device__ __forceinline__ void store_grad4(__nv_bfloat16* dst, float4 v, float mul) {
+  const float x[4] = {v.x * mul, v.y * mul, v.z * mul, v.w * mul};
+  store4(dst, x);
+}
+
 // A pair of (head, query tile) items that read the same key head: items 2p and
 // 2p + 1 of the heads' query tiles in order.
 struct PairUnit {
@@ -176,17 +219,13 @@ __device__ __forceinline__ int tile_of(const TcArgs& a, const PairUnit& w, int t
 }
 
 template <int KT>
-__device__ __forceinline__ PairUnit pair_unit(const TcArgs& a, const uint16_t* order, int64_t u) {
+__device__ __forceinline__ PairUnit pair_of(const TcArgs& a, int64_t b, int64_t kvh, int split,
+                                            int p) {
   const CrossGeom& g = a.g;
   PairUnit w;
-  const int64_t per_head = (int64_t)a.n_pairs * a.n_split;
-  const int64_t per_seq = per_head * g.kv_heads;
-  w.b = sequence_of(g, order, u / per_seq);
-  const int64_t rest = u % per_seq;
-  w.kvh = (int)(rest / per_head);
-  const int x = (int)(rest % per_head);
-  w.split = x / a.n_pairs;
-  const int p = x % a.n_pairs;
+  w.b = b;
+  w.kvh = (int)kvh;
+  w.split = split;
   const int all = g.group * a.n_qt;
   w.first = 2 * p;
   w.items = 2 * p + 1 < all ? 2 : 1;
@@ -196,6 +235,15 @@ __device__ __forceinline__ PairUnit pair_unit(const TcArgs& a, const uint16_t* o
   w.t0 = w.split * each < tiles ? w.split * each : tiles;
   w.n = tiles - w.t0 < each ? tiles - w.t0 : each;
   return w;
+}
+template <int KT>
+__device__ __forceinline__ PairUnit pair_unit(const TcArgs& a, const uint16_t* order, int64_t u) {
+  const int64_t per_head = (int64_t)a.n_pairs * a.n_split;
+  const int64_t per_seq = per_head * a.g.kv_heads;
+  const int64_t rest = u % per_seq;
+  const int x = (int)(rest % per_head);
+  return pair_of<KT>(a, sequence_of(a.g, order, u / per_seq), rest / per_head, x / a.n_pairs,
+                     x % a.n_pairs);
 }
 
 // =============================================================== forward
@@ -664,6 +712,107 @@ __device__ __forceinline__ void grads32(const uint32_t (&p)[32], const uint32_t 
 // As the forward kernel, over 64-key tiles: S_t, dP_t = dO_t V_j^T; dS_t as BF16
 // pairs in S_t's columns is the A operand of dQ_t += dS_t K_j. TMEM columns of
 // tile t from 256 t: S, dP, dQ.
+constexpr int kDealt = 128;  // most sequences of a table of steps
+
+// Steps of the pairs of all sequences: first[b] of the sequences before b. One
+// warp fills the table; without lengths every sequence has as many.
+__device__ __forceinline__ void step_table(const TcArgs& a, int keys, int64_t* first) {
+  const CrossGeom& g = a.g;
+  const int lane = threadIdx.x & 31;
+  const int64_t pairs = (int64_t)a.n_pairs * g.kv_heads;
+  int64_t sum = 0;
+  for (int64_t i0 = 0; i0 < g.batch; i0 += 32) {
+    const int64_t i = i0 + lane;
+    const int64_t n = i < g.batch ? (cross_len(g, i) + keys - 1) / keys * pairs : 0;
+    int64_t inc = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t x = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += x;
+    }
+    if (i < g.batch) first[i] = sum + inc - n;
+    sum += __shfl_sync(0xffffffffu, inc, 31);
+  }
+  if (lane == 0) first[g.batch] = sum;
+}
+
+// Where step s of all lies: its sequence, the pair, the key tile in the pair.
+struct StepAt {
+  int64_t b, pair, n;  // n: key tiles of the sequence
+  int j;
+};
+__device__ __forceinline__ StepAt step_at(const TcArgs& a, int keys, const int64_t* first, int64_t s) {
+  const CrossGeom& g = a.g;
+  StepAt x;
+  int64_t rest;
+  if (g.lens != nullptr) {
+    int64_t lo = 0, hi = g.batch;  // first[lo] <= s < first[hi]
+    while (hi - lo > 1) {
+      const int64_t mid = (lo + hi) >> 1;
+      if (first[mid] <= s) lo = mid;
+      else hi = mid;
+    }
+    x.b = lo;
+    x.n = (cross_len(g, lo) + keys - 1) / keys;
+    rest = s - first[lo];
+  } else {
+    x.n = (g.kv_len + keys - 1) / keys;
+    const int64_t per = x.n * a.n_pairs * g.kv_heads;
+    x.b = s / per;
+    rest = s % per;
+  }
+  x.pair = rest / x.n;
+  x.j = (int)(rest % x.n);
+  return x;
+}
+__device__ __forceinline__ int64_t steps_of_all(const TcArgs& a, int keys, const int64_t* first) {
+  const CrossGeom& g = a.g;
+  return g.lens != nullptr
+             ? first[g.batch]
+             : (g.kv_len + keys - 1) / keys * a.n_pairs * g.kv_heads * g.batch;
+}
+
+// A CTA's way through its work: whole units in a snake, or its range of steps.
+struct DqWalk {
+  int64_t r = 0, s = 0, end = 0;
+};
+struct DqUnit : PairUnit {
+  int j0, j1, slot;  // key tiles [j0, j1); slot of the partial sums, -1: the unit is whole
+};
+template <int KT>
+__device__ __forceinline__ bool dq_next(const TcArgs& a, const uint16_t* order, const int64_t* first,
+                                        int64_t total, DqWalk& k, DqUnit& w) {
+  const CrossGeom& g = a.g;
+  if (a.piece == nullptr) {
+    const int64_t u = snake(k.r, (int)blockIdx.x, (int)gridDim.x,
+                            (int64_t)a.n_pairs * g.kv_heads * g.batch);
+    if (u < 0) return false;
+    ++k.r;
+    static_cast<PairUnit&>(w) = pair_unit<KT>(a, order, u);
+    w.j0 = 0;
+    w.j1 = w.n;
+    w.slot = -1;
+    return true;
+  }
+  if (k.r == 0) {
+    k.r = 1;
+    k.s = border(total, blockIdx.x, gridDim.x);
+    k.end = border(total, blockIdx.x + 1, gridDim.x);
+  }
+  if (k.s >= k.end) return false;
+  const StepAt x = step_at(a, KT, first, k.s);
+  // pair_unit's numbering with the sequence in its natural place
+  static_cast<PairUnit&>(w) =
+      pair_of<KT>(a, x.b, x.pair / a.n_pairs, 0, (int)(x.pair % a.n_pairs));
+  w.j0 = x.j;
+  const int64_t stop = x.j + (k.end - k.s);
+  w.j1 = (int)(stop < x.n ? stop : x.n);
+  const bool first_piece = k.s == border(total, blockIdx.x, gridDim.x);
+  w.slot = w.j1 - w.j0 == x.n ? -1 : first_piece ? 0 : 1;
+  k.s += w.j1 - w.j0;
+  return true;
+}
+
 template <int HD>
 struct Dq {
   static constexpr int kKeys = 64;
@@ -705,11 +854,12 @@ cross_dq_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
   const uint32_t done_bar = sbars + 64u;
   const uint32_t tslot = bars + 8u * F::kBars;
   uint32_t* tslot_ptr = reinterpret_cast<uint32_t*>(sp + F::kBar + 8 * F::kBars);
+  // the order of the sequences, or the table of their steps
   uint16_t* order = reinterpret_cast<uint16_t*>(sp + F::kOrd);
+  int64_t* first = reinterpret_cast<int64_t*>(sp + F::kOrd);
 
   const CrossGeom& g = a.g;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t units = (int64_t)a.n_pairs * g.kv_heads * g.batch;
   const int ctas = (int)gridDim.x, cta = (int)blockIdx.x;
 
   if (threadIdx.x == 0) {
@@ -724,11 +874,13 @@ cross_dq_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
     fence_barrier_init();
   }
   if (warp == kMmaWarp) tmem_alloc(tslot, 512);
-  order_by_length(g, order);
+  if (a.piece == nullptr) order_by_length(g, order);
+  else if (g.lens != nullptr && warp == 0) step_table(a, F::kKeys, first);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tslot_ptr);
+  const int64_t total = a.piece == nullptr ? 0 : steps_of_all(a, F::kKeys, first);
   auto tS = [&](int t) { return tmem + 256u * t; };
   auto tDp = [&](int t) { return tmem + 256u * t + 64u; };
   auto tDq = [&](int t) { return tmem + 256u * t + 128u; };
@@ -737,10 +889,9 @@ cross_dq_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
     if (elect_one()) {
       bool ok = true;
       int gk = 0, ru = 0;
-      for (int64_t r = 0; ok; ++r) {
-        const int64_t u = snake(r, cta, ctas, units);
-        if (u < 0) break;
-        const PairUnit w = pair_unit<F::kKeys>(a, order, u);
+      DqWalk walk;
+      DqUnit w;
+      while (ok && dq_next<F::kKeys>(a, order, first, total, walk, w)) {
         if (w.n <= 0) continue;
         if (!mbar_wait(q_empty, (uint32_t)((ru & 1) ^ 1), g.err)) break;
         mbar_expect_tx(q_full, w.items * 2 * F::kTile);
@@ -750,7 +901,7 @@ cross_dq_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
             tma_load_4d(sQ(t) + c * kBlk128, &tmQ, c * 64, row, h * a.qh, (int)w.b * a.qb, q_full);
             tma_load_4d(sG(t) + c * kBlk128, &tmG, c * 64, row, h * a.dh, (int)w.b * a.db, q_full);
           }
-        for (int j = 0; j < w.n; ++j, ++gk) {
+        for (int j = w.j0; j < w.j1; ++j, ++gk) {
           const int st = gk % F::kStages, row = j * F::kKeys;
           if (!mbar_wait(kv_empty(st), (uint32_t)(((gk / F::kStages) & 1) ^ 1), g.err)) {
             ok = false;
@@ -818,10 +969,9 @@ cross_dq_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
       };
       using t0 = std::integral_constant<int, 0>;
       using t1 = std::integral_constant<int, 1>;
-      for (int64_t r = 0; ok; ++r) {
-        const int64_t u = snake(r, cta, ctas, units);
-        if (u < 0) break;
-        const PairUnit w = pair_unit<F::kKeys>(a, order, u);
+      DqWalk walk;
+      DqUnit w;
+      while (ok && dq_next<F::kKeys>(a, order, first, total, walk, w)) {
         if (w.n <= 0) continue;
         const bool two = w.items > 1;
         ok = mbar_wait(q_full, (uint32_t)(ru & 1), g.err) && kv_wait();
@@ -829,9 +979,9 @@ cross_dq_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
         issue_s(t0{});
         if (two) issue_s(t1{});
         kv_next();
-        for (int j = 0; j < w.n; ++j) {
-          const bool last = j + 1 == w.n;
-          const uint32_t more = j > 0 ? 1u : 0u;
+        for (int j = w.j0; j < w.j1; ++j) {
+          const bool last = j + 1 == w.j1;
+          const uint32_t more = j > w.j0 ? 1u : 0u;
           ok = (last || kv_wait()) && issue_dq(t0{}, more);
           if (!ok) break;
           if (last) mma_commit(dq_done(0));
@@ -863,12 +1013,11 @@ cross_dq_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
     const unsigned long long sl22 = f2_pack(sl2, sl2);
     bool ok = true;
     int gs = 0, gk = 0, gu = 0;
-    for (int64_t r = 0;; ++r) {
-      const int64_t u = snake(r, cta, ctas, units);
-      if (u < 0) break;
-      const PairUnit w = pair_unit<F::kKeys>(a, order, u);
+    DqWalk walk;
+    DqUnit w;
+    while (dq_next<F::kKeys>(a, order, first, total, walk, w)) {
       if (t >= w.items) {
-        gk += w.n > 0 ? w.n : 0;
+        gk += w.j1 > w.j0 ? w.j1 - w.j0 : 0;
         continue;
       }
       const int h = head_of(a, w, t);
@@ -877,7 +1026,7 @@ cross_dq_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
       const int64_t at = (w.b * g.heads + h) * a.q_pad + qi;
       const float nl = in ? a.nlse[at] : -INFINITY, dl = in ? a.delta[at] : 0.f;
       const unsigned long long nl2 = f2_pack(nl, nl), dl2 = f2_pack(dl, dl);
-      for (int j = 0; j < w.n; ++j, ++gs, ++gk) {
+      for (int j = w.j0; j < w.j1; ++j, ++gs, ++gk) {
         const int64_t left = w.len - (int64_t)j * F::kKeys;
         const bool tail = left < F::kKeys;
         const int lim = tail ? (int)left - 1 : F::kKeys - 1;
@@ -939,7 +1088,20 @@ cross_dq_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
         uint32_t v[32];
         tmem_ld32(tDq(t) + lanes + c * 32, v);
         tmem_wait_ld();
-        if (in && c * 32 < g.hd) store_cols32(dst + c * 32, v, g.scale, g.hd - c * 32);
+        if (w.slot >= 0)
+          store_piece32<HD>(piece_rows<HD>(a, cta, w.slot, t) + (int64_t)row * HD + c * 32, v);
+        else if (in && c * 32 < g.hd)
+          store_cols32(dst + c * 32, v, g.scale, g.hd - c * 32);
+      }
+    }
+    // sequences without keys have no steps
+    if (a.piece != nullptr && g.lens != nullptr) {
+      const int64_t rows = (int64_t)g.heads * g.q_len;
+      for (int64_t b = 0; b < g.batch; ++b) {
+        if (first[b + 1] != first[b]) continue;
+        for (int64_t i = (int64_t)cta * 256 + threadIdx.x; i < rows; i += (int64_t)ctas * 256)
+          zero_cols(static_cast<__nv_bfloat16*>(a.dq) + b * g.dqs[0] + i / g.q_len * g.dqs[1] +
+                        i % g.q_len * g.dqs[2], g.hd);
       }
     }
   }
@@ -952,6 +1114,37 @@ cross_dq_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
   }
 }
 
+// dQ of the pairs that a border of the steps cuts: a CTA per border and eighth of
+// the pair's 256 rows.
+template <int HD>
+__global__ void __launch_bounds__(256)
+cross_dq_join(const __grid_constant__ TcArgs a, int ctas) {
+  __shared__ int64_t first[kDealt];
+  wait_for_launch_before();
+  const CrossGeom& g = a.g;
+  constexpr int kKeys = Dq<HD>::kKeys;
+  if (g.lens != nullptr && threadIdx.x < 32) step_table(a, kKeys, first);
+  __syncthreads();
+  const int64_t total = steps_of_all(a, kKeys, first), c = (int64_t)blockIdx.x + 1;
+  const int64_t s = border(total, c, ctas);
+  if (s >= total) return;
+  const StepAt x = step_at(a, kKeys, first, s);
+  const int64_t begin = s - x.j;
+  // the unit begins here, or an earlier border has it
+  if (x.j == 0 || border(total, c - 1, ctas) > begin) return;
+  const PairUnit w = pair_of<kKeys>(a, x.b, x.pair / a.n_pairs, 0, (int)(x.pair % a.n_pairs));
+  constexpr int kVec = HD / 4;
+  for (int i = threadIdx.x; i < 32 * kVec; i += 256) {
+    const int rr = (int)blockIdx.y * 32 + i / kVec, t = rr / kRows, row = rr % kRows, col = i % kVec * 4;
+    if (t >= w.items || col >= g.hd) continue;
+    const int64_t qi = (int64_t)tile_of(a, w, t) * kRows + row;
+    if (qi >= g.q_len) continue;
+    const float4 v = sum_pieces<HD>(a, total, ctas, c, begin, x.n, t, row, col);
+    store_grad4(static_cast<__nv_bfloat16*>(a.dq) + w.b * g.dqs[0] + head_of(a, w, t) * g.dqs[1] +
+                    qi * g.dqs[2] + col, v, g.scale);
+  }
+}
+
 // ================================================================ dK and dV
 // A unit is a 128-key tile of a key head; its steps are the 64-query tiles of
 // all query heads that share it. Steps alternate between two score buffers and
@@ -961,6 +1154,101 @@ cross_dq_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
 // Nothing is masked: a row of a key behind the length only reaches its own
 // output row, which is stored as zeros, and the terms of a query row behind
 // q_len make its probabilities 0.
+//
+// Whole units go round in a snake as far as they fill all CTAs; the rest of them
+// is dealt out by steps.
+struct KvUnit {
+  int64_t b, len;
+  int kvh, kt;
+  int i0, i1, slot;  // steps [i0, i1); slot of the partial sums, -1: the unit is whole
+};
+struct KvWalk {
+  int64_t r = 0, s = -1, end = 0;
+};
+// first[i]: key tiles of the sequences before i, of one key head.
+__device__ __forceinline__ bool kv_table(const CrossGeom& g) {
+  return g.lens != nullptr && g.batch < kOrder;
+}
+__device__ __forceinline__ void tile_table(const CrossGeom& g, int64_t* first) {
+  const int lane = threadIdx.x & 31;
+  int64_t sum = 0;
+  for (int64_t i0 = 0; i0 < g.batch; i0 += 32) {
+    const int64_t i = i0 + lane;
+    const int64_t n = i < g.batch ? (cross_len(g, i) + kRows - 1) / kRows : 0;
+    int64_t inc = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t x = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += x;
+    }
+    if (i < g.batch) first[i] = sum + inc - n;
+    sum += __shfl_sync(0xffffffffu, inc, 31);
+  }
+  if (lane == 0) first[g.batch] = sum;
+}
+// Unit u: sequences outermost, then key heads, then tiles, so that tiles that run
+// at the same time read the same queries. With a table the units are exactly the
+// tiles that have keys; without one every tile is a unit.
+__device__ __forceinline__ KvUnit kv_unit(const CrossGeom& g, const int64_t* first, int64_t u,
+                                          int n_it) {
+  KvUnit w;
+  const int64_t all_tiles = (g.kv_len + kRows - 1) / kRows;
+  if (kv_table(g)) {
+    int64_t lo = 0, hi = g.batch;  // first[lo] * kv_heads <= u < first[hi] * kv_heads
+    while (hi - lo > 1) {
+      const int64_t mid = (lo + hi) >> 1;
+      if (first[mid] * g.kv_heads <= u) lo = mid;
+      else hi = mid;
+    }
+    w.b = lo;
+    const int64_t tiles = first[lo + 1] - first[lo];
+    const int64_t rest = u - first[lo] * g.kv_heads;
+    w.kvh = (int)(rest / tiles);
+    w.kt = (int)(rest % tiles);
+  } else {
+    w.b = u / (all_tiles * g.kv_heads);
+    const int64_t rest = u % (all_tiles * g.kv_heads);
+    w.kvh = (int)(rest / all_tiles);
+    w.kt = (int)(rest % all_tiles);
+  }
+  w.len = cross_len(g, w.b);
+  w.i0 = 0;
+  w.i1 = (int64_t)w.kt * kRows < w.len ? n_it : 0;
+  w.slot = -1;
+  return w;
+}
+__device__ __forceinline__ int64_t kv_units(const CrossGeom& g, const int64_t* first) {
+  return (kv_table(g) ? first[g.batch] : (g.kv_len + kRows - 1) / kRows * g.batch) * g.kv_heads;
+}
+// Units that go round whole; the others' steps are dealt out.
+__device__ __forceinline__ int64_t kv_whole(const TcArgs& a, int64_t units, int64_t ctas) {
+  return a.piece == nullptr ? units : units / ctas * ctas;
+}
+__device__ __forceinline__ bool kv_next(const TcArgs& a, const int64_t* first, int64_t units, int n_it,
+                                        KvWalk& k, KvUnit& w) {
+  const int64_t ctas = gridDim.x, cta = blockIdx.x;
+  const int64_t whole = kv_whole(a, units, ctas);
+  const int64_t total = (units - whole) * n_it;
+  if (k.s < 0) {
+    const int64_t u = snake(k.r, (int)cta, (int)ctas, whole);
+    if (u >= 0) {
+      ++k.r;
+      w = kv_unit(a.g, first, u, n_it);
+      return true;
+    }
+    k.s = border(total, cta, ctas);
+    k.end = border(total, cta + 1, ctas);
+  }
+  if (k.s >= k.end) return false;
+  w = kv_unit(a.g, first, whole + k.s / n_it, n_it);
+  w.i0 = (int)(k.s % n_it);
+  const int64_t stop = w.i0 + (k.end - k.s);
+  w.i1 = (int)(stop < n_it ? stop : n_it);
+  w.slot = w.i1 - w.i0 == n_it ? -1 : k.s == border(total, cta, ctas) ? 0 : 1;
+  k.s += w.i1 - w.i0;
+  return true;
+}
+
 template <int HD>
 struct Dkv {
   static constexpr int kQ = 64;                     // query rows of a step
@@ -1014,9 +1302,7 @@ cross_dkdv_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int ctas = (int)gridDim.x, cta = (int)blockIdx.x;
   const int64_t all_tiles = (g.kv_len + kRows - 1) / kRows;
-  // With a table of the sequences' tiles the units are exactly the tiles that
-  // have keys; without one every tile is a unit.
-  const bool table = g.lens != nullptr && g.batch < kOrder;
+  const bool table = kv_table(g);
   const int q_steps = a.q_pad / F::kQ;
   const int n_it = g.group * q_steps;
 
@@ -1033,22 +1319,7 @@ cross_dkdv_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
     fence_barrier_init();
   }
   if (warp == kMmaWarp) tmem_alloc(tslot, 512);
-  if (table && warp == 0) {
-    int64_t sum = 0;
-    for (int64_t i0 = 0; i0 < g.batch; i0 += 32) {
-      const int64_t i = i0 + lane;
-      int64_t n = i < g.batch ? (cross_len(g, i) + kRows - 1) / kRows : 0;
-      int64_t inc = n;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int64_t x = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += x;
-      }
-      if (i < g.batch) first[i] = sum + inc - n;
-      sum += __shfl_sync(0xffffffffu, inc, 31);
-    }
-    if (lane == 0) first[g.batch] = sum;
-  }
+  if (table && warp == 0) tile_table(g, first);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -1056,48 +1327,16 @@ cross_dkdv_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
   auto tS = [&](int t) { return tmem + 128u * t; };
   auto tDp = [&](int t) { return tmem + 128u * t + 64u; };
   const uint32_t tDv = tmem + 256u, tDk = tmem + 256u + HD;
-  const int64_t units = (table ? first[g.batch] : all_tiles * g.batch) * g.kv_heads;
-
-  struct Unit {
-    int64_t b, len;
-    int kvh, kt, n;
-  };
-  // sequences outermost, then key heads, then tiles: tiles that run at the same
-  // time read the same queries
-  auto unit = [&](int64_t u) {
-    Unit w;
-    if (table) {
-      int64_t lo = 0, hi = g.batch;  // first[lo] * kv_heads <= u < first[hi] * kv_heads
-      while (hi - lo > 1) {
-        const int64_t mid = (lo + hi) >> 1;
-        if (first[mid] * g.kv_heads <= u) lo = mid;
-        else hi = mid;
-      }
-      w.b = lo;
-      const int64_t tiles = first[lo + 1] - first[lo];
-      const int64_t rest = u - first[lo] * g.kv_heads;
-      w.kvh = (int)(rest / tiles);
-      w.kt = (int)(rest % tiles);
-    } else {
-      w.b = u / (all_tiles * g.kv_heads);
-      const int64_t rest = u % (all_tiles * g.kv_heads);
-      w.kvh = (int)(rest / all_tiles);
-      w.kt = (int)(rest % all_tiles);
-    }
-    w.len = cross_len(g, w.b);
-    w.n = (int64_t)w.kt * kRows < w.len ? n_it : 0;
-    return w;
-  };
+  const int64_t units = kv_units(g, first);
 
   if (warp == kTmaWarp) {
     if (elect_one()) {
       bool ok = true;
       int gq = 0, ru = 0;
-      for (int64_t r = 0; ok; ++r) {
-        const int64_t u = snake(r, cta, ctas, units);
-        if (u < 0) break;
-        const Unit w = unit(u);
-        if (w.n == 0) continue;
+      KvWalk walk;
+      KvUnit w;
+      while (ok && kv_next(a, first, units, n_it, walk, w)) {
+        if (w.i0 == w.i1) continue;
         const int kb = ru % F::kKvBufs;
         if (!mbar_wait(kv_empty(kb), (uint32_t)(((ru / F::kKvBufs) & 1) ^ 1), g.err)) break;
         mbar_expect_tx(kv_full(kb), 2 * F::kTile);
@@ -1107,7 +1346,7 @@ cross_dkdv_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
           tma_load_4d(sV(kb) + c * kBlk128, &tmV, c * 64, w.kt * kRows, w.kvh * a.vh,
                       (int)w.b * a.vb, kv_full(kb));
         }
-        for (int i = 0; i < w.n; ++i, ++gq) {
+        for (int i = w.i0; i < w.i1; ++i, ++gq) {
           const int st = gq % F::kStages;
           if (!mbar_wait(q_empty(st), (uint32_t)(((gq / F::kStages) & 1) ^ 1), g.err)) {
             ok = false;
@@ -1171,14 +1410,14 @@ cross_dkdv_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
       auto s_next = [&]() {
         if (++sst == F::kStages) sst = 0, sph ^= 1u;
       };
-      for (int64_t r = 0; ok; ++r) {
-        const int64_t u = snake(r, cta, ctas, units);
-        if (u < 0) break;
-        const Unit w = unit(u);
-        if (w.n == 0) continue;
+      KvWalk walk;
+      KvUnit w;
+      while (ok && kv_next(a, first, units, n_it, walk, w)) {
+        if (w.i0 == w.i1) continue;
         const int kb = ru % F::kKvBufs;
         ok = mbar_wait(kv_full(kb), (uint32_t)((ru / F::kKvBufs) & 1), g.err);
-        for (int i = 0; i < 2 && i < w.n && ok; ++i) {
+        const int n = w.i1 - w.i0;
+        for (int i = 0; i < 2 && i < n && ok; ++i) {
           ok = q_wait();
           if (!ok) break;
           issue_s(tb, kb);
@@ -1187,10 +1426,10 @@ cross_dkdv_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
           tb ^= 1u;
         }
         if (!ok) break;
-        for (int i = 0; i < w.n; ++i) {
+        for (int i = 0; i < n; ++i) {
           const uint32_t t = db;
           const uint32_t more = i > 0 ? 1u : 0u;
-          const bool next = i + 2 < w.n;
+          const bool next = i + 2 < n;
           const uint32_t aq = (uint32_t)gst * F::kStage, sc = tmem + 128u * t;
           ok = mbar_wait(p_full(t), gp, g.err) &&
                // the previous unit's dV and dK have been read
@@ -1240,11 +1479,11 @@ cross_dkdv_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
     const unsigned long long sl22 = f2_pack(sl2, sl2);
     bool ok = true;
     int gs = 0, ru = 0;
-    for (int64_t r = 0;; ++r) {
-      const int64_t u = snake(r, cta, ctas, units);
-      if (u < 0) break;
-      const Unit w = unit(u);
-      for (int i = 0; i < w.n; ++i) {
+    KvWalk walk;
+    KvUnit w;
+    while (kv_next(a, first, units, n_it, walk, w)) {
+      const int n_steps = w.i1 - w.i0;
+      for (int i = 0; i < n_steps; ++i) {
         const int s = gs + i;
         if ((s & 1) != t) continue;
         const int st = s % F::kStages;
@@ -1300,14 +1539,14 @@ cross_dkdv_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
         __syncwarp();
         if (lane == 0) mbar_arrive(ds_full(t));
       }
-      gs += w.n;
+      gs += n_steps;
       // warpgroup 0 stores dV, warpgroup 1 dK
       const int64_t kj = (int64_t)w.kt * kRows + row;
       const bool in = kj < g.kv_len;
       __nv_bfloat16* dst =
           t == 0 ? static_cast<__nv_bfloat16*>(a.dv) + w.b * g.dvs[0] + w.kvh * g.dvs[1] + kj * g.dvs[2]
                  : static_cast<__nv_bfloat16*>(a.dk) + w.b * g.dks[0] + w.kvh * g.dks[1] + kj * g.dks[2];
-      if (w.n == 0) {
+      if (n_steps == 0) {
         if (in) zero_cols(dst, g.hd);
         continue;
       }
@@ -1327,10 +1566,12 @@ cross_dkdv_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
           __syncwarp();
           if (lane == 0) mbar_arrive(acc_empty);
         }
-        if (!in || c * 32 >= g.hd) continue;
-        if (kj < w.len) store_cols32(dst + c * 32, v, mul, g.hd - c * 32);
+        if (w.slot >= 0)
+          store_piece32<HD>(piece_rows<HD>(a, cta, w.slot, t) + (int64_t)row * HD + c * 32, v);
+        else if (kj < w.len && c * 32 < g.hd)
+          store_cols32(dst + c * 32, v, mul, g.hd - c * 32);
       }
-      if (in && kj >= w.len) zero_cols(dst, g.hd);
+      if (in && kj >= w.len && w.slot < 0) zero_cols(dst, g.hd);
     }
     if (table) {  // the tiles without keys, which are no units
       for (int64_t i = cta; i < all_tiles * g.kv_heads * g.batch; i += ctas) {
@@ -1351,6 +1592,39 @@ cross_dkdv_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
     __syncwarp();
     tc_fence_after();
     tmem_dealloc(tmem, 512);
+  }
+}
+
+// dV and dK of the units that a border of the steps cuts: a CTA per border and
+// eighth of the 2 x 128 rows.
+template <int HD>
+__global__ void __launch_bounds__(256)
+cross_dkdv_join(const __grid_constant__ TcArgs a, int ctas) {
+  __shared__ int64_t first[kOrder];
+  wait_for_launch_before();
+  const CrossGeom& g = a.g;
+  if (kv_table(g) && threadIdx.x < 32) tile_table(g, first);
+  __syncthreads();
+  const int n_it = g.group * (a.q_pad / Dkv<HD>::kQ);
+  const int64_t units = kv_units(g, first), whole = kv_whole(a, units, ctas);
+  const int64_t total = (units - whole) * n_it, c = (int64_t)blockIdx.x + 1;
+  const int64_t s = border(total, c, ctas);
+  if (s >= total) return;
+  const int64_t begin = s / n_it * n_it;
+  // the unit begins here, or an earlier border has it
+  if (begin == s || border(total, c - 1, ctas) > begin) return;
+  const KvUnit w = kv_unit(g, first, whole + s / n_it, n_it);
+  constexpr int kVec = HD / 4;
+  for (int i = threadIdx.x; i < 32 * kVec; i += 256) {
+    const int rr = (int)blockIdx.y * 32 + i / kVec, t = rr / kRows, row = rr % kRows, col = i % kVec * 4;
+    const int64_t kj = (int64_t)w.kt * kRows + row;
+    if (col >= g.hd || kj >= g.kv_len) continue;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (kj < w.len) v = sum_pieces<HD>(a, total, ctas, c, begin, n_it, t, row, col);
+    __nv_bfloat16* dst =
+        t == 0 ? static_cast<__nv_bfloat16*>(a.dv) + w.b * g.dvs[0] + w.kvh * g.dvs[1] + kj * g.dvs[2]
+               : static_cast<__nv_bfloat16*>(a.dk) + w.b * g.dks[0] + w.kvh * g.dks[1] + kj * g.dks[2];
+    store_grad4(dst + col, v, t == 0 ? 1.f : g.scale);
   }
 }
 
@@ -1402,9 +1676,31 @@ magma_status_t fwd_tc(const void* q, const void* k, const void* v, TcArgs a, cud
   return check_launch("cross_fwd_tc");
 }
 
+// Whether the steps are dealt out: where whole units leave the CTAs idle for more
+// than this many steps on average (lengths that differ: at least half a unit's).
+// The pieces cost two stores of 128 rows and a second launch, about as long as 20
+// steps.
+constexpr int64_t kIdleSteps = 24;
+bool deal(const CrossGeom& g, int64_t units, int64_t steps) {
+  const int64_t n = num_sms();
+  if (units > 16 * n) return false;
+  const int64_t idle = steps * (ceil_div(units, n) * n - units) / n;
+  return std::max(idle, g.lens != nullptr ? steps / 2 : 0) > kIdleSteps;
+}
+bool deal_dkdv(const CrossGeom& g) {
+  return (g.lens == nullptr || g.batch < kOrder) &&
+         deal(g, ceil_div(g.kv_len, kRows) * g.kv_heads * g.batch,
+              (int64_t)g.group * ceil_div(g.q_len, 64));
+}
+bool deal_dq(const CrossGeom& g) {
+  const TcArgs a = args_of(g);
+  return (g.lens == nullptr || g.batch < kDealt) &&
+         deal(g, (int64_t)a.n_pairs * g.kv_heads * g.batch, ceil_div(g.kv_len, 64));
+}
+
 template <int HD>
-magma_status_t bwd_tc(const void* q, const void* k, const void* v, const void* d_o, TcArgs a,
-                      cudaStream_t s) {
+magma_status_t bwd_tc(const void* q, const void* k, const void* v, const void* d_o, float* piece,
+                      TcArgs a, cudaStream_t s) {
   const CrossGeom& g = a.g;
   CUtensorMap mq, mg, mk, mv;
   {
@@ -1415,9 +1711,14 @@ magma_status_t bwd_tc(const void* q, const void* k, const void* v, const void* d
     if (magma_status_t st = view_map(&mv, v, g.hd, g.kv_len, g.kv_heads, g.batch, g.vs, kRows, &a.vb, &a.vh)) return st;
     if (magma_status_t st = cross_smem<cross_dkdv_tc<HD>>(F::kSmem)) return st;
     const int64_t units = ceil_div(g.kv_len, kRows) * g.kv_heads * g.batch;
-    const unsigned ctas = (unsigned)std::min<int64_t>(units, num_sms());
+    a.piece = deal_dkdv(g) ? piece : nullptr;
+    const unsigned ctas = (unsigned)(a.piece ? num_sms() : std::min<int64_t>(units, num_sms()));
     cross_dkdv_tc<HD><<<ctas, kThreads, F::kSmem, s>>>(mq, mg, mk, mv, a);
     if (magma_status_t st = check_launch("cross_dkdv_tc")) return st;
+    if (a.piece)
+      if (magma_status_t st = launch_after(cross_dkdv_join<HD>, dim3(ctas - 1, 8), 256, 0, s,
+                                           "cross_dkdv_join", a, (int)ctas))
+        return st;
   }
   using F = Dq<HD>;
   if (magma_status_t st = view_map(&mq, q, g.hd, g.q_len, g.heads, g.batch, g.qs, kRows, &a.qb, &a.qh)) return st;
@@ -1426,9 +1727,12 @@ magma_status_t bwd_tc(const void* q, const void* k, const void* v, const void* d
   if (magma_status_t st = view_map(&mv, v, g.hd, g.kv_len, g.kv_heads, g.batch, g.vs, F::kKeys, &a.vb, &a.vh)) return st;
   if (magma_status_t st = cross_smem<cross_dq_tc<HD>>(F::kSmem)) return st;
   const int64_t units = (int64_t)a.n_pairs * g.kv_heads * g.batch;
-  const unsigned ctas = (unsigned)std::min<int64_t>(units, num_sms());
+  a.piece = deal_dq(g) ? piece : nullptr;
+  const unsigned ctas = (unsigned)(a.piece ? num_sms() : std::min<int64_t>(units, num_sms()));
   cross_dq_tc<HD><<<ctas, kThreads, F::kSmem, s>>>(mq, mg, mk, mv, a);
-  return check_launch("cross_dq_tc");
+  if (magma_status_t st = check_launch("cross_dq_tc")) return st;
+  if (a.piece == nullptr) return MAGMA_OK;
+  return launch_after(cross_dq_join<HD>, dim3(ctas - 1, 8), 256, 0, s, "cross_dq_join", a, (int)ctas);
 }
 
 }  // namespace
@@ -1484,8 +1788,18 @@ magma_status_t cross_fwd_tc_run(const void* q, const void* k, const void* v, voi
   return cross_join_parts(a.part, a.part_lse, o, lse, g, a.n_split, MAGMA_DTYPE_BF16, s);
 }
 
-size_t cross_tc_bwd_workspace(const CrossGeom& g) {
+// The row terms, then the pieces: two slots of two tiles a CTA. (Room for them is
+// asked for with and without lengths, which the query does not know of.)
+static size_t row_bytes(const CrossGeom& g) {
   return 2 * sizeof(float) * (size_t)g.batch * g.heads * (ceil_div(g.q_len, 64) * 64);
+}
+size_t cross_tc_bwd_workspace(const CrossGeom& g) {
+  static const int32_t some = 0;
+  CrossGeom l = g;
+  l.lens = &some;
+  const bool pieces = deal_dkdv(g) || deal_dq(g) || deal_dkdv(l) || deal_dq(l);
+  return row_bytes(g) +
+         (pieces ? (size_t)num_sms() * 4 * kRows * (g.hd <= 64 ? 64 : 128) * sizeof(float) : 0);
 }
 
 magma_status_t cross_bwd_tc_run(const void* q, const void* k, const void* v, const void* o,
@@ -1504,7 +1818,9 @@ magma_status_t cross_bwd_tc_run(const void* q, const void* k, const void* v, con
       static_cast<const __nv_bfloat16*>(o), static_cast<const __nv_bfloat16*>(d_o), lse, nlse, delta,
       g, a.q_pad);
   if (magma_status_t st = check_launch("cross_rows")) return st;
-  return g.hd <= 64 ? bwd_tc<64>(q, k, v, d_o, a, s) : bwd_tc<128>(q, k, v, d_o, a, s);
+  float* piece = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + row_bytes(g));
+  return g.hd <= 64 ? bwd_tc<64>(q, k, v, d_o, piece, a, s)
+                    : bwd_tc<128>(q, k, v, d_o, piece, a, s);
 }
 
 }  // namespace magma

@@ -181,6 +181,21 @@ def test_few_queries_over_long_sources(cuda, case, dtype):
     run_both(case, dtype)
 
 
+# few tiles with many steps: the gradient's steps are dealt out over the GPU and
+# units are put together from pieces, also next to sequences without keys
+@pytest.mark.parametrize("case,lens", [
+    ((1, 4, 1, 520, 300, 64), None), ((2, 8, 2, 450, 200, 128), [200, 77]),
+    ((3, 2, 1, 130, 2100, 64), [2100, 0, 1999]), ((2, 4, 4, 260, 1900, 128), [1, 1900]),
+    ((1, 2, 2, 1700, 2200, 80), None), ((5, 3, 1, 600, 700, 64), [0, 700, 64, 129, 500]),
+    ((1, 1, 1, 65, 9000, 128), None), ((4, 6, 2, 700, 1664, 96), [1664, 1000, 128, 1663]),
+])
+def test_gradient_with_steps_dealt_out(cuda, case, lens):
+    first = run_both(case, torch.bfloat16, lens=lens)
+    again = run_both(case, torch.bfloat16, lens=lens)
+    for a, b in zip(first[3], again[3]):
+        assert torch.equal(a, b)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("scale,std", [(0.0, 1.0), (1.0, 2.0), (1e-3, 30.0)])
 def test_scales(cuda, scale, std, dtype):
