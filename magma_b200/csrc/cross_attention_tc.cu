@@ -107,9 +107,9 @@ __device__ __forceinline__ uint32_t align1024(uint8_t* raw, uint8_t** p) {
 
 // The r-th unit of CTA c among n CTAs, even rounds in CTA order, odd ones
 // reversed; -1 past the end.
-__device__ __forceinline__ int64_t snake(int64_t r, int c, int n, int64_t units) {
-  const int64_t u = r * n + ((r & 1) ? n - 1 - c : c);
-  return u < units ? u : -1;
+__device__ __forceinline__ int snake(int r, int c, int n, int units) {
+  const int64_t u = (int64_t)r * n + ((r & 1) ? n - 1 - c : c);
+  return u < units ? (int)u : -1;
 }
 
 // order[rank] = sequence, longest first.
@@ -125,8 +125,7 @@ __device__ __forceinline__ void order_by_length(const CrossGeom& g, uint16_t* or
     order[rank] = (uint16_t)i;
   }
 }
-__device__ __forceinline__ int64_t sequence_of(const CrossGeom& g, const uint16_t* order,
-                                               int64_t rank) {
+__device__ __forceinline__ int sequence_of(const CrossGeom& g, const uint16_t* order, int rank) {
   return g.lens == nullptr || g.batch > kOrder ? rank : order[rank];
 }
 
@@ -140,18 +139,28 @@ __device__ __forceinline__ void zero_row(uint32_t tile, int r, int blocks, int b
                    : "memory");
 }
 
-// 32 F32 columns of a row times mul as BF16, those below `cols`.
+// 32 F32 columns of a row times mul as BF16, those below `cols`. A thread has a
+// row: 32-byte stores fill whole sectors, where the row's address allows them.
 __device__ __forceinline__ void store_cols32(__nv_bfloat16* dst, const uint32_t (&v)[32], float mul,
                                              int cols) {
+  uint32_t u[16];
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    if (q * 8 >= cols) break;
-    uint4 u;
-    u.x = pack_bf16(__uint_as_float(v[q * 8 + 0]) * mul, __uint_as_float(v[q * 8 + 1]) * mul);
-    u.y = pack_bf16(__uint_as_float(v[q * 8 + 2]) * mul, __uint_as_float(v[q * 8 + 3]) * mul);
-    u.z = pack_bf16(__uint_as_float(v[q * 8 + 4]) * mul, __uint_as_float(v[q * 8 + 5]) * mul);
-    u.w = pack_bf16(__uint_as_float(v[q * 8 + 6]) * mul, __uint_as_float(v[q * 8 + 7]) * mul);
-    reinterpret_cast<uint4*>(dst)[q] = u;
+  for (int e = 0; e < 16; ++e)
+    u[e] = pack_bf16(__uint_as_float(v[2 * e]) * mul, __uint_as_float(v[2 * e + 1]) * mul);
+  if ((reinterpret_cast<uintptr_t>(dst) & 31u) == 0 && cols % 16 == 0) {
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+      if (q * 16 < cols)
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst + 16 * q),
+                     "r"(u[8 * q]), "r"(u[8 * q + 1]), "r"(u[8 * q + 2]), "r"(u[8 * q + 3]),
+                     "r"(u[8 * q + 4]), "r"(u[8 * q + 5]), "r"(u[8 * q + 6]), "r"(u[8 * q + 7])
+                     : "memory");
+  } else {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (q * 8 < cols)
+        reinterpret_cast<uint4*>(dst)[q] =
+            make_uint4(u[4 * q], u[4 * q + 1], u[4 * q + 2], u[4 * q + 3]);
   }
 }
 __device__ __forceinline__ void zero_cols(__nv_bfloat16* dst, int hd) {
@@ -179,18 +188,27 @@ __device__ __forceinline__ void store_piece32(float* row, const uint32_t (&v)[32
   for (int q = 0; q < 8; ++q)
     reinterpret_cast<uint4*>(row)[q] = make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
 }
-// The unit of steps [begin, begin + n) that border c cuts: the sum over its
-// pieces of row `row`, columns [col, col + 4). Slot 0 of a CTA whose range begins
-// in the unit, slot 1 of the one whose range ends in it.
-template <int HD>
-__device__ __forceinline__ float4 sum_pieces(const TcArgs& a, int64_t total, int64_t ctas, int64_t c,
-                                             int64_t begin, int64_t n, int t, int row, int col) {
-  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+// The unit of steps [begin, begin + n) that border c cuts first: its pieces in
+// order, as CTA * 2 + slot. Slot 0 of a CTA whose range begins in the unit, slot 1
+// of the one whose range ends in it. One thread writes the list.
+constexpr int kMostPieces = 1024;
+__device__ __forceinline__ int list_pieces(int64_t total, int64_t ctas, int64_t c, int64_t begin,
+                                           int64_t n, int* list) {
+  int count = 0;
   for (int64_t i = c - 1; i < ctas && border(total, i, ctas) < begin + n; ++i) {
     if (border(total, i, ctas) == border(total, i + 1, ctas)) continue;  // nothing of its own
-    const int slot = border(total, i, ctas) >= begin ? 0 : 1;
+    list[count++] = (int)(i * 2 + (border(total, i, ctas) >= begin ? 0 : 1));
+  }
+  return count;
+}
+template <int HD>
+__device__ __forceinline__ float4 sum_pieces(const TcArgs& a, const int* list, int count, int t,
+                                             int row, int col) {
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int i = 0; i < count; ++i) {
     const float4 v = *reinterpret_cast<const float4*>(
-        piece_rows<HD>(a, i, slot, t) + (int64_t)row * HD + col);
+        piece_rows<HD>(a, list[i] >> 1, list[i] & 1, t) + (int64_t)row * HD + col);
     s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
   }
   return s;
@@ -219,12 +237,11 @@ __device__ __forceinline__ int tile_of(const TcArgs& a, const PairUnit& w, int t
 }
 
 template <int KT>
-__device__ __forceinline__ PairUnit pair_of(const TcArgs& a, int64_t b, int64_t kvh, int split,
-                                            int p) {
+__device__ __forceinline__ PairUnit pair_of(const TcArgs& a, int b, int kvh, int split, int p) {
   const CrossGeom& g = a.g;
   PairUnit w;
   w.b = b;
-  w.kvh = (int)kvh;
+  w.kvh = kvh;
   w.split = split;
   const int all = g.group * a.n_qt;
   w.first = 2 * p;
@@ -236,14 +253,15 @@ __device__ __forceinline__ PairUnit pair_of(const TcArgs& a, int64_t b, int64_t 
   w.n = tiles - w.t0 < each ? tiles - w.t0 : each;
   return w;
 }
+// Unit numbers fit 32 bits (the host checks): a 64-bit division costs as much as
+// half a tile.
 template <int KT>
-__device__ __forceinline__ PairUnit pair_unit(const TcArgs& a, const uint16_t* order, int64_t u) {
-  const int64_t per_head = (int64_t)a.n_pairs * a.n_split;
-  const int64_t per_seq = per_head * a.g.kv_heads;
-  const int64_t rest = u % per_seq;
-  const int x = (int)(rest % per_head);
-  return pair_of<KT>(a, sequence_of(a.g, order, u / per_seq), rest / per_head, x / a.n_pairs,
-                     x % a.n_pairs);
+__device__ __forceinline__ PairUnit pair_unit(const TcArgs& a, const uint16_t* order, int u) {
+  const uint32_t per_head = (uint32_t)(a.n_pairs * a.n_split);
+  const uint32_t head = (uint32_t)u / per_head, x = (uint32_t)u % per_head;
+  const uint32_t rank = head / (uint32_t)a.g.kv_heads, kvh = head % (uint32_t)a.g.kv_heads;
+  return pair_of<KT>(a, sequence_of(a.g, order, (int)rank), (int)kvh, (int)(x / (uint32_t)a.n_pairs),
+                     (int)(x % (uint32_t)a.n_pairs));
 }
 
 // =============================================================== forward
@@ -307,7 +325,7 @@ cross_fwd_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
 
   const CrossGeom& g = a.g;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t units = (int64_t)a.n_pairs * a.n_split * g.kv_heads * g.batch;
+  const int units = (int)(a.n_pairs * a.n_split * g.kv_heads * g.batch);
   const int ctas = (int)gridDim.x, cta = (int)blockIdx.x;
 
   if (threadIdx.x == 0) {
@@ -333,8 +351,8 @@ cross_fwd_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
       bool ok = true;
       int gk = 0;  // key tiles loaded so far
       int ru = 0;  // units that had keys
-      for (int64_t r = 0; ok; ++r) {
-        const int64_t u = snake(r, cta, ctas, units);
+      for (int r = 0; ok; ++r) {
+        const int u = snake(r, cta, ctas, units);
         if (u < 0) break;
         const PairUnit w = pair_unit<kRows>(a, order, u);
         if (w.n <= 0) continue;
@@ -424,8 +442,8 @@ cross_fwd_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
       };
       using t0 = std::integral_constant<int, 0>;
       using t1 = std::integral_constant<int, 1>;
-      for (int64_t r = 0; ok; ++r) {
-        const int64_t u = snake(r, cta, ctas, units);
+      for (int r = 0; ok; ++r) {
+        const int u = snake(r, cta, ctas, units);
         if (u < 0) break;
         const PairUnit w = pair_unit<kRows>(a, order, u);
         if (w.n <= 0) continue;
@@ -476,8 +494,8 @@ cross_fwd_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
     bool ok = true;
     int gs = 0;  // this warpgroup's steps so far
     int gk = 0;
-    for (int64_t r = 0;; ++r) {
-      const int64_t u = snake(r, cta, ctas, units);
+    for (int r = 0;; ++r) {
+      const int u = snake(r, cta, ctas, units);
       if (u < 0) break;
       const PairUnit w = pair_unit<kRows>(a, order, u);
       if (t >= w.items) {
@@ -712,80 +730,80 @@ __device__ __forceinline__ void grads32(const uint32_t (&p)[32], const uint32_t 
 // As the forward kernel, over 64-key tiles: S_t, dP_t = dO_t V_j^T; dS_t as BF16
 // pairs in S_t's columns is the A operand of dQ_t += dS_t K_j. TMEM columns of
 // tile t from 256 t: S, dP, dQ.
-constexpr int kDealt = 128;  // most sequences of a table of steps
+constexpr int kDealt = kOrder / 2;  // entries of a table of steps, in the place of the order
 
 // Steps of the pairs of all sequences: first[b] of the sequences before b. One
-// warp fills the table; without lengths every sequence has as many.
-__device__ __forceinline__ void step_table(const TcArgs& a, int keys, int64_t* first) {
+// warp fills the table; without lengths every sequence has as many. (The host
+// deals out fewer than 2^31 steps.)
+__device__ __forceinline__ void step_table(const TcArgs& a, int keys, int* first) {
   const CrossGeom& g = a.g;
   const int lane = threadIdx.x & 31;
-  const int64_t pairs = (int64_t)a.n_pairs * g.kv_heads;
-  int64_t sum = 0;
-  for (int64_t i0 = 0; i0 < g.batch; i0 += 32) {
-    const int64_t i = i0 + lane;
-    const int64_t n = i < g.batch ? (cross_len(g, i) + keys - 1) / keys * pairs : 0;
-    int64_t inc = n;
+  const int pairs = (int)(a.n_pairs * g.kv_heads), batch = (int)g.batch;
+  int sum = 0;
+  for (int i0 = 0; i0 < batch; i0 += 32) {
+    const int i = i0 + lane;
+    const int n = i < batch ? ((int)cross_len(g, i) + keys - 1) / keys * pairs : 0;
+    int inc = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t x = __shfl_up_sync(0xffffffffu, inc, o);
+      const int x = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += x;
     }
-    if (i < g.batch) first[i] = sum + inc - n;
+    if (i < batch) first[i] = sum + inc - n;
     sum += __shfl_sync(0xffffffffu, inc, 31);
   }
-  if (lane == 0) first[g.batch] = sum;
+  if (lane == 0) first[batch] = sum;
 }
 
 // Where step s of all lies: its sequence, the pair, the key tile in the pair.
 struct StepAt {
-  int64_t b, pair, n;  // n: key tiles of the sequence
-  int j;
+  int b, pair, n, j;  // n: key tiles of the sequence
 };
-__device__ __forceinline__ StepAt step_at(const TcArgs& a, int keys, const int64_t* first, int64_t s) {
+__device__ __forceinline__ StepAt step_at(const TcArgs& a, int keys, const int* first, int s) {
   const CrossGeom& g = a.g;
   StepAt x;
-  int64_t rest;
+  uint32_t rest;
   if (g.lens != nullptr) {
-    int64_t lo = 0, hi = g.batch;  // first[lo] <= s < first[hi]
+    int lo = 0, hi = (int)g.batch;  // first[lo] <= s < first[hi]
     while (hi - lo > 1) {
-      const int64_t mid = (lo + hi) >> 1;
+      const int mid = (lo + hi) >> 1;
       if (first[mid] <= s) lo = mid;
       else hi = mid;
     }
     x.b = lo;
-    x.n = (cross_len(g, lo) + keys - 1) / keys;
-    rest = s - first[lo];
+    x.n = ((int)cross_len(g, lo) + keys - 1) / keys;
+    rest = (uint32_t)(s - first[lo]);
   } else {
-    x.n = (g.kv_len + keys - 1) / keys;
-    const int64_t per = x.n * a.n_pairs * g.kv_heads;
-    x.b = s / per;
-    rest = s % per;
+    x.n = ((int)g.kv_len + keys - 1) / keys;
+    const uint32_t per = (uint32_t)(x.n * a.n_pairs * g.kv_heads);
+    x.b = (int)((uint32_t)s / per);
+    rest = (uint32_t)s % per;
   }
-  x.pair = rest / x.n;
-  x.j = (int)(rest % x.n);
+  x.pair = (int)(rest / (uint32_t)x.n);
+  x.j = (int)(rest % (uint32_t)x.n);
   return x;
 }
-__device__ __forceinline__ int64_t steps_of_all(const TcArgs& a, int keys, const int64_t* first) {
+__device__ __forceinline__ int steps_of_all(const TcArgs& a, int keys, const int* first) {
   const CrossGeom& g = a.g;
   return g.lens != nullptr
              ? first[g.batch]
-             : (g.kv_len + keys - 1) / keys * a.n_pairs * g.kv_heads * g.batch;
+             : (int)((g.kv_len + keys - 1) / keys * a.n_pairs * g.kv_heads * g.batch);
 }
 
 // A CTA's way through its work: whole units in a snake, or its range of steps.
 struct DqWalk {
-  int64_t r = 0, s = 0, end = 0;
+  int r = 0, s = 0, end = 0;
 };
 struct DqUnit : PairUnit {
   int j0, j1, slot;  // key tiles [j0, j1); slot of the partial sums, -1: the unit is whole
 };
 template <int KT>
-__device__ __forceinline__ bool dq_next(const TcArgs& a, const uint16_t* order, const int64_t* first,
-                                        int64_t total, DqWalk& k, DqUnit& w) {
+__device__ __forceinline__ bool dq_next(const TcArgs& a, const uint16_t* order, const int* first,
+                                        int total, DqWalk& k, DqUnit& w) {
   const CrossGeom& g = a.g;
   if (a.piece == nullptr) {
-    const int64_t u = snake(k.r, (int)blockIdx.x, (int)gridDim.x,
-                            (int64_t)a.n_pairs * g.kv_heads * g.batch);
+    const int u =
+        snake(k.r, (int)blockIdx.x, (int)gridDim.x, (int)(a.n_pairs * g.kv_heads * g.batch));
     if (u < 0) return false;
     ++k.r;
     static_cast<PairUnit&>(w) = pair_unit<KT>(a, order, u);
@@ -794,20 +812,19 @@ __device__ __forceinline__ bool dq_next(const TcArgs& a, const uint16_t* order, 
     w.slot = -1;
     return true;
   }
+  bool first_piece = false;
   if (k.r == 0) {
     k.r = 1;
-    k.s = border(total, blockIdx.x, gridDim.x);
-    k.end = border(total, blockIdx.x + 1, gridDim.x);
+    k.s = (int)border(total, blockIdx.x, gridDim.x);
+    k.end = (int)border(total, blockIdx.x + 1, gridDim.x);
+    first_piece = true;
   }
   if (k.s >= k.end) return false;
   const StepAt x = step_at(a, KT, first, k.s);
-  // pair_unit's numbering with the sequence in its natural place
-  static_cast<PairUnit&>(w) =
-      pair_of<KT>(a, x.b, x.pair / a.n_pairs, 0, (int)(x.pair % a.n_pairs));
+  static_cast<PairUnit&>(w) = pair_of<KT>(a, x.b, x.pair / a.n_pairs, 0, x.pair % a.n_pairs);
   w.j0 = x.j;
-  const int64_t stop = x.j + (k.end - k.s);
-  w.j1 = (int)(stop < x.n ? stop : x.n);
-  const bool first_piece = k.s == border(total, blockIdx.x, gridDim.x);
+  const int stop = x.j + (k.end - k.s);
+  w.j1 = stop < x.n ? stop : x.n;
   w.slot = w.j1 - w.j0 == x.n ? -1 : first_piece ? 0 : 1;
   k.s += w.j1 - w.j0;
   return true;
@@ -856,7 +873,7 @@ cross_dq_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
   uint32_t* tslot_ptr = reinterpret_cast<uint32_t*>(sp + F::kBar + 8 * F::kBars);
   // the order of the sequences, or the table of their steps
   uint16_t* order = reinterpret_cast<uint16_t*>(sp + F::kOrd);
-  int64_t* first = reinterpret_cast<int64_t*>(sp + F::kOrd);
+  int* first = reinterpret_cast<int*>(sp + F::kOrd);
 
   const CrossGeom& g = a.g;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -880,7 +897,7 @@ cross_dq_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tslot_ptr);
-  const int64_t total = a.piece == nullptr ? 0 : steps_of_all(a, F::kKeys, first);
+  const int total = a.piece == nullptr ? 0 : steps_of_all(a, F::kKeys, first);
   auto tS = [&](int t) { return tmem + 256u * t; };
   auto tDp = [&](int t) { return tmem + 256u * t + 64u; };
   auto tDq = [&](int t) { return tmem + 256u * t + 128u; };
@@ -1119,7 +1136,8 @@ cross_dq_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
 template <int HD>
 __global__ void __launch_bounds__(256)
 cross_dq_join(const __grid_constant__ TcArgs a, int ctas) {
-  __shared__ int64_t first[kDealt];
+  __shared__ int first[kDealt];
+  __shared__ int list[kMostPieces], count;
   wait_for_launch_before();
   const CrossGeom& g = a.g;
   constexpr int kKeys = Dq<HD>::kKeys;
@@ -1128,20 +1146,25 @@ cross_dq_join(const __grid_constant__ TcArgs a, int ctas) {
   const int64_t total = steps_of_all(a, kKeys, first), c = (int64_t)blockIdx.x + 1;
   const int64_t s = border(total, c, ctas);
   if (s >= total) return;
-  const StepAt x = step_at(a, kKeys, first, s);
+  const StepAt x = step_at(a, kKeys, first, (int)s);
   const int64_t begin = s - x.j;
   // the unit begins here, or an earlier border has it
   if (x.j == 0 || border(total, c - 1, ctas) > begin) return;
-  const PairUnit w = pair_of<kKeys>(a, x.b, x.pair / a.n_pairs, 0, (int)(x.pair % a.n_pairs));
+  const PairUnit w = pair_of<kKeys>(a, x.b, x.pair / a.n_pairs, 0, x.pair % a.n_pairs);
+  if (threadIdx.x == 0) count = list_pieces(total, ctas, c, begin, x.n, list);
+  __syncthreads();
   constexpr int kVec = HD / 4;
+  const int t = (int)blockIdx.y / 4;  // four CTAs a tile
+  if (t >= w.items) return;
+  const int h = head_of(a, w, t);
+  const int64_t q0 = (int64_t)tile_of(a, w, t) * kRows;
+  __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(a.dq) + w.b * g.dqs[0] + h * g.dqs[1];
+#pragma unroll 2
   for (int i = threadIdx.x; i < 32 * kVec; i += 256) {
-    const int rr = (int)blockIdx.y * 32 + i / kVec, t = rr / kRows, row = rr % kRows, col = i % kVec * 4;
-    if (t >= w.items || col >= g.hd) continue;
-    const int64_t qi = (int64_t)tile_of(a, w, t) * kRows + row;
-    if (qi >= g.q_len) continue;
-    const float4 v = sum_pieces<HD>(a, total, ctas, c, begin, x.n, t, row, col);
-    store_grad4(static_cast<__nv_bfloat16*>(a.dq) + w.b * g.dqs[0] + head_of(a, w, t) * g.dqs[1] +
-                    qi * g.dqs[2] + col, v, g.scale);
+    const int row = (int)(blockIdx.y % 4) * 32 + i / kVec, col = i % kVec * 4;
+    if (col >= g.hd || q0 + row >= g.q_len) continue;
+    store_grad4(dst + (q0 + row) * g.dqs[2] + col, sum_pieces<HD>(a, list, count, t, row, col),
+                g.scale);
   }
 }
 
@@ -1163,88 +1186,91 @@ struct KvUnit {
   int i0, i1, slot;  // steps [i0, i1); slot of the partial sums, -1: the unit is whole
 };
 struct KvWalk {
-  int64_t r = 0, s = -1, end = 0;
+  int r = 0, s = -1, end = 0;
 };
 // first[i]: key tiles of the sequences before i, of one key head.
 __device__ __forceinline__ bool kv_table(const CrossGeom& g) {
   return g.lens != nullptr && g.batch < kOrder;
 }
-__device__ __forceinline__ void tile_table(const CrossGeom& g, int64_t* first) {
-  const int lane = threadIdx.x & 31;
-  int64_t sum = 0;
-  for (int64_t i0 = 0; i0 < g.batch; i0 += 32) {
-    const int64_t i = i0 + lane;
-    const int64_t n = i < g.batch ? (cross_len(g, i) + kRows - 1) / kRows : 0;
-    int64_t inc = n;
+__device__ __forceinline__ void tile_table(const CrossGeom& g, int* first) {
+  const int lane = threadIdx.x & 31, batch = (int)g.batch;
+  int sum = 0;
+  for (int i0 = 0; i0 < batch; i0 += 32) {
+    const int i = i0 + lane;
+    const int n = i < batch ? (int)((cross_len(g, i) + kRows - 1) / kRows) : 0;
+    int inc = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t x = __shfl_up_sync(0xffffffffu, inc, o);
+      const int x = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += x;
     }
-    if (i < g.batch) first[i] = sum + inc - n;
+    if (i < batch) first[i] = sum + inc - n;
     sum += __shfl_sync(0xffffffffu, inc, 31);
   }
-  if (lane == 0) first[g.batch] = sum;
+  if (lane == 0) first[batch] = sum;
 }
 // Unit u: sequences outermost, then key heads, then tiles, so that tiles that run
 // at the same time read the same queries. With a table the units are exactly the
 // tiles that have keys; without one every tile is a unit.
-__device__ __forceinline__ KvUnit kv_unit(const CrossGeom& g, const int64_t* first, int64_t u,
-                                          int n_it) {
+__device__ __forceinline__ KvUnit kv_unit(const CrossGeom& g, const int* first, int u, int n_it) {
   KvUnit w;
-  const int64_t all_tiles = (g.kv_len + kRows - 1) / kRows;
+  const uint32_t heads = (uint32_t)g.kv_heads;
+  uint32_t tiles, rest;
   if (kv_table(g)) {
-    int64_t lo = 0, hi = g.batch;  // first[lo] * kv_heads <= u < first[hi] * kv_heads
+    int lo = 0, hi = (int)g.batch;  // first[lo] * heads <= u < first[hi] * heads
+    const int x = (int)((uint32_t)u / heads);
     while (hi - lo > 1) {
-      const int64_t mid = (lo + hi) >> 1;
-      if (first[mid] * g.kv_heads <= u) lo = mid;
+      const int mid = (lo + hi) >> 1;
+      if (first[mid] <= x) lo = mid;
       else hi = mid;
     }
     w.b = lo;
-    const int64_t tiles = first[lo + 1] - first[lo];
-    const int64_t rest = u - first[lo] * g.kv_heads;
-    w.kvh = (int)(rest / tiles);
-    w.kt = (int)(rest % tiles);
+    tiles = (uint32_t)(first[lo + 1] - first[lo]);
+    rest = (uint32_t)u - (uint32_t)first[lo] * heads;
   } else {
-    w.b = u / (all_tiles * g.kv_heads);
-    const int64_t rest = u % (all_tiles * g.kv_heads);
-    w.kvh = (int)(rest / all_tiles);
-    w.kt = (int)(rest % all_tiles);
+    tiles = (uint32_t)((g.kv_len + kRows - 1) / kRows);
+    w.b = (uint32_t)u / (tiles * heads);
+    rest = (uint32_t)u % (tiles * heads);
   }
+  w.kvh = (int)(rest / tiles);
+  w.kt = (int)(rest % tiles);
   w.len = cross_len(g, w.b);
   w.i0 = 0;
   w.i1 = (int64_t)w.kt * kRows < w.len ? n_it : 0;
   w.slot = -1;
   return w;
 }
-__device__ __forceinline__ int64_t kv_units(const CrossGeom& g, const int64_t* first) {
-  return (kv_table(g) ? first[g.batch] : (g.kv_len + kRows - 1) / kRows * g.batch) * g.kv_heads;
+__device__ __forceinline__ int kv_units(const CrossGeom& g, const int* first) {
+  return (int)((kv_table(g) ? first[g.batch] : (g.kv_len + kRows - 1) / kRows * g.batch) * g.kv_heads);
 }
 // Units that go round whole; the others' steps are dealt out.
-__device__ __forceinline__ int64_t kv_whole(const TcArgs& a, int64_t units, int64_t ctas) {
+__device__ __forceinline__ int kv_whole(const TcArgs& a, int units, int ctas) {
   return a.piece == nullptr ? units : units / ctas * ctas;
 }
-__device__ __forceinline__ bool kv_next(const TcArgs& a, const int64_t* first, int64_t units, int n_it,
+__device__ __forceinline__ bool kv_next(const TcArgs& a, const int* first, int units, int n_it,
                                         KvWalk& k, KvUnit& w) {
-  const int64_t ctas = gridDim.x, cta = blockIdx.x;
-  const int64_t whole = kv_whole(a, units, ctas);
-  const int64_t total = (units - whole) * n_it;
+  const int ctas = (int)gridDim.x, cta = (int)blockIdx.x;
+  const int whole = kv_whole(a, units, ctas);
+  bool first_piece = false;
   if (k.s < 0) {
-    const int64_t u = snake(k.r, (int)cta, (int)ctas, whole);
+    const int u = snake(k.r, cta, ctas, whole);
     if (u >= 0) {
       ++k.r;
       w = kv_unit(a.g, first, u, n_it);
       return true;
     }
-    k.s = border(total, cta, ctas);
-    k.end = border(total, cta + 1, ctas);
+    const int64_t total = (int64_t)(units - whole) * n_it;
+    k.s = (int)border(total, cta, ctas);
+    k.end = (int)border(total, cta + 1, ctas);
+    first_piece = true;
   }
   if (k.s >= k.end) return false;
-  w = kv_unit(a.g, first, whole + k.s / n_it, n_it);
-  w.i0 = (int)(k.s % n_it);
-  const int64_t stop = w.i0 + (k.end - k.s);
-  w.i1 = (int)(stop < n_it ? stop : n_it);
-  w.slot = w.i1 - w.i0 == n_it ? -1 : k.s == border(total, cta, ctas) ? 0 : 1;
+  const int u = (int)((uint32_t)k.s / (uint32_t)n_it);
+  w = kv_unit(a.g, first, whole + u, n_it);
+  w.i0 = k.s - u * n_it;
+  const int stop = w.i0 + (k.end - k.s);
+  w.i1 = stop < n_it ? stop : n_it;
+  w.slot = w.i1 - w.i0 == n_it ? -1 : first_piece ? 0 : 1;
   k.s += w.i1 - w.i0;
   return true;
 }
@@ -1263,7 +1289,7 @@ struct Dkv {
   static constexpr int kStats = kRing + kStages * kStage;   // [stage][nlse, delta]
   static constexpr int kBar = kStats + kStages * 2 * kQ * 4;
   static constexpr int kBars = 2 * kKvBufs + 2 * kStages + 8 + 3;
-  static constexpr int kSmem = kBar + kBars * 8 + 16 + 8 * kOrder + 16 + 1024;
+  static constexpr int kSmem = kBar + kBars * 8 + 8 + 4 * kOrder + 1024;
   static_assert(kSmem <= 232448, "shared memory");
 };
 
@@ -1295,8 +1321,7 @@ cross_dkdv_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
   const uint32_t tslot = bars + 8u * F::kBars;
   uint32_t* tslot_ptr = reinterpret_cast<uint32_t*>(sp + F::kBar + 8 * F::kBars);
   // first[i]: key tiles of the sequences before i
-  int64_t* first = reinterpret_cast<int64_t*>(
-      sp + ((F::kBar + 8 * F::kBars + 8 + 15) / 16) * 16);
+  int* first = reinterpret_cast<int*>(sp + F::kBar + 8 * F::kBars + 8);
 
   const CrossGeom& g = a.g;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -1327,7 +1352,7 @@ cross_dkdv_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
   auto tS = [&](int t) { return tmem + 128u * t; };
   auto tDp = [&](int t) { return tmem + 128u * t + 64u; };
   const uint32_t tDv = tmem + 256u, tDk = tmem + 256u + HD;
-  const int64_t units = kv_units(g, first);
+  const int units = kv_units(g, first);
 
   if (warp == kTmaWarp) {
     if (elect_one()) {
@@ -1480,8 +1505,10 @@ cross_dkdv_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
     bool ok = true;
     int gs = 0, ru = 0;
     KvWalk walk;
-    KvUnit w;
-    while (kv_next(a, first, units, n_it, walk, w)) {
+    KvUnit next;
+    bool have = kv_next(a, first, units, n_it, walk, next);
+    while (have) {
+      const KvUnit w = next;
       const int n_steps = w.i1 - w.i0;
       for (int i = 0; i < n_steps; ++i) {
         const int s = gs + i;
@@ -1540,6 +1567,7 @@ cross_dkdv_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
         if (lane == 0) mbar_arrive(ds_full(t));
       }
       gs += n_steps;
+      have = kv_next(a, first, units, n_it, walk, next);  // while the last products run
       // warpgroup 0 stores dV, warpgroup 1 dK
       const int64_t kj = (int64_t)w.kt * kRows + row;
       const bool in = kj < g.kv_len;
@@ -1600,31 +1628,36 @@ cross_dkdv_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
 template <int HD>
 __global__ void __launch_bounds__(256)
 cross_dkdv_join(const __grid_constant__ TcArgs a, int ctas) {
-  __shared__ int64_t first[kOrder];
+  __shared__ int first[kOrder];
+  __shared__ int list[kMostPieces], count;
   wait_for_launch_before();
   const CrossGeom& g = a.g;
   if (kv_table(g) && threadIdx.x < 32) tile_table(g, first);
   __syncthreads();
   const int n_it = g.group * (a.q_pad / Dkv<HD>::kQ);
-  const int64_t units = kv_units(g, first), whole = kv_whole(a, units, ctas);
-  const int64_t total = (units - whole) * n_it, c = (int64_t)blockIdx.x + 1;
+  const int units = kv_units(g, first), whole = kv_whole(a, units, ctas);
+  const int64_t total = (int64_t)(units - whole) * n_it, c = (int64_t)blockIdx.x + 1;
   const int64_t s = border(total, c, ctas);
   if (s >= total) return;
   const int64_t begin = s / n_it * n_it;
   // the unit begins here, or an earlier border has it
   if (begin == s || border(total, c - 1, ctas) > begin) return;
-  const KvUnit w = kv_unit(g, first, whole + s / n_it, n_it);
+  const KvUnit w = kv_unit(g, first, whole + (int)(s / n_it), n_it);
+  if (threadIdx.x == 0) count = list_pieces(total, ctas, c, begin, n_it, list);
+  __syncthreads();
   constexpr int kVec = HD / 4;
+  const int t = (int)blockIdx.y / 4;  // four CTAs a tile
+  __nv_bfloat16* dst = t == 0 ? static_cast<__nv_bfloat16*>(a.dv) + w.b * g.dvs[0] + w.kvh * g.dvs[1]
+                              : static_cast<__nv_bfloat16*>(a.dk) + w.b * g.dks[0] + w.kvh * g.dks[1];
+  const int64_t step = t == 0 ? g.dvs[2] : g.dks[2];
+#pragma unroll 2
   for (int i = threadIdx.x; i < 32 * kVec; i += 256) {
-    const int rr = (int)blockIdx.y * 32 + i / kVec, t = rr / kRows, row = rr % kRows, col = i % kVec * 4;
+    const int row = (int)(blockIdx.y % 4) * 32 + i / kVec, col = i % kVec * 4;
     const int64_t kj = (int64_t)w.kt * kRows + row;
     if (col >= g.hd || kj >= g.kv_len) continue;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (kj < w.len) v = sum_pieces<HD>(a, total, ctas, c, begin, n_it, t, row, col);
-    __nv_bfloat16* dst =
-        t == 0 ? static_cast<__nv_bfloat16*>(a.dv) + w.b * g.dvs[0] + w.kvh * g.dvs[1] + kj * g.dvs[2]
-               : static_cast<__nv_bfloat16*>(a.dk) + w.b * g.dks[0] + w.kvh * g.dks[1] + kj * g.dks[2];
-    store_grad4(dst + col, v, t == 0 ? 1.f : g.scale);
+    if (kj < w.len) v = sum_pieces<HD>(a, list, count, t, row, col);
+    store_grad4(dst + kj * step + col, v, t == 0 ? 1.f : g.scale);
   }
 }
 
@@ -1662,6 +1695,9 @@ TcArgs args_of(const CrossGeom& g) {
   return a;
 }
 
+// Units and steps are counted in 32 bits.
+bool fits32(int64_t a, int64_t b, int64_t c) { return (double)a * b * c < 1e9; }
+
 template <int HD>
 magma_status_t fwd_tc(const void* q, const void* k, const void* v, TcArgs a, cudaStream_t s) {
   const CrossGeom& g = a.g;
@@ -1683,7 +1719,7 @@ magma_status_t fwd_tc(const void* q, const void* k, const void* v, TcArgs a, cud
 constexpr int64_t kIdleSteps = 24;
 bool deal(const CrossGeom& g, int64_t units, int64_t steps) {
   const int64_t n = num_sms();
-  if (units > 16 * n) return false;
+  if (units > 16 * n || n > kMostPieces || steps > (1 << 18)) return false;
   const int64_t idle = steps * (ceil_div(units, n) * n - units) / n;
   return std::max(idle, g.lens != nullptr ? steps / 2 : 0) > kIdleSteps;
 }
@@ -1742,7 +1778,8 @@ bool cross_tc_fwd_supported(const void* q, const void* k, const void* v, const v
   return dtype == MAGMA_DTYPE_BF16 && g.hd % 8 == 0 && g.kv_len > 0 && g.q_len > 0 &&
          tc_strides(q, g.qs, g.q_len) && tc_strides(k, g.ks, g.kv_len) &&
          tc_strides(v, g.vs, g.kv_len) && tc_strides(o, g.os, g.q_len) &&
-         (int64_t)g.group * ceil_div(g.q_len, kRows) < (1LL << 30);
+         fits32(g.batch, g.kv_heads, ceil_div(g.kv_len, kRows)) &&
+         fits32(g.batch, g.heads, ceil_div(g.q_len, 64));
 }
 
 bool cross_tc_bwd_supported(const void* q, const void* k, const void* v, const void* o,
@@ -1750,8 +1787,7 @@ bool cross_tc_bwd_supported(const void* q, const void* k, const void* v, const v
                             const CrossGeom& g, magma_dtype_t dtype) {
   return cross_tc_fwd_supported(q, k, v, o, g, dtype) && tc_strides(d_o, g.dos, g.q_len) &&
          tc_strides(dq, g.dqs, g.q_len) && tc_strides(dk, g.dks, g.kv_len) &&
-         tc_strides(dv, g.dvs, g.kv_len) &&
-         (int64_t)g.group * ceil_div(g.q_len, 64) < (1LL << 31);
+         tc_strides(dv, g.dvs, g.kv_len);
 }
 
 // Parts of a source: as many as fill the SMs, at least four key tiles each (a
