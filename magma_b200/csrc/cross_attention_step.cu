@@ -4,7 +4,8 @@
 // The work is one read of K and V (4 flops per byte and query row), so the
 // source is cut into chunks, a CTA takes one chunk of one key head with all
 // query rows that read it (row = shared head * q_len + query), and the parts
-// are joined by their log-sum-exp (cross_join_parts). Keys from the length on
+// are joined by their log-sum-exp: by the cluster that the chunks of a short source
+// form, through distributed shared memory, or by cross_join_parts. Keys from the length on
 // are filled with zeros: what lies behind a length is never read.
 //
 //   cross_step_bf16  warp-level MMA (m16n8k16): WM x (4 / WM) warps over rows
@@ -14,9 +15,10 @@
 //                    what bounds this. K and V tiles come through a cp.async ring.
 //   cross_step_f32   FMA pipe: scores by key, sums by column, four warps over
 //                    the keys.
-#include <cmath>
+#include <cooperative_groups.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "cross_attention.cuh"
 #include "sm100.cuh"
@@ -25,8 +27,10 @@ namespace magma {
 namespace {
 
 using namespace sm100;
+namespace cg = cooperative_groups;
 
 constexpr int kThreads = 128;
+constexpr int kMaxCluster = 8;
 constexpr int kKeys = 64;  // keys of a BF16 tile
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -37,9 +41,10 @@ struct StepArgs {
   int groups, each;     // CTAs that share a chunk's rows, rows of one of them
   int n_chunk;          // chunks of the longest source
   int64_t chunk;        // keys of a chunk, a multiple of the tile
+  int cluster;          // the chunks of a source are a cluster, which joins them itself
   void* o;
   float* lse;
-  float* part;          // [chunk][b][h][q][hd], if n_chunk > 1
+  float* part;          // [chunk][b][h][q][hd], of several chunks that are no cluster
   float* part_lse;      // [chunk][b][h][q], natural logarithm
 };
 
@@ -51,11 +56,12 @@ struct Chunk {
 __device__ __forceinline__ Chunk chunk_of(const StepArgs& a) {
   Chunk c;
   int64_t i = blockIdx.x;
+  c.index = (int)(i % a.n_chunk);
+  i /= a.n_chunk;
   c.r0 = (int)(i % a.groups) * a.each;
   i /= a.groups;
-  c.index = (int)(i % a.n_chunk);
-  c.kvh = i / a.n_chunk % a.g.kv_heads;
-  c.b = i / a.n_chunk / a.g.kv_heads;
+  c.kvh = i % a.g.kv_heads;
+  c.b = i / a.g.kv_heads;
   const int64_t len = cross_len(a.g, c.b);
   c.k0 = c.index * a.chunk < len ? c.index * a.chunk : len;
   c.k1 = len - c.k0 < a.chunk ? len : c.k0 + a.chunk;
@@ -113,13 +119,93 @@ __device__ __forceinline__ void store_part(const StepArgs& a, const Chunk& c, in
   int64_t h, q;
   const int64_t at = row_at(a.g, c, r, &h, &q);
   const int64_t rows = a.g.batch * a.g.heads * a.g.q_len;
-  if (a.n_chunk > 1) {
+  if (a.part != nullptr) {
     store4(a.part + (c.index * rows + at) * a.g.hd + col, v);
     if (col == 0) a.part_lse[c.index * rows + at] = lse;
   } else {
     store4(static_cast<T*>(a.o) + c.b * a.g.os[0] + h * a.g.os[1] + q * a.g.os[2] + col, v);
     if (col == 0 && a.lse != nullptr) a.lse[at] = lse;
   }
+}
+
+// exp in the base that a kernel keeps its maxima in, and a maximum as a natural
+// logarithm.
+template <bool LOG2> __device__ __forceinline__ float exp_of(float x) {
+  if constexpr (LOG2) return ex2_approx(x);
+  else return expf(x);
+}
+template <bool LOG2> __device__ __forceinline__ float ln_of(float x) { return LOG2 ? x * kLn2 : x; }
+
+// The CTA's sums over its warps, and those of the cluster's CTAs. so: [warp][R][P]
+// sums, relative to the maximum in sml[warp * R + row]; WN warps share a row of
+// ROWS. A row's sum over the warps is put in the place of its first warp's, where
+// the other CTAs read it. fin: [ROWS].
+template <typename T, bool LOG2, int ROWS, int R, int WN, int HD, int P>
+__device__ __forceinline__ void finish(const StepArgs& a, const Chunk& c, float* so,
+                                       const float2* sml, float2* fin) {
+  constexpr int kVec = HD / 4;
+  const int tid = threadIdx.x;
+  for (int i = tid; i < ROWS * kVec; i += kThreads) {
+    const int r = i / kVec, col = i % kVec * 4;
+    if (c.r0 + r >= a.rows || col >= a.g.hd) continue;
+    const int w0 = r / R * WN, rr = r % R;
+    float mm = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < WN; ++w) mm = fmaxf(mm, sml[(w0 + w) * R + rr].x);
+    float total = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < WN; ++w) {
+      const float2 ml = sml[(w0 + w) * R + rr];
+      const float f = mm == -INFINITY ? 0.f : exp_of<LOG2>(ml.x - mm);
+      total += f * ml.y;
+      float x[4];
+      load4(so + ((w0 + w) * R + rr) * P + col, x);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = fmaf(f, x[e], o[e]);
+    }
+    if (a.cluster) {
+      store4(so + (w0 * R + rr) * P + col, o);
+      if (col == 0) fin[r] = make_float2(mm, total);
+      continue;
+    }
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] *= inv;
+    store_part<T>(a, c, c.r0 + r, col, o, total == 0.f ? -INFINITY : ln_of<LOG2>(mm) + logf(total));
+  }
+  if (!a.cluster) return;
+  cg::cluster_group cluster = cg::this_cluster();
+  cluster.sync();
+  for (int i = c.index * kThreads + tid; i < ROWS * kVec; i += a.n_chunk * kThreads) {
+    const int r = i / kVec, col = i % kVec * 4;
+    if (c.r0 + r >= a.rows || col >= a.g.hd) continue;
+    const int at = (r / R * WN * R + r % R) * P + col;
+    float2 ml[kMaxCluster];
+    float mm = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < kMaxCluster; ++k) {
+      if (k >= a.n_chunk) continue;
+      ml[k] = cluster.map_shared_rank(fin, k)[r];
+      mm = fmaxf(mm, ml[k].x);
+    }
+    float total = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < kMaxCluster; ++k) {
+      if (k >= a.n_chunk) continue;
+      const float f = mm == -INFINITY ? 0.f : exp_of<LOG2>(ml[k].x - mm);
+      total += f * ml[k].y;
+      const float4 x = *reinterpret_cast<const float4*>(cluster.map_shared_rank(so, k) + at);
+      o[0] = fmaf(f, x.x, o[0]);
+      o[1] = fmaf(f, x.y, o[1]);
+      o[2] = fmaf(f, x.z, o[2]);
+      o[3] = fmaf(f, x.w, o[3]);
+    }
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] *= inv;
+    store_part<T>(a, c, c.r0 + r, col, o, total == 0.f ? -INFINITY : ln_of<LOG2>(mm) + logf(total));
+  }
+  cluster.sync();  // the others have read this CTA's sums
 }
 
 // ---------------------------------------------------------------- BF16
@@ -135,14 +221,18 @@ struct Bf {
 
 template <int HD, int WM>
 __global__ void __launch_bounds__(kThreads)
-cross_step_bf16(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __restrict__ k,
-                const __nv_bfloat16* __restrict__ v, const __grid_constant__ StepArgs a) {
+cross_step_bf16(const void* __restrict__ qv, const void* __restrict__ kv,
+                const void* __restrict__ vv, const __grid_constant__ StepArgs a) {
+  const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(qv);
+  const __nv_bfloat16* k = static_cast<const __nv_bfloat16*>(kv);
+  const __nv_bfloat16* v = static_cast<const __nv_bfloat16*>(vv);
   using F = Bf<HD>;
   constexpr int WN = 4 / WM;         // warps over the keys of a tile
   constexpr int KW = kKeys / WN;     // keys of a warp
   constexpr int NT = KW / 8;         // its 8-key tiles
   constexpr int DT = HD / 8;         // 8-column tiles of the output
   extern __shared__ __align__(128) uint8_t sm[];
+  __shared__ float2 fin[WM * 16];
   const uint32_t base = smem_u32(sm);
   const CrossGeom& g = a.g;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -300,30 +390,7 @@ cross_step_bf16(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __rest
     if ((lane & 3) == 0) sml[warp * 16 + r] = make_float2(m[i], l[i]);
   }
   __syncthreads();
-  constexpr int kVec = HD / 4;
-  for (int i = tid; i < WM * 16 * kVec; i += kThreads) {
-    const int r = i / kVec, col = i % kVec * 4;
-    if (r >= a.rows || col >= g.hd) continue;
-    const int w0 = (r / 16) * WN, rr = r % 16;
-    float mm = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < WN; ++w) mm = fmaxf(mm, sml[(w0 + w) * 16 + rr].x);
-    float total = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int w = 0; w < WN; ++w) {
-      const float2 ml = sml[(w0 + w) * 16 + rr];
-      const float f = mm == -INFINITY ? 0.f : ex2_approx(ml.x - mm);
-      total += f * ml.y;
-      float x[4];
-      load4(so + ((w0 + w) * 16 + rr) * (HD + 4) + col, x);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] = fmaf(f, x[e], o[e]);
-    }
-    const float inv = total == 0.f ? 0.f : 1.f / total;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] *= inv;
-    store_part<__nv_bfloat16>(a, c, r, col, o, total == 0.f ? -INFINITY : mm * kLn2 + logf(total));
-  }
+  finish<__nv_bfloat16, true, WM * 16, 16, WN, HD, HD + 4>(a, c, so, sml, fin);
 }
 
 // ----------------------------------------------------------------- F32
@@ -337,14 +404,17 @@ constexpr int kF32Keys = 32;  // keys of the four warps' groups
 
 template <int HD, int RT>
 __global__ void __launch_bounds__(kThreads, RT == 8 ? 3 : HD == 128 ? 4 : 5)
-cross_step_f32(const float* __restrict__ q, const float* __restrict__ k,
-               const float* __restrict__ v, const __grid_constant__ StepArgs a) {
+cross_step_f32(const void* __restrict__ qv, const void* __restrict__ kv,
+               const void* __restrict__ vv, const __grid_constant__ StepArgs a) {
+  const float* q = static_cast<const float*>(qv);
+  const float* k = static_cast<const float*>(kv);
+  const float* v = static_cast<const float*>(vv);
   constexpr int kPieces = HD / 16;         // of a lane's share of a K row
   constexpr int kHalves = 128 / HD;        // keys that a V load covers
   constexpr int kLoads = 8 / kHalves;      // V loads of a group
   constexpr int kVec = HD / 4;
-  __shared__ float sh[4 * RT * HD];        // q, at the end the warps' sums
-  __shared__ float2 sml[4 * RT];
+  __shared__ __align__(16) float sh[4 * RT * HD];  // q, at the end the warps' sums
+  __shared__ float2 sml[4 * RT], fin[RT];
   const CrossGeom& g = a.g;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int kk = lane >> 2, part = lane & 3;
@@ -455,28 +525,7 @@ cross_step_f32(const float* __restrict__ q, const float* __restrict__ k,
     if (lane == 0) sml[warp * RT + r] = make_float2(m[r], l[r]);
   }
   __syncthreads();
-  for (int i = tid; i < RT * kVec; i += kThreads) {
-    const int r = i / kVec, d = i % kVec * 4;
-    if (c.r0 + r >= a.rows || d >= g.hd) continue;
-    float mm = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) mm = fmaxf(mm, sml[w * RT + r].x);
-    float total = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const float2 ml = sml[w * RT + r];
-      const float f = mm == -INFINITY ? 0.f : expf(ml.x - mm);
-      total += f * ml.y;
-      float x[4];
-      load4(sh + (w * RT + r) * HD + d, x);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] = fmaf(f, x[e], o[e]);
-    }
-    const float inv = total == 0.f ? 0.f : 1.f / total;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] *= inv;
-    store_part<float>(a, c, c.r0 + r, d, o, total == 0.f ? -INFINITY : mm + logf(total));
-  }
+  finish<float, false, RT, RT, 4, HD, HD>(a, c, sh, sml, fin);
 }
 
 // ---------------------------------------------------------------- host side
@@ -507,23 +556,44 @@ int64_t chunk_keys(const CrossGeom& g, magma_dtype_t dtype) {
   return ceil_div(keys, tile) * tile;
 }
 
+// Whether the chunks of a source are the CTAs of a cluster: calls too small to fill
+// the GPU twice. Longer ones are cut finer than a cluster is large; these are
+// over in the time that the second launch of the join takes.
+bool use_cluster(const CrossGeom& g, magma_dtype_t dtype) {
+  const int64_t heads =
+      g.batch * g.kv_heads * ceil_div((int64_t)g.group * g.q_len, rows_each(g, dtype));
+  return heads * kMaxCluster <= 6LL * num_sms() && g.kv_len <= 8192;
+}
+
+template <typename K>
+magma_status_t launch_step(K kernel, const void* q, const void* k, const void* v, const StepArgs& a,
+                           unsigned ctas, int smem, cudaStream_t s, const char* what) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = a.cluster ? (unsigned)a.n_chunk : 1u;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = a.cluster ? 1 : 0;
+  return cuda_status(cudaLaunchKernelEx(&cfg, kernel, q, k, v, a), what);
+}
+
 template <int HD, int WM>
 magma_status_t launch_bf16(const void* q, const void* k, const void* v, const StepArgs& a,
                            unsigned ctas, cudaStream_t s) {
   const int smem = Bf<HD>::kSmem;
   if (magma_status_t st = cross_smem<cross_step_bf16<HD, WM>>(smem)) return st;
-  cross_step_bf16<HD, WM><<<ctas, kThreads, smem, s>>>(
-      static_cast<const __nv_bfloat16*>(q), static_cast<const __nv_bfloat16*>(k),
-      static_cast<const __nv_bfloat16*>(v), a);
-  return check_launch("cross_step_bf16");
+  return launch_step(cross_step_bf16<HD, WM>, q, k, v, a, ctas, smem, s, "cross_step_bf16");
 }
 
 template <int HD, int RT>
 magma_status_t launch_f32(const void* q, const void* k, const void* v, const StepArgs& a,
                           unsigned ctas, cudaStream_t s) {
-  cross_step_f32<HD, RT><<<ctas, kThreads, 0, s>>>(
-      static_cast<const float*>(q), static_cast<const float*>(k), static_cast<const float*>(v), a);
-  return check_launch("cross_step_f32");
+  return launch_step(cross_step_f32<HD, RT>, q, k, v, a, ctas, 0, s, "cross_step_f32");
 }
 
 }  // namespace
@@ -543,6 +613,7 @@ bool cross_step_rows(const CrossGeom& g, magma_dtype_t dtype) {
 }
 
 size_t cross_step_workspace(const CrossGeom& g, magma_dtype_t dtype) {
+  if (use_cluster(g, dtype)) return 0;
   const int64_t n = ceil_div(g.kv_len, chunk_keys(g, dtype));
   return n <= 1 ? 0 : (size_t)n * g.batch * g.heads * g.q_len * (g.hd + 1) * sizeof(float);
 }
@@ -560,12 +631,14 @@ magma_status_t cross_step_run(const void* q, const void* k, const void* v, void*
   const int64_t tile = tile_keys(dtype);
   const int64_t rows = g.batch * g.heads * g.q_len;
   const size_t each = (size_t)rows * (g.hd + 1) * sizeof(float);
-  a.chunk = chunk_keys(g, dtype);
+  a.cluster = use_cluster(g, dtype) ? 1 : 0;
+  a.chunk = a.cluster ? ceil_div(g.kv_len, kMaxCluster * tile) * tile : chunk_keys(g, dtype);
   const int64_t room = workspace && aligned16(workspace) ? (int64_t)(workspace_bytes / each) : 0;
-  if (ceil_div(g.kv_len, a.chunk) > std::max<int64_t>(1, room))
+  if (!a.cluster && ceil_div(g.kv_len, a.chunk) > std::max<int64_t>(1, room))
     a.chunk = ceil_div(g.kv_len, std::max<int64_t>(1, room) * tile) * tile;
   a.n_chunk = (int)ceil_div(g.kv_len, a.chunk);
-  if (a.n_chunk > 1) {
+  if (a.n_chunk == 1) a.cluster = 0;
+  if (a.n_chunk > 1 && !a.cluster) {
     a.part = static_cast<float*>(workspace);
     a.part_lse = a.part + (size_t)a.n_chunk * rows * g.hd;
   }
@@ -580,7 +653,7 @@ magma_status_t cross_step_run(const void* q, const void* k, const void* v, void*
                            : (a.rows <= 16 ? launch_bf16<128, 1> : a.rows <= 32 ? launch_bf16<128, 2> : launch_bf16<128, 4>);
     st = run(q, k, v, a, ctas, s);
   }
-  if (st || a.n_chunk == 1) return st;
+  if (st || a.part == nullptr) return st;
   return cross_join_parts(a.part, a.part_lse, o, lse, g, a.n_chunk, dtype, s);
 }
 

@@ -853,6 +853,7 @@ cross_dq_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
             const __grid_constant__ TcArgs a) {
   using F = Dq<HD>;
   extern __shared__ uint8_t smem_raw[];
+  wait_for_launch_before();
   uint8_t* sp;
   const uint32_t base = align1024(smem_raw, &sp);
   auto sQ = [&](int t) { return base + F::kQ + 2 * t * F::kTile; };
@@ -1300,6 +1301,7 @@ cross_dkdv_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
               const __grid_constant__ TcArgs a) {
   using F = Dkv<HD>;
   extern __shared__ uint8_t smem_raw[];
+  wait_for_launch_before();
   uint8_t* sp;
   const uint32_t base = align1024(smem_raw, &sp);
   auto sK = [&](int kb) { return base + F::kKv + 2 * kb * F::kTile; };
@@ -1749,8 +1751,9 @@ magma_status_t bwd_tc(const void* q, const void* k, const void* v, const void* d
     const int64_t units = ceil_div(g.kv_len, kRows) * g.kv_heads * g.batch;
     a.piece = deal_dkdv(g) ? piece : nullptr;
     const unsigned ctas = (unsigned)(a.piece ? num_sms() : std::min<int64_t>(units, num_sms()));
-    cross_dkdv_tc<HD><<<ctas, kThreads, F::kSmem, s>>>(mq, mg, mk, mv, a);
-    if (magma_status_t st = check_launch("cross_dkdv_tc")) return st;
+    if (magma_status_t st = launch_after(cross_dkdv_tc<HD>, dim3(ctas), kThreads, F::kSmem, s,
+                                         "cross_dkdv_tc", mq, mg, mk, mv, a))
+      return st;
     if (a.piece)
       if (magma_status_t st = launch_after(cross_dkdv_join<HD>, dim3(ctas - 1, 8), 256, 0, s,
                                            "cross_dkdv_join", a, (int)ctas))
@@ -1765,8 +1768,9 @@ magma_status_t bwd_tc(const void* q, const void* k, const void* v, const void* d
   const int64_t units = (int64_t)a.n_pairs * g.kv_heads * g.batch;
   a.piece = deal_dq(g) ? piece : nullptr;
   const unsigned ctas = (unsigned)(a.piece ? num_sms() : std::min<int64_t>(units, num_sms()));
-  cross_dq_tc<HD><<<ctas, kThreads, F::kSmem, s>>>(mq, mg, mk, mv, a);
-  if (magma_status_t st = check_launch("cross_dq_tc")) return st;
+  if (magma_status_t st = launch_after(cross_dq_tc<HD>, dim3(ctas), kThreads, F::kSmem, s,
+                                       "cross_dq_tc", mq, mg, mk, mv, a))
+    return st;
   if (a.piece == nullptr) return MAGMA_OK;
   return launch_after(cross_dq_join<HD>, dim3(ctas - 1, 8), 256, 0, s, "cross_dq_join", a, (int)ctas);
 }
