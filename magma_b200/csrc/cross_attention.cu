@@ -121,11 +121,12 @@ size_t magma_cross_attention_bwd_workspace_size(int64_t batch, int64_t heads, in
                                                 int64_t q_len, int64_t kv_len, int64_t head_dim,
                                                 magma_dtype_t dtype) {
   if (batch <= 0 || heads <= 0 || q_len <= 0) return 0;
-  const size_t delta = sizeof(float) * (size_t)batch * (size_t)heads * (size_t)q_len;
-  if (dtype != MAGMA_DTYPE_BF16 || head_dim % 8 != 0 ||
-      !has_work(batch, heads, kv_heads, q_len, kv_len, head_dim))
-    return delta;
-  return cross_tc_bwd_workspace(sizes(batch, heads, kv_heads, q_len, kv_len, head_dim));
+  // without keys dQ = 0 and nothing but delta is formed
+  if (!has_work(batch, heads, kv_heads, q_len, kv_len, head_dim))
+    return (sizeof(float) * (size_t)batch * (size_t)heads * (size_t)q_len + 15) / 16 * 16;
+  const CrossGeom g = sizes(batch, heads, kv_heads, q_len, kv_len, head_dim);
+  return dtype == MAGMA_DTYPE_BF16 && head_dim % 8 == 0 ? cross_tc_bwd_workspace(g)
+                                                        : cross_simt_bwd_workspace(g);
 }
 
 magma_status_t magma_cross_attention_bwd(
@@ -163,7 +164,7 @@ magma_status_t magma_cross_attention_bwd(
                 "%s: a 16-byte aligned workspace of %zu bytes is needed", fn, need);
   if (cross_tc_bwd_supported(q, k, v, o, d_o, dq, dk, dv, g, dtype))
     return cross_bwd_tc_run(q, k, v, o, d_o, lse, dq, dk, dv, workspace, g, (cudaStream_t)stream);
-  return cross_bwd_simt(q, k, v, o, d_o, lse, dq, dk, dv, static_cast<float*>(workspace), g, dtype,
+  return cross_bwd_simt(q, k, v, o, d_o, lse, dq, dk, dv, g, dtype, workspace, workspace_bytes,
                         (cudaStream_t)stream);
 }
 

@@ -54,10 +54,11 @@ size_t cross_simt_fwd_workspace(const CrossGeom& g);
 magma_status_t cross_fwd_simt(const void* q, const void* k, const void* v, void* o, float* lse,
                               const CrossGeom& g, magma_dtype_t dtype, void* workspace,
                               size_t workspace_bytes, cudaStream_t s);
+size_t cross_simt_bwd_workspace(const CrossGeom& g);
 magma_status_t cross_bwd_simt(const void* q, const void* k, const void* v, const void* o,
                               const void* d_o, const float* lse, void* dq, void* dk, void* dv,
-                              float* delta, const CrossGeom& g, magma_dtype_t dtype,
-                              cudaStream_t s);
+                              const CrossGeom& g, magma_dtype_t dtype, void* workspace,
+                              size_t workspace_bytes, cudaStream_t s);
 
 // cross_attention_step.cu: few query rows per key head (_rows: as far as sizes
 // say), 16-byte aligned positions.

@@ -154,6 +154,14 @@ __device__ __forceinline__ int64_t row_index(const CrossGeom& g, const Block& x,
   return (x.b * g.heads + x.kvh * g.group + r / g.q_len) * g.q_len + r % g.q_len;
 }
 
+// Tiles [t0, t1) of a part.
+__device__ __forceinline__ void part_tiles(int64_t tiles, int part, int parts, int64_t& t0,
+                                           int64_t& t1) {
+  const int64_t each = (tiles + parts - 1) / parts;
+  t0 = part * each < tiles ? part * each : tiles;
+  t1 = tiles - t0 < each ? tiles : t0 + each;
+}
+
 struct FwdArgs {
   CrossGeom g;
   int parts;
@@ -162,35 +170,39 @@ struct FwdArgs {
 };
 
 // ------------------------------------------------------------------ forward
-// 128 threads; thread (ty, tx) has rows ty 4 + {0..3} and + 32, keys tx + 16 j,
-// columns tx 4 + {0..3} and + 64. K and V of a tile have a buffer each: V comes
-// in under the scores, the next K under the sums.
-template <int HD>
+// 128 threads; thread (ty, tx) has rows ty 4 + {0..3} and, of a 64-row tile, + 32,
+// keys tx + 16 j, columns tx 4 + {0..3} and + 64. K and V of a tile have a buffer
+// each: V comes in under the scores, the next K under the sums. 64-row tiles read
+// shared memory least (half its bandwidth at the FMA pipe's rate, 32-row tiles
+// three quarters); 32-row tiles are for calls that would otherwise not give the
+// SMs enough CTAs to even out.
+template <int HD, int BM>
 struct FwdTile {
   static constexpr int kKeys = HD == 64 ? 64 : 32;
+  static constexpr int kPp = BM + 4;  // pitch of the probabilities
   static constexpr int kSmem =
-      ((kRows + 2 * kKeys) * kPitch<HD> + kKeys * kP) * 4 + kRows * 8;
+      ((BM + 2 * kKeys) * kPitch<HD> + kKeys * kPp) * 4 + BM * 8;
 };
 
-template <int HD, typename T, bool VEC>
+template <int HD, int BM, typename T, bool VEC>
 __global__ void __launch_bounds__(128)
 cross_fwd(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
           T* __restrict__ o, float* __restrict__ lse, const __grid_constant__ FwdArgs a) {
-  constexpr int BN = FwdTile<HD>::kKeys, NK = BN / 16, ND = HD / 16;
+  constexpr int BN = FwdTile<HD, BM>::kKeys, kP = FwdTile<HD, BM>::kPp;
+  constexpr int NI = BM / 8, NP = NI / 2, NK = BN / 16, ND = HD / 16;
   extern __shared__ __align__(16) float sm[];
   float* Qs = sm;
-  float* Ks = Qs + kRows * kPitch<HD>;
+  float* Ks = Qs + BM * kPitch<HD>;
   float* Vs = Ks + BN * kPitch<HD>;
   float* Ps = Vs + BN * kPitch<HD>;                        // [key][row]
   int64_t* offs = reinterpret_cast<int64_t*>(Ps + BN * kP);  // of the query rows
   const CrossGeom& g = a.g;
   const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
   const int64_t rows = (int64_t)g.group * g.q_len;
-  const Block x = block_of((rows + kRows - 1) / kRows, g.kv_heads, a.parts);
-  const int64_t r0 = x.tile * kRows, len = cross_len(g, x.b);
-  const int64_t tiles = (len + BN - 1) / BN, each = (tiles + a.parts - 1) / a.parts;
-  const int64_t t0 = x.part * each < tiles ? x.part * each : tiles;
-  const int64_t t1 = tiles - t0 < each ? tiles : t0 + each;
+  const Block x = block_of((rows + BM - 1) / BM, g.kv_heads, a.parts);
+  const int64_t r0 = x.tile * BM, len = cross_len(g, x.b);
+  int64_t t0, t1;
+  part_tiles((len + BN - 1) / BN, x.part, a.parts, t0, t1);
   const T* kh = k + x.b * g.ks[0] + x.kvh * g.ks[1];
   const T* vh = v + x.b * g.vs[0] + x.kvh * g.vs[1];
   auto row = [&](int i) { return ty * 4 + (i & 3) + 32 * (i >> 2); };
@@ -204,29 +216,29 @@ cross_fwd(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict_
       return t * BN + r < len ? (t * BN + r) * g.vs[2] : (int64_t)-1;
     });
   };
-  if (tid < kRows) offs[tid] = row_offset(g, x, g.qs, r0 + tid);
+  if (tid < BM) offs[tid] = row_offset(g, x, g.qs, r0 + tid);
   __syncthreads();
-  load_rows<HD, kRows, VEC>(Qs, q, g.hd, [&](int r) { return offs[r]; });
+  load_rows<HD, BM, VEC>(Qs, q, g.hd, [&](int r) { return offs[r]; });
   if (t0 < t1) load_k(t0);
   cp_commit();
-  u64 acc[4][ND];
-  float m[8], l[8];
+  u64 acc[NP][ND];
+  float m[NI], l[NI];
 #pragma unroll
-  for (int p = 0; p < 4; ++p)
+  for (int p = 0; p < NP; ++p)
 #pragma unroll
     for (int c = 0; c < ND; ++c) acc[p][c] = 0ull;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) m[i] = -INFINITY, l[i] = 0.f;
+  for (int i = 0; i < NI; ++i) m[i] = -INFINITY, l[i] = 0.f;
   for (int64_t t = t0; t < t1; ++t) {
     cp_wait<0>();
     __syncthreads();  // K is there; the last tile's V and P have been used
     load_v(t);
     cp_commit();
-    float s[8][NK];
+    float s[NI][NK];
     dots<HD>(s, Qs, Ks, row, [&](int j) { return tx + 16 * j; });
-    float alpha[8];
+    float alpha[NI];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < NI; ++i) {
       float mx = -INFINITY;
 #pragma unroll
       for (int j = 0; j < NK; ++j) {
@@ -250,11 +262,11 @@ cross_fwd(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict_
 #pragma unroll
     for (int j = 0; j < NK; ++j)
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < NI / 4; ++h)
         *reinterpret_cast<float4*>(Ps + (tx + 16 * j) * kP + ty * 4 + 32 * h) =
             make_float4(s[4 * h][j], s[4 * h + 1][j], s[4 * h + 2][j], s[4 * h + 3][j]);
 #pragma unroll
-    for (int p = 0; p < 4; ++p) {
+    for (int p = 0; p < NP; ++p) {
       const u64 f = f2_pack(alpha[2 * p], alpha[2 * p + 1]);
 #pragma unroll
       for (int c = 0; c < ND; ++c) acc[p][c] = f2_mul(acc[p][c], f);
@@ -265,16 +277,20 @@ cross_fwd(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict_
     cp_commit();
 #pragma unroll 4
     for (int key = 0; key < BN; ++key) {
-      const ulonglong2 lo = *reinterpret_cast<const ulonglong2*>(Ps + key * kP + ty * 4);
-      const ulonglong2 hi = *reinterpret_cast<const ulonglong2*>(Ps + key * kP + ty * 4 + 32);
-      const u64 left[4] = {lo.x, lo.y, hi.x, hi.y};
+      u64 left[NP];
+#pragma unroll
+      for (int h = 0; h < NI / 4; ++h) {
+        const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(Ps + key * kP + ty * 4 + 32 * h);
+        left[2 * h] = x.x;
+        left[2 * h + 1] = x.y;
+      }
       add_products(acc, left, Vs + key * kPitch<HD>, tx);
     }
   }
   cp_wait<0>();
   const int64_t all = g.batch * g.heads * g.q_len;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < NI; ++i) {
 #pragma unroll
     for (int w = 8; w > 0; w >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], w);
     const int64_t r = r0 + row(i);
@@ -341,6 +357,14 @@ __device__ __forceinline__ void probs(float& s, float& dp, bool on, float scale,
   dp = on ? p * (dp - delta) : 0.f;
 }
 
+// Where few tiles have many steps, a tile's steps are split into parts, whose F32
+// sums are added up in order by cross_sum.
+struct BwdArgs {
+  CrossGeom g;
+  int kv_parts, q_parts;  // of the query rows in dK and dV, of the keys in dQ
+  float* part;            // [part][dV, dK][b][kvh][key][hd], or [part][b][h][q][hd]
+};
+
 // --------------------------------------------------------------- dK and dV
 // One CTA of 256 threads per (key tile, key head, sequence). Scores: thread (ty,
 // tx) has rows ty 4 + {0..3}, keys tx + 16 j. Sums: keys ty 4 + {0..3}, columns
@@ -352,7 +376,8 @@ __global__ void __launch_bounds__(256, HD == 64 ? 2 : 1)
 cross_dkdv(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
            const T* __restrict__ d_o, const float* __restrict__ lse,
            const float* __restrict__ delta, T* __restrict__ dk, T* __restrict__ dv,
-           const __grid_constant__ CrossGeom g) {
+           const __grid_constant__ BwdArgs a) {
+  const CrossGeom& g = a.g;
   constexpr int ND = HD / 16;
   extern __shared__ __align__(16) float sm[];
   float* Ks = sm;
@@ -366,9 +391,11 @@ cross_dkdv(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict
   int64_t* qo = reinterpret_cast<int64_t*>(Es + kRows);
   int64_t* go = qo + kRows;
   const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
-  const Block x = block_of((g.kv_len + kRows - 1) / kRows, g.kv_heads, 1);
+  const Block x = block_of((g.kv_len + kRows - 1) / kRows, g.kv_heads, a.kv_parts);
   const int64_t k0 = x.tile * kRows, len = cross_len(g, x.b);
   const int64_t rows = (int64_t)g.group * g.q_len;
+  int64_t t0, t1;
+  part_tiles((rows + kRows - 1) / kRows, x.part, a.kv_parts, t0, t1);
   u64 adk[2][ND], adv[2][ND];
 #pragma unroll
   for (int p = 0; p < 2; ++p)
@@ -380,7 +407,7 @@ cross_dkdv(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict
     };
     load_rows<HD, kRows, VEC>(Ks, k + x.b * g.ks[0] + x.kvh * g.ks[1], g.hd, key(g.ks[2]));
     load_rows<HD, kRows, VEC>(Vs, v + x.b * g.vs[0] + x.kvh * g.vs[1], g.hd, key(g.vs[2]));
-    for (int64_t r0 = 0; r0 < rows; r0 += kRows) {
+    for (int64_t r0 = t0 * kRows; r0 < t1 * kRows; r0 += kRows) {
       __syncthreads();
       if (tid < kRows) {
         qo[tid] = row_offset(g, x, g.qs, r0 + tid);
@@ -432,6 +459,13 @@ cross_dkdv(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict
       float a0, a1, b0, b1;
       f2_unpack(adk[i >> 1][c], a0, a1);
       f2_unpack(adv[i >> 1][c], b0, b1);
+      if (a.kv_parts > 1) {
+        const int64_t all = g.batch * g.kv_heads * g.kv_len * g.hd;
+        const int64_t at = ((x.b * g.kv_heads + x.kvh) * g.kv_len + kj) * g.hd + d;
+        a.part[2 * x.part * all + at] = i & 1 ? b1 : b0;
+        a.part[(2 * x.part + 1) * all + at] = i & 1 ? a1 : a0;
+        continue;
+      }
       dkh[kj * g.dks[2] + d] = from_f32<T>((i & 1 ? a1 : a0) * g.scale);
       dvh[kj * g.dvs[2] + d] = from_f32<T>(i & 1 ? b1 : b0);
     }
@@ -447,7 +481,8 @@ template <int HD, typename T, bool VEC>
 __global__ void __launch_bounds__(256, HD == 64 ? 2 : 1)
 cross_dq(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
          const T* __restrict__ d_o, const float* __restrict__ lse,
-         const float* __restrict__ delta, T* __restrict__ dq, const __grid_constant__ CrossGeom g) {
+         const float* __restrict__ delta, T* __restrict__ dq, const __grid_constant__ BwdArgs a) {
+  const CrossGeom& g = a.g;
   constexpr int ND = HD / 16;
   extern __shared__ __align__(16) float sm[];
   float* Qs = sm;
@@ -459,8 +494,10 @@ cross_dq(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__
   int64_t* go = qo + kRows;
   const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
   const int64_t rows = (int64_t)g.group * g.q_len;
-  const Block x = block_of((rows + kRows - 1) / kRows, g.kv_heads, 1);
+  const Block x = block_of((rows + kRows - 1) / kRows, g.kv_heads, a.q_parts);
   const int64_t r0 = x.tile * kRows, len = cross_len(g, x.b);
+  int64_t t0, t1;
+  part_tiles((len + kRows - 1) / kRows, x.part, a.q_parts, t0, t1);
   const T* kh = k + x.b * g.ks[0] + x.kvh * g.ks[1];
   const T* vh = v + x.b * g.vs[0] + x.kvh * g.vs[1];
   if (tid < kRows) {
@@ -480,7 +517,7 @@ cross_dq(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__
   for (int p = 0; p < 2; ++p)
 #pragma unroll
     for (int c = 0; c < ND; ++c) acc[p][c] = 0ull;
-  for (int64_t k0 = 0; k0 < len; k0 += kRows) {
+  for (int64_t k0 = t0 * kRows; k0 < t1 * kRows; k0 += kRows) {
     __syncthreads();
     auto key = [&](int64_t st) {
       return [&g, k0, len, st](int r) { return k0 + r < len ? (k0 + r) * st : (int64_t)-1; };
@@ -520,8 +557,35 @@ cross_dq(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__
       if (d >= g.hd) continue;
       float lo, hi;
       f2_unpack(acc[i >> 1][c], lo, hi);
-      dq[o + d] = from_f32<T>((i & 1 ? hi : lo) * g.scale);
+      const float y = i & 1 ? hi : lo;
+      if (a.q_parts > 1)
+        a.part[(x.part * g.batch * g.heads * g.q_len + row_index(g, x, r0 + row(i))) * g.hd + d] = y;
+      else
+        dq[o + d] = from_f32<T>(y * g.scale);
     }
+  }
+}
+
+// out[b][h][n][d] = mul * sum over the parts, in order; `step`: elements from a part
+// to the next.
+struct SumArgs {
+  const float* part;
+  int64_t step, heads, n, total;
+  int64_t st[3];
+  int parts, hd;
+  float mul;
+};
+template <typename T>
+__global__ void __launch_bounds__(256) cross_sum(const SumArgs a, T* __restrict__ out) {
+  wait_for_launch_before();
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.total;
+       i += (int64_t)gridDim.x * 256) {
+    float s = 0.f;
+#pragma unroll 4
+    for (int p = 0; p < a.parts; ++p) s += a.part[p * a.step + i];
+    const int64_t row = i / a.hd, n = row % a.n, bh = row / a.n;
+    out[bh / a.heads * a.st[0] + bh % a.heads * a.st[1] + n * a.st[2] + i % a.hd] =
+        from_f32<T>(s * a.mul);
   }
 }
 
@@ -534,34 +598,80 @@ magma_status_t blocks_of(int64_t tiles, int64_t heads, int64_t batch, int64_t pa
   return MAGMA_OK;
 }
 
-int64_t row_tiles(const CrossGeom& g) { return ceil_div((int64_t)g.group * g.q_len, kRows); }
+int64_t row_tiles(const CrossGeom& g, int rows = kRows) {
+  return ceil_div((int64_t)g.group * g.q_len, rows);
+}
 
 // Rows in 16-byte pieces.
 bool pieces(const void* p, const int64_t (&st)[3]) {
   return aligned16(p) && st[0] % 4 == 0 && st[1] % 4 == 0 && st[2] % 4 == 0;
 }
 
+// Rows of a forward tile: 32 where 64-row tiles would be fewer than four per SM
+// (8 x 12 heads, 200 queries over 83 to 333 keys: TIME32).
+int fwd_rows(const CrossGeom& g) {
+  return row_tiles(g) * g.kv_heads * g.batch < 4LL * num_sms() ? 32 : 64;
+}
+
+template <int HD, int BM, typename T, bool VEC>
+magma_status_t fwd_rows_of(const void* q, const void* k, const void* v, void* o, float* lse,
+                           const FwdArgs& a, cudaStream_t s) {
+  const CrossGeom& g = a.g;
+  constexpr int smem = FwdTile<HD, BM>::kSmem;
+  unsigned n;
+  if (magma_status_t st = cross_smem<cross_fwd<HD, BM, T, VEC>>(smem)) return st;
+  if (magma_status_t st = blocks_of(row_tiles(g, BM), g.kv_heads, g.batch, a.parts, &n)) return st;
+  cross_fwd<HD, BM, T, VEC><<<n, 128, smem, s>>>((const T*)q, (const T*)k, (const T*)v, (T*)o, lse, a);
+  return check_launch("cross_fwd");
+}
 template <int HD, typename T, bool VEC>
 magma_status_t fwd(const void* q, const void* k, const void* v, void* o, float* lse,
                    const FwdArgs& a, cudaStream_t s) {
-  const CrossGeom& g = a.g;
-  constexpr int smem = FwdTile<HD>::kSmem;
-  unsigned n;
-  if (magma_status_t st = cross_smem<cross_fwd<HD, T, VEC>>(smem)) return st;
-  if (magma_status_t st = blocks_of(row_tiles(g), g.kv_heads, g.batch, a.parts, &n)) return st;
-  cross_fwd<HD, T, VEC><<<n, 128, smem, s>>>((const T*)q, (const T*)k, (const T*)v, (T*)o, lse, a);
-  return check_launch("cross_fwd");
+  return fwd_rows(a.g) == 32 ? fwd_rows_of<HD, 32, T, VEC>(q, k, v, o, lse, a, s)
+                             : fwd_rows_of<HD, 64, T, VEC>(q, k, v, o, lse, a, s);
+}
+
+// Parts of a tile's steps where the tiles do not give every SM two CTAs: as many as
+// give it four, of at least two steps.
+int64_t grad_parts(int64_t ctas, int64_t steps) {
+  if (ctas >= 2 * num_sms()) return 1;
+  return std::max<int64_t>(1, std::min<int64_t>(4LL * num_sms() / std::max<int64_t>(ctas, 1), steps / 2));
+}
+int64_t kv_parts(const CrossGeom& g) {
+  return grad_parts(ceil_div(g.kv_len, kRows) * g.kv_heads * g.batch, row_tiles(g));
+}
+int64_t q_parts(const CrossGeom& g) {
+  return grad_parts(row_tiles(g) * g.kv_heads * g.batch, ceil_div(g.kv_len, kRows));
+}
+size_t kv_part_bytes(const CrossGeom& g) {
+  return 2 * sizeof(float) * (size_t)g.batch * g.kv_heads * g.kv_len * g.hd;
+}
+size_t q_part_bytes(const CrossGeom& g) {
+  return sizeof(float) * (size_t)g.batch * g.heads * g.q_len * g.hd;
+}
+size_t delta_bytes(const CrossGeom& g) {
+  return (sizeof(float) * (size_t)g.batch * g.heads * g.q_len + 15) / 16 * 16;
+}
+
+template <typename T>
+magma_status_t sum_parts(const float* part, int64_t step, int64_t parts, int64_t batch, int64_t heads,
+                         int64_t n, int hd, const int64_t (&st)[3], float mul, void* out,
+                         cudaStream_t s) {
+  SumArgs a{part, step, heads, n, batch * heads * n * hd, {st[0], st[1], st[2]}, (int)parts, hd, mul};
+  const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div(a.total, 256), 8LL * num_sms());
+  return launch_after(cross_sum<T>, dim3(blocks), 256, 0, s, "cross_sum", a, static_cast<T*>(out));
 }
 
 template <int HD, typename T, bool VEC>
 magma_status_t bwd(const void* q, const void* k, const void* v, const void* o, const void* d_o,
-                   const float* lse, void* dq, void* dk, void* dv, float* delta,
-                   const CrossGeom& g, cudaStream_t s) {
+                   const float* lse, void* dq, void* dk, void* dv, float* delta, const BwdArgs& a,
+                   cudaStream_t s) {
+  const CrossGeom& g = a.g;
   if (magma_status_t st = cross_smem<cross_dkdv<HD, T, VEC>>(kDkvSmem<HD>)) return st;
   if (magma_status_t st = cross_smem<cross_dq<HD, T, VEC>>(kDqSmem<HD>)) return st;
   unsigned nq = 0, nk = 0;
-  if (magma_status_t st = blocks_of(row_tiles(g), g.kv_heads, g.batch, 1, &nq)) return st;
-  if (magma_status_t st = blocks_of(ceil_div(g.kv_len, kRows), g.kv_heads, g.batch, 1, &nk)) return st;
+  if (magma_status_t st = blocks_of(row_tiles(g), g.kv_heads, g.batch, a.q_parts, &nq)) return st;
+  if (magma_status_t st = blocks_of(ceil_div(g.kv_len, kRows), g.kv_heads, g.batch, a.kv_parts, &nk)) return st;
   if (nq > 0) {
     const int64_t cap = 16LL * num_sms();
     const int64_t nd = ceil_div(g.batch * g.heads * g.q_len, 8);
@@ -570,13 +680,25 @@ magma_status_t bwd(const void* q, const void* k, const void* v, const void* o, c
   }
   if (nk > 0) {
     cross_dkdv<HD, T, VEC><<<nk, 256, kDkvSmem<HD>, s>>>((const T*)q, (const T*)k, (const T*)v,
-                                                         (const T*)d_o, lse, delta, (T*)dk, (T*)dv, g);
+                                                         (const T*)d_o, lse, delta, (T*)dk, (T*)dv, a);
     if (magma_status_t st = check_launch("cross_dkdv")) return st;
+    if (a.kv_parts > 1) {
+      const int64_t all = g.batch * g.kv_heads * g.kv_len * g.hd;
+      if (magma_status_t st = sum_parts<T>(a.part, 2 * all, a.kv_parts, g.batch, g.kv_heads, g.kv_len,
+                                           g.hd, g.dvs, 1.f, dv, s))
+        return st;
+      if (magma_status_t st = sum_parts<T>(a.part + all, 2 * all, a.kv_parts, g.batch, g.kv_heads,
+                                           g.kv_len, g.hd, g.dks, g.scale, dk, s))
+        return st;
+    }
   }
   if (nq > 0) {
     cross_dq<HD, T, VEC><<<nq, 256, kDqSmem<HD>, s>>>((const T*)q, (const T*)k, (const T*)v,
-                                                      (const T*)d_o, lse, delta, (T*)dq, g);
-    return check_launch("cross_dq");
+                                                      (const T*)d_o, lse, delta, (T*)dq, a);
+    if (magma_status_t st = check_launch("cross_dq")) return st;
+    if (a.q_parts > 1)
+      return sum_parts<T>(a.part, g.batch * g.heads * g.q_len * g.hd, a.q_parts, g.batch, g.heads,
+                          g.q_len, g.hd, g.dqs, g.scale, dq, s);
   }
   return MAGMA_OK;
 }
@@ -586,9 +708,9 @@ magma_status_t bwd(const void* q, const void* k, const void* v, const void* o, c
 // tiles take 73 us whole and 84 us in two parts each; 8 heads over 2, 40 queries,
 // 3000 keys: 42 us in 11 parts of four tiles, 34 us in 23 of two.)
 int64_t wanted_parts(const CrossGeom& g) {
-  const int64_t ctas = std::max<int64_t>(row_tiles(g) * g.kv_heads * g.batch, 1);
+  const int64_t ctas = std::max<int64_t>(row_tiles(g, fwd_rows(g)) * g.kv_heads * g.batch, 1);
   const int64_t tiles = ceil_div(g.kv_len, g.hd <= 64 ? 64 : 32);
-  if (ctas >= 2 * num_sms()) return 1;
+  if (ctas >= 4 * num_sms()) return 1;
   return std::max<int64_t>(1, std::min<int64_t>(6LL * num_sms() / ctas, tiles / 2));
 }
 
@@ -628,19 +750,35 @@ magma_status_t cross_fwd_simt(const void* q, const void* k, const void* v, void*
   return cross_join_parts(a.part, a.part_lse, o, lse, g, a.parts, dtype, s);
 }
 
+size_t cross_simt_bwd_workspace(const CrossGeom& g) {
+  const int64_t nk = kv_parts(g), nq = q_parts(g);
+  return delta_bytes(g) + std::max(nk > 1 ? nk * kv_part_bytes(g) : 0, nq > 1 ? nq * q_part_bytes(g) : 0);
+}
+
 magma_status_t cross_bwd_simt(const void* q, const void* k, const void* v, const void* o,
                               const void* d_o, const float* lse, void* dq, void* dk, void* dv,
-                              float* delta, const CrossGeom& g, magma_dtype_t dtype,
-                              cudaStream_t s) {
+                              const CrossGeom& g, magma_dtype_t dtype, void* workspace,
+                              size_t workspace_bytes, cudaStream_t s) {
+  float* delta = static_cast<float*>(workspace);
+  BwdArgs a{};
+  a.g = g;
+  a.kv_parts = a.q_parts = 1;
+  if (workspace_bytes > delta_bytes(g)) {
+    const size_t room = workspace_bytes - delta_bytes(g);
+    a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + delta_bytes(g));
+    if (g.kv_len > 0)
+      a.kv_parts = (int)std::max<int64_t>(1, std::min<int64_t>(kv_parts(g), room / kv_part_bytes(g)));
+    a.q_parts = (int)std::max<int64_t>(1, std::min<int64_t>(q_parts(g), room / q_part_bytes(g)));
+  }
   const bool vec = dtype == MAGMA_DTYPE_F32 && g.hd % 4 == 0 && pieces(q, g.qs) &&
                    pieces(k, g.ks) && pieces(v, g.vs) && pieces(d_o, g.dos);
   if (dtype == MAGMA_DTYPE_F32)
-    return g.hd <= 64 ? (vec ? bwd<64, float, true>(q, k, v, o, d_o, lse, dq, dk, dv, delta, g, s)
-                             : bwd<64, float, false>(q, k, v, o, d_o, lse, dq, dk, dv, delta, g, s))
-                      : (vec ? bwd<128, float, true>(q, k, v, o, d_o, lse, dq, dk, dv, delta, g, s)
-                             : bwd<128, float, false>(q, k, v, o, d_o, lse, dq, dk, dv, delta, g, s));
-  return g.hd <= 64 ? bwd<64, __nv_bfloat16, false>(q, k, v, o, d_o, lse, dq, dk, dv, delta, g, s)
-                    : bwd<128, __nv_bfloat16, false>(q, k, v, o, d_o, lse, dq, dk, dv, delta, g, s);
+    return g.hd <= 64 ? (vec ? bwd<64, float, true>(q, k, v, o, d_o, lse, dq, dk, dv, delta, a, s)
+                             : bwd<64, float, false>(q, k, v, o, d_o, lse, dq, dk, dv, delta, a, s))
+                      : (vec ? bwd<128, float, true>(q, k, v, o, d_o, lse, dq, dk, dv, delta, a, s)
+                             : bwd<128, float, false>(q, k, v, o, d_o, lse, dq, dk, dv, delta, a, s));
+  return g.hd <= 64 ? bwd<64, __nv_bfloat16, false>(q, k, v, o, d_o, lse, dq, dk, dv, delta, a, s)
+                    : bwd<128, __nv_bfloat16, false>(q, k, v, o, d_o, lse, dq, dk, dv, delta, a, s);
 }
 
 }  // namespace magma
