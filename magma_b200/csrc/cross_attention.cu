@@ -108,6 +108,7 @@ magma_status_t magma_cross_attention_fwd(const void* q, const void* k, const voi
   if (magma_status_t st = set_strides(fn, "o", o_strides, g.os, true, batch, heads, q_len, head_dim)) return st;
   if (batch == 0 || heads == 0 || q_len == 0) return MAGMA_OK;
   MAGMA_REQUIRE(q && o && (kv_len == 0 || (k && v)), "%s: NULL pointer", fn);
+  MAGMA_REQUIRE(o != q && o != k && o != v, "%s: o shares memory with an input", fn);
   if (cross_step_supported(q, k, v, o, g, dtype))
     return cross_step_run(q, k, v, o, lse, g, dtype, workspace, workspace_bytes,
                           (cudaStream_t)stream);
@@ -158,6 +159,15 @@ magma_status_t magma_cross_attention_bwd(
   const bool has_q = batch && heads && q_len, has_k = batch && kv_heads && kv_len;
   MAGMA_REQUIRE(!has_q || (q && o && d_o && lse && dq), "%s: NULL pointer", fn);
   MAGMA_REQUIRE(!has_k || (k && v && dk && dv), "%s: NULL pointer", fn);
+  const void* grads[] = {has_q ? dq : nullptr, has_k ? dk : nullptr, has_k ? dv : nullptr};
+  const void* inputs[] = {q, k, v, o, d_o};
+  for (int i = 0; i < 3; ++i) {
+    if (grads[i] == nullptr) continue;
+    for (const void* x : inputs)
+      MAGMA_REQUIRE(grads[i] != x, "%s: a gradient shares memory with an input", fn);
+    for (int j = 0; j < i; ++j)
+      MAGMA_REQUIRE(grads[i] != grads[j], "%s: two gradients share memory", fn);
+  }
   const size_t need = magma_cross_attention_bwd_workspace_size(batch, heads, kv_heads, q_len,
                                                                kv_len, head_dim, dtype);
   MAGMA_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned16(workspace)),

@@ -348,13 +348,27 @@ __device__ __forceinline__ void row_terms(const CrossGeom& g, const Block& x, in
   e = on ? delta[at] : 0.f;
 }
 
-// P and dS from the dot products; a key from len on takes no part, a query row
-// that is not there has lse = inf.
-__device__ __forceinline__ void probs(float& s, float& dp, bool on, float scale, float lse,
-                                      float delta) {
-  const float p = on ? expf(s * scale - lse) : 0.f;
-  s = p;
-  dp = on ? p * (dp - delta) : 0.f;
+// P and dS of a row's four keys from the dot products; a key from len on takes no
+// part, a query row that is not there has lse = inf. Where the tile has all keys
+// of the row (`whole`; the 16 threads of a row are half a warp), delta is formed
+// from P and dP: the stored O is rounded to the tensor's type, and a few keys do
+// not average that out.
+template <typename On>
+__device__ __forceinline__ void probs(float (&s)[4], float (&dp)[4], On on, float scale, float lse,
+                                      float delta, bool whole) {
+  float sum = 0.f;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    s[j] = on(j) ? expf(s[j] * scale - lse) : 0.f;
+    if (on(j)) sum = fmaf(s[j], dp[j], sum);
+  }
+  if (whole) {
+#pragma unroll
+    for (int w = 8; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+    delta = sum;
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) dp[j] = on(j) ? s[j] * (dp[j] - delta) : 0.f;
 }
 
 // Where few tiles have many steps, a tile's steps are split into parts, whose F32
@@ -426,14 +440,16 @@ cross_dkdv(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict
       dots<HD>(s, Qs, Ks, row, col);
       dots<HD>(dp, Gs, Vs, row, col);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < 4; ++i) {
+        const int r = row(i);
+        probs(s[i], dp[i], [&](int j) { return k0 + col(j) < len; }, g.scale, Ls[r], Es[r],
+              len <= kRows);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int r = row(i), c = col(j);
-          probs(s[i][j], dp[i][j], k0 + c < len, g.scale, Ls[r], Es[r]);
-          Ps[r * kP + c] = s[i][j];
-          Ds[r * kP + c] = dp[i][j];
+          Ps[r * kP + col(j)] = s[i][j];
+          Ds[r * kP + col(j)] = dp[i][j];
         }
+      }
       __syncthreads();
 #pragma unroll 4
       for (int r = 0; r < kRows; ++r) {
@@ -531,10 +547,11 @@ cross_dq(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__
     dots<HD>(s, Qs, Ks, row, col);
     dots<HD>(dp, Gs, Vs, row, col);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int i = 0; i < 4; ++i)
+      probs(s[i], dp[i], [&](int j) { return k0 + col(j) < len; }, g.scale, ls[i], es[i],
+            len <= kRows);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        probs(s[i][j], dp[i][j], k0 + col(j) < len, g.scale, ls[i], es[i]);
+    for (int j = 0; j < 4; ++j) {
       *reinterpret_cast<float4*>(Ds + col(j) * kP + ty * 4) =
           make_float4(dp[0][j], dp[1][j], dp[2][j], dp[3][j]);
     }
@@ -766,9 +783,10 @@ magma_status_t cross_bwd_simt(const void* q, const void* k, const void* v, const
   if (workspace_bytes > delta_bytes(g)) {
     const size_t room = workspace_bytes - delta_bytes(g);
     a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + delta_bytes(g));
-    if (g.kv_len > 0)
-      a.kv_parts = (int)std::max<int64_t>(1, std::min<int64_t>(kv_parts(g), room / kv_part_bytes(g)));
-    a.q_parts = (int)std::max<int64_t>(1, std::min<int64_t>(q_parts(g), room / q_part_bytes(g)));
+    if (const size_t each = kv_part_bytes(g))
+      a.kv_parts = (int)std::max<int64_t>(1, std::min<int64_t>(kv_parts(g), room / each));
+    if (const size_t each = q_part_bytes(g))
+      a.q_parts = (int)std::max<int64_t>(1, std::min<int64_t>(q_parts(g), room / each));
   }
   const bool vec = dtype == MAGMA_DTYPE_F32 && g.hd % 4 == 0 && pieces(q, g.qs) &&
                    pieces(k, g.ks) && pieces(v, g.vs) && pieces(d_o, g.dos);

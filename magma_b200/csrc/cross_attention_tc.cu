@@ -60,7 +60,7 @@ struct TcArgs {
   float* part;              // [split][b][h][q][hd] of a split source
   float* part_lse;          // [split][b][h][q]
   const float* nlse;        // [b][h][q_pad], -lse log2(e)
-  const float* delta;
+  float* delta;             // [b][h][q_pad], rowsum(dO O)
   float* piece;             // partial sums of units that several CTAs share, or NULL
   void* dq;
   void* dk;
@@ -1043,7 +1043,8 @@ cross_dq_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
       const bool in = qi < g.q_len;
       const int64_t at = (w.b * g.heads + h) * a.q_pad + qi;
       const float nl = in ? a.nlse[at] : -INFINITY, dl = in ? a.delta[at] : 0.f;
-      const unsigned long long nl2 = f2_pack(nl, nl), dl2 = f2_pack(dl, dl);
+      const unsigned long long nl2 = f2_pack(nl, nl);
+      unsigned long long dl2 = f2_pack(dl, dl);
       for (int j = w.j0; j < w.j1; ++j, ++gs, ++gk) {
         const int64_t left = w.len - (int64_t)j * F::kKeys;
         const bool tail = left < F::kKeys;
@@ -1063,6 +1064,23 @@ cross_dq_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) continue;
         tc_fence_after();
+        if (w.n == 1) {
+          // All keys of the row are here: delta = sum P dP without the rounding of
+          // the stored O, which a few keys do not average out. dK reads it too.
+          float sum = 0.f;
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            uint32_t vd[32];
+            tmem_ld32(tDp(t) + lanes + 32 * c, vd);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (32 * c + e <= lim)
+                sum = fmaf(__uint_as_float(vs[c][e]), __uint_as_float(vd[e]), sum);
+          }
+          dl2 = f2_pack(sum, sum);
+          if (in) a.delta[at] = sum;
+        }
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           uint32_t vd[32], pd[16];
@@ -1741,38 +1759,39 @@ magma_status_t bwd_tc(const void* q, const void* k, const void* v, const void* d
                       TcArgs a, cudaStream_t s) {
   const CrossGeom& g = a.g;
   CUtensorMap mq, mg, mk, mv;
-  {
-    using F = Dkv<HD>;
-    if (magma_status_t st = view_map(&mq, q, g.hd, g.q_len, g.heads, g.batch, g.qs, F::kQ, &a.qb, &a.qh)) return st;
-    if (magma_status_t st = view_map(&mg, d_o, g.hd, g.q_len, g.heads, g.batch, g.dos, F::kQ, &a.db, &a.dh)) return st;
-    if (magma_status_t st = view_map(&mk, k, g.hd, g.kv_len, g.kv_heads, g.batch, g.ks, kRows, &a.kb, &a.kh)) return st;
-    if (magma_status_t st = view_map(&mv, v, g.hd, g.kv_len, g.kv_heads, g.batch, g.vs, kRows, &a.vb, &a.vh)) return st;
-    if (magma_status_t st = cross_smem<cross_dkdv_tc<HD>>(F::kSmem)) return st;
-    const int64_t units = ceil_div(g.kv_len, kRows) * g.kv_heads * g.batch;
-    a.piece = deal_dkdv(g) ? piece : nullptr;
+  {  // dQ first: it writes the delta of short sources, which dK reads
+    using F = Dq<HD>;
+    if (magma_status_t st = view_map(&mq, q, g.hd, g.q_len, g.heads, g.batch, g.qs, kRows, &a.qb, &a.qh)) return st;
+    if (magma_status_t st = view_map(&mg, d_o, g.hd, g.q_len, g.heads, g.batch, g.dos, kRows, &a.db, &a.dh)) return st;
+    if (magma_status_t st = view_map(&mk, k, g.hd, g.kv_len, g.kv_heads, g.batch, g.ks, F::kKeys, &a.kb, &a.kh)) return st;
+    if (magma_status_t st = view_map(&mv, v, g.hd, g.kv_len, g.kv_heads, g.batch, g.vs, F::kKeys, &a.vb, &a.vh)) return st;
+    if (magma_status_t st = cross_smem<cross_dq_tc<HD>>(F::kSmem)) return st;
+    const int64_t units = (int64_t)a.n_pairs * g.kv_heads * g.batch;
+    a.piece = deal_dq(g) ? piece : nullptr;
     const unsigned ctas = (unsigned)(a.piece ? num_sms() : std::min<int64_t>(units, num_sms()));
-    if (magma_status_t st = launch_after(cross_dkdv_tc<HD>, dim3(ctas), kThreads, F::kSmem, s,
-                                         "cross_dkdv_tc", mq, mg, mk, mv, a))
+    if (magma_status_t st = launch_after(cross_dq_tc<HD>, dim3(ctas), kThreads, F::kSmem, s,
+                                         "cross_dq_tc", mq, mg, mk, mv, a))
       return st;
     if (a.piece)
-      if (magma_status_t st = launch_after(cross_dkdv_join<HD>, dim3(ctas - 1, 8), 256, 0, s,
-                                           "cross_dkdv_join", a, (int)ctas))
+      if (magma_status_t st = launch_after(cross_dq_join<HD>, dim3(ctas - 1, 8), 256, 0, s,
+                                           "cross_dq_join", a, (int)ctas))
         return st;
   }
-  using F = Dq<HD>;
-  if (magma_status_t st = view_map(&mq, q, g.hd, g.q_len, g.heads, g.batch, g.qs, kRows, &a.qb, &a.qh)) return st;
-  if (magma_status_t st = view_map(&mg, d_o, g.hd, g.q_len, g.heads, g.batch, g.dos, kRows, &a.db, &a.dh)) return st;
-  if (magma_status_t st = view_map(&mk, k, g.hd, g.kv_len, g.kv_heads, g.batch, g.ks, F::kKeys, &a.kb, &a.kh)) return st;
-  if (magma_status_t st = view_map(&mv, v, g.hd, g.kv_len, g.kv_heads, g.batch, g.vs, F::kKeys, &a.vb, &a.vh)) return st;
-  if (magma_status_t st = cross_smem<cross_dq_tc<HD>>(F::kSmem)) return st;
-  const int64_t units = (int64_t)a.n_pairs * g.kv_heads * g.batch;
-  a.piece = deal_dq(g) ? piece : nullptr;
+  using F = Dkv<HD>;
+  if (magma_status_t st = view_map(&mq, q, g.hd, g.q_len, g.heads, g.batch, g.qs, F::kQ, &a.qb, &a.qh)) return st;
+  if (magma_status_t st = view_map(&mg, d_o, g.hd, g.q_len, g.heads, g.batch, g.dos, F::kQ, &a.db, &a.dh)) return st;
+  if (magma_status_t st = view_map(&mk, k, g.hd, g.kv_len, g.kv_heads, g.batch, g.ks, kRows, &a.kb, &a.kh)) return st;
+  if (magma_status_t st = view_map(&mv, v, g.hd, g.kv_len, g.kv_heads, g.batch, g.vs, kRows, &a.vb, &a.vh)) return st;
+  if (magma_status_t st = cross_smem<cross_dkdv_tc<HD>>(F::kSmem)) return st;
+  const int64_t units = ceil_div(g.kv_len, kRows) * g.kv_heads * g.batch;
+  a.piece = deal_dkdv(g) ? piece : nullptr;
   const unsigned ctas = (unsigned)(a.piece ? num_sms() : std::min<int64_t>(units, num_sms()));
-  if (magma_status_t st = launch_after(cross_dq_tc<HD>, dim3(ctas), kThreads, F::kSmem, s,
-                                       "cross_dq_tc", mq, mg, mk, mv, a))
+  if (magma_status_t st = launch_after(cross_dkdv_tc<HD>, dim3(ctas), kThreads, F::kSmem, s,
+                                       "cross_dkdv_tc", mq, mg, mk, mv, a))
     return st;
   if (a.piece == nullptr) return MAGMA_OK;
-  return launch_after(cross_dq_join<HD>, dim3(ctas - 1, 8), 256, 0, s, "cross_dq_join", a, (int)ctas);
+  return launch_after(cross_dkdv_join<HD>, dim3(ctas - 1, 8), 256, 0, s, "cross_dkdv_join", a,
+                      (int)ctas);
 }
 
 }  // namespace

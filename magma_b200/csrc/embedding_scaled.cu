@@ -598,6 +598,7 @@ magma_status_t magma_embedding_scaled_fwd(const int32_t* tokens, const void* tab
   if (rows == 0 || dim == 0) return MAGMA_OK;
   MAGMA_REQUIRE(vocab > 0, "%s: an empty table", fn);
   MAGMA_REQUIRE(tokens && table && out, "%s: NULL pointer", fn);
+  MAGMA_REQUIRE(out != table && out != pos, "%s: out shares memory with an input", fn);
   MAGMA_REQUIRE(table_ld >= dim, "%s: table_ld %lld below dim %lld", fn, (long long)table_ld,
                 (long long)dim);
   const bool vec = vec_ok(table, table_ld, table_dtype, 8) && vec_ok(out, dim, out_dtype, 8) &&
@@ -634,6 +635,9 @@ magma_status_t magma_embedding_scaled_bwd(const int32_t* tokens, const void* dou
   MAGMA_REQUIRE(vocab == 0 || (dtable && dtable_ld >= dim), "%s: NULL dtable or dtable_ld below dim", fn);
   MAGMA_REQUIRE(rows == 0 || (tokens && dout && dout_ld >= dim),
                 "%s: NULL pointer or dout_ld below dim", fn);
+  MAGMA_REQUIRE(vocab == 0 || (dtable != dout && (const void*)dpos != dtable),
+                "%s: outputs share memory with dout or each other", fn);
+  MAGMA_REQUIRE(dpos == nullptr || (const void*)dpos != dout, "%s: dpos shares memory with dout", fn);
   const Layout l = layout(rows, dim);
   MAGMA_REQUIRE(rows == 0 || (workspace && workspace_bytes >= l.total && aligned16(workspace)),
                 "%s: a 16-byte aligned workspace of %lld bytes is needed", fn, (long long)l.total);

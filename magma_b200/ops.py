@@ -62,7 +62,12 @@ def workspace(nbytes: int, device: torch.device | None = None) -> torch.Tensor:
 # own from torch's allocator at each call, so that calls on several streams and
 # calls in captured graphs share none. Their smallest calls take a few
 # microseconds on the GPU, so the checks on the way there are kept short.
-_raw_stream = torch._C._cuda_getCurrentRawStream
+def _raw_stream(i: int) -> int:
+    return torch.cuda.current_stream(i).cuda_stream
+
+
+# the same value without the Stream object around it, where torch has it
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)
 _I64x12, _I64x24 = C.c_int64 * 12, C.c_int64 * 24
 
 

@@ -10,6 +10,7 @@ from magma_b200 import lib
 torch = pytest.importorskip("torch")
 
 BUF = 0x100000  # an aligned address that a refused call never touches
+OUT, OUT2, OUT3 = 0x10000000, 0x20000000, 0x30000000  # and others for outputs
 
 
 def refused(name, *args):
@@ -24,13 +25,13 @@ def st(*v):
 
 
 # ------------------------------------------------------------------- embedding
-def emb_fwd(tokens=BUF, table=BUF, ld=8, pos=None, out=BUF, batch=2, seq=3, dim=8, vocab=5,
+def emb_fwd(tokens=BUF, table=BUF, ld=8, pos=None, out=OUT, batch=2, seq=3, dim=8, vocab=5,
             ti=lib.F32, to=lib.F32):
     return ("magma_embedding_scaled_fwd", tokens, table, ld, pos, out, batch, seq, dim, vocab, 1.0,
             ti, to, None)
 
 
-def emb_bwd(tokens=BUF, dout=BUF, dout_ld=8, dtable=BUF, dtable_ld=8, batch=2, seq=3, dim=8,
+def emb_bwd(tokens=BUF, dout=BUF, dout_ld=8, dtable=OUT, dtable_ld=8, batch=2, seq=3, dim=8,
             vocab=5, pad=-1, ti=lib.F32, to=lib.F32, ws=BUF, ws_bytes=1 << 20):
     return ("magma_embedding_scaled_bwd", tokens, dout, dout_ld, dtable, dtable_ld, None, batch,
             seq, dim, vocab, 1.0, pad, 0, 0, ti, to, ws, ws_bytes, None)
@@ -40,7 +41,7 @@ def emb_bwd(tokens=BUF, dout=BUF, dout_ld=8, dtable=BUF, dtable_ld=8, batch=2, s
     (dict(batch=-1), "negative"), (dict(dim=1 << 23), "too large"), (dict(ti=lib.S32), "dtypes"),
     (dict(to=7), "dtypes"), (dict(tokens=None), "NULL"), (dict(table=None), "NULL"),
     (dict(out=None), "NULL"), (dict(ld=7), "table_ld"), (dict(vocab=0), "empty table"),
-    (dict(batch=1 << 20, seq=1 << 20), "2^31"),
+    (dict(batch=1 << 20, seq=1 << 20), "2^31"), (dict(out=BUF), "shares memory"),
 ])
 def test_embedding_lookup_refuses(change, word):
     assert word in refused(*emb_fwd(**change))
@@ -51,6 +52,7 @@ def test_embedding_lookup_refuses(change, word):
     (dict(pad=-2), "padding_idx"), (dict(dout=None), "NULL"), (dict(dtable=None), "NULL"),
     (dict(dout_ld=7), "dout_ld"), (dict(dtable_ld=0), "dtable_ld"), (dict(ws=None), "workspace"),
     (dict(ws_bytes=64), "workspace"), (dict(ws=BUF + 8), "workspace"), (dict(vocab=0), "empty"),
+    (dict(dtable=BUF), "share memory"),
 ])
 def test_embedding_gradient_refuses(change, word):
     assert word in refused(*emb_bwd(**change))
@@ -64,7 +66,7 @@ def test_embedding_without_rows_does_nothing():
 
 
 # ------------------------------------------------------------- cross attention
-def fwd(q=BUF, k=BUF, v=BUF, o=BUF, batch=2, heads=4, kv_heads=2, m=3, n=5, hd=8, scale=1.0,
+def fwd(q=BUF, k=BUF, v=BUF, o=OUT, batch=2, heads=4, kv_heads=2, m=3, n=5, hd=8, scale=1.0,
         dt=lib.F32, so=None, sq=None):
     sq = sq or st(heads * m * hd, m * hd, hd)
     sk = st(kv_heads * n * hd, n * hd, hd)
@@ -72,11 +74,11 @@ def fwd(q=BUF, k=BUF, v=BUF, o=BUF, batch=2, heads=4, kv_heads=2, m=3, n=5, hd=8
             sq, sk, sk, so or st(heads * m * hd, m * hd, hd), scale, dt, None, 0, None)
 
 
-def bwd(lse=BUF, dq=BUF, dk=BUF, ws=BUF, ws_bytes=1 << 20, sdk=None, sdq=None, heads=4, kv_heads=2,
+def bwd(lse=BUF, dq=OUT, dk=OUT2, dv=OUT3, ws=BUF, ws_bytes=1 << 20, sdk=None, sdq=None, heads=4, kv_heads=2,
         m=3, n=5, hd=8, batch=2):
     sq = st(heads * m * hd, m * hd, hd)
     sk = st(kv_heads * n * hd, n * hd, hd)
-    return ("magma_cross_attention_bwd", BUF, BUF, BUF, BUF, BUF, lse, None, dq, dk, BUF, batch,
+    return ("magma_cross_attention_bwd", BUF, BUF, BUF, BUF, BUF, lse, None, dq, dk, dv, batch,
             heads, kv_heads, m, n, hd, sq, sk, sk, sq, sq, sdq or sq, sdk or sk, sk, 1.0, lib.F32,
             ws, ws_bytes, None)
 
@@ -88,7 +90,7 @@ def bwd(lse=BUF, dq=BUF, dk=BUF, ws=BUF, ws_bytes=1 << 20, sdk=None, sdq=None, h
     (dict(scale=-1.0), "scale"), (dict(q=None), "NULL"), (dict(k=None), "NULL"),
     (dict(v=None), "NULL"), (dict(o=None), "NULL"), (dict(sq=st(-1, 8, 8)), "stride"),
     (dict(so=st(96, 0, 8)), "share memory"), (dict(so=st(96, 24, 7)), "share memory"),
-    (dict(so=st(8, 8, 8)), "share memory"),
+    (dict(so=st(8, 8, 8)), "share memory"), (dict(o=BUF), "shares memory"),
 ])
 def test_cross_attention_refuses(change, word):
     assert word in refused(*fwd(**change))
@@ -98,6 +100,7 @@ def test_cross_attention_refuses(change, word):
     (dict(lse=None), "NULL"), (dict(dq=None), "NULL"), (dict(dk=None), "NULL"),
     (dict(ws=None), "workspace"), (dict(ws_bytes=16), "workspace"), (dict(ws=BUF + 4), "workspace"),
     (dict(sdk=st(80, 0, 8)), "share memory"), (dict(sdq=st(0, 24, 8)), "share memory"),
+    (dict(dq=BUF), "shares memory"), (dict(dv=OUT2), "share memory"),
 ])
 def test_cross_attention_gradient_refuses(change, word):
     assert word in refused(*bwd(**change))

@@ -291,6 +291,62 @@ def test_front_end_refuses(cuda):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_no_queries_or_no_keys(cuda, dtype):
+    """Nothing to attend with: dK and dV are 0. Nothing to attend to: O and dQ are 0."""
+    from magma_b200 import ops
+    q, k, v, do, _ = make(12, 2, 4, 2, 5, 9, 64, dtype)
+    none = q[:, :, :0]
+    o, lse = ops.cross_attention_fwd(none, k, v)
+    assert o.shape == none.shape and lse.shape == none.shape[:3]
+    _, dk, dv = ops.cross_attention_bwd(none, k, v, o, o, lse)
+    assert bool((dk == 0).all()) and bool((dv == 0).all())
+    o, lse = ops.cross_attention_fwd(q, k[:, :, :0], v[:, :, :0])
+    assert bool((o == 0).all()) and bool((lse == -math.inf).all())
+    dq, dk, _ = ops.cross_attention_bwd(q, k[:, :, :0], v[:, :, :0], o, do, lse)
+    assert bool((dq == 0).all()) and dk.shape[2] == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("case", [(2, 4, 2, 1, 3000, 64), (1, 2, 1, 90, 4000, 128),
+                                  (2, 4, 4, 3, 500, 64), (1, 2, 2, 600, 64, 64)])
+def test_smaller_workspaces(cuda, case, dtype):
+    """The forward pass takes any workspace; the gradient refuses one that is too small."""
+    import ctypes as C
+
+    from magma_b200 import lib, ops
+    b, h, g, m, n, d = case
+    q, k, v, do, _ = make(13, b, h, g, m, n, d, dtype)
+    want, bound = reference(q, k, v, do, None, d ** -0.5)
+    dt = lib.F32 if dtype == torch.float32 else lib.BF16
+    st = lambda t: C.addressof(keep.setdefault(id(t), (C.c_int64 * 3)(*t.stride()[:3])))  # noqa: E731
+    keep = {}
+    need = lib.query("magma_cross_attention_fwd_workspace_size", b, h, g, m, n, d, dt)
+    for size in {0, 16, need // 3 // 16 * 16, need, need + 4096}:
+        ws = torch.empty(size, dtype=torch.uint8, device="cuda") if size else None
+        o, lse = torch.empty_like(q), torch.empty(b, h, m, device="cuda")
+        lib.call("magma_cross_attention_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
+                 lse.data_ptr(), None, b, h, g, m, n, d, st(q), st(k), st(v), st(o), d ** -0.5, dt,
+                 ws.data_ptr() if size else None, size, torch.cuda.current_stream().cuda_stream)
+        check(o, want[0], bound[0], "o")
+        check(lse, want[1], bound[1], "lse")
+    need = lib.query("magma_cross_attention_bwd_workspace_size", b, h, g, m, n, d, dt)
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+    grads = [torch.empty_like(t) for t in (q, k, v)]
+
+    def bwd(size):
+        lib.call("magma_cross_attention_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
+                 do.data_ptr(), lse.data_ptr(), None, *[t.data_ptr() for t in grads], b, h, g, m, n,
+                 d, st(q), st(k), st(v), st(o), st(do), *[st(t) for t in grads], d ** -0.5, dt,
+                 ws.data_ptr(), size, torch.cuda.current_stream().cuda_stream)
+
+    with pytest.raises(lib.MagmaError):
+        bwd(need - 16)
+    bwd(need)
+    for x, w, e in zip(grads, want[2:], bound[2:]):
+        check(x, w, e, "gradient")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("m", [1, 150])
 def test_captured_graphs_and_streams(cuda, m, dtype):
     """Two captured graphs and eager calls on two streams at once, on new inputs."""
