@@ -494,12 +494,16 @@ cross_fwd_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
     bool ok = true;
     int gs = 0;  // this warpgroup's steps so far
     int gk = 0;
-    for (int r = 0;; ++r) {
-      const int u = snake(r, cta, ctas, units);
-      if (u < 0) break;
-      const PairUnit w = pair_unit<kRows>(a, order, u);
+    int r = 0;
+    int u = snake(r, cta, ctas, units);
+    PairUnit next{};
+    if (u >= 0) next = pair_unit<kRows>(a, order, u);
+    while (u >= 0) {
+      const PairUnit w = next;
+      u = snake(++r, cta, ctas, units);
       if (t >= w.items) {
         gk += w.n > 0 ? w.n : 0;
+        if (u >= 0) next = pair_unit<kRows>(a, order, u);
         continue;
       }
       const int h = head_of(a, w, t);
@@ -543,11 +547,14 @@ cross_fwd_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
         const float mx = fmaxf(fmaxf(fmaxf(mx8[0], mx8[1]), fmaxf(mx8[2], mx8[3])),
                                fmaxf(fmaxf(mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7])));
         const float m_new = fmaxf(m_run, mx * sl2);
-        // the previous P V has read P_t and added into O_t
-        if (gs >= 1 && !mbar_wait(pv_done(t), (uint32_t)((gs - 1) & 1), g.err)) ok = false;
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) continue;
-        tc_fence_after();
+        // The previous P V has read P_t and added into O_t (head size 128: S_t was
+        // issued behind it, and is there).
+        if constexpr (!F::kOver) {
+          if (gs >= 1 && !mbar_wait(pv_done(t), (uint32_t)((gs - 1) & 1), g.err)) ok = false;
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) continue;
+          tc_fence_after();
+        }
         if (j == 0) {
           m_run = m_new == -INFINITY ? 0.f : m_new;
         } else if (__any_sync(0xffffffffu, m_new > m_run + kRescaleLog2)) {
@@ -613,6 +620,7 @@ cross_fwd_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
         f2_unpack(rs2[1], b0, b1);
         l_run += (a0 + a1) + (b0 + b1);
       }
+      if (u >= 0) next = pair_unit<kRows>(a, order, u);  // while the last product runs
       if (ok && w.n > 0 && !mbar_wait(pv_done(t), (uint32_t)((gs - 1) & 1), g.err)) ok = false;
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) continue;
@@ -1032,10 +1040,13 @@ cross_dq_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
     bool ok = true;
     int gs = 0, gk = 0, gu = 0;
     DqWalk walk;
-    DqUnit w;
-    while (dq_next<F::kKeys>(a, order, first, total, walk, w)) {
+    DqUnit next;
+    bool have = dq_next<F::kKeys>(a, order, first, total, walk, next);
+    while (have) {
+      const DqUnit w = next;
       if (t >= w.items) {
         gk += w.j1 > w.j0 ? w.j1 - w.j0 : 0;
+        have = dq_next<F::kKeys>(a, order, first, total, walk, next);
         continue;
       }
       const int h = head_of(a, w, t);
@@ -1110,6 +1121,7 @@ cross_dq_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
       }
       __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(a.dq) + w.b * g.dqs[0] + h * g.dqs[1] +
                            qi * g.dqs[2];
+      have = dq_next<F::kKeys>(a, order, first, total, walk, next);  // while the last products run
       if (w.n <= 0) {
         if (in) zero_cols(dst, g.hd);
         continue;
