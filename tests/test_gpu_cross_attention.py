@@ -318,8 +318,12 @@ def test_smaller_workspaces(cuda, case, dtype):
     q, k, v, do, _ = make(13, b, h, g, m, n, d, dtype)
     want, bound = reference(q, k, v, do, None, d ** -0.5)
     dt = lib.F32 if dtype == torch.float32 else lib.BF16
-    st = lambda t: C.addressof(keep.setdefault(id(t), (C.c_int64 * 3)(*t.stride()[:3])))  # noqa: E731
-    keep = {}
+    keep = []
+
+    def st(t):
+        keep.append((C.c_int64 * 3)(*t.stride()[:3]))
+        return C.addressof(keep[-1])
+
     need = lib.query("magma_cross_attention_fwd_workspace_size", b, h, g, m, n, d, dt)
     for size in {0, 16, need // 3 // 16 * 16, need, need + 4096}:
         ws = torch.empty(size, dtype=torch.uint8, device="cuda") if size else None
