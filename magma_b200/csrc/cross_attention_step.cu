@@ -544,25 +544,27 @@ int rows_each(const CrossGeom& g, magma_dtype_t dtype) {
 }
 
 // Keys of a chunk: sixteen CTAs per SM, so that lengths that differ even out, but
-// chunks below 256 keys only where there are not six CTAs per SM: each chunk costs
-// a part and its share of the join.
+// chunks below 256 keys only where there are not four CTAs per SM, which is what
+// runs at once: each chunk costs a part and its share of the join. (F32, 4 x 32
+// heads over 8, 4000 keys: six CTAs per SM 39 us, four 31 us, two 32 us.)
 int64_t chunk_keys(const CrossGeom& g, magma_dtype_t dtype) {
   const int64_t tile = tile_keys(dtype);
   const int64_t heads =
       g.batch * g.kv_heads * ceil_div((int64_t)g.group * g.q_len, rows_each(g, dtype));
   const int64_t many = ceil_div(g.kv_len * heads, 16LL * num_sms());
-  const int64_t few = ceil_div(g.kv_len * heads, 6LL * num_sms());
+  const int64_t few = ceil_div(g.kv_len * heads, 4LL * num_sms());
   const int64_t keys = std::max(many, std::min<int64_t>(256, few));
   return ceil_div(keys, tile) * tile;
 }
 
-// Whether the chunks of a source are the CTAs of a cluster: calls too small to fill
-// the GPU twice. Longer ones are cut finer than a cluster is large; these are
-// over in the time that the second launch of the join takes.
+// Whether the chunks of a source are the CTAs of a cluster: eight of them for heads
+// that do not fill the GPU, while a CTA's chunk stays short. (BF16,
+// head size 64: 8 heads, 1000 keys 5.6 us in clusters, 7.0 us with the join; 4 x 8
+// heads, 2000 keys 7.6 and 9.3 us; F32, 4 x 32 heads over 8, 4000 keys 39 and 31 us.)
 bool use_cluster(const CrossGeom& g, magma_dtype_t dtype) {
   const int64_t heads =
       g.batch * g.kv_heads * ceil_div((int64_t)g.group * g.q_len, rows_each(g, dtype));
-  return heads * kMaxCluster <= 6LL * num_sms() && g.kv_len <= 8192;
+  return heads * kMaxCluster <= 6LL * num_sms() && g.kv_len <= (dtype == MAGMA_DTYPE_F32 ? 2048 : 4096);
 }
 
 template <typename K>

@@ -1858,13 +1858,13 @@ bool cross_tc_bwd_supported(const void* q, const void* k, const void* v, const v
          tc_strides(dv, g.dvs, g.kv_len);
 }
 
-// Parts of a source: as many as fill the SMs, at least four key tiles each (a
+// Parts of a source: as many as fill the SMs, at least two key tiles each (a
 // part costs its share of the join: one F32 row per query and part).
 static int64_t wanted_splits(const CrossGeom& g) {
   const TcArgs a = args_of(g);
   const int64_t units = (int64_t)a.n_pairs * g.kv_heads * g.batch;
   const int64_t tiles = ceil_div(g.kv_len, kRows);
-  return std::max<int64_t>(1, std::min<int64_t>(num_sms() / std::max<int64_t>(units, 1), tiles / 4));
+  return std::max<int64_t>(1, std::min<int64_t>(num_sms() / std::max<int64_t>(units, 1), tiles / 2));
 }
 
 size_t cross_tc_fwd_workspace(const CrossGeom& g) {
