@@ -4,7 +4,9 @@
  * training step: LayerNorm fwd/bwd, causal attention fwd/bwd, the Linear
  * contraction (GEMM), the generic Adam update, and the glue ops on the same
  * graphs (embedding, softmax cross-entropy, GELU/ReLU, bias gradient,
- * dtype conversion).
+ * dtype conversion); and for the operators that encoder-decoder models add
+ * (scaled embedding and its gradient, attention over another sequence's keys
+ * and values, gradient norm and clipping over separate tensors).
  *
  * Conventions follow Magma's PJRT C shim
  * (Sources/CXLARuntime/include/PJRTSimpleWrapper.h):
