@@ -464,17 +464,23 @@ cross_fwd_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
       };
       using t0 = std::integral_constant<int, 0>;
       using t1 = std::integral_constant<int, 1>;
-      for (int r = 0; ok; ++r) {
-        const int u = snake(r, cta, ctas, units);
-        if (u < 0) break;
-        const PairUnit w = pair_unit<kRows>(a, order, u);
-        if (w.n <= 0) continue;
+      int r = 0, u = snake(0, cta, ctas, units);
+      PairUnit next{};
+      if (u >= 0) next = pair_unit<kRows>(a, order, u);
+      while (ok && u >= 0) {
+        const PairUnit w = next;
+        u = snake(++r, cta, ctas, units);
+        if (w.n <= 0) {
+          if (u >= 0) next = pair_unit<kRows>(a, order, u);
+          continue;
+        }
         const int qb = ru % F::kQBufs;
         const bool two = w.items > 1;
         ok = mbar_wait(q_full(qb), (uint32_t)((ru / F::kQBufs) & 1), g.err) && k_wait() &&
              issue_s(t0{}, qb) && (!two || issue_s(t1{}, qb));
         if (!ok) break;
         k_next();
+        if (u >= 0) next = pair_unit<kRows>(a, order, u);  // while the first products run
         for (int j = 0; j < w.n; ++j) {
           const bool last = j + 1 == w.n;
           const uint32_t more = j > 0 ? 1u : 0u;
@@ -1029,15 +1035,21 @@ cross_dq_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
       using t0 = std::integral_constant<int, 0>;
       using t1 = std::integral_constant<int, 1>;
       DqWalk walk;
-      DqUnit w;
-      while (ok && dq_next<F::kKeys>(a, order, first, total, walk, w)) {
-        if (w.n <= 0) continue;
+      DqUnit next;
+      bool have = dq_next<F::kKeys>(a, order, first, total, walk, next);
+      while (ok && have) {
+        const DqUnit w = next;
+        if (w.n <= 0) {
+          have = dq_next<F::kKeys>(a, order, first, total, walk, next);
+          continue;
+        }
         const bool two = w.items > 1;
         ok = mbar_wait(q_full, (uint32_t)(ru & 1), g.err) && kv_wait();
         if (!ok) break;
         issue_s(t0{});
         if (two) issue_s(t1{});
         kv_next();
+        have = dq_next<F::kKeys>(a, order, first, total, walk, next);  // while they run
         for (int j = w.j0; j < w.j1; ++j) {
           const bool last = j + 1 == w.j1;
           const uint32_t more = j > w.j0 ? 1u : 0u;
@@ -1501,9 +1513,14 @@ cross_dkdv_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
         if (++sst == F::kStages) sst = 0, sph ^= 1u;
       };
       KvWalk walk;
-      KvUnit w;
-      while (ok && kv_next(a, first, units, n_it, walk, w)) {
-        if (w.i0 == w.i1) continue;
+      KvUnit next;
+      bool have = kv_next(a, first, units, n_it, walk, next);
+      while (ok && have) {
+        const KvUnit w = next;
+        if (w.i0 == w.i1) {
+          have = kv_next(a, first, units, n_it, walk, next);
+          continue;
+        }
         const int kb = ru % F::kKvBufs;
         ok = mbar_wait(kv_full(kb), (uint32_t)((ru / F::kKvBufs) & 1), g.err);
         const int n = w.i1 - w.i0;
@@ -1516,15 +1533,16 @@ cross_dkdv_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
           tb ^= 1u;
         }
         if (!ok) break;
+        have = kv_next(a, first, units, n_it, walk, next);  // while the first products run
         for (int i = 0; i < n; ++i) {
           const uint32_t t = db;
           const uint32_t more = i > 0 ? 1u : 0u;
-          const bool next = i + 2 < n;
+          const bool follows = i + 2 < n;
           const uint32_t aq = (uint32_t)gst * F::kStage, sc = tmem + 128u * t;
           ok = mbar_wait(p_full(t), gp, g.err) &&
                // the previous unit's dV and dK have been read
                (i > 0 || ru == 0 || mbar_wait(acc_empty, (uint32_t)((ru - 1) & 1), g.err)) &&
-               (!next || q_wait());
+               (!follows || q_wait());
           if (!ok) break;
           tc_fence_after();
           {
@@ -1533,7 +1551,7 @@ cross_dkdv_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
             for (int kk = 0; kk < F::kQ / 16; ++kk)
               mma_bf16_ts(tDv, sc + kk * 8, desc_add(dgm, kk * 2048), idG, kk > 0 ? 1u : more);
           }
-          if (next) issue_s(t, kb);  // behind dV, which reads P^T in the same columns
+          if (follows) issue_s(t, kb);  // behind dV, which reads P^T in the same columns
           ok = mbar_wait(ds_full(t), gp, g.err);
           if (!ok) break;
           tc_fence_after();
@@ -1544,7 +1562,7 @@ cross_dkdv_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
               mma_bf16_ts(tDk, sc + 64u + kk * 8, desc_add(dqm, kk * 2048), idG, kk > 0 ? 1u : more);
           }
           mma_commit(q_empty(gst));
-          if (next) {
+          if (follows) {
             issue_dp(t, kb);
             s_next();
             tb ^= 1u;
