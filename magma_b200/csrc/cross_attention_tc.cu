@@ -221,7 +221,9 @@ __device__ __forceinline__ void store_grad4(__nv_bfloat16* dst, float4 v, float 
 // 2^x of a pair on the FMA pipe, for x up to 8: x = n + f with n the nearest whole
 // number (in the low bits of x + 1.5 2^23), the minimax polynomial of degree 5 of
 // 2^f on [-1/2, 1/2] (Remez exchange, relative error 7.5e-8), n added to the
-// exponent; 0 below 2^-126, as ex2.approx.ftz.
+// exponent; 0 below 2^-126, as ex2.approx.ftz. A NaN becomes FLT_MAX (the bits of
+// the canonical NaN, 0x7FFFFFFF, shifted and added to themselves), which the
+// caller's sum has to turn back.
 __device__ __forceinline__ void ex2_pair_fma(unsigned long long x, float& p0, float& p1) {
   const unsigned long long magic = f2_pack(12582912.f, 12582912.f);
   const unsigned long long t = f2_add(x, magic);
@@ -238,6 +240,12 @@ __device__ __forceinline__ void ex2_pair_fma(unsigned long long x, float& p0, fl
   f2_unpack(y, y0, y1);
   p0 = x0 < -126.f ? 0.f : __uint_as_float(__float_as_uint(t0) * 0x800000u + __float_as_uint(y0));
   p1 = x1 < -126.f ? 0.f : __uint_as_float(__float_as_uint(t1) * 0x800000u + __float_as_uint(y1));
+}
+
+// A sum of kv_len exponentials below 2^8 stays below 2^40: more is the FLT_MAX that
+// ex2_pair_fma made of a NaN score.
+__device__ __forceinline__ float nan_sum(float l) {
+  return l > 1e30f ? __int_as_float(0x7fffffff) : l;
 }
 
 // A pair of (head, query tile) items that read the same key head: items 2p and
@@ -588,7 +596,7 @@ cross_fwd_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
         } else if (__any_sync(0xffffffffu, m_new > m_run + kRescaleLog2)) {
           const float alpha = ex2_approx(m_run - m_new);
           m_run = m_new;
-          l_run *= alpha;
+          l_run = nan_sum(l_run) * alpha;
 #pragma unroll
           for (int c = 0; c < HD / 16; ++c) {
             uint32_t o[16];
@@ -664,6 +672,7 @@ cross_fwd_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) continue;
       tc_fence_after();
+      l_run = nan_sum(l_run);
       const float inv = l_run == 0.f ? 0.f : 1.0f / l_run;  // no keys: a zero row
       const float lse = l_run == 0.f ? -INFINITY : m_run * kLn2 + logf(l_run);
       const int64_t at = (w.b * g.heads + h) * g.q_len + qi;

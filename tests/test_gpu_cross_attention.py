@@ -431,3 +431,25 @@ def test_gradient_against_differences(cuda):
     got = sum((g.double() * e).sum().item() for g, e in zip(grads, dirs))
     off = sum((b * e.abs()).sum().item() for b, e in zip(bound[2:], dirs))
     assert abs(got - quot[1]) <= off + 4 * abs(quot[0] - quot[1]) / 3 + 1e-9 * abs(quot[1])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("d", [64, 128])
+def test_nan_key_reaches_every_row(dtype, d):
+    """A NaN in a key that counts makes its scores NaN, whichever column of a tile
+    it is in, and with them the rows of its heads; other heads stay finite."""
+    from magma_b200 import ops
+    q, k, v, do, _ = make(77, 1, 8, 8, 130, 200, d, dtype)
+    clean, _ = ops.cross_attention_fwd(q, k, v)
+    for h in range(8):
+        k[0, h, 128 + h, 0] = float("nan")
+    k[0, 7, 135, 0] = 0.5
+    o, lse = ops.cross_attention_fwd(q, k, v)
+    assert torch.isnan(o[0, :7]).all() and torch.isnan(lse[0, :7]).all()
+    assert torch.isfinite(o[0, 7]).all()
+    for h in range(8):
+        k[0, h, 128 + h, 0] = 0.5
+        k[0, h, h, 0] = float("nan")
+    o, lse = ops.cross_attention_fwd(q, k, v)
+    assert torch.isnan(o).all() and torch.isnan(lse).all()
+    assert torch.isfinite(clean).all()
