@@ -2,23 +2,41 @@
 // tcgen05 tensor cores: BF16, F32 accumulation, head sizes that are multiples
 // of 8 up to 128 (padded to 64 or 128 columns by the tensor maps' zero fill).
 //
-//   cross_fwd_tc    O_t += P_t V_j over the key tiles j, S_t = Q_t K_j^T
-//   cross_rows      -lse log2(e) and delta = rowsum(dO O) of every query row
-//   cross_dkdv_tc   dV += P^T dO, dK += dS^T Q over the query tiles of every
-//                   head that shares the key head
-//   cross_dq_tc     dQ_t += dS_t K_j over the key tiles
+//   cross_fwd_tc     O_t += P_t V_j over the key tiles j, S_t = Q_t K_j^T
+//   cross_rows       -lse log2(e) and delta = rowsum(dO O) of every query row
+//   cross_dq_tc      dQ_t += dS_t K_j over the key tiles
+//   cross_dkdv_tc    dV += P^T dO, dK += dS^T Q over the query tiles of every
+//                    head that shares the key head
+//   cross_dq_join, cross_dkdv_join  the pieces of the sums that two CTAs shared
 //
 // Formulas as in cross_attention_simt.cu. The gradient recomputes S and dP in
 // both of its passes (14 instead of 10 products of the size of S) and needs no
-// partial tiles in memory and no atomics: every output element has one owner.
+// atomics: an output element is added up by one CTA, or in pieces that a join
+// adds in a fixed order, so the result is the same on every run.
 //
 // All three products kernels have the same frame: persistent, one CTA per SM, a
-// TMA warp, a warp whose first lane issues the MMAs, and two warpgroups (thread
-// = row) that turn score tiles into probabilities; while one works the tensor
-// cores run for the other. Lengths that differ between the sequences are dealt
+// TMA warp, a warp with one elected lane that issues the MMAs (elect.sync, not
+// lane == 0: with it the compiler keeps descriptors and barriers in uniform
+// registers; the gradient of 2 x 32 heads of 128, 2048 queries, 4096 keys, 1233 ->
+// 924 us), and
+// two warpgroups (thread = row) that turn score tiles into probabilities; while
+// one works the tensor cores run for the other. Lengths that differ between the sequences are dealt
 // out longest first in a snake over the CTAs. Rows of V (forward) or K (dQ) from
 // the length on are set to zero in shared memory before a product reads them,
 // so whatever lies behind a length meets a probability of 0 only as 0.
+//
+// What bounds them. Forward of 4 x 32 heads over 8 of size 128, 2048 queries, up to
+// 4096 keys: 324 to 331 us, 1.2 PFLOP/s, what the tensor cores' power limit leaves
+// (385 us when it is repeated for seconds); head size 64: 275 to 295 us, bound by
+// the exponentials, which are as many for half the products. Gradient of 2 x 32
+// heads over 8 of size 128, 2048 queries, 4096 keys: 800 to 850 us (rows 16, dQ 350
+// and its join 17, dK and dV 430 and 13), 0.83 PFLOP/s of the 10 products that are
+// needed, 1.16 of the 14 that are done. 8 x 16 heads of 64, 512 queries, up to 1024
+// keys: 86 us (rows 8, dQ 38, dK and dV 48). There a 64-query step takes some 1250
+// cycles where its products take 700: the issuing lane's waits and the warpgroups'
+// chain S -> P -> dS. Two issuing warps (S, P^T and dV; dP, dS^T and dK), three score
+// buffers, four warpgroups of 32 columns, warpgroups that take turns at the
+// exponentials took 88 to 93 us.
 #include <cuda.h>
 
 #include <algorithm>
@@ -301,7 +319,9 @@ __device__ __forceinline__ PairUnit pair_unit(const TcArgs& a, const uint16_t* o
 // size 128: S_t at 128 t, O_t at 256 + 128 t, and P_t takes the first half of
 // S_t's columns: S_t(j + 1) follows P_t(j) V_j, and the other tile's softmax
 // covers the wait. O_t is rescaled only when a row's maximum grows by more than
-// 2^8 (the stale maximum is exact after the final division).
+// 2^8 (the stale maximum is exact after the final division). P is rounded to BF16
+// for P V, the row's sum adds the probabilities as they were before: the quotient is
+// off by the rounding of each P, half a step.
 template <int HD>
 struct Fwd {
   static constexpr bool kOver = HD == 128;
@@ -721,7 +741,8 @@ cross_fwd_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
 // =========================================================== rows of the gradient
 // nlse = -lse log2(e), delta = rowsum(dO O), rows padded to a multiple of 64 with
 // (-inf, 0): the exponential of a row that is not there, or that had no
-// probabilities, is 0. Eight threads a row.
+// probabilities, is 0. Eight threads a row. One read of O and dO: 16 us for the 67 MB
+// of 2 x 32 heads, 2048 rows of 128 (4.2 TB/s).
 __global__ void __launch_bounds__(256)
 cross_rows(const __nv_bfloat16* __restrict__ o, const __nv_bfloat16* __restrict__ d_o,
            const float* __restrict__ lse, float* __restrict__ nlse, float* __restrict__ delta,

@@ -25,6 +25,13 @@
 //  3. emb_join     adds the parts of each crossing run in order.
 // The order of the additions depends on the tokens alone (no atomics on
 // floating values), so the result is the same on every run.
+//
+// What bounds it (GPU time of the three launches): 32768 rows of 1024 BF16, 50257
+// tokens: 35 + 16 + 9 us, the 206 MB of the table's F32 gradient and the 67 MB of
+// dout at 4.6 TB/s; writing the zeros takes longer than the sort beside it. 16384
+// rows of 384, 65 tokens: 10 + 9 + 8 us alone, 18 behind one another (a launch may
+// begin before the one before it ends): the sort's two passes through the
+// cluster, not the 26 MB.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -39,7 +46,8 @@ namespace cg = cooperative_groups;
 
 // ---- lookup --------------------------------------------------------------------
 // A warp per row and pass of U vectors a lane, all loads of a pass first. HBM
-// bound: the table and position rows are read and the output written once.
+// bound: the table and position rows are read and the output written once (32 x 1024
+// rows of 1024 F32: 40 to 42 us, 6.5 TB/s; 16 rows of 512 BF16: 2.1 us, a launch).
 template <typename TI, typename TO, int V>
 __global__ void __launch_bounds__(128)
 emb_lookup(const int32_t* __restrict__ tokens, const TI* __restrict__ table, int64_t table_ld,
