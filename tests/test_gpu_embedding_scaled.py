@@ -112,6 +112,32 @@ def test_gradient(cuda, b, n, d, v, kind, td, tt):
     assert ops.device_error_check() == 0
 
 
+# Small tables under many rows, long rows, and sizes around the tiles' borders.
+MORE = [(16, 1024, 384, 65, "any"), (4, 2048, 1000, 192, "any"), (4, 2048, 1000, 193, "any"),
+        (2, 1024, 33, 7, "few"), (2, 1025, 33, 7, "few"), (8, 512, 4800, 5, "any"), (1, 1, 31, 192, "any"),
+        (1, 300, 512, 257, "few"), (2, 1000, 512, 3001, "few"), (1, 2500, 1024, 312, "any"),
+        (1, 2497, 1024, 312, "any")]
+
+
+@pytest.mark.parametrize("td,tt", [(F32, F32), (BF16, F32), (F32, BF16), (BF16, BF16)])
+@pytest.mark.parametrize("b,n,d,v,kind", MORE)
+def test_gradient_of_small_tables_and_long_rows(cuda, b, n, d, v, kind, td, tt):
+    test_gradient(cuda, b, n, d, v, kind, td, tt)
+
+
+def test_bad_tokens_of_a_small_table(cuda):
+    from magma_b200 import lib, ops
+    tok, dout = batch(11, 8, 1024, 640, 30, F32)
+    tok[0, 5], tok[7, 1023], tok[3, 3] = -1, 30, 2 ** 31 - 1
+    got, _ = ops.embedding_scaled_bwd(tok, dout, 30)
+    with pytest.raises(lib.MagmaError):
+        ops.device_error_check()
+    t = tok.reshape(-1)
+    good = (t >= 0) & (t < 30)
+    want, bound = gradient_reference(t[good], dout[good], 30, 1.0, None)
+    check(got, want, bound, "dtable")
+
+
 @pytest.mark.parametrize("tt", [F32, BF16])
 @pytest.mark.parametrize("d", [64, 77])
 def test_gradient_accumulates(cuda, d, tt):
