@@ -22,8 +22,8 @@
 // pairs along the row index for the second products, whose left operand is
 // written to shared memory with that index contiguous. Rows are padded by 16
 // bytes, which spreads 16-byte reads of neighbouring rows over the banks. (F32, 8 x 12
-// heads of 64, 200 queries over 114 to 333 keys: 59 us, 18.5 of the FMA pipe's 74
-// TFLOP/s; 672 CTAs of 32 rows last 1 to 6 tiles each, and a tile's loads, maximum
+// heads of 64, 200 queries over 114 to 333 keys: 57 us, 19.4 of the FMA pipe's 74
+// TFLOP/s; 2 x 16 heads of 128, 1024 x 1024: 33.8; 672 CTAs of 32 rows last 1 to 6 tiles each, and a tile's loads, maximum
 // and exponentials take as long as its products.)
 #include <algorithm>
 #include <cmath>
@@ -146,6 +146,23 @@ __device__ __forceinline__ Block block_of(int64_t tiles, int64_t heads, int part
   return x;
 }
 
+// The sequence in place i of the sequences by length, the longest first: the CTAs of
+// the longest ones, which come last to an end, start first (8 x 12 heads, 200 queries
+// over 114 to 333 keys, the shortest first 68 us, the longest first 57; the gradient
+// of 4 x 8 heads, 700 over up to 900 keys, as they come 592 and 499 us). Every warp
+// finds it by itself; beyond 32 sequences the CTAs are so many that they even out.
+__device__ __forceinline__ int64_t longest_first(const CrossGeom& g, int64_t i) {
+  if (g.lens == nullptr || g.batch > 32) return i;
+  const int lane = threadIdx.x & 31, n = (int)g.batch;
+  const int mine = lane < n ? g.lens[lane] : -1;
+  int rank = 0;
+  for (int o = 0; o < n; ++o) {
+    const int other = __shfl_sync(0xffffffffu, mine, o);
+    rank += other > mine || (other == mine && o < lane);
+  }
+  return __ffs(__ballot_sync(0xffffffffu, lane < n && rank == (int)i)) - 1;
+}
+
 // Offset of listed query row r of a [B, H, Sq, D] tensor, -1 behind the last.
 __device__ __forceinline__ int64_t row_offset(const CrossGeom& g, const Block& x,
                                               const int64_t (&st)[3], int64_t r) {
@@ -178,7 +195,10 @@ struct FwdArgs {
 // each: V comes in under the scores, the next K under the sums. 64-row tiles read
 // shared memory least (half its bandwidth at the FMA pipe's rate, 32-row tiles
 // three quarters); 32-row tiles are for calls that would otherwise not give the
-// SMs enough CTAs to even out.
+// SMs enough CTAs to even out. Four CTAs per SM (128 registers) where that is
+// possible: 2 x 16 heads of 128, 1024 x 1024, 552 -> 509 us; the 32-row tiles of head
+// size 64 do better with the 134 registers that they ask for (8 x 12 heads, 200 x
+// 114..333: 56.6 and 58.4 us).
 template <int HD, int BM>
 struct FwdTile {
   static constexpr int kKeys = HD == 64 ? 64 : 32;
@@ -188,7 +208,7 @@ struct FwdTile {
 };
 
 template <int HD, int BM, typename T, bool VEC>
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(128, HD == 64 && BM == 32 ? 1 : 4)
 cross_fwd(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
           T* __restrict__ o, float* __restrict__ lse, const __grid_constant__ FwdArgs a) {
   constexpr int BN = FwdTile<HD, BM>::kKeys, kP = FwdTile<HD, BM>::kPp;
@@ -202,7 +222,8 @@ cross_fwd(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict_
   const CrossGeom& g = a.g;
   const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
   const int64_t rows = (int64_t)g.group * g.q_len;
-  const Block x = block_of((rows + BM - 1) / BM, g.kv_heads, a.parts);
+  Block x = block_of((rows + BM - 1) / BM, g.kv_heads, a.parts);
+  x.b = longest_first(g, x.b);
   const int64_t r0 = x.tile * BM, len = cross_len(g, x.b);
   int64_t t0, t1;
   part_tiles((len + BN - 1) / BN, x.part, a.parts, t0, t1);
@@ -239,15 +260,24 @@ cross_fwd(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict_
     cp_commit();
     float s[NI][NK];
     dots<HD>(s, Qs, Ks, row, [&](int j) { return tx + 16 * j; });
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+      for (int j = 0; j < NK; ++j) s[i][j] *= g.scale;
+    if (len - t * BN < BN) {  // the thread's keys that are not there
+      const int left = (int)(len - t * BN) - tx;
+#pragma unroll
+      for (int j = 0; j < NK; ++j)
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+          if (16 * j >= left) s[i][j] = -INFINITY;
+    }
     float alpha[NI];
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       float mx = -INFINITY;
 #pragma unroll
-      for (int j = 0; j < NK; ++j) {
-        s[i][j] = t * BN + tx + 16 * j < len ? s[i][j] * g.scale : -INFINITY;
-        mx = fmaxf(mx, s[i][j]);
-      }
+      for (int j = 0; j < NK; ++j) mx = fmaxf(mx, s[i][j]);
 #pragma unroll
       for (int w = 8; w > 0; w >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
       const float mn = fmaxf(m[i], mx);
@@ -513,7 +543,8 @@ cross_dq(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__
   int64_t* go = qo + kRows;
   const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
   const int64_t rows = (int64_t)g.group * g.q_len;
-  const Block x = block_of((rows + kRows - 1) / kRows, g.kv_heads, a.q_parts);
+  Block x = block_of((rows + kRows - 1) / kRows, g.kv_heads, a.q_parts);
+  x.b = longest_first(g, x.b);
   const int64_t r0 = x.tile * kRows, len = cross_len(g, x.b);
   int64_t t0, t1;
   part_tiles((len + kRows - 1) / kRows, x.part, a.q_parts, t0, t1);
