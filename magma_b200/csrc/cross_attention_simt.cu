@@ -23,8 +23,9 @@
 // written to shared memory with that index contiguous. Rows are padded by 16
 // bytes, which spreads 16-byte reads of neighbouring rows over the banks. (F32, 8 x 12
 // heads of 64, 200 queries over 114 to 333 keys: 57 us, 19.4 of the FMA pipe's 74
-// TFLOP/s; 2 x 16 heads of 128, 1024 x 1024: 33.8; 672 CTAs of 32 rows last 1 to 6 tiles each, and a tile's loads, maximum
-// and exponentials take as long as its products.)
+// TFLOP/s: 672 CTAs of 32 rows last two to six tiles each, and a tile's loads, maximum
+// and exponentials take as long as its products. 2 x 16 heads of 128, 1024 x 1024:
+// 508 us, 33.8 TFLOP/s.)
 #include <algorithm>
 #include <cmath>
 
@@ -659,8 +660,8 @@ bool pieces(const void* p, const int64_t (&st)[3]) {
 }
 
 // Rows of a forward tile: 32 where 64-row tiles would be fewer than four per SM
-// (8 x 12 heads of 64, 200 queries over 114 to 333 keys: 59 to 63 us, with 64 rows 68
-// to 73).
+// (8 x 12 heads of 64, 200 queries over 114 to 333 keys: 57 us; before the
+// longest came first 59 to 63, and with 64 rows 68 to 73).
 int fwd_rows(const CrossGeom& g) {
   return row_tiles(g) * g.kv_heads * g.batch < 4LL * num_sms() ? 32 : 64;
 }
