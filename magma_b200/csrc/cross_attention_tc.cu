@@ -803,9 +803,37 @@ __device__ __forceinline__ void grads32(const uint32_t (&p)[32], const uint32_t 
   }
 }
 
+// What the BF16 pairs of 32 columns leave of their F32 values, as BF16 pairs.
+__device__ __forceinline__ void rest16(const uint32_t (&x)[32], const uint32_t (&hi)[16],
+                                       uint32_t (&lo)[16]) {
+#pragma unroll
+  for (int e = 0; e < 16; ++e)
+    lo[e] = pack_bf16(__uint_as_float(x[2 * e]) - __uint_as_float(hi[e] << 16),
+                      __uint_as_float(x[2 * e + 1]) - __uint_as_float(hi[e] & 0xFFFF0000u));
+}
+// dS of 32 columns as F32, in place of dP.
+template <typename DL>
+__device__ __forceinline__ void grads32_f32(const uint32_t (&p)[32], uint32_t (&vd)[32], DL dl) {
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    float d0, d1;
+    f2_unpack(f2_mul(f2_pack(__uint_as_float(p[2 * e]), __uint_as_float(p[2 * e + 1])),
+                     f2_sub(f2_pack(__uint_as_float(vd[2 * e]), __uint_as_float(vd[2 * e + 1])),
+                            dl(e))), d0, d1);
+    vd[2 * e] = __float_as_uint(d0);
+    vd[2 * e + 1] = __float_as_uint(d1);
+  }
+}
+__device__ __forceinline__ void pack32(const uint32_t (&x)[32], uint32_t (&hi)[16]) {
+#pragma unroll
+  for (int e = 0; e < 16; ++e)
+    hi[e] = pack_bf16(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
+}
+
 // =================================================================== dQ
 // As the forward kernel, over 64-key tiles: S_t, dP_t = dO_t V_j^T; dS_t as BF16
-// pairs in S_t's columns is the A operand of dQ_t += dS_t K_j. TMEM columns of
+// pairs in S_t's columns is the A operand of dQ_t += dS_t K_j (SPLIT: in two terms, as
+// in cross_dkdv_tc). TMEM columns of
 // tile t from 256 t: S, dP, dQ.
 constexpr int kDealt = kOrder / 2;  // entries of a table of steps, in the place of the order
 
@@ -923,7 +951,7 @@ struct Dq {
   static_assert(kSmem <= 232448, "shared memory");
 };
 
-template <int HD>
+template <int HD, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1)
 cross_dq_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmG,
             const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
@@ -1060,6 +1088,11 @@ cross_dq_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
 #pragma unroll
         for (int kk = 0; kk < F::kKeys / 16; ++kk)
           mma_bf16_ts(tDq(t), tS(t) + kk * 8, desc_add(dk, kk * 2048), idQ, kk > 0 ? 1u : more);
+        if constexpr (SPLIT) {
+#pragma unroll
+          for (int kk = 0; kk < F::kKeys / 16; ++kk)
+            mma_bf16_ts(tDq(t), tS(t) + 32u + kk * 8, desc_add(dk, kk * 2048), idQ, 1u);
+        }
         return true;
       };
       using t0 = std::integral_constant<int, 0>;
@@ -1172,14 +1205,24 @@ cross_dq_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
           uint32_t vd[32], pd[16];
           tmem_ld32(tDp(t) + lanes + 32 * c, vd);
           tmem_wait_ld();
-          grads32(vs[c], vd, [&](int) { return dl2; }, pd);
-          if (tail) {
+          auto mask = [&](uint32_t(&x)[16]) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-              if (32 * c + 2 * e > lim) pd[e] &= 0xFFFF0000u;
-              if (32 * c + 2 * e + 1 > lim) pd[e] &= 0x0000FFFFu;
+              if (32 * c + 2 * e > lim) x[e] &= 0xFFFF0000u;
+              if (32 * c + 2 * e + 1 > lim) x[e] &= 0x0000FFFFu;
             }
+          };
+          if constexpr (SPLIT) {
+            uint32_t pl[16];
+            grads32_f32(vs[c], vd, [&](int) { return dl2; });
+            pack32(vd, pd);
+            rest16(vd, pd, pl);
+            if (tail) mask(pl);
+            tmem_st16(tS(t) + lanes + 32 + 16 * c, pl);
+          } else {
+            grads32(vs[c], vd, [&](int) { return dl2; }, pd);
           }
+          if (tail) mask(pd);
           tmem_st16(tS(t) + lanes + 16 * c, pd);  // S_t is in registers
         }
         if (tail && t == 0 && row < F::kKeys) {  // warps 0 and 1
@@ -1279,7 +1322,8 @@ cross_dq_join(const __grid_constant__ TcArgs a, int ctas) {
 // all query heads that share it. Steps alternate between two score buffers and
 // the two warpgroups: S^T = K Q^T, dP^T = V dO^T (thread = key row); P^T and
 // dS^T as BF16 pairs in the same columns are the A operands of dV += P^T dO and
-// dK += dS^T Q. TMEM columns of buffer t from 128 t: S^T, dP^T; then dV, dK.
+// dK += dS^T Q (SPLIT: what the pairs left of the F32 values, as pairs in the upper
+// half of the columns, is a second A operand). TMEM columns of buffer t from 128 t: S^T, dP^T; then dV, dK.
 // Nothing is masked: a row of a key behind the length only reaches its own
 // output row, which is stored as zeros, and the terms of a query row behind
 // q_len make its probabilities 0.
@@ -1399,7 +1443,7 @@ struct Dkv {
   static_assert(kSmem <= 232448, "shared memory");
 };
 
-template <int HD>
+template <int HD, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1)
 cross_dkdv_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmG,
               const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
@@ -1580,6 +1624,11 @@ cross_dkdv_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
 #pragma unroll
             for (int kk = 0; kk < F::kQ / 16; ++kk)
               mma_bf16_ts(tDv, sc + kk * 8, desc_add(dgm, kk * 2048), idG, kk > 0 ? 1u : more);
+            if constexpr (SPLIT) {
+#pragma unroll
+              for (int kk = 0; kk < F::kQ / 16; ++kk)
+                mma_bf16_ts(tDv, sc + 32u + kk * 8, desc_add(dgm, kk * 2048), idG, 1u);
+            }
           }
           if (follows) issue_s(t, kb);  // behind dV, which reads P^T in the same columns
           ok = mbar_wait(ds_full(t), gp, g.err);
@@ -1590,6 +1639,11 @@ cross_dkdv_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
 #pragma unroll
             for (int kk = 0; kk < F::kQ / 16; ++kk)
               mma_bf16_ts(tDk, sc + 64u + kk * 8, desc_add(dqm, kk * 2048), idG, kk > 0 ? 1u : more);
+            if constexpr (SPLIT) {
+#pragma unroll
+              for (int kk = 0; kk < F::kQ / 16; ++kk)
+                mma_bf16_ts(tDk, sc + 96u + kk * 8, desc_add(dqm, kk * 2048), idG, 1u);
+            }
           }
           mma_commit(q_empty(gst));
           if (follows) {
@@ -1655,6 +1709,11 @@ cross_dkdv_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
           for (int e = 0; e < 16; ++e)
             pp[e] = pack_bf16(__uint_as_float(vs[c][2 * e]), __uint_as_float(vs[c][2 * e + 1]));
           tmem_st16(tS(t) + lanes + 16 * c, pp);  // S^T is in registers
+          if constexpr (SPLIT) {
+            uint32_t pl[16];
+            rest16(vs[c], pp, pl);
+            tmem_st16(tS(t) + lanes + 32 + 16 * c, pl);
+          }
         }
         tmem_wait_st();
         tc_fence_before();
@@ -1671,7 +1730,15 @@ cross_dkdv_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           uint32_t pd[16];
-          grads32(vs[c], vd[c], terms(dl, c), pd);
+          if constexpr (SPLIT) {
+            uint32_t pl[16];
+            grads32_f32(vs[c], vd[c], terms(dl, c));
+            pack32(vd[c], pd);
+            rest16(vd[c], pd, pl);
+            tmem_st16(tDp(t) + lanes + 32 + 16 * c, pl);
+          } else {
+            grads32(vs[c], vd[c], terms(dl, c), pd);
+          }
           tmem_st16(tDp(t) + lanes + 16 * c, pd);
         }
         tmem_wait_st();
@@ -1847,7 +1914,19 @@ bool deal_dq(const CrossGeom& g) {
          deal(g, (int64_t)a.n_pairs * g.kv_heads * g.batch, ceil_div(g.kv_len, 64));
 }
 
-template <int HD>
+// Whether P and dS go into the products as two BF16 terms, the rounded value and what
+// it left: where no CTA has more than a step of dQ. The sums of a large gradient
+// have the error of their own rounding times sqrt(2) with single terms; that of
+// a small one scatters around it (measured: up to 1.6), and there the second
+// product hides in the launches' latency (2 x 8 heads, 128 x 128: 15.2 and 16.2 us at head
+// size 64, 17.9 and 19.5 at 128). With more steps it costs a seventh to a fifth
+// (2 x 16 heads, 512 x 512: 27.4 and 31.7 us; 8 x 16 heads, 512 x 1024: 105 and 125).
+bool one_step(const CrossGeom& g) {
+  const TcArgs a = args_of(g);
+  return (double)a.n_pairs * g.kv_heads * g.batch * ceil_div(g.kv_len, 64) <= (double)num_sms();
+}
+
+template <int HD, bool SPLIT>
 magma_status_t bwd_tc(const void* q, const void* k, const void* v, const void* d_o, float* piece,
                       TcArgs a, cudaStream_t s) {
   const CrossGeom& g = a.g;
@@ -1858,11 +1937,11 @@ magma_status_t bwd_tc(const void* q, const void* k, const void* v, const void* d
     if (magma_status_t st = view_map(&mg, d_o, g.hd, g.q_len, g.heads, g.batch, g.dos, kRows, &a.db, &a.dh)) return st;
     if (magma_status_t st = view_map(&mk, k, g.hd, g.kv_len, g.kv_heads, g.batch, g.ks, F::kKeys, &a.kb, &a.kh)) return st;
     if (magma_status_t st = view_map(&mv, v, g.hd, g.kv_len, g.kv_heads, g.batch, g.vs, F::kKeys, &a.vb, &a.vh)) return st;
-    if (magma_status_t st = cross_smem<cross_dq_tc<HD>>(F::kSmem)) return st;
+    if (magma_status_t st = cross_smem<cross_dq_tc<HD, SPLIT>>(F::kSmem)) return st;
     const int64_t units = (int64_t)a.n_pairs * g.kv_heads * g.batch;
     a.piece = deal_dq(g) ? piece : nullptr;
     const unsigned ctas = (unsigned)(a.piece ? num_sms() : std::min<int64_t>(units, num_sms()));
-    if (magma_status_t st = launch_after(cross_dq_tc<HD>, dim3(ctas), kThreads, F::kSmem, s,
+    if (magma_status_t st = launch_after(cross_dq_tc<HD, SPLIT>, dim3(ctas), kThreads, F::kSmem, s,
                                          "cross_dq_tc", mq, mg, mk, mv, a))
       return st;
     if (a.piece)
@@ -1875,11 +1954,11 @@ magma_status_t bwd_tc(const void* q, const void* k, const void* v, const void* d
   if (magma_status_t st = view_map(&mg, d_o, g.hd, g.q_len, g.heads, g.batch, g.dos, F::kQ, &a.db, &a.dh)) return st;
   if (magma_status_t st = view_map(&mk, k, g.hd, g.kv_len, g.kv_heads, g.batch, g.ks, kRows, &a.kb, &a.kh)) return st;
   if (magma_status_t st = view_map(&mv, v, g.hd, g.kv_len, g.kv_heads, g.batch, g.vs, kRows, &a.vb, &a.vh)) return st;
-  if (magma_status_t st = cross_smem<cross_dkdv_tc<HD>>(F::kSmem)) return st;
+  if (magma_status_t st = cross_smem<cross_dkdv_tc<HD, SPLIT>>(F::kSmem)) return st;
   const int64_t units = ceil_div(g.kv_len, kRows) * g.kv_heads * g.batch;
   a.piece = deal_dkdv(g) ? piece : nullptr;
   const unsigned ctas = (unsigned)(a.piece ? num_sms() : std::min<int64_t>(units, num_sms()));
-  if (magma_status_t st = launch_after(cross_dkdv_tc<HD>, dim3(ctas), kThreads, F::kSmem, s,
+  if (magma_status_t st = launch_after(cross_dkdv_tc<HD, SPLIT>, dim3(ctas), kThreads, F::kSmem, s,
                                        "cross_dkdv_tc", mq, mg, mk, mv, a))
     return st;
   if (a.piece == nullptr) return MAGMA_OK;
@@ -1971,8 +2050,9 @@ magma_status_t cross_bwd_tc_run(const void* q, const void* k, const void* v, con
       g, a.q_pad);
   if (magma_status_t st = check_launch("cross_rows")) return st;
   float* piece = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + row_bytes(g));
-  return g.hd <= 64 ? bwd_tc<64>(q, k, v, d_o, piece, a, s)
-                    : bwd_tc<128>(q, k, v, d_o, piece, a, s);
+  auto* run = one_step(g) ? (g.hd <= 64 ? bwd_tc<64, true> : bwd_tc<128, true>)
+                           : (g.hd <= 64 ? bwd_tc<64, false> : bwd_tc<128, false>);
+  return run(q, k, v, d_o, piece, a, s);
 }
 
 }  // namespace magma
