@@ -1915,15 +1915,17 @@ bool deal_dq(const CrossGeom& g) {
 }
 
 // Whether P and dS go into the products as two BF16 terms, the rounded value and what
-// it left: where no CTA has more than a step of dQ. The sums of a large gradient
-// have the error of their own rounding times sqrt(2) with single terms; that of
-// a small one scatters around it (measured: up to 1.6), and there the second
+// it left: where no CTA has more than a step of dQ, and where dQ or dK has few rows.
+// The sums of a large gradient have the error of their own rounding times sqrt(2)
+// with single terms; that of a small one scatters around it (measured: up to 1.6; 256
+// rows of 32 under 16 sources of 65 keys 1.53), and in small calls the second
 // product hides in the launches' latency (2 x 8 heads, 128 x 128: 15.2 and 16.2 us at head
 // size 64, 17.9 and 19.5 at 128). With more steps it costs a seventh to a fifth
 // (2 x 16 heads, 512 x 512: 27.4 and 31.7 us; 8 x 16 heads, 512 x 1024: 105 and 125).
-bool one_step(const CrossGeom& g) {
+bool two_terms(const CrossGeom& g) {
   const TcArgs a = args_of(g);
-  return (double)a.n_pairs * g.kv_heads * g.batch * ceil_div(g.kv_len, 64) <= (double)num_sms();
+  return g.batch * g.heads * g.q_len <= 1024 || g.batch * g.kv_heads * g.kv_len <= 1024 ||
+         (double)a.n_pairs * g.kv_heads * g.batch * ceil_div(g.kv_len, 64) <= (double)num_sms();
 }
 
 template <int HD, bool SPLIT>
@@ -2050,7 +2052,7 @@ magma_status_t cross_bwd_tc_run(const void* q, const void* k, const void* v, con
       g, a.q_pad);
   if (magma_status_t st = check_launch("cross_rows")) return st;
   float* piece = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + row_bytes(g));
-  auto* run = one_step(g) ? (g.hd <= 64 ? bwd_tc<64, true> : bwd_tc<128, true>)
+  auto* run = two_terms(g) ? (g.hd <= 64 ? bwd_tc<64, true> : bwd_tc<128, true>)
                            : (g.hd <= 64 ? bwd_tc<64, false> : bwd_tc<128, false>);
   return run(q, k, v, d_o, piece, a, s);
 }
