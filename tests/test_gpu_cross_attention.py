@@ -476,3 +476,14 @@ def test_small_gradients_have_the_error_of_their_rounding(cuda, case):
         err = (a.double() - want).norm()
         least = (want.to(torch.bfloat16).double() - want).norm()
         assert err <= 1.15 * least, (name, (err / least).item())
+
+
+# more sequences than the tables of lengths and steps hold, and than a warp ranks
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("case", [(600, 2, 1, 40, 150, 64), (300, 2, 2, 30, 100, 128),
+                                  (512, 1, 1, 70, 200, 32), (33, 4, 2, 65, 130, 64)])
+def test_many_sequences(cuda, case, dtype):
+    b, n = case[0], case[4]
+    run_both(case, dtype, lens=[(37 * i) % (n + 1) for i in range(b)])
+    if b == 600:
+        run_both(case, dtype)
