@@ -286,6 +286,11 @@ namespace magma {
 __device__ __forceinline__ void wait_for_launch_before() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }
+// Lets the next launch begin as soon as every CTA of this one has called it; what
+// depends on this launch's results still waits for its end.
+__device__ __forceinline__ void let_next_launch_begin() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
 template <typename... P, typename... A>
 magma_status_t launch_after(void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem,
                             cudaStream_t stream, const char* what, A&&... args) {

@@ -80,6 +80,8 @@ struct TcArgs {
   const float* nlse;        // [b][h][q_pad], -lse log2(e)
   float* delta;             // [b][h][q_pad], rowsum(dO O)
   float* piece;             // partial sums of units that several CTAs share, or NULL
+  // dK and dV may begin while dQ is ending: the row terms are there by then
+  int early;
   void* dq;
   void* dk;
   void* dv;
@@ -749,6 +751,7 @@ cross_rows(const __nv_bfloat16* __restrict__ o, const __nv_bfloat16* __restrict_
            const float* __restrict__ lse, float* __restrict__ nlse, float* __restrict__ delta,
            const CrossGeom g, int q_pad) {
   constexpr int kEach = 4;
+  let_next_launch_begin();
   const uint32_t per_head = (uint32_t)q_pad / 64, bh = blockIdx.x / per_head;
   const uint32_t b = bh / (uint32_t)g.heads, h = bh % (uint32_t)g.heads;
   const int64_t q0 = (int64_t)(blockIdx.x % per_head) * 64 + (threadIdx.x >> 3);
@@ -976,7 +979,6 @@ cross_dq_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
             const __grid_constant__ TcArgs a) {
   using F = Dq<HD>;
   extern __shared__ uint8_t smem_raw[];
-  wait_for_launch_before();
   uint8_t* sp;
   const uint32_t base = align1024(smem_raw, &sp);
   auto sQ = [&](int t) { return base + F::kQ + 2 * t * F::kTile; };
@@ -1158,6 +1160,8 @@ cross_dq_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
       mbar_wait(done_bar, 0, g.err);
     }
   } else {
+    wait_for_launch_before();  // for the row terms
+    if (a.piece == nullptr) let_next_launch_begin();
     const int t = warp >> 2;
     const int row = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
@@ -1468,7 +1472,7 @@ cross_dkdv_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
               const __grid_constant__ TcArgs a) {
   using F = Dkv<HD>;
   extern __shared__ uint8_t smem_raw[];
-  wait_for_launch_before();
+  if (!a.early) wait_for_launch_before();
   uint8_t* sp;
   const uint32_t base = align1024(smem_raw, &sp);
   auto sK = [&](int kb) { return base + F::kKv + 2 * kb * F::kTile; };
@@ -1531,6 +1535,7 @@ cross_dkdv_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
       KvUnit w;
       while (ok && kv_next(a, first, units, n_it, walk, w)) {
         if (w.i0 == w.i1) continue;
+        if (w.len <= Dq<HD>::kKeys) wait_for_launch_before();  // dQ forms the delta of these
         const int kb = ru % F::kKvBufs;
         if (!mbar_wait(kv_empty(kb), (uint32_t)(((ru / F::kKvBufs) & 1) ^ 1), g.err)) break;
         mbar_expect_tx(kv_full(kb), 2 * F::kTile);
@@ -1812,6 +1817,8 @@ cross_dkdv_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
       }
     }
   }
+  // This launch's end stands for that of the one before it too.
+  wait_for_launch_before();
   tc_fence_before();
   __syncthreads();
   if (warp == kMmaWarp) {
@@ -1975,6 +1982,7 @@ magma_status_t bwd_tc(const void* q, const void* k, const void* v, const void* d
   if (magma_status_t st = view_map(&mk, k, g.hd, g.kv_len, g.kv_heads, g.batch, g.ks, kRows, &a.kb, &a.kh)) return st;
   if (magma_status_t st = view_map(&mv, v, g.hd, g.kv_len, g.kv_heads, g.batch, g.vs, kRows, &a.vb, &a.vh)) return st;
   if (magma_status_t st = cross_smem<cross_dkdv_tc<HD, SPLIT>>(F::kSmem)) return st;
+  a.early = a.piece == nullptr;
   const int64_t units = ceil_div(g.kv_len, kRows) * g.kv_heads * g.batch;
   a.piece = deal_dkdv(g) ? piece : nullptr;
   const unsigned ctas = (unsigned)(a.piece ? num_sms() : std::min<int64_t>(units, num_sms()));
