@@ -32,11 +32,12 @@
 // heads over 8 of size 128, 2048 queries, 4096 keys: 800 to 850 us (rows 16, dQ 350
 // and its join 17, dK and dV 430 and 13), 0.83 PFLOP/s of the 10 products that are
 // needed, 1.16 of the 14 that are done. 8 x 16 heads of 64, 512 queries, up to 1024
-// keys: 86 us (rows 8, dQ 38, dK and dV 48). There a 64-query step takes some 1250
+// keys: 80 us (rows 7, dQ 38, dK and dV 48 alone; each begins beside the end of the one
+// before it, without that 84). There a 64-query step takes some 1250
 // cycles where its products take 700: the issuing lane's waits and the warpgroups'
 // chain S -> P -> dS. Two issuing warps (S, P^T and dV; dP, dS^T and dK), three score
 // buffers, four warpgroups of 32 columns, warpgroups that take turns at the
-// exponentials took 88 to 93 us.
+// exponentials took 2 to 7 us more.
 #include <cuda.h>
 
 #include <algorithm>
