@@ -33,6 +33,9 @@ magma_status_t set_strides(const char* fn, const char* what, const int64_t* from
   return MAGMA_OK;
 }
 
+// An address that is none of an element's would fault in the kernel.
+bool on_element(const void* p, size_t size) { return reinterpret_cast<uintptr_t>(p) % size == 0; }
+
 CrossGeom sizes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t q_len, int64_t kv_len,
                 int64_t hd) {
   CrossGeom g{};
@@ -109,6 +112,10 @@ magma_status_t magma_cross_attention_fwd(const void* q, const void* k, const voi
   if (batch == 0 || heads == 0 || q_len == 0) return MAGMA_OK;
   MAGMA_REQUIRE(q && o && (kv_len == 0 || (k && v)), "%s: NULL pointer", fn);
   MAGMA_REQUIRE(o != q && o != k && o != v, "%s: o shares memory with an input", fn);
+  const void* tensors[] = {q, k, v, o};
+  for (const void* x : tensors)
+    MAGMA_REQUIRE(on_element(x, dtype_size(dtype)), "%s: an address off its elements", fn);
+  MAGMA_REQUIRE(on_element(lse, 4) && on_element(kv_lens, 4), "%s: an address off its elements", fn);
   if (cross_step_supported(q, k, v, o, g, dtype))
     return cross_step_run(q, k, v, o, lse, g, dtype, workspace, workspace_bytes,
                           (cudaStream_t)stream);
@@ -168,6 +175,10 @@ magma_status_t magma_cross_attention_bwd(
     for (int j = 0; j < i; ++j)
       MAGMA_REQUIRE(grads[i] != grads[j], "%s: two gradients share memory", fn);
   }
+  const void* tensors[] = {q, k, v, o, d_o, dq, dk, dv};
+  for (const void* x : tensors)
+    MAGMA_REQUIRE(on_element(x, dtype_size(dtype)), "%s: an address off its elements", fn);
+  MAGMA_REQUIRE(on_element(lse, 4) && on_element(kv_lens, 4), "%s: an address off its elements", fn);
   const size_t need = magma_cross_attention_bwd_workspace_size(batch, heads, kv_heads, q_len,
                                                                kv_len, head_dim, dtype);
   MAGMA_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned16(workspace)),

@@ -578,6 +578,9 @@ magma_status_t launch_lookup(const int32_t* tokens, const void* table, int64_t l
   return check_launch("emb_lookup");
 }
 
+// An address that is none of an element's would fault in the kernel.
+bool on_element(const void* p, size_t size) { return reinterpret_cast<uintptr_t>(p) % size == 0; }
+
 magma_status_t check_sizes(const char* fn, int64_t batch, int64_t seq, int64_t dim, int64_t vocab) {
   MAGMA_REQUIRE(batch >= 0 && seq >= 0 && dim >= 0 && vocab >= 0, "%s: negative size", fn);
   MAGMA_REQUIRE(vocab < 0x7FFFFFFFLL && dim <= (1LL << 22), "%s: vocab or dim too large", fn);
@@ -609,6 +612,9 @@ magma_status_t magma_embedding_scaled_fwd(const int32_t* tokens, const void* tab
   MAGMA_REQUIRE(out != table && out != pos, "%s: out shares memory with an input", fn);
   MAGMA_REQUIRE(table_ld >= dim, "%s: table_ld %lld below dim %lld", fn, (long long)table_ld,
                 (long long)dim);
+  MAGMA_REQUIRE(on_element(tokens, 4) && on_element(table, dtype_size(table_dtype)) &&
+                    on_element(pos, dtype_size(table_dtype)) && on_element(out, dtype_size(out_dtype)),
+                "%s: an address off its elements", fn);
   const bool vec = vec_ok(table, table_ld, table_dtype, 8) && vec_ok(out, dim, out_dtype, 8) &&
                    (pos == nullptr || vec_ok(pos, dim, table_dtype, 8));
   cudaStream_t cs = (cudaStream_t)stream;
@@ -646,6 +652,9 @@ magma_status_t magma_embedding_scaled_bwd(const int32_t* tokens, const void* dou
   MAGMA_REQUIRE(vocab == 0 || (dtable != dout && (const void*)dpos != dtable),
                 "%s: outputs share memory with dout or each other", fn);
   MAGMA_REQUIRE(dpos == nullptr || (const void*)dpos != dout, "%s: dpos shares memory with dout", fn);
+  MAGMA_REQUIRE(on_element(tokens, 4) && on_element(dout, dtype_size(dout_dtype)) &&
+                    on_element(dtable, dtype_size(dtable_dtype)) && on_element(dpos, 4),
+                "%s: an address off its elements", fn);
   const Layout l = layout(rows, dim);
   MAGMA_REQUIRE(rows == 0 || (workspace && workspace_bytes >= l.total && aligned16(workspace)),
                 "%s: a 16-byte aligned workspace of %lld bytes is needed", fn, (long long)l.total);

@@ -169,3 +169,15 @@ def test_front_end_refuses_host_tensors_and_wrong_lists():
     with pytest.raises(ValueError, match="added to"):
         ops.embedding_scaled_bwd(torch.zeros(1, 2, dtype=torch.int32), torch.zeros(2, 8), 5,
                                  accumulate=True)
+
+
+# ---------------------------------------------------------- addresses off elements
+@pytest.mark.parametrize("args", [
+    fwd(q=BUF + 2), fwd(k=BUF + 1), fwd(v=BUF + 3), fwd(o=OUT + 2), fwd(q=BUF + 1, dt=lib.BF16),
+    fwd(o=OUT + 1, dt=lib.BF16), bwd(lse=BUF + 2), bwd(dq=OUT + 2), bwd(dk=OUT2 + 1), bwd(dv=OUT3 + 2),
+    emb_fwd(tokens=BUF + 2), emb_fwd(table=BUF + 2), emb_fwd(out=OUT + 1, to=lib.BF16),
+    emb_fwd(pos=BUF + 2), emb_bwd(tokens=BUF + 1), emb_bwd(dout=BUF + 2),
+    emb_bwd(dtable=OUT + 1, to=lib.BF16),
+])
+def test_addresses_off_their_elements_are_refused(args):
+    assert "off its elements" in refused(*args)
