@@ -261,7 +261,8 @@ MAGMA_API magma_status_t magma_attention_bwd(const void* q, const void* k, const
  * query head h reads key head h / (heads / kv_heads). Every tensor has its own
  * (batch, head, position) strides in elements, the last dimension is
  * contiguous; an input's stride may be 0, an output's positions may not share
- * memory. kv_lens (int32 [batch] on the device, NULL: kv_len for all) may leave
+ * memory, with one another or with any other tensor of the call (an output that
+ * begins where another tensor does is refused). kv_lens (int32 [batch] on the device, NULL: kv_len for all) may leave
  * a sequence without keys: its rows of O are 0, its lse -infinity and its
  * gradients 0. Keys and values from kv_lens[b] on have no influence, whatever
  * they hold. A length outside [0, kv_len] is clamped and recorded in the device
@@ -287,7 +288,9 @@ MAGMA_API magma_status_t magma_cross_attention_fwd(const void* q, const void* k,
  * dV = P^T dO; dS = P * (dO V^T - rowsum(dO*O)); dQ = scale * dS K;
  * dK = scale * dS^T Q, dK and dV summed over the query heads of a key head.
  * dQ, dK and dV are written whole (keys from kv_lens[b] on get zeros), in a
- * fixed order of additions. The workspace of the query's size is needed. */
+ * fixed order of additions. The workspace of the query's size is needed.
+ * BF16: P and dS enter the products rounded to BF16, in small calls in two terms
+ * (value and remainder), and each gradient is rounded once when stored. */
 MAGMA_API size_t magma_cross_attention_bwd_workspace_size(int64_t batch, int64_t heads,
                                           int64_t kv_heads, int64_t q_len, int64_t kv_len,
                                           int64_t head_dim, magma_dtype_t dtype);
