@@ -3,8 +3,11 @@
 // Each part holds a row's normalised O_s and lse_s. With M the largest lse_s,
 //   O = sum_s exp(lse_s - M) O_s / sum_s exp(lse_s - M),
 //   lse = M + log sum_s exp(lse_s - M).
-// A part without keys has lse -inf and is not read. W warps a row (four for many
-// parts, whose reads would follow one another otherwise), four columns a lane.
+// A part without keys has lse -inf and adds nothing. A part with a NaN score has lse
+// NaN, which the maximum passes over and its exponential brings into the sums: the
+// parts are left out only where the lse of every one of them is -inf. W warps a row
+// (four for many parts, whose reads would follow one another otherwise), four columns
+// a lane.
 #include <cmath>
 
 #include "cross_attention.cuh"
@@ -28,13 +31,19 @@ cross_join(const float* __restrict__ part, const float* __restrict__ part_lse, T
   const int64_t i = (int64_t)blockIdx.x * kRows + warp / W;
   const bool row_on = i < rows;
   float m = -INFINITY;
+  bool some = false;  // a part that is not empty
   if (row_on)
-    for (int s = lane; s < n_part; s += 32) m = fmaxf(m, part_lse[s * rows + i]);
+    for (int s = lane; s < n_part; s += 32) {
+      const float x = part_lse[s * rows + i];
+      some = some || x != -INFINITY;
+      m = fmaxf(m, x);
+    }
   m = warp_max(m);
+  some = __any_sync(0xffffffffu, some);
   float total = 0.f;
   float acc[4] = {0.f, 0.f, 0.f, 0.f};
   const int c = lane * 4;
-  if (m != -INFINITY) {
+  if (some) {
     const int s0 = n_part * w / W, s1 = n_part * (w + 1) / W;
 #pragma unroll 8
     for (int s = s0; s < s1; ++s) {

@@ -1,0 +1,55 @@
+"""Cross attention at its edges: values that are no ordinary numbers, and sizes of
+zero. Tolerances are those of test_gpu_cross_attention."""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from test_gpu_cross_attention import check, make, reference  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.float32, torch.bfloat16]
+
+# Sources that are cut into parts: a few queries in chunks, query tiles too few for
+# the GPU (BF16: tensor cores, F32: FMA pipe), and one that is not cut in BF16.
+SPLIT = [(1, 8, 8, 1, 5000, 64), (2, 8, 2, 4, 9000, 128), (1, 2, 2, 100, 6000, 64),
+         (1, 2, 1, 70, 6000, 128), (1, 8, 8, 130, 200, 64)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("case", SPLIT)
+def test_nan_query_of_a_split_source(cuda, case, dtype):
+    """Every part's scores of that row are NaN: so are its output and lse, and no
+    other row's."""
+    from magma_b200 import ops
+    b, h, g, m, n, d = case
+    q, k, v, do, _ = make(31, b, h, g, m, n, d, dtype)
+    want, bound = reference(q, k, v, do, None, d ** -0.5)
+    bad = torch.zeros(b, h, m, dtype=torch.bool, device="cuda")
+    bad[0, h - 1, m - 1] = True
+    q[bad, d - 1] = math.nan
+    o, lse = ops.cross_attention_fwd(q, k, v)
+    assert bool(torch.isnan(o[bad]).all()) and bool(torch.isnan(lse[bad]).all())
+    check(o[~bad], want[0][~bad], bound[0][~bad], "o")
+    check(lse[~bad], want[1][~bad], bound[1][~bad], "lse")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("case", SPLIT)
+def test_nan_key_where_one_part_has_keys(cuda, case, dtype):
+    """A sequence so short that only the first part has keys, one of them NaN: the
+    empty parts do not make its rows those of a sequence without keys."""
+    from magma_b200 import ops
+    _, h, g, m, n, d = case
+    q, k, v, do, lens = make(32, 3, h, g, m, n, d, dtype, [n, 20, 0])
+    want, bound = reference(q, k, v, do, lens, d ** -0.5)
+    k[1, 0, 3, 0] = math.nan
+    o, lse = ops.cross_attention_fwd(q, k, v, kv_lens=lens)
+    bad = torch.zeros(3, h, m, dtype=torch.bool, device="cuda")
+    bad[1, :h // g] = True
+    assert bool(torch.isnan(o[bad]).all()) and bool(torch.isnan(lse[bad]).all())
+    check(o[~bad], want[0][~bad], bound[0][~bad], "o")
+    check(lse[~bad], want[1][~bad], bound[1][~bad], "lse")
+    assert bool((o[2] == 0).all()) and bool((lse[2] == -math.inf).all())
