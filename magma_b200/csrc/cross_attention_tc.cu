@@ -41,6 +41,7 @@
 #include <cuda.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <type_traits>
 
 #include "cross_attention.cuh"
@@ -615,7 +616,8 @@ cross_fwd_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CU
           tc_fence_after();
         }
         if (j == 0) {
-          m_run = m_new == -INFINITY ? 0.f : m_new;
+          // scores of -inf alone: below any other, so that the first one to come rescales
+          m_run = fmaxf(m_new, -FLT_MAX);
         } else if (__any_sync(0xffffffffu, m_new > m_run + kRescaleLog2)) {
           const float alpha = ex2_approx(m_run - m_new);
           m_run = m_new;

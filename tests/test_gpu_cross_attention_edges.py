@@ -53,3 +53,22 @@ def test_nan_key_where_one_part_has_keys(cuda, case, dtype):
     check(o[~bad], want[0][~bad], bound[0][~bad], "o")
     check(lse[~bad], want[1][~bad], bound[1][~bad], "lse")
     assert bool((o[2] == 0).all()) and bool((lse[2] == -math.inf).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("case", [(1, 2, 2, 200, 300, 64), (1, 2, 1, 200, 300, 128),
+                                  (1, 2, 2, 100, 6000, 64), (2, 4, 2, 130, 700, 96),
+                                  (1, 2, 2, 3, 300, 64), (3, 40, 40, 300, 400, 64)])
+def test_first_keys_score_minus_infinity(cuda, case, dtype):
+    """The first 128 keys' scores are -inf, the others' about -500: the output is
+    that of the other keys, however far below 0 their largest score is."""
+    from magma_b200 import ops
+    b, h, g, m, n, d = case
+    q, k, v, do, _ = make(33, b, h, g, m, n, d, dtype)
+    q[..., 0] = 1.0
+    k[..., 0] = -4000.0 / 64 ** 0.5 * d ** 0.5
+    k[:, :, :128, 0] = -math.inf
+    want, bound = reference(q, k[:, :, 128:], v[:, :, 128:], do, None, d ** -0.5)
+    o, lse = ops.cross_attention_fwd(q, k, v)
+    check(o, want[0], bound[0], "o")
+    check(lse, want[1], bound[1], "lse")
