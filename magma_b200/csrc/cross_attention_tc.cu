@@ -1999,9 +1999,12 @@ magma_status_t bwd_tc(const void* q, const void* k, const void* v, const void* d
 
 }  // namespace
 
+// Without sequences or query heads there is no grid to launch; the FMA-pipe kernels
+// write what such a call has to write (zeros to dK and dV).
 bool cross_tc_fwd_supported(const void* q, const void* k, const void* v, const void* o,
                             const CrossGeom& g, magma_dtype_t dtype) {
   return dtype == MAGMA_DTYPE_BF16 && g.hd % 8 == 0 && g.kv_len > 0 && g.q_len > 0 &&
+         g.batch > 0 && g.heads > 0 &&
          tc_strides(q, g.qs, g.q_len) && tc_strides(k, g.ks, g.kv_len) &&
          tc_strides(v, g.vs, g.kv_len) && tc_strides(o, g.os, g.q_len) &&
          fits32(g.batch, g.kv_heads, ceil_div(g.kv_len, kRows)) &&

@@ -72,3 +72,17 @@ def test_first_keys_score_minus_infinity(cuda, case, dtype):
     o, lse = ops.cross_attention_fwd(q, k, v)
     check(o, want[0], bound[0], "o")
     check(lse, want[1], bound[1], "lse")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("b,h,g", [(2, 0, 2), (0, 4, 2), (0, 0, 0), (2, 0, 0)])
+def test_gradient_without_heads_or_sequences(cuda, b, h, g, dtype):
+    """No query heads: dK and dV are 0. No sequences: nothing to write."""
+    from magma_b200 import ops
+    q = torch.ones(b, h, 70, 64, device="cuda", dtype=dtype)
+    k = torch.ones(b, g, 200, 64, device="cuda", dtype=dtype)
+    o, lse = ops.cross_attention_fwd(q, k, k)
+    assert o.shape == q.shape and lse.shape == (b, h, 70)
+    dk, dv = torch.full_like(k, 7.0), torch.full_like(k, 7.0)
+    dq, dk, dv = ops.cross_attention_bwd(q, k, k, o, q, lse, dk=dk, dv=dv)
+    assert dq.shape == q.shape and bool((dk == 0).all()) and bool((dv == 0).all())
