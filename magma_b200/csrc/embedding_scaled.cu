@@ -460,7 +460,8 @@ __device__ __forceinline__ int64_t tiles_of_run(const GradArgs& a, const uint32_
   return lo;
 }
 
-// One CTA per tile and 32 V columns: if a run begins in the tile and goes on
+// One CTA per tile and 32 V columns, and further ones where these outnumber the grid's
+// second dimension: if a run begins in the tile and goes on
 // behind it, its parts are added in four stretches of tiles, a warp each, and
 // the stretches in order.
 template <typename TT, int V>
@@ -475,29 +476,33 @@ __global__ void __launch_bounds__(kSumThreads) emb_join(const __grid_constant__ 
   if (p0 > 0 && key[p0] == t && key[p0 - 1] == t) return;  // began earlier
   const int64_t n = tiles_of_run(a, key, tile, t);  // tiles with a head part
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int col = (blockIdx.y * 32 + lane) * V;
   const int64_t j0 = tile + 1 + n * warp / 4, j1 = tile + 1 + n * (warp + 1) / 4;
-  float acc[V] = {};
-  if (col < a.dim) {
-    if (warp == 0) load_v<float, V>(a.tail + tile * a.dim + col, acc);
-    const float* src = a.head + col;
+  for (int c0 = blockIdx.y * 32 * V; c0 < a.dim; c0 += gridDim.y * 32 * V) {
+    const int col = c0 + lane * V;
+    float acc[V] = {};
+    if (col < a.dim) {
+      if (warp == 0) load_v<float, V>(a.tail + tile * a.dim + col, acc);
+      const float* src = a.head + col;
 #pragma unroll 8
-    for (int64_t j = j0; j < j1; ++j) {
-      float v[V];
-      load_v<float, V>(src + j * a.dim, v);
+      for (int64_t j = j0; j < j1; ++j) {
+        float v[V];
+        load_v<float, V>(src + j * a.dim, v);
 #pragma unroll
-      for (int e = 0; e < V; ++e) acc[e] += v[e];
+        for (int e = 0; e < V; ++e) acc[e] += v[e];
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) part[warp][lane * V + e] = acc[e];
     }
+    __syncthreads();
+    if (warp == 0 && col < a.dim) {
 #pragma unroll
-    for (int e = 0; e < V; ++e) part[warp][lane * V + e] = acc[e];
+      for (int w = 1; w < kSumThreads / 32; ++w)
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc[e] += part[w][lane * V + e];
+      store_grad<TT, V>(a, t, col, acc);
+    }
+    __syncthreads();
   }
-  __syncthreads();
-  if (warp != 0 || col >= a.dim) return;
-#pragma unroll
-  for (int w = 1; w < kSumThreads / 32; ++w)
-#pragma unroll
-    for (int e = 0; e < V; ++e) acc[e] += part[w][lane * V + e];
-  store_grad<TT, V>(a, t, col, acc);
 }
 
 // Places of a tile: many tiles for short batches, and few parts of a run for
@@ -562,8 +567,9 @@ magma_status_t launch_grad(const GradArgs& a, cudaStream_t cs) {
     return st;
   if (a.tiles < 2) return MAGMA_OK;  // no border for a run to cross
   return launch_after(emb_join<TT, V>,
-                      dim3((unsigned)(a.tiles - 1), (unsigned)ceil_div(a.dim, 32 * V)), kSumThreads, 0,
-                      cs, "emb_join", a);
+                      dim3((unsigned)(a.tiles - 1),
+                           (unsigned)std::min<int64_t>(ceil_div(a.dim, 32 * V), 65535)),
+                      kSumThreads, 0, cs, "emb_join", a);
 }
 
 template <typename TI, typename TO>
