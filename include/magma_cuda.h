@@ -264,11 +264,11 @@ MAGMA_API magma_status_t magma_attention_bwd(const void* q, const void* k, const
  * memory, with one another or with any other tensor of the call (an output that
  * begins where another tensor does is refused). kv_lens (int32 [batch] on the
  * device, NULL: kv_len for all) may leave a sequence without keys: its rows of O
- * are 0, its lse -infinity and its gradients 0. Keys and values from kv_lens[b] on have no influence, whatever
- * they hold. A length outside [0, kv_len] is clamped and recorded in the device
+ * are 0, its lse -infinity and its gradients 0. Keys and values from kv_lens[b]
+ * on have no influence, whatever they hold. A length outside [0, kv_len] is clamped and recorded in the device
  * error word. lse [batch, heads, q_len] F32 is the row log-sum-exp of the scaled
- * scores (NULL: not written). dtype F32 or BF16, head_dim <= 128, scale finite
- * and not negative.
+ * scores (NULL: not written). dtype F32 or BF16, head_dim <= 128, lengths
+ * at most 2^31 - 64, scale finite and not negative.
  * workspace (16-byte aligned) may be smaller than the query's answer, or NULL:
  * the forward pass then splits long sources into fewer parts. Calls that
  * overlap on the GPU need workspaces of their own. */

@@ -49,12 +49,15 @@ CrossGeom sizes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t q_len, i
   return g;
 }
 
+// Lengths are padded to multiples of 64 in 32-bit counters.
+constexpr int64_t kMaxLen = (1LL << 31) - 64;
+
 // Whether a workspace query is about a call that launches anything.
 bool has_work(int64_t batch, int64_t heads, int64_t kv_heads, int64_t q_len, int64_t kv_len,
               int64_t hd) {
   return batch > 0 && heads > 0 && kv_heads > 0 && q_len > 0 && kv_len > 0 && hd > 0 && hd <= 128 &&
-         batch < 65536 && heads < 65536 && heads % kv_heads == 0 && q_len < (1LL << 31) &&
-         kv_len < (1LL << 31);
+         batch < 65536 && heads < 65536 && heads % kv_heads == 0 && q_len <= kMaxLen &&
+         kv_len <= kMaxLen;
 }
 
 magma_status_t geometry(const char* fn, const int32_t* kv_lens, int64_t batch, int64_t heads,
@@ -63,7 +66,7 @@ magma_status_t geometry(const char* fn, const int32_t* kv_lens, int64_t batch, i
   MAGMA_REQUIRE(batch >= 0 && heads >= 0 && kv_heads >= 0 && q_len >= 0 && kv_len >= 0,
                 "%s: negative size", fn);
   MAGMA_REQUIRE(batch < 65536 && heads < 65536, "%s: batch and heads must be < 65536", fn);
-  MAGMA_REQUIRE(q_len < (1LL << 31) && kv_len < (1LL << 31), "%s: lengths must be < 2^31", fn);
+  MAGMA_REQUIRE(q_len <= kMaxLen && kv_len <= kMaxLen, "%s: lengths must be at most 2^31 - 64", fn);
   MAGMA_REQUIRE(hd >= 1 && hd <= 128, "%s: head_dim %lld outside [1, 128]", fn, (long long)hd);
   MAGMA_REQUIRE(kv_heads == 0 ? heads == 0 : heads % kv_heads == 0,
                 "%s: heads (%lld) must be a multiple of kv_heads (%lld)", fn, (long long)heads,
