@@ -261,8 +261,9 @@ MAGMA_API magma_status_t magma_attention_bwd(const void* q, const void* k, const
  * query head h reads key head h / (heads / kv_heads). Every tensor has its own
  * (batch, head, position) strides in elements, the last dimension is
  * contiguous; an input's stride may be 0, an output's positions may not share
- * memory, with one another or with any other tensor of the call (an output that
- * begins where another tensor does is refused). kv_lens (int32 [batch] on the
+ * memory, with one another or with any other tensor of the call: such a call is
+ * refused (views that lie between one another, as those of fused projections do,
+ * share none). kv_lens (int32 [batch] on the
  * device, NULL: kv_len for all) may leave a sequence without keys: its rows of O
  * are 0, its lse -infinity and its gradients 0. Keys and values from kv_lens[b]
  * on have no influence, whatever they hold. A length outside [0, kv_len] is clamped and recorded in the device
@@ -376,9 +377,9 @@ MAGMA_API magma_status_t magma_adam_step_clipped(float* params, const float* gra
  * norm). grads, out, sizes and the dtypes (F32 or BF16, each tensor its own) are
  * host arrays of `count` entries, read before the call returns; a tensor of size
  * 0 may be NULL. out[i] may be grads[i] itself (same address and dtype); apart
- * from that an output may not share memory with any tensor of the call. The
- * squares are added in 64 bits. norm is a device F32 scalar. workspace: 8-byte
- * aligned, magma_grad_norm_multi_workspace_size(count) bytes of device memory.
+ * from that an output may not share memory with any tensor of the call, the norm
+ * among them: such a call is refused. The squares are added in 64 bits. norm is a
+ * device F32 scalar. workspace: 8-byte aligned, magma_grad_norm_multi_workspace_size(count) bytes of device memory.
  * magma_grad_norm_multi writes the norm only. */
 MAGMA_API int64_t magma_grad_norm_multi_workspace_size(int32_t count);
 MAGMA_API magma_status_t magma_grad_norm_multi(const void* const* grads, const int64_t* sizes,
@@ -447,7 +448,8 @@ MAGMA_API magma_status_t magma_embedding_bwd_deterministic(const int32_t* tokens
  * table [vocab, dim] with rows table_ld elements apart, pos [>= seq, dim]
  * (NULL: none) in table_dtype; out [batch*seq, dim] in out_dtype; F32 or BF16,
  * F32 arithmetic. A token outside [0, vocab) contributes a zero row and is
- * recorded in the device error word. */
+ * recorded in the device error word. out may not share memory with an input, here
+ * and below outputs neither with inputs nor with one another (refused). */
 MAGMA_API magma_status_t magma_embedding_scaled_fwd(const int32_t* tokens, const void* table,
                                    int64_t table_ld, const void* pos, void* out, int64_t batch,
                                    int64_t seq, int64_t dim, int64_t vocab, float scale,

@@ -3,6 +3,7 @@
 #include <cmath>
 
 #include "cross_attention.cuh"
+#include "memory_views.cuh"
 
 using namespace magma;
 
@@ -33,8 +34,15 @@ magma_status_t set_strides(const char* fn, const char* what, const int64_t* from
   return MAGMA_OK;
 }
 
-// An address that is none of an element's would fault in the kernel.
-bool on_element(const void* p, size_t size) { return reinterpret_cast<uintptr_t>(p) % size == 0; }
+MemView view(const void* p, const CrossGeom& g, int64_t heads, int64_t len, const int64_t (&st)[3],
+             magma_dtype_t dtype) {
+  const int64_t e = (int64_t)dtype_size(dtype);
+  return {p, g.hd * e, {g.batch, heads, len}, {st[0] * e, st[1] * e, st[2] * e}};
+}
+MemView lse_view(const float* lse, const CrossGeom& g) {
+  return {lse, 4 * g.q_len, {g.batch, g.heads, 1}, {4 * g.heads * g.q_len, 4 * g.q_len, 0}};
+}
+MemView lens_view(const CrossGeom& g) { return {g.lens, 4 * g.batch}; }
 
 CrossGeom sizes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t q_len, int64_t kv_len,
                 int64_t hd) {
@@ -114,11 +122,19 @@ magma_status_t magma_cross_attention_fwd(const void* q, const void* k, const voi
   if (magma_status_t st = set_strides(fn, "o", o_strides, g.os, true, batch, heads, q_len, head_dim)) return st;
   if (batch == 0 || heads == 0 || q_len == 0) return MAGMA_OK;
   MAGMA_REQUIRE(q && o && (kv_len == 0 || (k && v)), "%s: NULL pointer", fn);
-  MAGMA_REQUIRE(o != q && o != k && o != v, "%s: o shares memory with an input", fn);
   const void* tensors[] = {q, k, v, o};
   for (const void* x : tensors)
     MAGMA_REQUIRE(on_element(x, dtype_size(dtype)), "%s: an address off its elements", fn);
   MAGMA_REQUIRE(on_element(lse, 4) && on_element(kv_lens, 4), "%s: an address off its elements", fn);
+  const MemView inputs[] = {view(q, g, heads, q_len, g.qs, dtype),
+                            view(k, g, kv_heads, kv_len, g.ks, dtype),
+                            view(v, g, kv_heads, kv_len, g.vs, dtype), lens_view(g)};
+  const MemView ov = view(o, g, heads, q_len, g.os, dtype), lv = lse_view(lse, g);
+  for (const MemView& x : inputs) {
+    MAGMA_REQUIRE(!share_memory(ov, x), "%s: o shares memory with an input", fn);
+    MAGMA_REQUIRE(!share_memory(lv, x), "%s: lse shares memory with an input", fn);
+  }
+  MAGMA_REQUIRE(!share_memory(ov, lv), "%s: o and lse share memory", fn);
   if (cross_step_supported(q, k, v, o, g, dtype))
     return cross_step_run(q, k, v, o, lse, g, dtype, workspace, workspace_bytes,
                           (cudaStream_t)stream);
@@ -169,19 +185,24 @@ magma_status_t magma_cross_attention_bwd(
   const bool has_q = batch && heads && q_len, has_k = batch && kv_heads && kv_len;
   MAGMA_REQUIRE(!has_q || (q && o && d_o && lse && dq), "%s: NULL pointer", fn);
   MAGMA_REQUIRE(!has_k || (k && v && dk && dv), "%s: NULL pointer", fn);
-  const void* grads[] = {has_q ? dq : nullptr, has_k ? dk : nullptr, has_k ? dv : nullptr};
-  const void* inputs[] = {q, k, v, o, d_o};
-  for (int i = 0; i < 3; ++i) {
-    if (grads[i] == nullptr) continue;
-    for (const void* x : inputs)
-      MAGMA_REQUIRE(grads[i] != x, "%s: a gradient shares memory with an input", fn);
-    for (int j = 0; j < i; ++j)
-      MAGMA_REQUIRE(grads[i] != grads[j], "%s: two gradients share memory", fn);
-  }
   const void* tensors[] = {q, k, v, o, d_o, dq, dk, dv};
   for (const void* x : tensors)
     MAGMA_REQUIRE(on_element(x, dtype_size(dtype)), "%s: an address off its elements", fn);
   MAGMA_REQUIRE(on_element(lse, 4) && on_element(kv_lens, 4), "%s: an address off its elements", fn);
+  const MemView inputs[] = {view(q, g, heads, q_len, g.qs, dtype),
+                            view(k, g, kv_heads, kv_len, g.ks, dtype),
+                            view(v, g, kv_heads, kv_len, g.vs, dtype),
+                            view(o, g, heads, q_len, g.os, dtype),
+                            view(d_o, g, heads, q_len, g.dos, dtype), lse_view(lse, g), lens_view(g)};
+  const MemView grads[] = {view(dq, g, heads, q_len, g.dqs, dtype),
+                           view(dk, g, kv_heads, kv_len, g.dks, dtype),
+                           view(dv, g, kv_heads, kv_len, g.dvs, dtype)};
+  for (int i = 0; i < 3; ++i) {
+    for (const MemView& x : inputs)
+      MAGMA_REQUIRE(!share_memory(grads[i], x), "%s: a gradient shares memory with an input", fn);
+    for (int j = 0; j < i; ++j)
+      MAGMA_REQUIRE(!share_memory(grads[i], grads[j]), "%s: two gradients share memory", fn);
+  }
   const size_t need = magma_cross_attention_bwd_workspace_size(batch, heads, kv_heads, q_len,
                                                                kv_len, head_dim, dtype);
   MAGMA_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned16(workspace)),

@@ -37,6 +37,7 @@
 #include <algorithm>
 
 #include "common.cuh"
+#include "memory_views.cuh"
 #include "sm100.cuh"
 
 namespace magma {
@@ -584,8 +585,11 @@ magma_status_t launch_lookup(const int32_t* tokens, const void* table, int64_t l
   return check_launch("emb_lookup");
 }
 
-// An address that is none of an element's would fault in the kernel.
-bool on_element(const void* p, size_t size) { return reinterpret_cast<uintptr_t>(p) % size == 0; }
+// n rows of dim elements, ld apart.
+MemView rows_view(const void* p, int64_t n, int64_t dim, int64_t ld, magma_dtype_t t) {
+  const int64_t e = (int64_t)dtype_size(t);
+  return {p, dim * e, {n, 1, 1}, {ld * e, 0, 0}};
+}
 
 magma_status_t check_sizes(const char* fn, int64_t batch, int64_t seq, int64_t dim, int64_t vocab) {
   MAGMA_REQUIRE(batch >= 0 && seq >= 0 && dim >= 0 && vocab >= 0, "%s: negative size", fn);
@@ -615,12 +619,16 @@ magma_status_t magma_embedding_scaled_fwd(const int32_t* tokens, const void* tab
   if (rows == 0 || dim == 0) return MAGMA_OK;
   MAGMA_REQUIRE(vocab > 0, "%s: an empty table", fn);
   MAGMA_REQUIRE(tokens && table && out, "%s: NULL pointer", fn);
-  MAGMA_REQUIRE(out != table && out != pos, "%s: out shares memory with an input", fn);
   MAGMA_REQUIRE(table_ld >= dim, "%s: table_ld %lld below dim %lld", fn, (long long)table_ld,
                 (long long)dim);
   MAGMA_REQUIRE(on_element(tokens, 4) && on_element(table, dtype_size(table_dtype)) &&
                     on_element(pos, dtype_size(table_dtype)) && on_element(out, dtype_size(out_dtype)),
                 "%s: an address off its elements", fn);
+  const MemView ov = rows_view(out, rows, dim, dim, out_dtype);
+  const MemView inputs[] = {rows_view(table, vocab, dim, table_ld, table_dtype),
+                            rows_view(pos, seq, dim, dim, table_dtype), {tokens, 4 * rows}};
+  for (const MemView& x : inputs)
+    MAGMA_REQUIRE(!share_memory(ov, x), "%s: out shares memory with an input", fn);
   const bool vec = vec_ok(table, table_ld, table_dtype, 8) && vec_ok(out, dim, out_dtype, 8) &&
                    (pos == nullptr || vec_ok(pos, dim, table_dtype, 8));
   cudaStream_t cs = (cudaStream_t)stream;
@@ -655,12 +663,16 @@ magma_status_t magma_embedding_scaled_bwd(const int32_t* tokens, const void* dou
   MAGMA_REQUIRE(vocab == 0 || (dtable && dtable_ld >= dim), "%s: NULL dtable or dtable_ld below dim", fn);
   MAGMA_REQUIRE(rows == 0 || (tokens && dout && dout_ld >= dim),
                 "%s: NULL pointer or dout_ld below dim", fn);
-  MAGMA_REQUIRE(vocab == 0 || (dtable != dout && (const void*)dpos != dtable),
-                "%s: outputs share memory with dout or each other", fn);
-  MAGMA_REQUIRE(dpos == nullptr || (const void*)dpos != dout, "%s: dpos shares memory with dout", fn);
   MAGMA_REQUIRE(on_element(tokens, 4) && on_element(dout, dtype_size(dout_dtype)) &&
                     on_element(dtable, dtype_size(dtable_dtype)) && on_element(dpos, 4),
                 "%s: an address off its elements", fn);
+  const MemView tv = rows_view(dtable, vocab, dim, dtable_ld, dtable_dtype);
+  const MemView pv = rows_view(dpos, seq, dim, dim, MAGMA_DTYPE_F32);
+  const MemView inputs[] = {rows_view(dout, rows, dim, dout_ld, dout_dtype), {tokens, 4 * rows}};
+  for (const MemView& x : inputs)
+    MAGMA_REQUIRE(!share_memory(tv, x) && !share_memory(pv, x),
+                  "%s: outputs share memory with an input", fn);
+  MAGMA_REQUIRE(!share_memory(tv, pv), "%s: dtable and dpos share memory", fn);
   const Layout l = layout(rows, dim);
   MAGMA_REQUIRE(rows == 0 || (workspace && workspace_bytes >= l.total && aligned16(workspace)),
                 "%s: a 16-byte aligned workspace of %lld bytes is needed", fn, (long long)l.total);

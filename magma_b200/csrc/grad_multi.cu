@@ -240,15 +240,17 @@ magma_status_t check(const char* fn, const Tensors& t) {
 }
 
 // An output may be its own gradient (same address and dtype); otherwise it may
-// share no memory with any other tensor of the call, which another block reads
-// or writes at the same time.
-magma_status_t check_overlap(const char* fn, const Tensors& t) {
+// share no memory with any other tensor of the call, the norm among them, which
+// another block reads or writes at the same time.
+magma_status_t check_overlap(const char* fn, const Tensors& t, const float* norm) {
   struct Range {
     uintptr_t begin, end;
     bool out;
   };
   std::vector<Range> r;
-  r.reserve(2 * (size_t)t.count);
+  r.reserve(2 * (size_t)t.count + 1);
+  const uintptr_t n = reinterpret_cast<uintptr_t>(norm);
+  r.push_back({n, n + sizeof(float), true});
   for (int32_t k = 0; k < t.count; ++k) {
     if (t.sizes[k] == 0) continue;
     const uintptr_t g = reinterpret_cast<uintptr_t>(t.g[k]);
@@ -342,7 +344,7 @@ magma_status_t run(const char* fn, const Tensors& t, float grad_scale, float max
                 "%s: an 8-byte aligned workspace is needed", fn);
   if (t.out) {
     try {
-      if (magma_status_t st = check_overlap(fn, t)) return st;
+      if (magma_status_t st = check_overlap(fn, t, norm)) return st;
     } catch (const std::bad_alloc&) {
       return fail(MAGMA_RESOURCE_EXHAUSTED, "%s: out of host memory", fn);
     }
