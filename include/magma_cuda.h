@@ -379,7 +379,8 @@ MAGMA_API magma_status_t magma_adam_step_clipped(float* params, const float* gra
  * 0 may be NULL. out[i] may be grads[i] itself (same address and dtype); apart
  * from that an output may not share memory with any tensor of the call, the norm
  * among them: such a call is refused. The squares are added in 64 bits. norm is a
- * device F32 scalar. workspace: 8-byte aligned, magma_grad_norm_multi_workspace_size(count) bytes of device memory.
+ * device F32 scalar. workspace: 8-byte aligned,
+ * magma_grad_norm_multi_workspace_size(count) bytes of device memory.
  * magma_grad_norm_multi writes the norm only. */
 MAGMA_API int64_t magma_grad_norm_multi_workspace_size(int32_t count);
 MAGMA_API magma_status_t magma_grad_norm_multi(const void* const* grads, const int64_t* sizes,

@@ -29,6 +29,7 @@
 #include <vector>
 
 #include "common.cuh"
+#include "memory_views.cuh"
 
 namespace magma {
 namespace {
@@ -231,9 +232,8 @@ magma_status_t check(const char* fn, const Tensors& t) {
                   fn, k);
     if (t.sizes[k] == 0) continue;
     MAGMA_REQUIRE(t.g[k] && (!t.out || t.out[k]), "%s: NULL tensor at %d", fn, k);
-    MAGMA_REQUIRE(reinterpret_cast<uintptr_t>(t.g[k]) % dtype_size(t.g_dtypes[k]) == 0 &&
-                      (!t.out || reinterpret_cast<uintptr_t>(t.out[k]) %
-                                         dtype_size(t.out_dtypes[k]) == 0),
+    MAGMA_REQUIRE(on_element(t.g[k], dtype_size(t.g_dtypes[k])) &&
+                      (!t.out || on_element(t.out[k], dtype_size(t.out_dtypes[k]))),
                   "%s: tensor %d is not aligned to its element size", fn, k);
   }
   return MAGMA_OK;
@@ -338,7 +338,8 @@ magma_status_t run_lists(const char* fn, const Tensors& t, float grad_scale, flo
 magma_status_t run(const char* fn, const Tensors& t, float grad_scale, float max_norm, float* norm,
                    void* workspace, int64_t workspace_bytes, void* stream) {
   if (magma_status_t st = check(fn, t)) return st;
-  MAGMA_REQUIRE(norm != nullptr, "%s: NULL norm", fn);
+  MAGMA_REQUIRE(norm != nullptr && on_element(norm, sizeof(float)),
+                "%s: NULL norm, or one off its element", fn);
   MAGMA_REQUIRE(workspace != nullptr && workspace_bytes >= 0 &&
                     (reinterpret_cast<uintptr_t>(workspace) & 7u) == 0,
                 "%s: an 8-byte aligned workspace is needed", fn);
