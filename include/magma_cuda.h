@@ -266,7 +266,8 @@ MAGMA_API magma_status_t magma_attention_bwd(const void* q, const void* k, const
  * share none). kv_lens (int32 [batch] on the
  * device, NULL: kv_len for all) may leave a sequence without keys: its rows of O
  * are 0, its lse -infinity and its gradients 0. Keys and values from kv_lens[b]
- * on have no influence, whatever they hold. A length outside [0, kv_len] is clamped and recorded in the device
+ * on have no influence, whatever they hold. A row of scores that are all -infinity
+ * comes out as one without keys; a NaN or +infinity among them makes it NaN. A length outside [0, kv_len] is clamped and recorded in the device
  * error word. lse [batch, heads, q_len] F32 is the row log-sum-exp of the scaled
  * scores (NULL: not written). dtype F32 or BF16, head_dim <= 128, lengths
  * at most 2^31 - 64, scale finite and not negative.

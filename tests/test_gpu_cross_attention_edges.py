@@ -86,3 +86,51 @@ def test_gradient_without_heads_or_sequences(cuda, b, h, g, dtype):
     dk, dv = torch.full_like(k, 7.0), torch.full_like(k, 7.0)
     dq, dk, dv = ops.cross_attention_bwd(q, k, k, o, q, lse, dk=dk, dv=dv)
     assert dq.shape == q.shape and bool((dk == 0).all()) and bool((dv == 0).all())
+
+
+# every path: a few queries in a cluster, in joined chunks, in one chunk; tensor cores or
+# FMA pipe whole and in parts; an odd head size
+PATHS = SPLIT + [(1, 8, 8, 1, 777, 64), (2, 4, 4, 1, 20, 64), (2, 8, 8, 200, 300, 128),
+                 (2, 4, 2, 150, 260, 33)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("case", PATHS)
+@pytest.mark.parametrize("last", [False, True])
+def test_an_infinite_score(cuda, case, dtype, last):
+    """One key's score of a row is +inf: inf - inf has no value, and the row is NaN. The
+    other rows' score of that key is -inf: it has no part in them."""
+    from magma_b200 import ops
+    b, h, g, m, n, d = case
+    q, k, v, do, _ = make(34, b, h, g, m, n, d, dtype)
+    at = n - 1 if last else 0
+    q[..., 0] = -1.0
+    q[0, 0, m - 1, 0] = 1.0
+    k[0, 0, at, 0] = math.inf
+    keep = torch.arange(n, device="cuda") != at
+    want, bound = reference(q[:1], k[:1, :, keep], v[:1, :, keep], do[:1], None, d ** -0.5)
+    o, lse = ops.cross_attention_fwd(q, k, v)
+    assert bool(torch.isnan(o[0, 0, m - 1]).all()) and math.isnan(lse[0, 0, m - 1].item())
+    rows = slice(0, m - 1) if m > 1 else slice(0, 0)
+    check(o[0, 0, rows], want[0][0, 0, rows], bound[0][0, 0, rows], "o")
+    check(lse[0, 0, rows], want[1][0, 0, rows], bound[1][0, 0, rows], "lse")
+    assert bool(torch.isfinite(o[b - 1, h - 1]).all()) and bool(torch.isfinite(lse[b - 1, h - 1]).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("case", PATHS)
+def test_a_row_of_scores_that_are_minus_infinity(cuda, case, dtype):
+    """It comes out as a row without keys, on every path."""
+    from magma_b200 import ops
+    b, h, g, m, n, d = case
+    q, k, v, do, _ = make(35, b, h, g, m, n, d, dtype)
+    want, bound = reference(q, k, v, do, None, d ** -0.5)
+    q[0, 0, m - 1] = 0.0
+    q[0, 0, m - 1, 0] = 1.0
+    k[0, 0, :, 0] = -math.inf
+    o, lse = ops.cross_attention_fwd(q, k, v)
+    assert bool((o[0, 0, m - 1] == 0).all()) and lse[0, 0, m - 1].item() == -math.inf
+    if b * g == 1:  # all heads read these keys
+        return
+    check(o[b - 1, h - 1], want[0][b - 1, h - 1], bound[0][b - 1, h - 1], "o")
+    check(lse[b - 1, h - 1], want[1][b - 1, h - 1], bound[1][b - 1, h - 1], "lse")
