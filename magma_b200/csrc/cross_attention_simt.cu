@@ -685,7 +685,11 @@ magma_status_t fwd(const void* q, const void* k, const void* v, void* o, float* 
 }
 
 // Parts of a tile's steps where the tiles do not give every SM two CTAs: as many as
-// give it four, of at least two steps.
+// give it four, of at least two steps. (Gradients in F32, whole, in parts for two CTAs
+// per SM, and for four: 8 heads over 2 of 64, 40 x 3000, 407, 70 and 70 us; 8 heads, 200 x
+// 333, 97, 55 and 55; 6 x 8 heads, 256 x 512, 226, 226 and 213; 4 heads of 128, 1024 x
+// 1024, 478, 286 and 320. With CTAs for most SMs already the parts cost more than they
+// give: 4 x 8 heads of 64, 512 x 512, 252, 252 and 288.)
 int64_t grad_parts(int64_t ctas, int64_t steps) {
   if (ctas >= 2 * num_sms()) return 1;
   return std::max<int64_t>(1, std::min<int64_t>(4LL * num_sms() / std::max<int64_t>(ctas, 1), steps / 2));

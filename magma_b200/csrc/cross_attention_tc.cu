@@ -1,6 +1,10 @@
 // Attention of queries over the keys and values of another sequence on the
 // tcgen05 tensor cores: BF16, F32 accumulation, head sizes that are multiples
-// of 8 up to 128 (padded to 64 or 128 columns by the tensor maps' zero fill).
+// of 8 up to 128, padded to 64 or 128 columns by the tensor maps' zero fill. The
+// products run over the padded columns, so that their counts are constants: sizes
+// between cost almost what the next of the two does (8 x 16 heads, 512 queries, 1024
+// keys, forward and gradient: 32 columns 33 and 91 us, 64 35 and 101, 80 39 and 133, 96
+// 40 and 136, 128 41 and 142).
 //
 //   cross_fwd_tc     O_t += P_t V_j over the key tiles j, S_t = Q_t K_j^T
 //   cross_rows       -lse log2(e) and delta = rowsum(dO O) of every query row
@@ -241,9 +245,10 @@ __device__ __forceinline__ void store_grad4(__nv_bfloat16* dst, float4 v, float 
 }
 
 // 2^x of a pair on the FMA pipe, for x up to 8: x = n + f with n the nearest whole
-// number (in the low bits of x + 1.5 2^23), the minimax polynomial of degree 5 of
-// 2^f on [-1/2, 1/2] (Remez exchange, relative error 7.5e-8), n added to the
-// exponent; 0 below 2^-126, as ex2.approx.ftz. A NaN becomes FLT_MAX (the bits of
+// number (in the low bits of x + 1.5 2^23), a polynomial of degree 5 for 2^f on
+// [-1/2, 1/2], n added to the exponent (the minimax polynomial by Remez exchange, whose
+// relative error of 7.5e-8 its coefficients' rounding to F32 makes 1.55e-7, at most
+// 2.2e-7 with the roundings of the F32 evaluation); 0 below 2^-126, as ex2.approx.ftz. A NaN becomes FLT_MAX (the bits of
 // the canonical NaN, 0x7FFFFFFF, shifted and added to themselves), which the
 // caller's sum has to turn back.
 __device__ __forceinline__ void ex2_pair_fma(unsigned long long x, float& p0, float& p1) {
@@ -2020,7 +2025,10 @@ bool cross_tc_bwd_supported(const void* q, const void* k, const void* v, const v
 }
 
 // Parts of a source: as many as fill the SMs, at least two key tiles each (a
-// part costs its share of the join: one F32 row per query and part).
+// part costs its share of the join: one F32 row per query and part). Unsplit, and in
+// parts of at least two tiles, one, four: 2 heads of 64, 100 x 6000, 57, 13, 12 and 14
+// us; 8 heads of 128, 256 x 4096, 58, 24, 25 and 21; 16 heads of 64, 128 x 1024, 14, 11, 11
+// and 13. Short sources lose by it: 4 x 8 heads of 128, 256 x 512, 14, 20, 21 and 14.
 static int64_t wanted_splits(const CrossGeom& g) {
   const TcArgs a = args_of(g);
   const int64_t units = (int64_t)a.n_pairs * g.kv_heads * g.batch;

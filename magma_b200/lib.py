@@ -175,7 +175,10 @@ SIGNATURES = {
     "magma_scale": (None, [_vp, _i64, _f, _vp]),
 }
 
-# Kernel launches one successful call of each op makes (for launch accounting).
+# Kernel launches one successful call of each op makes (for launch accounting). The
+# least of them where it depends on sizes: cross attention adds one where the forward
+# pass splits its source and one to three for sums in parts of the gradient, lists of
+# more than 1024 tensors two per further 1024.
 KERNELS_PER_CALL = {
     "magma_layernorm_fwd": 1, "magma_layernorm_bwd": 2, "magma_layernorm_bwd_noalloc": 2,
     "magma_layernorm_bwd_residual": 2,
