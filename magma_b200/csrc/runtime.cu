@@ -41,6 +41,7 @@ magma_status_t fail(magma_status_t code, const char* fmt, ...) {
 
 magma_status_t cuda_status(cudaError_t err, const char* what) {
   if (err == cudaSuccess) return MAGMA_OK;
+  cudaGetLastError();  // reported here: the next launch check must not find it again
   magma_status_t code = MAGMA_INTERNAL;
   if (err == cudaErrorMemoryAllocation) code = MAGMA_RESOURCE_EXHAUSTED;
   else if (err == cudaErrorInvalidValue || err == cudaErrorInvalidDevicePointer ||
