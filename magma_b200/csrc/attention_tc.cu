@@ -28,6 +28,7 @@
 // kernel winds down instead of hanging).
 #include <cuda.h>
 
+#include <cfloat>
 #include <type_traits>
 
 #include "common.cuh"
@@ -409,7 +410,8 @@ attn_fwd_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
         if (ok) {
           tc_fence_after();
           if (j == 0) {
-            m_run = m_new == -INFINITY ? 0.f : m_new;
+            // scores of -inf alone: below any other, so that the first one to come rescales
+            m_run = fmaxf(m_new, -FLT_MAX);
           } else if (__any_sync(0xffffffffu, m_new > m_run + kRescaleLog2)) {
             const float alpha = ex2_approx(m_run - m_new);
             m_run = m_new;
